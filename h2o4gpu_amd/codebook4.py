@@ -1,0 +1,186 @@
+"""4-bit matrices whose 16 values are a codebook (as k-means finds it) and whose groups of columns
+have a scale each, and their products with tokens.
+
+    from h2o4gpu_amd import codebook4
+    packed = codebook4.quantize(W, group=128)      # W (out, cols): the codebook comes from KMeans
+    y = codebook4.product(x, packed)               # x (tokens, cols) -> (tokens, out)
+
+Element (n, k) of such a matrix is codebook[code(n, k)] * scales[n, k // group]. A matrix per expert
+(a leading axis) is multiplied with the rows that an ExpertOrder gives each expert:
+
+    rows = codebook4.experts_product(x, packed, order)
+    y = experts.combine(rows, weights, order)
+
+The products are for serving and have no gradient. Streams and graphs as in h2o4gpu_amd.experts.
+"""
+import numpy as np
+import torch
+
+from .experts import _TYPES, _call, _order_of, _rows, _tensor, _type_of
+from .libs import experts_hip
+
+
+class Codebook4:
+    """A 4-bit matrix (out, cols), or one per expert (experts, out, cols).
+
+    codes: uint8 (..., out, bytes), two columns a byte, the even one in the low half; bytes is at least
+    cols / 2 rounded up. They are kept as they are where rows are contiguous, 16-byte aligned and a
+    multiple of 16 bytes long, otherwise copied once into such rows.
+    scales: (..., out, ceil(cols / group)), float32, bfloat16 or float16; group is a multiple of 32.
+    codebook: (16,) or (experts, 16) finite values in the type of the tokens.
+    """
+
+    __slots__ = ("codes", "scales", "codebook", "cols", "group", "out", "n_experts", "pitch", "_args")
+
+    def __init__(self, codes, scales, codebook, cols, group):
+        lead = codes.dim() - 2 if isinstance(codes, torch.Tensor) else 0
+        if lead not in (0, 1):
+            raise ValueError("codes must be (out, bytes) or (experts, out, bytes), got %s" % (tuple(codes.shape),))
+        _tensor("codes", codes, 2 + lead, dtype=torch.uint8)
+        _tensor("scales", scales, 2 + lead, codes.device)
+        _type_of("scales", scales)
+        _tensor("codebook", codebook, codebook.dim() if isinstance(codebook, torch.Tensor) else 1, codes.device)
+        _type_of("codebook", codebook)
+        cols, group = int(cols), int(group)
+        if group < 32 or group % 32:
+            raise ValueError("group must be a multiple of 32, got %d" % group)
+        if cols < 1 or codes.shape[-1] < (cols + 1) // 2:
+            raise ValueError("%d bytes a row do not hold %d columns" % (codes.shape[-1], cols))
+        if codes.shape[-2] < 1 or (lead and not 1 <= codes.shape[0] <= experts_hip.MAX_EXPERTS):
+            raise ValueError("codes must have rows (and 1 to %d experts), got %s" % (experts_hip.MAX_EXPERTS,
+                                                                                     tuple(codes.shape)))
+        groups = -(-cols // group)
+        if tuple(scales.shape) != tuple(codes.shape[:-1]) + (groups,):
+            raise ValueError("scales must be %s, got %s" % (tuple(codes.shape[:-1]) + (groups,),
+                                                            tuple(scales.shape)))
+        if tuple(codebook.shape) != (16,) and not (lead and tuple(codebook.shape) == (codes.shape[0], 16)):
+            raise ValueError("codebook must have 16 values%s, got shape %s" % (
+                " (or 16 for each expert)" if lead else "", tuple(codebook.shape)))
+        pitch = -(-codes.shape[-1] // 16) * 16
+        if pitch != codes.shape[-1] or not codes.is_contiguous() or codes.data_ptr() % 16:
+            padded = codes.new_zeros(codes.shape[:-1] + (pitch,))
+            padded[..., :codes.shape[-1]] = codes
+            codes = padded
+        self.codes, self.scales, self.codebook = codes, scales.contiguous(), codebook.contiguous()
+        self.cols, self.group, self.out, self.pitch = cols, group, codes.shape[-2], pitch
+        self.n_experts = codes.shape[0] if lead else 0
+        self._args = (self.codes.data_ptr(), pitch, _TYPES[scales.dtype], self.scales.data_ptr(),
+                      self.codebook.data_ptr())
+
+    @property
+    def dtype(self):
+        """The type of the tokens that this matrix multiplies."""
+        return self.codebook.dtype
+
+    def dequantize(self):
+        """The matrix as a float32 tensor (for checks and for training on)."""
+        table = self.codebook.float()
+        pair = torch.arange(256, device=table.device)
+        table = torch.stack([table[..., pair & 15], table[..., pair >> 4]], -1)  # (..., 256, 2)
+        index = self.codes.to(torch.int64)
+        if table.dim() == 2:
+            w = table[index]
+        else:
+            w = table[torch.arange(self.n_experts, device=index.device)[:, None, None], index]
+        return w.flatten(-2)[..., :self.cols] * self.scales.float().repeat_interleave(self.group, -1)[..., :self.cols]
+
+
+def fit_codebook(values, sample=1 << 20, seed=0):
+    """The 16 centroids k-means finds for `values` (a GPU tensor, any shape), ascending, float32."""
+    from .solvers.kmeans import KMeans
+    flat = values.reshape(-1)
+    if flat.numel() > sample:  # evenly spaced: repeatable, and every part of the matrix is in it
+        flat = flat[torch.arange(sample, device=flat.device) * (flat.numel() // sample)]
+    flat = flat.float()
+    flat = flat[torch.isfinite(flat)]
+    if flat.numel() < 16:
+        raise ValueError("a codebook needs at least 16 finite values, got %d" % flat.numel())
+    at = torch.linspace(0.5 / 16, 1 - 0.5 / 16, 16, device=flat.device)
+    start = torch.sort(flat).values[(at * (flat.numel() - 1)).long()]
+    model = KMeans(n_clusters=16, init=start.cpu().numpy()[:, None], max_iter=100, tol=1e-9, random_state=seed)
+    model.fit(flat[:, None].contiguous())
+    return torch.from_numpy(np.sort(model.cluster_centers_.reshape(-1))).float().to(flat.device)
+
+
+def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
+    """Codebook4 of `weights`, (out, cols) or (experts, out, cols).
+
+    A group's scale is its largest magnitude over `top`, and every element gets the code of the entry
+    nearest to element / scale. codebook: 16 values (top: the one that a group's largest magnitude
+    stands for, e.g. 7 for the integers -8 .. 7); None fits it to the scaled elements with k-means.
+    It is rounded to the weights' type before the codes are chosen. scale_dtype defaults to that type.
+    """
+    _tensor("weights", weights, weights.dim() if isinstance(weights, torch.Tensor) and weights.dim() == 3 else 2)
+    code = _type_of("weights", weights)
+    group, top = int(group), float(top)
+    if group < 32 or group % 32:
+        raise ValueError("group must be a multiple of 32, got %d" % group)
+    if min(weights.shape) < 1:
+        raise ValueError("weights are empty: %s" % (tuple(weights.shape),))
+    if not 0.0 < top <= 3.4e38:
+        raise ValueError("top must be positive and finite, got %r" % top)
+    cols = weights.shape[-1]
+    flat = weights.detach().reshape(-1, cols)
+    if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < cols):
+        flat = flat.contiguous()
+    groups, pitch = -(-cols // group), -(-cols // 32) * 16
+    if codebook is None:
+        if top != 1.0:
+            raise ValueError("top goes with a given codebook; one that is fitted has 1")
+        part = flat[torch.arange(min(flat.shape[0], 4096), device=flat.device) *
+                    (flat.shape[0] // min(flat.shape[0], 4096))].float()
+        padded = torch.nn.functional.pad(part, (0, groups * group - cols)).reshape(part.shape[0], groups, group)
+        scaled = padded / padded.abs().amax(2, keepdim=True).clamp_min(1e-38)
+        codebook = fit_codebook(scaled.reshape(part.shape[0], -1)[:, :cols])
+    _tensor("codebook", codebook, 1, weights.device)
+    if codebook.shape[0] != 16:
+        raise ValueError("codebook must have 16 values, got %d" % codebook.shape[0])
+    codebook = codebook.to(weights.dtype).contiguous()
+    codes = torch.empty((flat.shape[0], pitch), dtype=torch.uint8, device=flat.device)
+    scales = torch.empty((flat.shape[0], groups), dtype=scale_dtype or weights.dtype, device=flat.device)
+    ptr, stride = _rows("weights", flat)
+    _call(flat.device, "h2o4gpu_codebook4_quantize", code, flat.shape[0], cols, group, top, ptr, stride,
+          codebook.data_ptr(), codes.data_ptr(), pitch, _type_of("scales", scales), scales.data_ptr())
+    lead = tuple(weights.shape[:-1])
+    return Codebook4(codes.reshape(lead + (pitch,)), scales.reshape(lead + (groups,)), codebook, cols, group)
+
+
+def _tokens(x, weights):
+    if not isinstance(weights, Codebook4):
+        raise TypeError("weights must be a Codebook4, got %s" % type(weights).__name__)
+    _tensor("x", x, 2, weights.codes.device, weights.dtype)
+    if x.shape[1] != weights.cols:
+        raise ValueError("x must be (tokens, %d), got %s" % (weights.cols, tuple(x.shape)))
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("products with 4-bit matrices have no gradient: detach x, or multiply with dequantize()")
+    return _rows("x", x)
+
+
+def product(x, weights):
+    """(tokens, out) = x (tokens, cols) times the transpose of a Codebook4 matrix; products and sums in
+    float32, rounded once to the type of x."""
+    ptr, stride = _tokens(x, weights)
+    if weights.n_experts:
+        raise ValueError("weights hold a matrix per expert: experts_product multiplies with those")
+    y = torch.empty((x.shape[0], weights.out), dtype=x.dtype, device=x.device)
+    _call(x.device, "h2o4gpu_codebook4_product", _TYPES[x.dtype], x.shape[0], weights.out, weights.cols,
+          weights.group, ptr, stride, *weights._args, y.data_ptr(), weights.out)
+    return y
+
+
+def experts_product(x, weights, order):
+    """(tokens * top_k, out), rows in expert order: the token of every slot of `order` times the
+    transpose of its expert's matrix; zeros behind order.offsets[-1]. Only the matrices of experts that
+    have a token are read."""
+    ptr, stride = _tokens(x, weights)
+    _order_of(order, x.device)
+    if not weights.n_experts or weights.n_experts != order.n_experts:
+        raise ValueError("order has %d experts, weights %d" % (order.n_experts, weights.n_experts))
+    if x.shape[0] != order.tokens:
+        raise ValueError("x must be (%d, %d), got %s" % (order.tokens, weights.cols, tuple(x.shape)))
+    y = torch.empty((order.tokens * order.top_k, weights.out), dtype=x.dtype, device=x.device)
+    _call(x.device, "h2o4gpu_codebook4_experts_product", _TYPES[x.dtype], order.tokens, order.top_k,
+          weights.n_experts, weights.out, weights.cols, weights.group, ptr, stride, *weights._args,
+          16 if weights.codebook.dim() == 2 else 0, order.order.data_ptr(), order.offsets.data_ptr(), y.data_ptr(),
+          weights.out)
+    return y
