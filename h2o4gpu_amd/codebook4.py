@@ -24,13 +24,14 @@ class Codebook4:
     """A 4-bit matrix (out, cols), or one per expert (experts, out, cols).
 
     codes: uint8 (..., out, bytes), two columns a byte, the even one in the low half; bytes is at least
-    cols / 2 rounded up. They are kept as they are where rows are contiguous, 16-byte aligned and a
-    multiple of 16 bytes long, otherwise copied once into such rows.
-    scales: (..., out, ceil(cols / group)), float32, bfloat16 or float16; group is a multiple of 32.
-    codebook: (16,) or (experts, 16) finite values in the type of the tokens.
+    cols / 2 rounded up. scales: (..., out, ceil(cols / group)), float32, bfloat16 or float16; group is a
+    multiple of 32. codebook: (16,) or (experts, 16) finite values in the type of the tokens.
+
+    Codes and scales are copied once into the order that the products read them in (`laid_codes`,
+    `laid_scales`); those passed in are not needed afterwards.
     """
 
-    __slots__ = ("codes", "scales", "codebook", "cols", "group", "out", "n_experts", "pitch", "_args")
+    __slots__ = ("laid_codes", "laid_scales", "codebook", "cols", "group", "out", "n_experts", "_args")
 
     def __init__(self, codes, scales, codebook, cols, group):
         lead = codes.dim() - 2 if isinstance(codes, torch.Tensor) else 0
@@ -56,16 +57,38 @@ class Codebook4:
         if tuple(codebook.shape) != (16,) and not (lead and tuple(codebook.shape) == (codes.shape[0], 16)):
             raise ValueError("codebook must have 16 values%s, got shape %s" % (
                 " (or 16 for each expert)" if lead else "", tuple(codebook.shape)))
-        pitch = -(-codes.shape[-1] // 16) * 16
-        if pitch != codes.shape[-1] or not codes.is_contiguous() or codes.data_ptr() % 16:
-            padded = codes.new_zeros(codes.shape[:-1] + (pitch,))
-            padded[..., :codes.shape[-1]] = codes
-            codes = padded
-        self.codes, self.scales, self.codebook = codes, scales.contiguous(), codebook.contiguous()
-        self.cols, self.group, self.out, self.pitch = cols, group, codes.shape[-2], pitch
+        codes, scales, device = codes.contiguous(), scales.contiguous(), codes.device
+        self.codebook, self.cols, self.group, self.out = codebook.contiguous(), cols, group, codes.shape[-2]
         self.n_experts = codes.shape[0] if lead else 0
-        self._args = (self.codes.data_ptr(), pitch, _TYPES[scales.dtype], self.scales.data_ptr(),
-                      self.codebook.data_ptr())
+        count, lib = max(1, self.n_experts), experts_hip.lib()
+        kind = _TYPES[scales.dtype]
+        nbytes = lib.h2o4gpu_codebook4_codes_bytes(count, self.out, cols)
+        if nbytes == 0:
+            raise ValueError("a matrix of %d x %d is beyond what the products take" % (self.out, cols))
+        self.laid_codes = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        nbytes = lib.h2o4gpu_codebook4_scales_bytes(count, self.out, cols, group, kind)
+        self.laid_scales = torch.empty(nbytes // scales.element_size(), dtype=scales.dtype, device=device)
+        _call(device, "h2o4gpu_codebook4_layout", count, self.out, cols, group, codes.data_ptr(), codes.shape[-1],
+              kind, scales.data_ptr(), self.laid_codes.data_ptr(), self.laid_scales.data_ptr())
+        self._args = (self.laid_codes.data_ptr(), kind, self.laid_scales.data_ptr(), self.codebook.data_ptr())
+
+    def codes(self):
+        """The codes, one a byte: uint8 (..., out, cols)."""
+        count, tiles, subs = max(1, self.n_experts), -(-self.out // 16), -(-self.cols // 128)
+        # (tile, 128 columns, q, row, 32 columns, bytes of 8) -> (tile, row, 128 columns, 32 columns, q, bytes)
+        raw = self.laid_codes.view(count, tiles, subs, 4, 16, 4, 4).permute(0, 1, 4, 2, 5, 3, 6)
+        raw = raw.reshape(count, tiles * 16, subs * 64)[:, :self.out]
+        codes = torch.stack([raw & 15, raw >> 4], -1).flatten(-2)[..., :self.cols]
+        return codes if self.n_experts else codes[0]
+
+    def scales(self):
+        """The scales, (..., out, ceil(cols / group))."""
+        count, tiles, subs = max(1, self.n_experts), -(-self.out // 16), -(-self.cols // 128)
+        per = 1 if self.group % 128 == 0 else 2 if self.group % 64 == 0 else 4
+        laid = self.laid_scales.view(count, tiles, subs, 16, per).permute(0, 1, 3, 2, 4)
+        laid = laid.reshape(count, tiles * 16, subs * per)[:, :self.out]
+        laid = laid[..., ::self.group * per // 128].contiguous()[..., :-(-self.cols // self.group)]
+        return laid if self.n_experts else laid[0]
 
     @property
     def dtype(self):
@@ -74,15 +97,12 @@ class Codebook4:
 
     def dequantize(self):
         """The matrix as a float32 tensor (for checks and for training on)."""
-        table = self.codebook.float()
-        pair = torch.arange(256, device=table.device)
-        table = torch.stack([table[..., pair & 15], table[..., pair >> 4]], -1)  # (..., 256, 2)
-        index = self.codes.to(torch.int64)
+        table, codes = self.codebook.float(), self.codes().to(torch.int64)
         if table.dim() == 2:
-            w = table[index]
+            values = table[torch.arange(self.n_experts, device=codes.device)[:, None, None], codes]
         else:
-            w = table[torch.arange(self.n_experts, device=index.device)[:, None, None], index]
-        return w.flatten(-2)[..., :self.cols] * self.scales.float().repeat_interleave(self.group, -1)[..., :self.cols]
+            values = table[codes]
+        return values * self.scales().float().repeat_interleave(self.group, -1)[..., :self.cols]
 
 
 def fit_codebook(values, sample=1 << 20, seed=0):
@@ -123,7 +143,7 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
     flat = weights.detach().reshape(-1, cols)
     if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < cols):
         flat = flat.contiguous()
-    groups, pitch = -(-cols // group), -(-cols // 32) * 16
+    groups, pitch = -(-cols // group), -(-cols // 2)
     if codebook is None:
         if top != 1.0:
             raise ValueError("top goes with a given codebook; one that is fitted has 1")
@@ -148,7 +168,7 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
 def _tokens(x, weights):
     if not isinstance(weights, Codebook4):
         raise TypeError("weights must be a Codebook4, got %s" % type(weights).__name__)
-    _tensor("x", x, 2, weights.codes.device, weights.dtype)
+    _tensor("x", x, 2, weights.laid_codes.device, weights.dtype)
     if x.shape[1] != weights.cols:
         raise ValueError("x must be (tokens, %d), got %s" % (weights.cols, tuple(x.shape)))
     if x.requires_grad and torch.is_grad_enabled():

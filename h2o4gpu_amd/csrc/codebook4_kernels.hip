@@ -17,9 +17,8 @@ __global__ __launch_bounds__(256) void quantize4_kernel(const T *w, int64_t ws, 
                                                         float top, const T *book, uint8_t *codes, int64_t pitch,
                                                         S *scales) {
   const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= out) return;
   const int groups = (cols + group - 1) / group;
+  for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < out; n += (int64_t)gridDim.x * 4) {
   for (int g = 0; g < groups; g++) {
     const int lo = g * group, hi = lo + group < cols ? lo + group : cols;
     float most = 0.f;
@@ -50,6 +49,7 @@ __global__ __launch_bounds__(256) void quantize4_kernel(const T *w, int64_t ws, 
     }
   }
   for (int64_t b = (cols + 1) / 2 + lane; b < pitch; b += 64) codes[n * pitch + b] = 0;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -63,11 +63,15 @@ struct RowSource {
   int64_t rows = 0;  // of y
 };
 
+// A matrix (or one per expert) in the order the product reads it, see launch_layout4.
 struct Matrix4 {
-  const uint8_t *codes = nullptr;
-  int64_t pitch = 0, out = 0;
-  int cols = 0, group = 0, groups = 0;
+  const uint4 *codes = nullptr;
+  const void *scales = nullptr;
+  const void *books = nullptr;
   int64_t book_stride = 0;
+  int64_t out = 0;
+  int cols = 0;
+  int per = 1;  // scales of a row for 128 columns
 };
 
 // The product on the matrix cores. x is the "A" operand (rows of the result tile: 16 tokens), the
@@ -75,20 +79,21 @@ struct Matrix4 {
 // applies is its own column's:
 //   A[i = lane % 16][k = VK * (lane / 16) + 0 .. VK-1], B[k likewise][j = lane % 16],
 //   accumulator v: D[i = 4 * (lane / 16) + v][j = lane % 16].
-// A wavefront takes 128 columns of the matrix at a time: lane (r, q) loads the 16 bytes of row r that
-// hold group-of-32 number q, and a 4 x 4 transposition between the four lane groups and the four
-// registers (four swaps) gives every lane 8 columns of each 32, so that no instruction mixes columns of
-// two scales. Codes become values through a table of pairs in LDS, indexed by a whole byte: 256
-// entries, each once per bank that a lane may read from, so the reads never collide (a table in
-// registers takes 3.1 vector instructions a code, this one takes one and half a read). Products are
-// exact in float, sums are float; the scale is applied to the sum over its group.
+// The matrix lies in tiles of 16 rows and 128 columns, each the 1024 bytes that a wavefront loads at once:
+// lane (r, q) has 8 columns of each 32 of row r, so that no instruction mixes columns of two scales,
+// and a wavefront that goes along its columns reads one stretch of memory. (Read from rows as they
+// are, 64 bytes of 16 rows at a time and 2 bytes of 16 rows of scales, 8192 x 8192 takes 16 us at one
+// token.) Codes become values through a table of pairs in LDS, indexed by a whole byte: 256
+// entries of 256 bytes, each with a copy of the pair for every bank, so that reads do not collide and an
+// address is one byte permutation (a table in registers takes 3.1 vector instructions a code, this one
+// half an instruction and half a read). Products are exact in float, sums are float; the scale is
+// applied to the sum over its group.
 template <typename T>
 struct Mfma4;
 
 template <>
 struct Mfma4<bfloat16_t> {
   typedef bfloat16_t vec __attribute__((ext_vector_type(8)));
-  static constexpr int COPIES = 32;  // of the pair table: 4 bytes each
   static __device__ __forceinline__ floatx4 mma(const unsigned *a, const unsigned *b, floatx4 c) {
     vec va, vb;
     __builtin_memcpy(&va, a, 16);
@@ -100,7 +105,6 @@ struct Mfma4<bfloat16_t> {
 template <>
 struct Mfma4<float16_t> {
   typedef float16_t vec __attribute__((ext_vector_type(8)));
-  static constexpr int COPIES = 32;
   static __device__ __forceinline__ floatx4 mma(const unsigned *a, const unsigned *b, floatx4 c) {
     vec va, vb;
     __builtin_memcpy(&va, a, 16);
@@ -111,7 +115,6 @@ struct Mfma4<float16_t> {
 
 template <>
 struct Mfma4<float> {
-  static constexpr int COPIES = 16;  // 8 bytes each
   static __device__ __forceinline__ floatx4 mma(const unsigned *a, const unsigned *b, floatx4 c) {
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -120,12 +123,12 @@ struct Mfma4<float> {
   }
 };
 
-static const int TABLE_BYTES = 256 * 128;
+static const int TABLE_BYTES = 256 * 256;
 
 // The same bytes at an address that is only aligned to its elements.
 typedef unsigned uintx4_u __attribute__((ext_vector_type(4), aligned(2)));
 
-// 8 values of x as 32-bit words; the last columns of a row with zeros behind them.
+// 8 values of x as 32-bit words.
 template <typename T>
 __device__ __forceinline__ void load_x8(const T *at, unsigned (&w)[2 * sizeof(T)]) {
 #pragma unroll
@@ -137,325 +140,558 @@ __device__ __forceinline__ void load_x8(const T *at, unsigned (&w)[2 * sizeof(T)
     w[4 * i + 3] = v[3];
   }
 }
+// (left: columns from `at` to the row's end, negative behind it; at[left - 1] is the row's last)
 template <typename T>
 __device__ __forceinline__ void load_x8_end(const T *at, int left, unsigned (&w)[2 * sizeof(T)]) {
+  if (left >= 8) {
+    load_x8<T>(at, w);
+    return;
+  }
+  // (as if new here: 32 offsets made ahead of the loops would take the registers of the loops)
+  asm volatile("" : "+v"(left));
   T v[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = i < left ? at[i] : (T)0.f;
+  for (int i = 0; i < 8; i++) v[i] = at[i < left ? i : left - 1];  // every load on its way before the first is used
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = i < left ? v[i] : (T)0.f;
   __builtin_memcpy(w, v, sizeof(v));
 }
 
-// 8 codes as 8 values: byte b of the word names a pair.
+// 8 codes as 8 values: byte b of the word names a pair, whose copy for this lane lies lane_at into the entry.
+// The table is the first thing in LDS (address 0): an address that had to be added to would cost as much as
+// the permutation that makes it.
 template <typename T>
-__device__ __forceinline__ void decode8(const char *table, unsigned word, unsigned lane_at,
+__device__ __forceinline__ void decode8(unsigned word, unsigned lane_at,
                                         unsigned (&w)[2 * sizeof(T)]) {
-  const unsigned at0 = ((word << 7) & 0x7f80u) | lane_at, at1 = ((word >> 1) & 0x7f80u) | lane_at;
-  const unsigned at2 = ((word >> 9) & 0x7f80u) | lane_at, at3 = ((word >> 17) & 0x7f80u) | lane_at;
-  typedef typename std::conditional<sizeof(T) == 4, uint2, unsigned>::type Pair;
-  const Pair p[4] = {*reinterpret_cast<const Pair *>(table + at0), *reinterpret_cast<const Pair *>(table + at1),
-                     *reinterpret_cast<const Pair *>(table + at2), *reinterpret_cast<const Pair *>(table + at3)};
+  typedef unsigned Two __attribute__((ext_vector_type(2)));
+  typedef typename std::conditional<sizeof(T) == 4, Two, unsigned>::type Pair;
+  typedef const __attribute__((address_space(3))) Pair *LdsPair;
+  // address = 256 * byte + lane_at: result bytes 0, 0, word's byte b, lane_at's byte 0
+  const unsigned at[4] = {__builtin_amdgcn_perm(word, lane_at, 0x0c0c0400), __builtin_amdgcn_perm(word, lane_at, 0x0c0c0500),
+                          __builtin_amdgcn_perm(word, lane_at, 0x0c0c0600), __builtin_amdgcn_perm(word, lane_at, 0x0c0c0700)};
+  Pair p[4];
+#pragma unroll
+  for (int b = 0; b < 4; b++) p[b] = *reinterpret_cast<LdsPair>((uint32_t)at[b]);
   __builtin_memcpy(w, p, sizeof(p));
-}
-
-// A scale of 32 or of 16 bits, the latter of either type.
-__device__ __forceinline__ float scale_value(float v, bool) { return v; }
-__device__ __forceinline__ float scale_value(uint16_t v, bool brain) {
-  float16_t h;
-  __builtin_memcpy(&h, &v, 2);
-  return brain ? __uint_as_float((unsigned)v << 16) : (float)h;
 }
 
 struct Product4Args {
   Matrix4 m;
-  bool brain;                // 16-bit scales are bfloat16
   RowSource src;
   int64_t xs, ys;
-  unsigned per_scale;        // how many 32s (FINE) or 128s of columns share a scale
-  unsigned per_scale_magic;  // ceil(2^32 / per_scale); 0 where that is 1
+  int splits;  // wavefronts that share a tile's columns
 };
 
-// What a wavefront has in flight: U times 128 columns of the matrix.
-template <typename T, typename S, int MT, int NT, int U, bool FINE>
-struct Stage {
-  uint4 words[U][NT];
-  S scale[U][NT][FINE ? 4 : 1];  // as they lie in memory: nothing waits for them before they are used
-  unsigned x[U][MT][4][2 * sizeof(T)];
+// A workgroup's expert and rows of y; hi <= lo where it has none.
+struct Share {
+  int expert = 0;
+  int64_t lo = 0, hi = 0;
 };
 
-// acc += scale * (x times 128 columns of the matrix's transpose).
-template <typename T, typename S, int MT, int NT, int U, bool FINE>
-__device__ __forceinline__ void multiply(const Stage<T, S, MT, NT, U, FINE> &st, int u, const char *table,
-                                         unsigned lane_at, bool brain, floatx4 (&acc)[MT][NT]) {
+// With experts, blockIdx.y is one, or, where there are fewer rows than experts, a row: the workgroups of an
+// expert's first row then have all of its rows. The last blockIdx.y writes zeros to the rows that have none.
+template <typename T>
+__device__ __forceinline__ Share share_of(const Product4Args &a, int *found, T *y) {
+  Share s;
+  s.hi = a.src.rows;
+  if (!a.src.offsets) return s;
+  const int E = a.src.experts;
+  if (blockIdx.y == gridDim.y - 1) {
+    for (int64_t p = a.src.offsets[E] + blockIdx.x; p < s.hi; p += gridDim.x)
+      for (int64_t n = threadIdx.x; n < a.m.out; n += blockDim.x) y[p * a.ys + n] = (T)0.f;
+    s.hi = 0;
+    return s;
+  }
+  if ((int)gridDim.y - 1 == E) {
+    s.expert = blockIdx.y;
+    s.lo = a.src.offsets[s.expert];
+    s.hi = a.src.offsets[s.expert + 1];
+    return s;
+  }
+  if (threadIdx.x == 0) found[0] = -1;
+  __syncthreads();
+  const int p = blockIdx.y;
+  for (int i = threadIdx.x; i < E; i += blockDim.x) {
+    const int from = a.src.offsets[i], to = a.src.offsets[i + 1];
+    if (from == p && to > p) {
+      found[0] = i;
+      found[1] = to;
+    }
+  }
+  __syncthreads();
+  s.expert = __builtin_amdgcn_readfirstlane(found[0]);
+  s.lo = p;
+  s.hi = s.expert >= 0 ? __builtin_amdgcn_readfirstlane(found[1]) : p;
+  __syncthreads();
+  return s;
+}
+
+// Where row p of y has its x.
+template <typename T>
+__device__ __forceinline__ const T *x_row(const T *x, const Product4Args &a, int64_t p) {
+  return x + (a.src.order ? (int64_t)((unsigned)a.src.order[p] / (unsigned)a.src.top_k) : p) * a.xs;
+}
+
+// The pair table of an expert's codebook: 16 lanes write an entry, a wavefront four in a row, so that no two
+// lanes write to one bank.
+template <typename T>
+__device__ __forceinline__ void make_table(char *lds, const Matrix4 &m, int e) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r = lane & 15;
+  const float held = (float)static_cast<const T *>(m.books)[e * m.book_stride + r];
+  for (int byte = wave * 4 + (lane >> 4); byte < 256; byte += waves * 4) {
+    const T low = (T)__shfl(held, byte & 15, 64), high = (T)__shfl(held, byte >> 4, 64);
+    T pair[16 / sizeof(T)];
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const uint4 w = st.words[u][t];
-    const auto s02 = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
-    const auto s13 = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
-    const auto d01 = __builtin_amdgcn_permlane16_swap(s02[0], s13[0], false, false);
-    const auto d23 = __builtin_amdgcn_permlane16_swap(s02[1], s13[1], false, false);
-    const unsigned d[4] = {d01[0], d01[1], d23[0], d23[1]};
-    floatx4 part[MT] = {};
+    for (int c = 0; c < (int)(16 / sizeof(T)); c += 2) {
+      pair[c] = low;
+      pair[c + 1] = high;
+    }
+    uint4 four;
+    __builtin_memcpy(&four, pair, 16);
+    *reinterpret_cast<uint4 *>(lds + byte * 256 + r * 16) = four;
+  }
+  __syncthreads();
+}
+
+// The 128 columns of NT tiles, on their way to or in registers: scales as they lie in memory, so that nothing
+// waits for them before they are used.
+template <typename S, int NT, int PER>
+struct Tiles {
+  struct alignas(sizeof(S) * PER) Scales {
+    S v[PER];
+  };
+  uint4 words[NT];
+  Scales scale[NT];
+};
+
+// A wavefront's place in the matrix.
+template <typename S, int NT, int PER>
+struct Reader {
+  typedef Tiles<S, NT, PER> Held;
+  const uint4 *codes;
+  const typename Held::Scales *scales;
+  int64_t at[NT];
+
+  __device__ __forceinline__ Reader(const Matrix4 &m, int e, int tiles16, int subs) {
+    codes = m.codes + (int64_t)e * tiles16 * subs * 64 + (threadIdx.x & 63);
+    scales = static_cast<const typename Held::Scales *>(m.scales) + (int64_t)e * tiles16 * subs * 16 +
+             (threadIdx.x & 15);
+  }
+  __device__ __forceinline__ void move_to(int tile, int tiles16, int subs) {  // (behind the last tile: the last again)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      unsigned b[2 * sizeof(T)];
-      decode8<T>(table, d[i], lane_at, b);
+    for (int t = 0; t < NT; t++) at[t] = (int64_t)(tile + t < tiles16 ? tile + t : tiles16 - 1) * subs;
+  }
+  __device__ __forceinline__ void fetch(Held &h, int sub) const {
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        part[m] = Mfma4<T>::mma(st.x[u][m][i], b, part[m]);
-        if (FINE || i == 3) {
+    for (int t = 0; t < NT; t++) {
+      h.words[t] = codes[(at[t] + sub) * 64];
+      h.scale[t] = scales[(at[t] + sub) * 16];
+    }
+  }
+};
+
+// One tile's 128 columns as values: 4 operands of a product. Every table read is on its way before what follows.
+template <typename T>
+__device__ __forceinline__ void decode(const uint4 &words, unsigned lane_at, unsigned (&b)[4][2 * sizeof(T)]) {
+  const unsigned d[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-          for (int v = 0; v < 4; v++)
-            acc[m][t][v] = fmaf(scale_value(st.scale[u][t][FINE ? i : 0], brain), part[m][v], acc[m][t][v]);
-          part[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 4; i++) decode8<T>(d[i], lane_at, b[i]);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Both kernels: a workgroup's wavefronts have blockDim / 64 / splits tiles of 16 * NT columns of y at a time;
+// `splits` wavefronts share a tile's columns of the matrix, each a stretch of them, 128 at a time with the
+// next R on their way, and add their sums up in LDS. PER: scales of a row for 128 columns (1, 2 or 4).
+
+// Up to MP rows of y at a time (1 or 4). A product's 16 rows of x are these rows in G = 16 / MP pieces of 128
+// columns, loaded once for G tiles of the matrix: the result's row p * MP + m is y's row m with piece p, and of
+// each product only the rows of the tile's own piece are kept.
+template <typename T, typename S, int MP, int PER>
+__global__ __launch_bounds__(512, sizeof(T) == 2 ? 4 : 2) void product4_few_kernel(const T *x, T *y, Product4Args a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int G = 16 / MP, SETS = MP == 4 ? 2 : 1;
+  constexpr int R = MP == 4 && PER > 1 ? 2 : 4;  // (as many as there are registers for)
+  typedef unsigned Frag[4][2 * sizeof(T)];
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  float *red = reinterpret_cast<float *>(lds + TABLE_BYTES);
+  const int teams = waves / a.splits, team = wave / a.splits, part = wave % a.splits;
+  const int tiles16 = (int)((a.m.out + 15) >> 4), subs = (a.m.cols + 127) >> 7;
+  const Share share = share_of(a, reinterpret_cast<int *>(red), y);
+  const int64_t begin = share.lo + (int64_t)blockIdx.z * MP, hi = share.hi;
+  if (begin >= hi) return;
+  const unsigned lane_at = (lane * 2 * sizeof(T)) & 255;
+  const int cols = a.m.cols, full = cols >> 7;
+  const int first = full * part / a.splits, count = full * (part + 1) / a.splits - first;
+  Reader<S, 1, PER> reader(a.m, share.expert, tiles16, subs);
+
+  bool have_table = false;
+  for (int tile0 = blockIdx.x * teams; tile0 < tiles16; tile0 += gridDim.x * teams) {
+    const int tile = tile0 + team;
+    const bool mine = tile < tiles16;
+    reader.move_to(tile, tiles16, subs);
+    for (int64_t lo = begin; lo < hi; lo += (int64_t)gridDim.z * MP) {
+      const T *row = x_row(x, a, lo + r % MP < hi ? lo + r % MP : hi - 1) + 8 * q;
+      const auto load_x = [&](Frag &xf, int b) {  // (pieces behind the last tile: the last tile's again)
+        const int64_t at = (int64_t)(first + (b + r / MP < count ? b + r / MP : count - 1)) * 128;
+#pragma unroll
+        for (int i = 0; i < 4; i++) load_x8<T>(row + (at + 32 * i), xf[i]);
+      };
+      float acc[MP] = {};  // over the pieces of lanes q
+      // j: the piece, of which the last two bits are known when this is compiled
+      const auto multiply = [&](const Frag &xf, const Tiles<S, 1, PER> &h, int j, int piece) {
+        Frag bf;
+        decode<T>(h.words[0], lane_at, bf);
+        const bool own = q == piece * MP / 4;
+        floatx4 sum = {};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          sum = Mfma4<T>::mma(xf[i], bf[i], sum);
+          if ((i + 1) % (4 / PER) == 0) {
+            const float by = (float)h.scale[0].v[i * PER / 4];
+#pragma unroll
+            for (int m = 0; m < MP; m++) acc[m] = own ? fmaf(by, sum[(MP * j + m) & 3], acc[m]) : acc[m];
+            sum = floatx4{0.f, 0.f, 0.f, 0.f};
+          }
+        }
+      };
+      Tiles<S, 1, PER> held[R];
+      Frag xf[SETS];
+      if (mine && count > 0) {
+        load_x(xf[0], 0);
+#pragma unroll
+        for (int j = 0; j < R; j++)
+          if (j < count) reader.fetch(held[j], first + j);
+      }
+      if (!have_table) make_table<T>(lds, a.m, share.expert);
+      have_table = true;
+      if (mine) {
+        const auto four = [&](const Frag &now, int b) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if (b + j >= count) break;
+            multiply(now, held[j % R], j, (b + j) % G);
+            if (b + j + R < count) reader.fetch(held[j % R], first + b + j + R);
+          }
+        };
+        if (SETS == 1) {
+          for (int b = 0; b < count; b += 4) {
+            if (b > 0 && b % G == 0) load_x(xf[0], b);
+            four(xf[0], b);
+          }
+        } else {  // a set of x lasts for four tiles: the next is on its way meanwhile
+          for (int b = 0; b < count; b += 8) {
+            if (b + 4 < count) load_x(xf[SETS - 1], b + 4);
+            four(xf[0], b);
+            if (b + 4 >= count) break;
+            if (b + 8 < count) load_x(xf[0], b + 8);
+            four(xf[SETS - 1], b + 4);
+          }
+        }
+        if ((cols & 127) && part == 0) {  // the columns behind the last whole 128 (part 0 has the fewest before)
+          reader.fetch(held[0], full);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int k = full * 128 + 32 * i;
+            load_x8_end<T>(row + k, cols - k - 8 * q, xf[0][i]);
+          }
+          multiply(xf[0], held[0], 0, 0);
+        }
+      }
+      // the four lanes of a column and the wavefronts of a tile, in their order
+      const int tokens = hi - lo < MP ? (int)(hi - lo) : MP;
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MP; m++) red[(wave * MP + m) * 64 + lane] = acc[m];
+      __syncthreads();
+      for (int i = lane + 64 * part; mine && i < tokens * 16; i += 64 * a.splits) {
+        const int m = i >> 4, c = i & 15;
+        const int64_t n = 16 * (int64_t)tile + c;
+        if (n < a.m.out) {
+          const float *from = red + (team * a.splits * MP + m) * 64 + c;
+          float sum = 0.f;
+          for (int w = 0; w < a.splits; w++, from += MP * 64) sum += (from[0] + from[16]) + (from[32] + from[48]);
+          y[(lo + m) * a.ys + n] = (T)sum;
         }
       }
     }
   }
 }
 
-// A workgroup has 16 * NT columns of y and 16 * MT rows of it at a time; its wavefronts share the
-// columns of the matrix, 128 * U to each in turn, the next ones on their way while the last are
-// multiplied, and add their sums up in LDS. Rows of x behind the last one and rows of the matrix behind
-// y's last column are read from the nearest that is there: their results are not written. FINE: scales
-// change every 32 columns, not only every 128.
-template <typename T, typename S, int MT, int NT, int U, bool FINE>
-__global__ __launch_bounds__(512) void product4_kernel(const T *x, const S *scales, const T *books, T *y,
-                                                       Product4Args a) {
+// 16 * MT rows of y at a time, a row of x in each of a product's 16. Rows of x behind the last one are read from
+// the last: their results are not written.
+template <typename T, typename S, int MT, int NT, int R, int PER>
+__global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  typedef Stage<T, S, MT, NT, U, FINE> Stg;
-  constexpr int P = 2 * sizeof(T);  // bytes of a pair
+  typedef unsigned XFrag[MT][4][2 * sizeof(T)];
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   float *red = reinterpret_cast<float *>(lds + TABLE_BYTES);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
-
-  int e = 0;
-  int64_t lo = 0, hi = a.src.rows;
-  if (a.src.offsets) {
-    const int E = a.src.experts;
-    if (blockIdx.y == gridDim.y - 1) {  // zeros for the rows that have no expert
-      lo = a.src.offsets[E];
-      for (int64_t p = lo + blockIdx.z * waves + wave; p < hi; p += gridDim.z * waves)
-        for (int c = lane; c < 16 * NT; c += 64)
-          if (n0 + c < a.m.out) y[p * a.ys + n0 + c] = (T)0.f;
-      return;
-    }
-    if ((int)gridDim.y - 1 == E) {
-      e = blockIdx.y;
-      lo = a.src.offsets[e];
-      hi = a.src.offsets[e + 1];
-    } else {  // fewer rows than experts: the workgroups of an expert's first row have all of its rows
-      int *found = reinterpret_cast<int *>(red);
-      if (threadIdx.x == 0) found[0] = -1;
-      __syncthreads();
-      const int p = blockIdx.y;
-      for (int i = threadIdx.x; i < E; i += blockDim.x) {
-        const int from = a.src.offsets[i], to = a.src.offsets[i + 1];
-        if (from == p && to > p) {
-          found[0] = i;
-          found[1] = to;
-        }
-      }
-      __syncthreads();
-      e = __builtin_amdgcn_readfirstlane(found[0]);
-      lo = p;
-      hi = e >= 0 ? found[1] : lo;
-      __syncthreads();
-    }
-  }
-  lo += (int64_t)blockIdx.z * (16 * MT);
-  if (lo >= hi) return;
-
-  const unsigned lane_at = (lane & (Mfma4<T>::COPIES - 1)) * P;
+  const int teams = waves / a.splits, team = wave / a.splits, part = wave % a.splits;
+  const int tiles16 = (int)((a.m.out + 15) >> 4), subs = (a.m.cols + 127) >> 7;
+  const Share share = share_of(a, reinterpret_cast<int *>(red), y);
+  const int64_t begin = share.lo + (int64_t)blockIdx.z * (16 * MT), hi = share.hi;
+  if (begin >= hi) return;
+  const unsigned lane_at = (lane * 2 * sizeof(T)) & 255;
   const int cols = a.m.cols, full = cols >> 7;
-  const uint8_t *code[NT];
-  const S *scale[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int64_t n = n0 + 16 * t + r < a.m.out ? n0 + 16 * t + r : a.m.out - 1;
-    code[t] = a.m.codes + (e * a.m.out + n) * a.m.pitch;
-    scale[t] = scales + (e * a.m.out + n) * a.m.groups;
-  }
-  const T *row[MT];
-  const auto rows_from = [&](int64_t first) {
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-      const int64_t p = first + 16 * t + r < hi ? first + 16 * t + r : hi - 1;
-      row[t] = x + (a.src.order ? a.src.order[p] / a.src.top_k : p) * a.xs;
-    }
-  };
-  const auto load_scales = [&](Stg &st, int u, int sub) {
-#pragma unroll
-    for (int i = 0; i < (FINE ? 4 : 1); i++) {
-      const unsigned unit = FINE ? sub * 4 + i : sub;
-      unsigned g = a.per_scale_magic ? __umulhi(unit, a.per_scale_magic) : unit;
-      g = g < (unsigned)a.m.groups ? g : a.m.groups - 1;
-#pragma unroll
-      for (int t = 0; t < NT; t++) st.scale[u][t][i] = scale[t][g];
-    }
-  };
-  const auto fetch = [&](Stg &st, int s0) {
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int sub = s0 + u < full ? s0 + u : full - 1;
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-        st.words[u][t] = *reinterpret_cast<const uint4 *>(code[t] + ((int64_t)sub * 64 + q * 16));
-      load_scales(st, u, sub);
-#pragma unroll
-      for (int t = 0; t < MT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) load_x8<T>(row[t] + (sub * 128 + 32 * i + 8 * q), st.x[u][t][i]);
-    }
-  };
-  const auto table = [&]() {  // thread t writes copies of entry t / 2
-    const T *book = books + e * a.m.book_stride;
-    for (int i = threadIdx.x; i < 512; i += blockDim.x) {
-      const int byte = i >> 1;
-      T pair[16 / sizeof(T)];
-#pragma unroll
-      for (int c = 0; c < (int)(16 / sizeof(T)); c += 2) {
-        pair[c] = book[byte & 15];
-        pair[c + 1] = book[byte >> 4];
-      }
-      uint4 four;
-      __builtin_memcpy(&four, pair, 16);
-#pragma unroll
-      for (int c = 0; c < 4; c++) *reinterpret_cast<uint4 *>(lds + i * 64 + c * 16) = four;
-    }
-    __syncthreads();
-  };
+  const int first = full * part / a.splits, count = full * (part + 1) / a.splits - first;
+  Reader<S, NT, PER> reader(a.m, share.expert, tiles16, subs);
 
   bool have_table = false;
-  for (; lo < hi; lo += (int64_t)gridDim.z * (16 * MT)) {
-    rows_from(lo);
-    floatx4 acc[MT][NT] = {};
-    const int step = waves * U;
-    Stg st[2];
-    int s = wave * U;
-    if (s < full) fetch(st[0], s);
-    if (!have_table) table();
-    have_table = true;
-    while (s < full) {
-      if (s + step < full) fetch(st[1], s + step);
+  for (int tile0 = blockIdx.x * teams; tile0 * NT < tiles16; tile0 += gridDim.x * teams) {
+    const int tile = (tile0 + team) * NT;
+    const bool mine = tile < tiles16;
+    reader.move_to(tile, tiles16, subs);
+    for (int64_t lo = begin; lo < hi; lo += (int64_t)gridDim.z * (16 * MT)) {
+      const T *row[MT];
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (s + u < full) multiply(st[0], u, lds, lane_at, a.brain, acc);
-      s += step;
-      if (s >= full) break;
-      if (s + step < full) fetch(st[0], s + step);
+      for (int t = 0; t < MT; t++) row[t] = x_row(x, a, lo + 16 * t + r < hi ? lo + 16 * t + r : hi - 1) + 8 * q;
+      floatx4 acc[MT][NT] = {};
+      Tiles<S, NT, PER> held[R];
+      XFrag xf[R];
+      const auto fetch = [&](int j, int sub) {
+        reader.fetch(held[j], sub);
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (s + u < full) multiply(st[1], u, lds, lane_at, a.brain, acc);
-      s += step;
-    }
-    if ((cols & 127) && wave == full % waves) {  // the columns behind the last whole 128
-      Stage<T, S, MT, NT, 1, FINE> end;
-      const int64_t last = a.m.pitch - 16, at = (int64_t)full * 64 + q * 16;
+        for (int t = 0; t < MT; t++)
 #pragma unroll
-      for (int t = 0; t < NT; t++) end.words[0][t] = *reinterpret_cast<const uint4 *>(code[t] + (at < last ? at : last));
-#pragma unroll
-      for (int i = 0; i < (FINE ? 4 : 1); i++) {
-        const unsigned unit = FINE ? full * 4 + i : full;
-        unsigned g = a.per_scale_magic ? __umulhi(unit, a.per_scale_magic) : unit;
-        g = g < (unsigned)a.m.groups ? g : a.m.groups - 1;
-#pragma unroll
-        for (int t = 0; t < NT; t++) end.scale[0][t][i] = scale[t][g];
-      }
-#pragma unroll
-      for (int t = 0; t < MT; t++)
+          for (int i = 0; i < 4; i++) load_x8<T>(row[t] + ((int64_t)sub * 128 + 32 * i), xf[j][t][i]);
+      };
+      const auto multiply = [&](int st, int t) {
+        unsigned b[4][2 * sizeof(T)];
+        decode<T>(held[st].words[t], lane_at, b);
+        floatx4 sum[MT] = {};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int k = full * 128 + 32 * i + 8 * q;
-          load_x8_end<T>(row[t] + k, cols - k, end.x[0][t][i]);
+#pragma unroll
+          for (int m = 0; m < MT; m++) {
+            sum[m] = Mfma4<T>::mma(xf[st][m][i], b[i], sum[m]);
+            if ((i + 1) % (4 / PER) == 0) {
+              const float sc = (float)held[st].scale[t].v[i * PER / 4];
+#pragma unroll
+              for (int v = 0; v < 4; v++) acc[m][t][v] = fmaf(sc, sum[m][v], acc[m][t][v]);
+              sum[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+            }
+          }
         }
-      multiply(end, 0, lds, lane_at, a.brain, acc);
-    }
-    // the wavefronts' sums, in their order
+      };
+      if (mine) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-      __syncthreads();
+        for (int j = 0; j < R; j++)
+          if (j < count) fetch(j, first + j);
+      }
+      if (!have_table) make_table<T>(lds, a.m, share.expert);
+      have_table = true;
+      if (mine) {
+        for (int b = 0; b < count; b += R) {
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+          for (int j = 0; j < R; j++) {
+            if (b + j >= count) break;
 #pragma unroll
-        for (int v = 0; v < 4; v++) red[(wave * (4 * NT) + 4 * t + v) * 64 + lane] = acc[m][t][v];
-      __syncthreads();
-      for (int i = threadIdx.x; i < 4 * NT * 64; i += blockDim.x) {
-        // i = (token, column): 16 neighbours write 16 columns of one row
-        const int token = i / (16 * NT), c = i % (16 * NT);
-        const int64_t p = lo + 16 * m + token, n = n0 + c;
-        if (p < hi && n < a.m.out) {
-          const int at = (4 * (c >> 4) + (token & 3)) * 64 + (token >> 2) * 16 + (c & 15);
-          float sum = 0.f;
-          for (int w = 0; w < waves; w++) sum += red[w * (4 * NT * 64) + at];
-          y[p * a.ys + n] = (T)sum;
+            for (int t = 0; t < NT; t++) multiply(j, t);
+            if (b + R + j < count) fetch(j, first + b + R + j);
+          }
+        }
+        if ((cols & 127) && part == 0) {  // the columns behind the last whole 128 (part 0 has the fewest before)
+          reader.fetch(held[0], full);
+#pragma unroll
+          for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int k = full * 128 + 32 * i;
+              load_x8_end<T>(row[t] + k, cols - k - 8 * q, xf[0][t][i]);
+            }
+#pragma unroll
+          for (int t = 0; t < NT; t++) multiply(0, t);
+        }
+      }
+      // the sums of a tile's wavefronts, in their order
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const int tokens = hi - lo - 16 * m < 16 ? (int)(hi - lo - 16 * m) : 16;
+        if (tokens <= 0) break;
+        if (a.splits == 1) {
+          if (mine) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int v = 0; v < 4; v++) {
+                const int64_t n = 16 * (int64_t)(tile + t) + r;
+                if (4 * q + v < tokens && n < a.m.out) y[(lo + 16 * m + 4 * q + v) * a.ys + n] = (T)acc[m][t][v];
+              }
+          }
+          continue;
+        }
+        __syncthreads();
+        if (4 * q < tokens) {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) red[(wave * (4 * NT) + 4 * t + v) * 64 + lane] = acc[m][t][v];
+        }
+        __syncthreads();
+        // (token, column): 16 neighbours write 16 columns of one row
+        for (int i = lane + 64 * part; mine && i < tokens * 16 * NT; i += 64 * a.splits) {
+          const int token = i / (16 * NT), c = i % (16 * NT);
+          const int64_t n = 16 * (int64_t)tile + c;
+          if (n < a.m.out) {
+            const float *from = red + team * a.splits * (4 * NT * 64) + (4 * (c >> 4) + (token & 3)) * 64 +
+                                (token >> 2) * 16 + (c & 15);
+            float sum = 0.f;
+            for (int w = 0; w < a.splits; w++) sum += from[w * (4 * NT * 64)];
+            y[(lo + 16 * m + token) * a.ys + n] = (T)sum;
+          }
         }
       }
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the order the product reads a matrix in
+// ---------------------------------------------------------------------------
+
+// Tile (row / 16, column / 128), lane (r, q): 16 bytes whose word i holds row r's columns 32 i + 8 q .. + 7
+// of the tile. Scales: a tile's 16 rows, one each, or four each (one per 32 columns) where a group ends
+// within 128. Rows and columns behind the matrix have code 0 and scale 0.
+__global__ __launch_bounds__(256) void layout4_codes_kernel(const uint8_t *codes, int64_t pitch, int64_t out, int cols,
+                                                            int64_t tiles16, int subs, int64_t lanes, uint4 *to) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < lanes; i += (int64_t)gridDim.x * 256) {
+    const int lane = i & 63, r = lane & 15, q = lane >> 4;
+    const int sub = (i >> 6) % subs;
+    const int64_t tile = (i >> 6) / subs, e = tile / tiles16, n = (tile % tiles16) * 16 + r;
+    const uint8_t *row = codes + (e * out + n) * pitch;
+    unsigned w[4] = {0, 0, 0, 0};
+    if (n < out)
+      for (int j = 0; j < 4; j++)
+        for (int b = 0; b < 4; b++) {
+          const int k = sub * 128 + 32 * j + 8 * q + 2 * b;
+          unsigned v = k < cols ? row[k / 2] : 0;
+          if (k + 1 >= cols) v &= 15;
+          w[j] |= v << (8 * b);
+        }
+    to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename S>
+__global__ __launch_bounds__(256) void layout4_scales_kernel(const S *scales, int64_t out, int groups, int group,
+                                                             int64_t tiles16, int subs, int per, int64_t count,
+                                                             S *to) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const int p = i % per, r = (i / per) & 15;
+    const int64_t t = i / per / 16, tile = t / subs, e = tile / tiles16, n = (tile % tiles16) * 16 + r;
+    const int g = ((t % subs) * 128 + p * (128 / per)) / group;
+    to[i] = n < out && g < groups ? scales[(e * out + n) * groups + g] : (S)0;
   }
 }
 
 static const size_t MOST_OUT = 1 << 24, MOST_COLS4 = 1000000, MOST_ROWS4 = 2147483646;
 
-static bool matrix_ok(int dtype, size_t out, size_t cols, int group, const void *codes, size_t pitch, int scale_dtype,
-                      const void *scales, const void *book) {
-  return known_type(dtype) && known_type(scale_dtype) && out >= 1 && out <= MOST_OUT && cols >= 1 &&
-         cols <= MOST_COLS4 && group >= 32 && group % 32 == 0 && codes && aligned_to(codes, 16) && pitch % 16 == 0 &&
-         pitch >= (cols + 1) / 2 && pitch <= ((size_t)1 << 32) && scales &&
-         aligned_to(scales, type_size(scale_dtype)) && book && aligned_to(book, type_size(dtype));
+static bool sizes_ok(size_t experts, size_t out, size_t cols, int group) {
+  return experts >= 1 && experts <= H2O4GPU_EXPERTS_MAX_EXPERTS && out >= 1 && out <= MOST_OUT && cols >= 1 &&
+         cols <= MOST_COLS4 && group >= 32 && group % 32 == 0;
 }
 
 static bool strided_ok(int dtype, const void *p, size_t stride, size_t cols) {
   return p && aligned_to(p, type_size(dtype)) && stride >= cols && stride <= ((size_t)1 << 40);
 }
 
-template <typename T, typename S, int MT, int NT, int U, bool FINE>
-static int launch_product4(const T *x, const S *scales, const T *book, T *y, const Product4Args &a, int waves,
-                           hipStream_t s) {
-  const size_t lds = TABLE_BYTES + (size_t)waves * 4 * NT * 64 * sizeof(float);
-  const void *kernel = reinterpret_cast<const void *>(product4_kernel<T, S, MT, NT, U, FINE>);
-  KM_TRY(ensure_dynamic_lds(kernel, lds));
-  const unsigned gx = (unsigned)((a.m.out + 16 * NT - 1) / (16 * NT));
-  unsigned gy = 1, gz = 1;
-  const int64_t tiles = (a.src.rows + 16 * MT - 1) / (16 * MT);
-  if (a.src.offsets)
+// Rows of codes and scales as quantize writes them.
+static bool packed_ok(const void *codes, size_t pitch, size_t cols, int scale_dtype, const void *scales) {
+  return codes && pitch >= (cols + 1) / 2 && pitch <= ((size_t)1 << 32) && known_type(scale_dtype) && scales &&
+         aligned_to(scales, type_size(scale_dtype));
+}
+
+static size_t tiles_of(size_t out) { return (out + 15) / 16; }
+static size_t subs_of(size_t cols) { return (cols + 127) / 128; }
+static int scales_per_sub(int group) { return group % 128 == 0 ? 1 : group % 64 == 0 ? 2 : 4; }
+static unsigned blocks_for(size_t items) { return (unsigned)((items + 255) / 256 < 65536 ? (items + 255) / 256 : 65536); }
+
+// rows: of y that a workgroup has at a time, tile: columns of y a team of wavefronts has.
+template <typename T>
+static int launch_product4(void (*kernel)(const T *, T *, Product4Args), int rows, int tile, const T *x, T *y,
+                           Product4Args a, int waves, int splits, hipStream_t s) {
+  const size_t lds = TABLE_BYTES + (size_t)waves * 64 * (tile / 16) * (rows < 4 ? rows : 4) * sizeof(float);
+  KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
+  a.splits = splits;
+  const int teams = waves / splits;
+  const unsigned tiles = (unsigned)((a.m.out + tile - 1) / tile);
+  unsigned gx = (tiles + teams - 1) / teams, gy = 1, gz = 1;
+  if (a.src.offsets) {
     gy = (unsigned)(a.src.rows < a.src.experts ? a.src.rows : a.src.experts) + 1;
-  else  // a workgroup that has several tiles of tokens makes its table once
-    gz = (unsigned)(tiles < 256 ? tiles : 256);
-  hipLaunchKernelGGL((product4_kernel<T, S, MT, NT, U, FINE>), dim3(gx, gy, gz), dim3(64 * waves), lds, s, x, scales,
-                     book, y, a);
+  } else {
+    const int64_t steps = (a.src.rows + rows - 1) / rows;
+    gz = (unsigned)(steps < 256 ? steps : 256);
+  }
+  // no more workgroups than run at once, twice over: one that has several tiles makes its table once
+  const unsigned most = 1024 / (gy * gz) > 0 ? 1024 / (gy * gz) : 1;
+  if (gx > most) gx = most;
+  hipLaunchKernelGGL(kernel, dim3(gx, gy, gz), dim3(64 * waves), lds, s, x, y, a);
   return launched();
 }
 
-static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m, int scale_dtype, const void *scales,
-                    const void *book, const RowSource &src, void *y, size_t y_stride, hipStream_t s) {
+static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m, int scale_dtype,
+                    const RowSource &src, void *y, size_t y_stride, hipStream_t s) {
   Product4Args a;
   a.m = m;
-  a.brain = scale_dtype == H2O4GPU_EXPERTS_BFLOAT16;
   a.src = src;
   a.xs = (int64_t)x_stride;
   a.ys = (int64_t)y_stride;
-  const bool fine = m.group % 128 != 0;
-  const unsigned unit = fine ? 32 : 128;
-  a.per_scale = (unsigned)m.group / unit;
-  const unsigned most = (unsigned)m.cols / unit + 1;
-  if (a.per_scale > most) a.per_scale = most;
-  a.per_scale_magic = a.per_scale == 1 ? 0u : (unsigned)((0x100000000ull + a.per_scale - 1) / a.per_scale);
-  const int subs = (m.cols + 127) / 128;
-  int waves = 8;
-  while (waves > 1 && waves / 2 >= subs) waves /= 2;
+  const int subs = (int)subs_of(m.cols);
+  const int64_t tiles = (int64_t)tiles_of(m.out);
+  // rows that a matrix has, about, and matrices (or workgroups along the rows of one)
+  const int64_t shares = !src.offsets ? 1 : src.rows < src.experts ? src.rows : src.experts;
+  const int64_t rows = (src.rows + shares - 1) / shares;
+  // Rows of y at a time, in 16s. x is read once for every 16 * NT columns of y, from an L2 that gives some
+  // 13 TB/s, so with many rows wide tiles pay: 64 x 8192 x 8192 takes 26 us with 2 x 4 tiles, 42 with 2 x 2, 37 with
+  // 4 x 2; 33 rows 25 with 3 x 2, 26 with 2 x 4, 32 with 2 x 2.
+  const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 ? 3 : 2;
+  const int64_t steps = src.offsets ? 1 : (src.rows + 16 * mt - 1) / (16 * mt);
+  // Columns of y at a time: as wide as leaves a workgroup for every CU (16 rows x 8192 x 8192: 15 us with 32, 20
+  // with 16, 18 with 64; 64 experts of 2048 x 4096: 53 us with 64, 80 with 32, 101 with 16).
+  const int64_t all = tiles * shares * steps;
+  const bool few = rows <= (src.offsets ? 2 : 4);
+  const int nt = few ? 1 : all >= 1024 && mt < 3 && (mt == 1 || m.per < 4) ? 4 : all >= 512 ? 2 : 1;
+  // Wavefronts that share a tile: as few as give every CU two workgroups of eight.
+  const int waves = 8;
+  int splits = 8;
+  while (splits > 1 && (splits / 2 >= subs || (all + nt - 1) / nt * (splits / 2) >= 4096)) splits /= 2;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    const auto with_scales = [&](auto *ts) {
-      typedef typename std::remove_const<typename std::remove_pointer<decltype(ts)>::type>::type S;
-      const T *tx = static_cast<const T *>(x), *tb = static_cast<const T *>(book);
-      T *ty = static_cast<T *>(y);
-      return fine ? launch_product4<T, S, 1, 1, 2, true>(tx, ts, tb, ty, a, waves, s)
-                  : launch_product4<T, S, 1, 1, 2, false>(tx, ts, tb, ty, a, waves, s);
-    };
-    return scale_dtype == H2O4GPU_EXPERTS_FLOAT32 ? with_scales(static_cast<const float *>(scales))
-                                                  : with_scales(static_cast<const uint16_t *>(scales));
+    const T *tx = static_cast<const T *>(x);
+    T *ty = static_cast<T *>(y);
+    return with_type(scale_dtype, [&](auto stag) {
+      typedef typename decltype(stag)::type S;
+#define FEW(MP)                                                                                              \
+  launch_product4(m.per == 1   ? product4_few_kernel<T, S, MP, 1>                                            \
+                  : m.per == 2 ? product4_few_kernel<T, S, MP, 2>                                            \
+                               : product4_few_kernel<T, S, MP, 4>,                                           \
+                  MP, 16, tx, ty, a, waves, splits, s)
+#define MANY(MT, NT, R)                                                                                      \
+  launch_product4(m.per == 1   ? product4_kernel<T, S, MT, NT, R, 1>                                         \
+                  : m.per == 2 ? product4_kernel<T, S, MT, NT, R, 2>                                         \
+                               : product4_kernel<T, S, MT, NT, R, 4>,                                        \
+                  16 * MT, 16 * NT, tx, ty, a, waves, splits, s)
+      // PROBE HERE
+      if (src.rows == 1) return FEW(1);
+      if (few) return FEW(4);
+      // (a float takes twice the registers: no more than 2 x 2)
+      if constexpr (sizeof(T) == 2) {
+        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : nt == 2 ? MANY(1, 2, 2) : MANY(1, 4, 2);
+        if (mt == 3) return nt == 1 ? MANY(3, 1, 1) : MANY(3, 2, 1);
+        if (nt == 4)  // (four scales for 128 columns take too many registers here)
+          return launch_product4(m.per == 1 ? product4_kernel<T, S, 2, 4, 1, 1> : product4_kernel<T, S, 2, 4, 1, 2>, 32,
+                                 64, tx, ty, a, waves, splits, s);
+        return nt == 1 ? MANY(2, 1, 2) : MANY(2, 2, 1);
+      } else {
+        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : MANY(1, 2, 2);
+        return nt == 1 ? MANY(2, 1, 1) : MANY(2, 2, 1);
+      }
+#undef FEW
+#undef MANY
+    });
   });
 }
 
@@ -466,59 +702,99 @@ using namespace kmhip;
 KM_API int h2o4gpu_codebook4_quantize(int dtype, size_t out, size_t cols, int group, float top, const void *d_w,
                                       size_t w_stride, const void *d_codebook, void *d_codes, size_t codes_pitch,
                                       int scale_dtype, void *d_scales, void *stream) {
-  if (!matrix_ok(dtype, out, cols, group, d_codes, codes_pitch, scale_dtype, d_scales, d_codebook) ||
-      !strided_ok(dtype, d_w, w_stride, cols) || !(top > 0.f) || !isfinite(top))
+  if (!known_type(dtype) || out < 1 || out > MOST_ROWS4 || !sizes_ok(1, 1, cols, group) ||
+      !packed_ok(d_codes, codes_pitch, cols, scale_dtype, d_scales) || !d_codebook ||
+      !aligned_to(d_codebook, type_size(dtype)) || !strided_ok(dtype, d_w, w_stride, cols) || !(top > 0.f) ||
+      !isfinite(top))
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
     return with_type(scale_dtype, [&](auto stag) {
       typedef typename decltype(stag)::type S;
-      hipLaunchKernelGGL((quantize4_kernel<T, S>), dim3((unsigned)((out + 3) / 4)), dim3(256), 0,
-                         static_cast<hipStream_t>(stream), static_cast<const T *>(d_w), (int64_t)w_stride,
-                         (int64_t)out, (int)cols, group, top, static_cast<const T *>(d_codebook),
+      hipLaunchKernelGGL((quantize4_kernel<T, S>), dim3((unsigned)((out + 3) / 4 < 65536 ? (out + 3) / 4 : 65536)),
+                         dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(d_w),
+                         (int64_t)w_stride, (int64_t)out, (int)cols, group, top, static_cast<const T *>(d_codebook),
                          static_cast<uint8_t *>(d_codes), (int64_t)codes_pitch, static_cast<S *>(d_scales));
       return launched();
     });
   });
 }
 
-static Matrix4 matrix4(size_t out, size_t cols, int group, const void *codes, size_t pitch, size_t book_stride) {
-  Matrix4 m;
-  m.codes = static_cast<const uint8_t *>(codes);
-  m.pitch = (int64_t)pitch;
-  m.out = (int64_t)out;
-  m.cols = (int)cols;
-  m.group = group;
-  m.groups = (int)((cols + group - 1) / group);
-  m.book_stride = (int64_t)book_stride;
-  return m;
+KM_API size_t h2o4gpu_codebook4_codes_bytes(size_t experts, size_t out, size_t cols) {
+  return sizes_ok(experts, out, cols, 32) ? experts * tiles_of(out) * subs_of(cols) * 1024 : 0;
+}
+
+KM_API size_t h2o4gpu_codebook4_scales_bytes(size_t experts, size_t out, size_t cols, int group, int scale_dtype) {
+  if (!sizes_ok(experts, out, cols, group) || !known_type(scale_dtype)) return 0;
+  return experts * tiles_of(out) * subs_of(cols) * 16 * scales_per_sub(group) * type_size(scale_dtype);
+}
+
+KM_API int h2o4gpu_codebook4_layout(size_t experts, size_t out, size_t cols, int group, const void *d_codes,
+                                    size_t codes_pitch, int scale_dtype, const void *d_scales, void *d_laid_codes,
+                                    void *d_laid_scales, void *stream) {
+  if (!sizes_ok(experts, out, cols, group) || !packed_ok(d_codes, codes_pitch, cols, scale_dtype, d_scales) ||
+      !d_laid_codes || !aligned_to(d_laid_codes, 16) || !d_laid_scales || !aligned_to(d_laid_scales, 16))
+    return H2O4GPU_KMEANS_EARG;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t tiles16 = (int64_t)tiles_of(out), lanes = (int64_t)experts * tiles16 * subs_of(cols) * 64;
+  hipLaunchKernelGGL(layout4_codes_kernel, dim3(blocks_for(lanes)), dim3(256), 0, s,
+                     static_cast<const uint8_t *>(d_codes), (int64_t)codes_pitch, (int64_t)out, (int)cols, tiles16,
+                     (int)subs_of(cols), lanes, static_cast<uint4 *>(d_laid_codes));
+  KM_TRY(launched());
+  const int per = scales_per_sub(group), groups = (int)((cols + group - 1) / group);
+  const int64_t count = (int64_t)experts * tiles16 * subs_of(cols) * 16 * per;
+  const auto with_scales = [&](auto zero) {
+    typedef decltype(zero) S;
+    hipLaunchKernelGGL(layout4_scales_kernel<S>, dim3(blocks_for(count)), dim3(256), 0, s,
+                       static_cast<const S *>(d_scales), (int64_t)out, groups, group, tiles16, (int)subs_of(cols),
+                       per, count, static_cast<S *>(d_laid_scales));
+    return launched();
+  };
+  return scale_dtype == H2O4GPU_EXPERTS_FLOAT32 ? with_scales(0.f) : with_scales((uint16_t)0);
+}
+
+// The checks that both products share, and the matrix.
+static bool laid_out(int dtype, size_t experts, size_t out, size_t cols, int group, const void *codes,
+                     int scale_dtype, const void *scales, const void *book, size_t book_stride, Matrix4 *m) {
+  if (!known_type(dtype) || !known_type(scale_dtype) || !sizes_ok(experts, out, cols, group) || !codes ||
+      !aligned_to(codes, 16) || !scales || !aligned_to(scales, 16) || !book || !aligned_to(book, type_size(dtype)) ||
+      (book_stride != 0 && book_stride < 16) || book_stride > ((size_t)1 << 32))
+    return false;
+  m->codes = static_cast<const uint4 *>(codes);
+  m->scales = scales;
+  m->books = book;
+  m->book_stride = (int64_t)book_stride;
+  m->out = (int64_t)out;
+  m->cols = (int)cols;
+  m->per = scales_per_sub(group);
+  return true;
 }
 
 KM_API int h2o4gpu_codebook4_product(int dtype, size_t rows, size_t out, size_t cols, int group, const void *d_x,
-                                     size_t x_stride, const void *d_codes, size_t codes_pitch, int scale_dtype,
-                                     const void *d_scales, const void *d_codebook, void *d_y, size_t y_stride,
+                                     size_t x_stride, const void *d_laid_codes, int scale_dtype,
+                                     const void *d_laid_scales, const void *d_codebook, void *d_y, size_t y_stride,
                                      void *stream) {
-  if (!matrix_ok(dtype, out, cols, group, d_codes, codes_pitch, scale_dtype, d_scales, d_codebook) ||
+  Matrix4 m;
+  if (!laid_out(dtype, 1, out, cols, group, d_laid_codes, scale_dtype, d_laid_scales, d_codebook, 0, &m) ||
       rows > MOST_ROWS4)
     return H2O4GPU_KMEANS_EARG;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
   if (!strided_ok(dtype, d_x, x_stride, cols) || !strided_ok(dtype, d_y, y_stride, out)) return H2O4GPU_KMEANS_EARG;
   RowSource src;
   src.rows = (int64_t)rows;
-  return product4(dtype, d_x, x_stride, matrix4(out, cols, group, d_codes, codes_pitch, 0), scale_dtype, d_scales,
-                  d_codebook, src, d_y, y_stride, static_cast<hipStream_t>(stream));
+  return product4(dtype, d_x, x_stride, m, scale_dtype, src, d_y, y_stride, static_cast<hipStream_t>(stream));
 }
 
 KM_API int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int experts, size_t out,
                                              size_t cols, int group, const void *d_x, size_t x_stride,
-                                             const void *d_codes, size_t codes_pitch, int scale_dtype,
-                                             const void *d_scales, const void *d_codebook, size_t codebook_stride,
-                                             const int *d_order, const int *d_offsets, void *d_y, size_t y_stride,
-                                             void *stream) {
-  if (!matrix_ok(dtype, out, cols, group, d_codes, codes_pitch, scale_dtype, d_scales, d_codebook) || experts < 1 ||
-      experts > H2O4GPU_EXPERTS_MAX_EXPERTS || top_k < 1 || top_k > H2O4GPU_EXPERTS_MAX_TOP_K ||
-      tokens > MOST_ROWS4 / (size_t)top_k || (codebook_stride != 0 && codebook_stride < 16) ||
-      codebook_stride > ((size_t)1 << 32))
+                                             const void *d_laid_codes, int scale_dtype, const void *d_laid_scales,
+                                             const void *d_codebook, size_t codebook_stride, const int *d_order,
+                                             const int *d_offsets, void *d_y, size_t y_stride, void *stream) {
+  Matrix4 m;
+  if (experts < 1 ||
+      !laid_out(dtype, (size_t)experts, out, cols, group, d_laid_codes, scale_dtype, d_laid_scales, d_codebook,
+                codebook_stride, &m) ||
+      top_k < 1 || top_k > H2O4GPU_EXPERTS_MAX_TOP_K || tokens > MOST_ROWS4 / (size_t)top_k)
     return H2O4GPU_KMEANS_EARG;
   if (tokens == 0) return H2O4GPU_KMEANS_OK;
   if (!strided_ok(dtype, d_x, x_stride, cols) || !strided_ok(dtype, d_y, y_stride, out) || !d_order || !d_offsets ||
@@ -530,6 +806,5 @@ KM_API int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k
   src.top_k = top_k;
   src.experts = experts;
   src.rows = (int64_t)tokens * top_k;
-  return product4(dtype, d_x, x_stride, matrix4(out, cols, group, d_codes, codes_pitch, codebook_stride), scale_dtype,
-                  d_scales, d_codebook, src, d_y, y_stride, static_cast<hipStream_t>(stream));
+  return product4(dtype, d_x, x_stride, m, scale_dtype, src, d_y, y_stride, static_cast<hipStream_t>(stream));
 }

@@ -38,11 +38,15 @@ PROTOTYPES = {
                                                  c_void_p]),
     "h2o4gpu_codebook4_quantize": (c_int, [c_int, c_size_t, c_size_t, c_int, c_float, c_void_p, c_size_t, c_void_p,
                                            c_void_p, c_size_t, c_int, c_void_p, c_void_p]),
+    "h2o4gpu_codebook4_codes_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
+    "h2o4gpu_codebook4_scales_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t, c_int, c_int]),
+    "h2o4gpu_codebook4_layout": (c_int, [c_size_t, c_size_t, c_size_t, c_int, c_void_p, c_size_t, c_int, c_void_p,
+                                         c_void_p, c_void_p, c_void_p]),
     "h2o4gpu_codebook4_product": (c_int, [c_int, c_size_t, c_size_t, c_size_t, c_int, c_void_p, c_size_t, c_void_p,
-                                          c_size_t, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                          c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "h2o4gpu_codebook4_experts_product": (c_int, [c_int, c_size_t, c_int, c_int, c_size_t, c_size_t, c_int,
-                                                  c_void_p, c_size_t, c_void_p, c_size_t, c_int, c_void_p, c_void_p,
-                                                  c_size_t, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                                  c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_size_t,
+                                                  c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

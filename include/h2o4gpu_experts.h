@@ -89,9 +89,9 @@ int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k, size_t
                                      size_t drows_stride, float *d_dweights, void *stream);
 
 /* A 4-bit matrix [out][cols]: codes are 4 bits each, the even column in a byte's low half, rows
- * codes_pitch bytes apart (a multiple of 16, d_codes 16-byte aligned; what lies behind column cols is
- * not used); scales [out][ceil(cols / group)], group a multiple of 32, `scale_dtype`; codebook: 16
- * finite values of `dtype`. Element (n, k) is codebook[code(n, k)] * scales[n][k / group].
+ * codes_pitch bytes apart (at least cols / 2, rounded up); scales [out][ceil(cols / group)] of
+ * `scale_dtype`, group a multiple of 32; codebook: 16 finite values of `dtype`. Element (n, k) is
+ * codebook[code(n, k)] * scales[n][k / group].
  *
  * quantize: codes and scales of a matrix d_w of `dtype`. A group's scale is its largest magnitude
  * over `top` (> 0: the codebook's value that this magnitude stands for), rounded to scale_dtype (1
@@ -100,21 +100,32 @@ int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k, size_t
 int h2o4gpu_codebook4_quantize(int dtype, size_t out, size_t cols, int group, float top, const void *d_w,
                                size_t w_stride, const void *d_codebook, void *d_codes, size_t codes_pitch,
                                int scale_dtype, void *d_scales, void *stream);
+/* The order in which the products read a matrix, or `experts` matrices one behind another (codes
+ * [experts][out][codes_pitch], scales [experts][out][groups]): made once from codes and scales, which are not
+ * needed any more. d_laid_codes: codes_bytes() bytes, d_laid_scales: scales_bytes() bytes, both 16-byte
+ * aligned. A tile of 16 rows and 128 columns is 1024 bytes of codes: 64 times 16 bytes, number 16 q + r
+ * of which holds in its word i the columns 32 i + 8 q .. + 7 of row r; tiles of a row of tiles follow
+ * each other. Its scales are 16, one a row, or, where group is no multiple of 128, 16 x 2 (a multiple of
+ * 64) or 16 x 4. Behind the matrix's last row and column lie zeros. The byte counts are 0 for bad arguments. */
+size_t h2o4gpu_codebook4_codes_bytes(size_t experts, size_t out, size_t cols);
+size_t h2o4gpu_codebook4_scales_bytes(size_t experts, size_t out, size_t cols, int group, int scale_dtype);
+int h2o4gpu_codebook4_layout(size_t experts, size_t out, size_t cols, int group, const void *d_codes,
+                             size_t codes_pitch, int scale_dtype, const void *d_scales, void *d_laid_codes,
+                             void *d_laid_scales, void *stream);
 /* d_y [rows][out] = d_x [rows][cols] times the matrix's transpose; products and sums in float, one
  * rounding at the end. */
 int h2o4gpu_codebook4_product(int dtype, size_t rows, size_t out, size_t cols, int group, const void *d_x,
-                              size_t x_stride, const void *d_codes, size_t codes_pitch, int scale_dtype,
-                              const void *d_scales, const void *d_codebook, void *d_y, size_t y_stride,
-                              void *stream);
+                              size_t x_stride, const void *d_laid_codes, int scale_dtype, const void *d_laid_scales,
+                              const void *d_codebook, void *d_y, size_t y_stride, void *stream);
 /* The same with a matrix per expert, rows in expert order (experts_sort on [tokens][top_k] choices):
  * d_y[p] = d_x[d_order[p] / top_k] times the transpose of the matrix whose rows p is among; zeros
- * for the rows behind d_offsets[experts]. codes [experts][out][codes_pitch], scales
- * [experts][out][groups]; codebook of expert e at d_codebook + e * codebook_stride (0: one for all). */
+ * for the rows behind d_offsets[experts]. Codebook of expert e at d_codebook + e * codebook_stride (0:
+ * one for all). */
 int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int experts, size_t out, size_t cols,
-                                      int group, const void *d_x, size_t x_stride, const void *d_codes,
-                                      size_t codes_pitch, int scale_dtype, const void *d_scales,
-                                      const void *d_codebook, size_t codebook_stride, const int *d_order,
-                                      const int *d_offsets, void *d_y, size_t y_stride, void *stream);
+                                      int group, const void *d_x, size_t x_stride, const void *d_laid_codes,
+                                      int scale_dtype, const void *d_laid_scales, const void *d_codebook,
+                                      size_t codebook_stride, const int *d_order, const int *d_offsets, void *d_y,
+                                      size_t y_stride, void *stream);
 
 #ifdef __cplusplus
 }

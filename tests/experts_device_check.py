@@ -318,7 +318,7 @@ def check_quantize(c):
     top = 1.0 if c["data"] != "huge" else 2.0
     q = codebook4.quantize(W.cuda(), group, book.cuda(), top=top, scale_dtype=sdt)
     groups = -(-K // group)
-    codes, scales = q.codes.cpu(), q.scales.cpu()
+    codes, scales = q.codes().cpu(), q.scales().cpu()
     assert q.dtype == dt and scales.dtype == sdt
     for g in range(groups):
         part = W[:, g * group:(g + 1) * group]
@@ -331,11 +331,7 @@ def check_quantize(c):
         off = torch.where(torch.isnan(off), math.inf, off)
         code = torch.argmin(off, 2)
         k = torch.arange(g * group, min(K, (g + 1) * group))
-        got = (codes[:, k // 2].long() >> (4 * (k % 2))) & 15
-        same(got, code, "codes")
-    if K % 2:
-        same(codes[:, K // 2] >> 4, torch.zeros(N, dtype=torch.uint8), "half byte behind the row")
-    assert int(codes[:, (K + 1) // 2:].sum()) == 0, "bytes behind the row"
+        same(codes[:, k].long(), code, "codes")
 
 
 # ---- single checks ------------------------------------------------------------------------------------
@@ -489,16 +485,21 @@ def check_c_refusals(_):
     earg("h2o4gpu_experts_dispatch", 0, 1, 2, 0, p, 8, p, p, 8, None)
     earg("h2o4gpu_experts_combine", 0, 1, 2, 8, p, 8, None, p, p, 8, None)
     earg("h2o4gpu_experts_combine_backward", 0, 1, 2, 8, p, 8, p, 8, p, p, p, 8, None, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 32, p, 64, p + 4, 32, 0, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 32, p, 64, p, 24, 0, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 32, p, 64, p, 16, 0, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 40, p, 64, p, 32, 0, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 32, p, 64, p, 32, 7, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_product", 0, 1, 4, 64, 32, p, 64, p, 32, 0, p, p, p, 3, None)
-    earg("h2o4gpu_codebook4_experts_product", 0, 1, 2, 0, 4, 64, 32, p, 64, p, 32, 0, p, p, 0, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_experts_product", 0, 1, 2, 3, 4, 64, 32, p, 64, p, 32, 0, p, p, 8, p, p, p, 4, None)
-    earg("h2o4gpu_codebook4_experts_product", 0, 1, 2, 3, 4, 64, 32, p, 64, p, 32, 0, p, p, 0, None, p, p, 4, None)
+    product = [0, 1, 4, 64, 32, p, 64, p, 0, p, p, p, 4, None]
+    for at, value in ((0, 3), (1, 2 ** 31), (2, 0), (3, 0), (3, 2 ** 21), (4, 40), (4, 0), (5, None), (5, p + 2), (6, 63),
+                      (7, None), (7, p + 4), (8, 7), (9, None), (9, p + 8), (10, None), (11, None), (12, 3)):
+        earg("h2o4gpu_codebook4_product", *(product[:at] + [value] + product[at + 1:]))
+    many = [0, 1, 2, 3, 4, 64, 32, p, 64, p, 0, p, p, 0, p, p, p, 4, None]
+    for at, value in ((0, -1), (1, 2 ** 31), (2, 0), (2, 65), (3, 0), (3, 16385), (4, 0), (5, 0), (6, 33), (7, None),
+                      (8, 2), (9, p + 1), (10, 3), (11, None), (12, p + 1), (13, 8), (14, None), (15, p + 2), (16, None),
+                      (17, 1)):
+        earg("h2o4gpu_codebook4_experts_product", *(many[:at] + [value] + many[at + 1:]))
     earg("h2o4gpu_codebook4_quantize", 0, 4, 64, 32, 0.0, p, 64, p, p, 32, 0, p, None)
+    earg("h2o4gpu_codebook4_quantize", 0, 4, 64, 32, 1.0, p, 64, p, p, 31, 0, p, None)
+    earg("h2o4gpu_codebook4_layout", 1, 4, 64, 32, p, 31, 0, p, p, p, None)
+    earg("h2o4gpu_codebook4_layout", 1, 4, 64, 32, p, 32, 0, p, p + 4, p, None)
+    assert L.h2o4gpu_codebook4_codes_bytes(0, 4, 4) == 0 and L.h2o4gpu_codebook4_scales_bytes(1, 4, 4, 31, 0) == 0
+    assert L.h2o4gpu_codebook4_codes_bytes(2, 17, 129) == 2 * 2 * 2 * 1024
     torch.cuda.synchronize()
     assert float(t.abs().sum()) == 0.0
 

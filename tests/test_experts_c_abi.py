@@ -50,5 +50,6 @@ def test_bad_arguments_are_refused_without_a_device():
     assert lib.h2o4gpu_experts_sort(10, 4, None, 16, 16, 16, None, 0, None) == -2
     assert lib.h2o4gpu_experts_dispatch(0, 3, 2, 8, 16, 4, 16, 16, 8, None) == -2
     assert lib.h2o4gpu_experts_combine(0, 3, 2, 8, 16, 8, None, 16, 16, 8, None) == -2
-    assert lib.h2o4gpu_codebook4_product(0, 1, 4, 64, 31, 16, 64, 16, 32, 0, 16, 16, 16, 4, None) == -2
-    assert lib.h2o4gpu_codebook4_product(0, 1, 4, 64, 32, 16, 64, 8, 32, 0, 16, 16, 16, 4, None) == -2
+    assert lib.h2o4gpu_codebook4_product(0, 1, 4, 64, 31, 16, 64, 16, 0, 16, 16, 16, 4, None) == -2
+    assert lib.h2o4gpu_codebook4_product(0, 1, 4, 64, 32, 16, 64, 8, 0, 16, 16, 16, 4, None) == -2
+    assert lib.h2o4gpu_codebook4_layout(1, 4, 64, 32, 16, 31, 0, 16, 16, 16, None) == -2
