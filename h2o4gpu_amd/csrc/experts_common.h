@@ -18,6 +18,12 @@ struct Tag {
   typedef T type;
 };
 
+// A number as a type, for lambdas that pick a kernel.
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 // f(Tag<T>()) for the element type a caller names, EARG for a number that is none.
 template <typename F>
 inline int with_type(int dtype, F f) {

@@ -84,50 +84,335 @@ __global__ __launch_bounds__(256) void route_any_kernel(const T *scores, int64_t
   }
 }
 
-// One wavefront a row: inner = sum of w g over the chosen, then every expert's gradient.
-template <typename T, bool LARGEST, bool ALL>
-__global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, int64_t rs, int64_t es, int64_t rows,
-                                                             int E, int K, float scale, const int *experts,
-                                                             const float *weights, const float *dweights,
-                                                             T *dscores, int64_t drs, int64_t des) {
-  const int lane = threadIdx.x & 63;
-  const float sign = LARGEST ? scale : -scale;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
-  int e_mine = -1;
-  float w = 0.f, g = 0.f;
-  if (lane < K) {
-    e_mine = experts[row * K + lane];
-    w = weights[row * K + lane];
-    g = e_mine >= 0 ? dweights[row * K + lane] : 0.f;
+// Lane i's value from lane i ^ 1, i ^ 2, the mirrored lane of its 8 and of its 16, or the lane 16 or 32 further:
+// what a reduction over 2, 4, 8, 16, 32 or 64 lanes takes in turn.
+template <int STEP>
+__device__ __forceinline__ unsigned from_step(unsigned v) {
+  if (STEP == 0) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);   // quad_perm 1 0 3 2
+  if (STEP == 1) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  if (STEP == 2) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  if (STEP == 3) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true);  // row_mirror
+  const bool low = STEP == 4 ? !(threadIdx.x & 16) : !(threadIdx.x & 32);
+  if (STEP == 4) {
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return low ? s[1] : s[0];
   }
-  float inner = e_mine >= 0 ? w * g : 0.f;
-  for (int m = 32; m >= 1; m >>= 1) inner += __shfl_xor(inner, m, WAVE);
-  const int e0 = __shfl(e_mine, 0, WAVE);
-  const float w0 = __shfl(w, 0, WAVE);
-  const float ninf = -__builtin_huge_valf();
-  float top = ninf;
-  if (ALL && e0 >= 0) top = score_key<LARGEST>((float)scores[row * rs + e0 * es]);
-  for (int base = 0; base < E; base += WAVE) {
-    const int e = base + lane;
-    float p = 0.f, ge = 0.f;
-    bool chosen = false;
-    for (int j = 0; j < K; j++) {
-      const int ej = __shfl(e_mine, j, WAVE);
-      const float wj = __shfl(w, j, WAVE), gj = __shfl(g, j, WAVE);
-      if (ej == e && ej >= 0) {
-        p = wj;
-        ge = gj;
-        chosen = true;
+  const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return low ? s[1] : s[0];
+}
+
+// A score as a number whose largest is the best: 0 for one that is not available. Zeros of either sign are one.
+__device__ __forceinline__ unsigned rank_of(float s, bool largest) {
+  const float k = largest ? s : -s;
+  const unsigned u = __float_as_uint(k == 0.f ? 0.f : k);
+  return k > -__builtin_huge_valf() ? ((int)u < 0 ? ~u : u | 0x80000000u) : 0;
+}
+__device__ __forceinline__ float key_of(unsigned rank) {
+  return __uint_as_float((int)rank < 0 ? rank & 0x7fffffffu : ~rank);
+}
+
+// The better of (rank, index) and that of the lane a step away, over LANES lanes.
+template <int LANES, int STEP = 0>
+__device__ __forceinline__ void best_of(unsigned &rank, unsigned &index) {
+  if constexpr ((1 << STEP) < LANES) {
+    const unsigned r = from_step<STEP>(rank), i = from_step<STEP>(index);
+    const bool take = r > rank || (r == rank && i < index);
+    rank = take ? r : rank;
+    index = take ? i : index;
+    best_of<LANES, STEP + 1>(rank, index);
+  }
+}
+template <int LANES, int STEP = 0>
+__device__ __forceinline__ float sum_of(float v) {
+  if constexpr ((1 << STEP) < LANES)
+    return sum_of<LANES, STEP + 1>(v + __uint_as_float(from_step<STEP>(__float_as_uint(v))));
+  return v;
+}
+
+// Rows whose scores lie side by side, at most LANES * NV of them: LANES lanes have a row in registers, W scores in
+// a row each at a time. Every round takes the best that is left (a lane's own best, then across the lanes) and
+// strikes it out. Lane j ends with choice j. 16384 rows of 256 bfloat16, eight chosen of all: 10 us (40 with
+// the kernel above).
+template <typename T, bool ALL, int LANES, int NV>
+__global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_t rs, int64_t rows, int E, int K,
+                                                         bool largest, float scale, int *experts, float *weights) {
+  constexpr int W = NV < (int)(16 / sizeof(T)) ? NV : (int)(16 / sizeof(T));
+  const int lane = threadIdx.x & (LANES - 1);
+  const int64_t step = (int64_t)gridDim.x * (256 / LANES);
+  for (int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
+    const T *s = scores + row * rs;
+    unsigned rank[NV];
+#pragma unroll
+    for (int c = 0; c < NV / W; c++) {
+      const int e = (c * LANES + lane) * W;
+      struct __attribute__((packed, aligned(sizeof(T)))) Some {
+        T v[W];
+      } some;
+      if (e + W <= E) {
+        some = *reinterpret_cast<const Some *>(s + e);
+#pragma unroll
+        for (int i = 0; i < W; i++) rank[c * W + i] = rank_of((float)some.v[i], largest);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; i++) rank[c * W + i] = e + i < E ? rank_of((float)s[e + i], largest) : 0;
       }
     }
-    if (e >= E) continue;
-    if (ALL && !chosen && e0 >= 0) {
-      const float k = score_key<LARGEST>((float)scores[row * rs + e * es]);
-      if (k != ninf) p = w0 * softmax_term(k, top, scale);
+    unsigned all[NV];
+    if (ALL) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) all[i] = rank[i];
     }
-    const float d = p != 0.f ? sign * p * (ge - inner) : 0.f;
-    dscores[row * drs + e * des] = (T)d;
+    unsigned mine = 0, first = 0;
+    int mine_e = -1;
+    float total = 0.f;
+    for (int j = 0; j < K; j++) {
+      unsigned r = 0, at = 0;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const bool better = rank[i] > r;
+        r = better ? rank[i] : r;
+        at = better ? (i / W * LANES * W + i % W) : at;
+      }
+      at += lane * W;
+      const unsigned own = at;
+      best_of<LANES>(r, at);
+      if (r == 0) break;
+      if (j == 0) first = r;
+      if (!ALL) total += softmax_term(key_of(r), key_of(first), scale);
+      mine = lane == j ? r : mine;
+      mine_e = lane == j ? (int)at : mine_e;
+      if (own == at) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) rank[i] = i / W * LANES * W + i % W + lane * W == at ? 0 : rank[i];
+      }
+    }
+    if (ALL) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) total += all[i] ? softmax_term(key_of(all[i]), key_of(first), scale) : 0.f;
+      total = sum_of<LANES>(total);
+    }
+    if (lane < K) {
+      experts[row * K + lane] = mine_e;
+      weights[row * K + lane] = mine ? softmax_term(key_of(mine), key_of(first), scale) / total : 0.f;
+    }
   }
+}
+
+// Scores of one expert side by side (row stride 1, the distances of transform): a lane has a row and walks down
+// its experts with its best KT in order. The wavefronts of a workgroup each walk a stretch of
+// the experts, and the first joins their lists (a later stretch's equal score stays behind). 1M rows x 64, two
+// chosen: 60 us.
+template <typename T, bool ALL, int KT>
+__global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, int64_t es, int64_t rows, int E, int K,
+                                                             bool largest, float scale, int *experts, float *weights) {
+  extern __shared__ float lists[];  // [parts][2 KT + 1][64]: keys, experts, sums over all
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, parts = blockDim.x >> 6;
+  const float ninf = -__builtin_huge_valf();
+  const int lo = (int)((int64_t)E * part / parts), hi = (int)((int64_t)E * (part + 1) / parts);
+  for (int64_t row0 = (int64_t)blockIdx.x * 64; row0 < rows; row0 += (int64_t)gridDim.x * 64) {
+    const int64_t row = row0 + lane < rows ? row0 + lane : rows - 1;
+    float key[KT], sum = 0.f;
+    int id[KT];
+#pragma unroll
+    for (int j = 0; j < KT; j++) {
+      key[j] = ninf;
+      id[j] = -1;
+    }
+    const auto insert = [&](float k, int e) {
+#pragma unroll
+      for (int j = KT - 1; j >= 0; j--) {
+        const bool here = k > key[j], above = j > 0 && k > key[j > 0 ? j - 1 : 0];
+        key[j] = above ? key[j > 0 ? j - 1 : 0] : here ? k : key[j];
+        id[j] = above ? id[j > 0 ? j - 1 : 0] : here ? e : id[j];
+      }
+    };
+    const T *s = scores + row;
+    for (int e0 = lo; e0 < hi; e0 += 8) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = s[(int64_t)(e0 + i < hi ? e0 + i : hi - 1) * es];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (e0 + i >= hi) break;
+        const float f = largest ? (float)v[i] : -(float)v[i];
+        if (ALL && f > ninf) {  // (sums are of terms against the best so far)
+          if (f > key[0])
+            sum = key[0] > ninf ? sum * softmax_term(key[0], f, scale) + 1.f : 1.f;
+          else
+            sum += softmax_term(f, key[0], scale);
+        }
+        if (f > key[KT - 1]) insert(f, e0 + i);
+      }
+    }
+    if (parts > 1) {
+      __syncthreads();
+      float *mine = lists + (size_t)part * (2 * KT + 1) * 64 + lane;
+#pragma unroll
+      for (int j = 0; j < KT; j++) {
+        mine[2 * j * 64] = key[j];
+        mine[(2 * j + 1) * 64] = __int_as_float(id[j]);
+      }
+      mine[2 * KT * 64] = sum;
+      __syncthreads();
+      if (part > 0) continue;
+      for (int p = 1; p < parts; p++) {
+        const float *other = lists + (size_t)p * (2 * KT + 1) * 64 + lane;
+        if (ALL) {
+          const float top = other[0], its = other[2 * KT * 64];
+          if (top > key[0])
+            sum = (key[0] > ninf ? sum * softmax_term(key[0], top, scale) : 0.f) + its;
+          else if (top > ninf)
+            sum += its * softmax_term(top, key[0], scale);
+        }
+#pragma unroll
+        for (int j = 0; j < KT; j++) {
+          const float k = other[2 * j * 64];
+          if (k > key[KT - 1]) insert(k, __float_as_int(other[(2 * j + 1) * 64]));
+        }
+      }
+    }
+    if (row0 + lane >= rows) continue;
+    float p[KT], total = 0.f;
+#pragma unroll
+    for (int j = 0; j < KT; j++) {
+      p[j] = j < K && id[j] >= 0 ? softmax_term(key[j], key[0], scale) : 0.f;
+      total += p[j];
+    }
+    if (ALL) total = sum;
+#pragma unroll
+    for (int j = 0; j < KT; j++)
+      if (j < K) {
+        experts[row * K + j] = id[j];
+        weights[row * K + j] = id[j] >= 0 ? p[j] / total : 0.f;
+      }
+  }
+}
+
+// One wavefront a row, any strides: inner = sum of w g over the chosen, then every expert's gradient, in LDS 1024 at
+// a time where the chosen ones' are put in their places.
+template <typename T, bool ALL>
+__global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, int64_t rs, int64_t es, int64_t rows,
+                                                             int E, int K, bool largest, float scale,
+                                                             const int *experts, const float *weights,
+                                                             const float *dweights, T *dscores, int64_t drs,
+                                                             int64_t des) {
+  __shared__ float held[4][1024];
+  const int lane = threadIdx.x & 63;
+  float *mine = held[threadIdx.x >> 6];
+  const float sign = largest ? scale : -scale, ninf = -__builtin_huge_valf();
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+    int e_mine = -1;
+    float w = 0.f, g = 0.f;
+    if (lane < K) {
+      e_mine = experts[row * K + lane];
+      w = weights[row * K + lane];
+      g = e_mine >= 0 ? dweights[row * K + lane] : 0.f;
+    }
+    const float inner = sum_of<64>(w != 0.f ? w * g : 0.f);
+    const int e0 = __builtin_amdgcn_readfirstlane(e_mine);
+    const float w0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(w)));
+    float top = 0.f;
+    if (ALL && e0 >= 0) top = (largest ? 1.f : -1.f) * (float)scores[row * rs + e0 * es];
+    const float own = w != 0.f ? sign * w * (g - inner) : 0.f, rest = ALL && e0 >= 0 ? -sign * w0 * inner : 0.f;
+    for (int base = 0; base < E; base += 1024) {
+      const int end = E - base < 1024 ? E - base : 1024;
+      for (int i = lane; i < end; i += WAVE) {
+        float d = 0.f;
+        if (ALL && rest != 0.f) {
+          const float s = (float)scores[row * rs + (base + i) * es], k = largest ? s : -s;
+          const float p = k > ninf ? softmax_term(k, top, scale) : 0.f;
+          d = p != 0.f ? rest * p : 0.f;
+        }
+        mine[i] = d;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (e_mine >= base && e_mine < base + end) mine[e_mine - base] = own;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int i = lane; i < end; i += WAVE) dscores[row * drs + (base + i) * des] = (T)mine[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
+// Scores and gradients of one expert side by side: a lane has a row. Its chosen experts in ascending order, so that
+// one comparison an expert tells whether the next of them is reached.
+template <typename T, bool ALL, int KT>
+__global__ __launch_bounds__(256) void route_backward_columns_kernel(const T *scores, int64_t es, int64_t rows, int E,
+                                                                     int K, bool largest, float scale,
+                                                                     const int *experts, const float *weights,
+                                                                     const float *dweights, T *dscores, int64_t des) {
+  const float sign = largest ? scale : -scale, ninf = -__builtin_huge_valf();
+  const int lo = (int)((int64_t)E * blockIdx.y / gridDim.y), hi = (int)((int64_t)E * (blockIdx.y + 1) / gridDim.y);
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < rows; row += (int64_t)gridDim.x * 256) {
+    int id[KT];
+    float d[KT], inner = 0.f;
+    float w0 = 0.f;
+    int e0 = -1;
+#pragma unroll
+    for (int j = 0; j < KT; j++) {
+      id[j] = j < K ? experts[row * K + j] : -1;
+      const float w = j < K ? weights[row * K + j] : 0.f;
+      const float g = id[j] >= 0 ? dweights[row * K + j] : 0.f;
+      inner += w != 0.f ? w * g : 0.f;
+      d[j] = g;
+      if (j == 0) {
+        e0 = id[0];
+        w0 = w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < KT; j++) {
+      const float w = j < K ? weights[row * K + j] : 0.f;
+      d[j] = w != 0.f ? sign * w * (d[j] - inner) : 0.f;
+    }
+    float top = 0.f;
+    if (ALL && e0 >= 0) top = (largest ? 1.f : -1.f) * (float)scores[row + e0 * es];
+    const float rest = ALL && e0 >= 0 ? -sign * w0 * inner : 0.f;
+    // ascending experts, those that are none (and those before this stretch) last
+#pragma unroll
+    for (int j = 0; j < KT; j++) id[j] = id[j] >= lo ? id[j] : 0x7fffffff;
+#pragma unroll
+    for (int a = 0; a < KT - 1; a++)
+#pragma unroll
+      for (int b = 0; b < KT - 1 - a; b++) {
+        const bool swap = id[b] > id[b + 1];
+        const int i = swap ? id[b] : id[b + 1];
+        const float v = swap ? d[b] : d[b + 1];
+        id[b] = swap ? id[b + 1] : id[b];
+        d[b] = swap ? d[b + 1] : d[b];
+        id[b + 1] = i;
+        d[b + 1] = v;
+      }
+    for (int u0 = lo; u0 < hi; u0 += 8) {
+      T v[8];
+      if (ALL) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = scores[row + (int64_t)(u0 + i < hi ? u0 + i : hi - 1) * es];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (u0 + i >= hi) break;
+        float out = 0.f;
+        if (ALL) {
+          const float k = largest ? (float)v[i] : -(float)v[i];
+          const float p = k > ninf ? softmax_term(k, top, scale) : 0.f;
+          out = p != 0.f && rest != 0.f ? rest * p : 0.f;
+        }
+        if (u0 + i == id[0]) {
+          out = d[0];
+#pragma unroll
+          for (int j = 0; j < KT - 1; j++) {
+            id[j] = id[j + 1];
+            d[j] = d[j + 1];
+          }
+          id[KT - 1] = 0x7fffffff;
+        }
+        dscores[row + (int64_t)(u0 + i) * des] = (T)out;
+      }
+    }
   }
 }
 
@@ -135,103 +420,166 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, in
 // order by expert: a stable counting sort
 // ---------------------------------------------------------------------------
 
-// Slots of one workgroup of the counting pass and of the placing one.
-static const int SORT_CHUNK = 8192;
+// A workgroup of up to 8 wavefronts has a chunk of slots, each wavefront a stretch of it, 64 slots at a time and at
+// most SORT_STEPS times. Two slots of a wavefront find that they name the same expert by comparing a bit of
+// all 64 numbers at a time, so that no order depends on when an addition happens.
+static const int SORT_STEPS = 4, SORT_WAVES = 8;
+static const size_t SORT_LDS = 150u << 10;
 
-static int sort_blocks(size_t slots) { return (int)((slots + SORT_CHUNK - 1) / SORT_CHUNK); }
+// How a launch cuts its slots. One workgroup: a single launch. Some: their histograms first, which every
+// placing workgroup adds up by itself. More than SORT_SCAN: a third launch adds them up in between.
+static const int SORT_SCAN = 64;
+struct SortShape {
+  int waves, chunk, blocks;
+};
+static SortShape sort_shape(size_t slots, int experts) {
+  SortShape s;
+  s.waves = SORT_WAVES;
+  while (s.waves > 1 && (((size_t)s.waves * (experts + 2) + 2 * (experts + 1)) * sizeof(int) > SORT_LDS || (size_t)s.waves * 32 >= slots))
+    s.waves >>= 1;
+  s.chunk = s.waves * WAVE * SORT_STEPS;
+  s.blocks = (int)((slots + s.chunk - 1) / s.chunk);
+  if (s.blocks < 1) s.blocks = 1;
+  return s;
+}
 
 __device__ __forceinline__ int bucket_of(int e, int E) { return (unsigned)e < (unsigned)E ? e : E; }
 
-__global__ __launch_bounds__(1024) void expert_count_kernel(const int *experts, int64_t slots, int E, int *hist) {
+__global__ __launch_bounds__(512) void expert_count_kernel(const int *experts, int64_t slots, int E, int chunk,
+                                                           int *hist) {
   extern __shared__ int cnt[];
   for (int i = threadIdx.x; i <= E; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  const int64_t lo = (int64_t)blockIdx.x * SORT_CHUNK;
-  const int64_t hi = lo + SORT_CHUNK < slots ? lo + SORT_CHUNK : slots;
+  const int64_t lo = (int64_t)blockIdx.x * chunk;
+  const int64_t hi = lo + chunk < slots ? lo + chunk : slots;
+#pragma unroll 4
   for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&cnt[bucket_of(experts[i], E)], 1);
   __syncthreads();
   for (int i = threadIdx.x; i <= E; i += blockDim.x) hist[(int64_t)blockIdx.x * (E + 1) + i] = cnt[i];
 }
 
-// One workgroup of `waves` wavefronts places a chunk: wavefront w has the w-th part of it and
-// counters of its own, so that equal experts keep their slots' order. LDS: counters [waves][E + 1],
-// scan [blockDim].
-__global__ __launch_bounds__(1024) void expert_place_kernel(const int *experts, int64_t slots, int E, int bits,
-                                                            const int *hist, int blocks, int *order, int *position,
-                                                            int *offsets) {
+// hist[c][b] -> how many of bucket b are in the chunks before c; the last row receives the totals. A wavefront
+// has a bucket, its lanes chunks in a row.
+__global__ __launch_bounds__(256) void expert_scan_kernel(int *hist, int blocks, int B) {
+  const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b >= B) return;
+  int before = 0;
+  for (int c0 = 0; c0 < blocks; c0 += WAVE) {
+    const int c = c0 + lane;
+    const int h = c < blocks ? hist[(int64_t)c * B + b] : 0;
+    int sum = h;
+    for (int m = 1; m < WAVE; m <<= 1) {
+      const int add = __shfl_up(sum, m, WAVE);
+      if (lane >= m) sum += add;
+    }
+    if (c < blocks) hist[(int64_t)c * B + b] = before + sum - h;
+    before += __shfl(sum, WAVE - 1, WAVE);
+  }
+  if (lane == 0) hist[(int64_t)blocks * B + b] = before;
+}
+
+// LDS: counters [waves][E + 1], a sum per wavefront, and where the histograms are added up here totals and
+// counts before [E + 1] each. scanned: hist is expert_scan_kernel's.
+__global__ __launch_bounds__(512) void expert_place_kernel(const int *experts, int64_t slots, int E, int bits, int chunk,
+                                                           const int *hist, int blocks, bool scanned, int *order,
+                                                           int *position, int *offsets) {
   extern __shared__ int lds[];
   const int B = E + 1, waves = blockDim.x / WAVE, lane = threadIdx.x & 63, w = threadIdx.x / WAVE;
-  int *cnt = lds;
-  int *scan = lds + waves * B;
-  for (int i = threadIdx.x; i < waves * B; i += blockDim.x) cnt[i] = 0;
-  __syncthreads();
-  const int64_t lo = (int64_t)blockIdx.x * SORT_CHUNK;
-  const int64_t hi = lo + SORT_CHUNK < slots ? lo + SORT_CHUNK : slots;
+  int *cnt = lds, *sums = lds + waves * B, *totals = sums + waves, *befores = totals + B;
+  const int64_t lo = (int64_t)blockIdx.x * chunk;
+  const int64_t hi = lo + chunk < slots ? lo + chunk : slots;
   const int64_t part = ((hi - lo + waves - 1) / waves + WAVE - 1) / WAVE * WAVE;
   const int64_t wlo = lo + w * part, whi = wlo + part < hi ? wlo + part : hi;
-  for (int64_t i = wlo + lane; i < whi; i += WAVE) atomicAdd(&cnt[w * B + bucket_of(experts[i], E)], 1);
-  __syncthreads();
-  // every bucket's place for this chunk: thread t has `per` buckets in a row
-  const int per = (B + blockDim.x - 1) / blockDim.x;
-  const int b0 = threadIdx.x * per;
-  int sum = 0;
-  for (int b = b0; b < b0 + per && b < B; b++) {
-    if (blocks == 1) {
-      for (int v = 0; v < waves; v++) sum += cnt[v * B + b];
-    } else {
-      for (int c = 0; c < blocks; c++) sum += hist[(int64_t)c * B + b];
-    }
+  int id[SORT_STEPS], local[SORT_STEPS];
+#pragma unroll
+  for (int k = 0; k < SORT_STEPS; k++) {
+    const int64_t i = wlo + k * WAVE + lane;
+    id[k] = i < whi ? experts[i] : 0;
   }
-  scan[threadIdx.x] = sum;
+  const int per = (B + blockDim.x - 1) / blockDim.x, b0 = threadIdx.x * per;
+  for (int i = threadIdx.x; i < waves * B; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  for (int m = 1; m < (int)blockDim.x; m <<= 1) {
-    const int add = (int)threadIdx.x >= m ? scan[threadIdx.x - m] : 0;
-    __syncthreads();
-    scan[threadIdx.x] += add;
-    __syncthreads();
-  }
-  int at = scan[threadIdx.x] - sum;
-  for (int b = b0; b < b0 + per && b < B; b++) {
-    if (blockIdx.x == 0) offsets[b] = at;
-    int total = 0, before = 0;
-    if (blocks > 1) {
-      for (int c = 0; c < blocks; c++) {
-        const int h = hist[(int64_t)c * B + b];
-        total += h;
-        if (c < (int)blockIdx.x) before += h;
-      }
-    }
-    int run = at + before;
-    for (int v = 0; v < waves; v++) {
-      const int c = cnt[v * B + b];
-      cnt[v * B + b] = run;
-      run += c;
-      if (blocks == 1) total += c;
-    }
-    at += total;
-  }
-  __syncthreads();
-  for (int64_t base = wlo; base < whi; base += WAVE) {
-    const int64_t i = base + lane;
-    const bool in = i < whi;
-    const int b = in ? bucket_of(experts[i], E) : 0;
+  // place of a slot among its wavefront's of the same expert
+#pragma unroll
+  for (int k = 0; k < SORT_STEPS; k++) {
+    if (wlo + k * WAVE >= whi) break;
+    const bool in = wlo + k * WAVE + lane < whi;
+    const int b = bucket_of(id[k], E);
     unsigned long long same = __ballot(in);
     for (int t = 0; t < bits; t++) {
       const bool bit = (b >> t) & 1;
-      const unsigned long long v = __ballot(in && bit);
+      const unsigned long long v = __ballot(bit);
       same &= bit ? v : ~v;
     }
+    id[k] = b;
     if (in) {
       const int rank = __popcll(same & ((1ull << lane) - 1));
       const int start = cnt[w * B + b];
-      const int p = start + rank;
-      order[p] = (int)i;
-      position[i] = b < E ? p : ~p;
+      local[k] = start + rank;
       __builtin_amdgcn_wave_barrier();
       if (rank == 0) cnt[w * B + b] = start + __popcll(same);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // every bucket's place for this chunk: how many are in all, and in the chunks before
+  int sum = 0;
+  for (int b = b0; b < b0 + per && b < B; b++) {
+    int total = 0, before = 0;
+    if (blocks == 1) {
+      for (int v = 0; v < waves; v++) total += cnt[v * B + b];
+    } else if (scanned) {
+      total = hist[(int64_t)blocks * B + b];
+    } else {
+#pragma unroll 16
+      for (int c = 0; c < blocks; c++) {
+        const int h = hist[(int64_t)c * B + b];
+        total += h;
+        before += c < (int)blockIdx.x ? h : 0;
+      }
+    }
+    if (blocks > 1 && !scanned) {
+      totals[b] = total;
+      befores[b] = before;
+    }
+    sum += total;
+  }
+  int upto = sum;
+  for (int m = 1; m < WAVE; m <<= 1) {
+    const int add = __shfl_up(upto, m, WAVE);
+    if (lane >= m) upto += add;
+  }
+  if (lane == WAVE - 1) sums[w] = upto;
+  __syncthreads();
+  int at = upto - sum;
+  for (int v = 0; v < w; v++) at += sums[v];
+  for (int b = b0; b < b0 + per && b < B; b++) {
+    if (blockIdx.x == 0) offsets[b] = at;
+    int run = at, next = at;
+    if (scanned) {
+      next += hist[(int64_t)blocks * B + b];
+      run += hist[(int64_t)blockIdx.x * B + b];
+    } else if (blocks > 1) {
+      next += totals[b];
+      run += befores[b];
+    }
+    for (int v = 0; v < waves; v++) {
+      const int c = cnt[v * B + b];
+      cnt[v * B + b] = run;
+      run += c;
+    }
+    at = blocks > 1 ? next : run;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < SORT_STEPS; k++) {
+    const int64_t i = wlo + k * WAVE + lane;
+    if (i < whi) {
+      const int p = cnt[w * B + id[k]] + local[k];
+      order[p] = (int)i;
+      position[i] = id[k] < E ? p : ~p;
+    }
   }
 }
 
@@ -239,61 +587,230 @@ __global__ __launch_bounds__(1024) void expert_place_kernel(const int *experts, 
 // rows out and back
 // ---------------------------------------------------------------------------
 
-// dst[place(t, j)] = src[t], zeros where the slot has no expert.
+// Rows move in pieces of 16 bytes, at addresses that are only aligned to their elements (one load or store all
+// the same); the elements behind a row's last whole piece move one by one.
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx4_u __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
-__global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss, const int *position, int64_t tokens,
-                                                        int K, int d, T *dst, int64_t ds) {
-  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-  for (int j = 0; j < K; j++) {
-    const int p = position[t * K + j];
-    T *to = dst + (int64_t)(p < 0 ? ~p : p) * ds;
-    for (int c = threadIdx.x; c < d; c += blockDim.x) to[c] = p < 0 ? (T)0.f : src[t * ss + c];
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ uintx4 load(const T *row, int piece) {
+    return *reinterpret_cast<const uintx4_u *>(row + (int64_t)piece * N);
   }
-}
+  static __device__ __forceinline__ void store(T *row, int piece, uintx4 v) {
+    *reinterpret_cast<uintx4_u *>(row + (int64_t)piece * N) = v;
+  }
+  static __device__ __forceinline__ void unpack(uintx4 v, float (&f)[N]) {
+    T e[N];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = (float)e[i];
+  }
+  static __device__ __forceinline__ uintx4 pack(const float (&f)[N]) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) e[i] = (T)f[i];
+    uintx4 v;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+  }
+};
 
-// dst[t] = sum over j of (w[t][j] *) src[place(t, j)].
-template <typename T, bool WEIGHTED>
-__global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss, const float *w, const int *position,
-                                                        int64_t tokens, int K, int d, T *dst, int64_t ds) {
-  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-  for (int c = threadIdx.x; c < d; c += blockDim.x) {
-    float acc = 0.f;
-    for (int j = 0; j < K; j++) {
-      const int p = position[t * K + j];
-      if (p < 0) continue;
-      const float v = (float)src[(int64_t)p * ss + c];
-      acc = WEIGHTED ? fmaf(w[t * K + j], v, acc) : acc + v;
+// How the threads of a launch share the tokens' rows: 2^lanes_log2 lanes to a row (as many as it has pieces, 64
+// at most), U pieces each, and blockIdx.y further stretches of a long row. Neighbouring lanes have
+// neighbouring pieces.
+struct RowShare {
+  int64_t tokens;
+  int K, d, lanes_log2;
+};
+
+// dst[place(t, j)] = src[t], zeros where the slot has no expert. A row is read once for its top_k places.
+template <typename T, int U>
+__global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss, const int *position, RowShare a,
+                                                        T *dst, int64_t ds) {
+  constexpr int N = Row<T>::N;
+  const int lanes = 1 << a.lanes_log2, whole = a.d / N, lane = threadIdx.x & (lanes - 1);
+  const int first = (int)blockIdx.y * lanes * U + lane;
+  const int64_t step = (int64_t)gridDim.x * (256 >> a.lanes_log2);
+  for (int64_t t = (int64_t)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2); t < a.tokens; t += step) {
+    const T *row = src + t * ss;
+    uintx4 p[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (first + u * lanes < whole) p[u] = Row<T>::load(row, first + u * lanes);
+    for (int j = 0; j < a.K; j++) {
+      const int at = position[t * a.K + j];
+      T *to = dst + (int64_t)(at < 0 ? ~at : at) * ds;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (first + u * lanes < whole) Row<T>::store(to, first + u * lanes, at < 0 ? uintx4{0, 0, 0, 0} : p[u]);
     }
-    dst[t * ds + c] = (T)acc;
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64_t os, const T *rows, int64_t rs,
-                                                            const float *w, const int *position, int64_t tokens,
-                                                            int K, int d, T *drows, int64_t drs, float *dw) {
-  __shared__ float part[4];
-  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-  for (int j = 0; j < K; j++) {
-    const int p = position[t * K + j];
-    const int64_t at = p < 0 ? ~p : p;
-    const float wj = p < 0 ? 0.f : w[t * K + j];
-    float acc = 0.f;
-    for (int c = threadIdx.x; c < d; c += blockDim.x) {
-      if (p < 0) {
-        drows[at * drs + c] = (T)0.f;
-        continue;
+    if (blockIdx.y == 0)
+      for (int c = whole * N + lane; c < a.d; c += lanes) {
+        const T v = row[c];
+        for (int j = 0; j < a.K; j++) {
+          const int at = position[t * a.K + j];
+          dst[(int64_t)(at < 0 ? ~at : at) * ds + c] = at < 0 ? (T)0.f : v;
+        }
       }
-      const float g = (float)dout[t * os + c];
-      acc = fmaf(g, (float)rows[at * rs + c], acc);
-      drows[at * drs + c] = (T)(wj * g);
-    }
-    for (int m = 32; m >= 1; m >>= 1) acc += __shfl_xor(acc, m, WAVE);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
-    __syncthreads();
-    if (threadIdx.x == 0) dw[t * K + j] = (part[0] + part[1]) + (part[2] + part[3]);
   }
+}
+
+// dst[t] = sum over j of (w[t][j] *) src[place(t, j)], j ascending; four rows of them on their way at a time.
+template <typename T, int U, bool WEIGHTED>
+__global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss, const float *w, const int *position,
+                                                        RowShare a, T *dst, int64_t ds) {
+  constexpr int N = Row<T>::N;
+  const int lanes = 1 << a.lanes_log2, whole = a.d / N, lane = threadIdx.x & (lanes - 1);
+  const int first = (int)blockIdx.y * lanes * U + lane, stride = gridDim.y * lanes * U;
+  const int64_t step = (int64_t)gridDim.x * (256 >> a.lanes_log2);
+  for (int64_t t = (int64_t)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2); t < a.tokens; t += step) {
+    for (int i0 = first; i0 < whole; i0 += stride) {
+      float acc[U][N] = {};
+      for (int j0 = 0; j0 < a.K; j0 += 4) {
+        int at[4];
+        float by[4];
+        uintx4 p[4][U];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          at[j] = j0 + j < a.K ? position[t * a.K + j0 + j] : -1;
+          by[j] = WEIGHTED && j0 + j < a.K ? w[t * a.K + j0 + j] : 1.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int u = 0; u < U; u++)
+            if (at[j] >= 0 && i0 + u * lanes < whole)
+              p[j][u] = Row<T>::load(src + (int64_t)at[j] * ss, i0 + u * lanes);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (at[j] >= 0) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+              float v[N];
+              Row<T>::unpack(p[j][u], v);
+#pragma unroll
+              for (int e = 0; e < N; e++) acc[u][e] = WEIGHTED ? fmaf(by[j], v[e], acc[u][e]) : acc[u][e] + v[e];
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (i0 + u * lanes < whole) Row<T>::store(dst + t * ds, i0 + u * lanes, Row<T>::pack(acc[u]));
+    }
+    if (blockIdx.y == 0)
+      for (int c = whole * N + lane; c < a.d; c += lanes) {
+        float sum = 0.f;
+        for (int j = 0; j < a.K; j++) {
+          const int at = position[t * a.K + j];
+          if (at < 0) continue;
+          const float v = (float)src[(int64_t)at * ss + c];
+          sum = WEIGHTED ? fmaf(w[t * a.K + j], v, sum) : sum + v;
+        }
+        dst[t * ds + c] = (T)sum;
+      }
+  }
+}
+
+// Both gradients of the weighted sum in one pass over the rows: J of a token's places at a time. SPLIT: the
+// four wavefronts of a workgroup share a token's row, otherwise each has tokens of its own.
+template <typename T, int U, int J, bool SPLIT>
+__global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64_t os, const T *rows, int64_t rs,
+                                                            const float *w, const int *position, RowShare a,
+                                                            T *drows, int64_t drs, float *dw) {
+  constexpr int N = Row<T>::N;
+  __shared__ float part[SPLIT ? 4 * J : 1];
+  const int lanes = 1 << a.lanes_log2, whole = a.d / N, wave = threadIdx.x >> 6;
+  const int lane = SPLIT ? threadIdx.x : threadIdx.x & (lanes - 1), stride = SPLIT ? 256 : lanes;
+  const int per = SPLIT ? 1 : 256 >> a.lanes_log2, width = SPLIT ? WAVE : lanes;
+  const int64_t step = (int64_t)gridDim.x * per;
+  for (int64_t t = (int64_t)blockIdx.x * per + (SPLIT ? 0 : threadIdx.x >> a.lanes_log2); t < a.tokens; t += step) {
+    const T *g_row = dout + t * os;
+    for (int j0 = 0; j0 < a.K; j0 += J) {
+      int at[J];
+      float by[J], dot[J] = {};
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        at[j] = j0 + j < a.K ? position[t * a.K + j0 + j] : -1;
+        by[j] = j0 + j < a.K ? w[t * a.K + j0 + j] : 0.f;
+      }
+      for (int i0 = lane; i0 < whole; i0 += stride * U) {
+        uintx4 g[U], y[J][U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (i0 + u * stride < whole) g[u] = Row<T>::load(g_row, i0 + u * stride);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+          for (int u = 0; u < U; u++)
+            if (at[j] >= 0 && i0 + u * stride < whole) y[j][u] = Row<T>::load(rows + (int64_t)at[j] * rs, i0 + u * stride);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          if (i0 + u * stride >= whole) break;
+          float gv[N];
+          Row<T>::unpack(g[u], gv);
+#pragma unroll
+          for (int j = 0; j < J; j++) {
+            if (at[j] >= 0) {
+              float yv[N], out[N];
+              Row<T>::unpack(y[j][u], yv);
+#pragma unroll
+              for (int e = 0; e < N; e++) {
+                dot[j] = fmaf(gv[e], yv[e], dot[j]);
+                out[e] = by[j] * gv[e];
+              }
+              Row<T>::store(drows + (int64_t)at[j] * drs, i0 + u * stride, Row<T>::pack(out));
+            } else if (j0 + j < a.K) {
+              Row<T>::store(drows + (int64_t)~at[j] * drs, i0 + u * stride, uintx4{0, 0, 0, 0});
+            }
+          }
+        }
+      }
+      for (int c = whole * N + lane; c < a.d; c += stride) {
+        const float gv = (float)g_row[c];
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+          if (j0 + j >= a.K) break;
+          if (at[j] >= 0) dot[j] = fmaf(gv, (float)rows[(int64_t)at[j] * rs + c], dot[j]);
+          drows[(int64_t)(at[j] < 0 ? ~at[j] : at[j]) * drs + c] = at[j] < 0 ? (T)0.f : (T)(by[j] * gv);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; j++)
+        for (int m = width >> 1; m >= 1; m >>= 1) dot[j] += __shfl_xor(dot[j], m, WAVE);
+      if (SPLIT) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+          for (int j = 0; j < J; j++) part[wave * J + j] = dot[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < J && j0 + (int)threadIdx.x < a.K)
+          dw[t * a.K + j0 + threadIdx.x] = (part[threadIdx.x] + part[J + threadIdx.x]) +
+                                           (part[2 * J + threadIdx.x] + part[3 * J + threadIdx.x]);
+      } else if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < J; j++)
+          if (j0 + j < a.K) dw[t * a.K + j0 + j] = dot[j];
+      }
+    }
+  }
+}
+
+// The share of rows of d elements of T, U pieces to a lane, and its grid.
+template <typename T>
+static RowShare share_rows(size_t tokens, int top_k, size_t cols, int U, dim3 *grid) {
+  RowShare a;
+  a.tokens = (int64_t)tokens;
+  a.K = top_k;
+  a.d = (int)cols;
+  const int pieces = (int)((cols + Row<T>::N - 1) / Row<T>::N);
+  a.lanes_log2 = 0;
+  while (a.lanes_log2 < 6 && (1 << a.lanes_log2) * U < pieces) a.lanes_log2++;
+  const int lanes = 1 << a.lanes_log2;
+  const size_t per = 256 >> a.lanes_log2;
+  *grid = dim3(grid_of((tokens + per - 1) / per), (unsigned)((pieces + lanes * U - 1) / (lanes * U)));
+  return a;
 }
 
 // ---------------------------------------------------------------------------
@@ -333,11 +850,42 @@ KM_API int h2o4gpu_experts_route(int dtype, size_t rows, int experts, int top_k,
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
+    const T *scores = static_cast<const T *>(d_scores);
+    const int64_t n = (int64_t)rows;
+    // columns: lists of up to eight stay in registers (longer ones go the general way)
+    if (row_stride == 1 && expert_stride != 1 && top_k <= 8) {
+      const auto columns = [&](auto all, auto kt) {
+        constexpr int KT = decltype(kt)::value;
+        int parts = 1;  // until there are some 2048 wavefronts, or a stretch is as short as a load's eight
+        while (parts < 16 && (n + 63) / 64 * parts < 2048 && experts / (parts * 2) >= 8) parts *= 2;
+        hipLaunchKernelGGL((route_columns_kernel<T, decltype(all)::value, KT>), dim3(grid_of((rows + 63) / 64)),
+                           dim3(64 * parts), parts > 1 ? sizeof(float) * parts * (2 * KT + 1) * 64 : 0, s, scores,
+                           (int64_t)expert_stride, n, experts, top_k, largest != 0, scale, d_experts, d_weights);
+        return launched();
+      };
+      const auto by_k = [&](auto all) {
+        return top_k == 1 ? columns(all, Int<1>()) : top_k == 2 ? columns(all, Int<2>())
+               : top_k <= 4 ? columns(all, Int<4>()) : columns(all, Int<8>());
+      };
+      return over_all ? by_k(Int<1>()) : by_k(Int<0>());
+    }
+    const auto in_rows = [&](auto lanes, auto nv) {
+      constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
+      auto kernel = over_all ? route_rows_kernel<T, true, L, NV> : route_rows_kernel<T, false, L, NV>;
+      hipLaunchKernelGGL(kernel, dim3(grid_of((rows * L + 255) / 256)), dim3(256), 0, s, scores, (int64_t)row_stride, n,
+                         experts, top_k, largest != 0, scale, d_experts, d_weights);
+      return launched();
+    };
+    if (expert_stride == 1 && experts <= 1024) {
+      if (experts <= 16 && top_k <= 4) return in_rows(Int<4>(), Int<4>());
+      if (experts <= 64 && top_k <= 16) return in_rows(Int<16>(), Int<4>());
+      if (experts <= 256 && top_k <= 16) return in_rows(Int<16>(), Int<16>());
+      return in_rows(Int<64>(), Int<16>());
+    }
     auto kernel = largest ? (over_all ? route_any_kernel<T, true, true> : route_any_kernel<T, true, false>)
                           : (over_all ? route_any_kernel<T, false, true> : route_any_kernel<T, false, false>);
-    hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 3) / 4)), dim3(256), 0, s, static_cast<const T *>(d_scores),
-                       (int64_t)row_stride, (int64_t)expert_stride, (int64_t)rows, experts, top_k, scale, d_experts,
-                       d_weights);
+    hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 3) / 4)), dim3(256), 0, s, scores, (int64_t)row_stride,
+                       (int64_t)expert_stride, n, experts, top_k, scale, d_experts, d_weights);
     return launched();
   });
 }
@@ -358,21 +906,34 @@ KM_API int h2o4gpu_experts_route_backward(int dtype, size_t rows, int experts, i
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    auto kernel = largest ? (over_all ? route_backward_kernel<T, true, true> : route_backward_kernel<T, true, false>)
-                          : (over_all ? route_backward_kernel<T, false, true>
-                                      : route_backward_kernel<T, false, false>);
-    hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 3) / 4)), dim3(256), 0, s, static_cast<const T *>(d_scores),
-                       (int64_t)row_stride, (int64_t)expert_stride, (int64_t)rows, experts, top_k, scale, d_experts,
-                       d_weights, d_dweights, static_cast<T *>(d_dscores), (int64_t)drow_stride,
-                       (int64_t)dexpert_stride);
+    const T *scores = static_cast<const T *>(d_scores);
+    T *dscores = static_cast<T *>(d_dscores);
+    const int64_t n = (int64_t)rows;
+    if (row_stride == 1 && drow_stride == 1 && dexpert_stride != 1 && top_k <= 8) {
+      unsigned parts = 1;
+      while ((n + 255) / 256 * parts < 512 && experts / (int)(parts * 2) >= 16) parts *= 2;
+      const dim3 grid(grid_of((rows + 255) / 256), parts);
+      const auto columns = [&](auto kt) {
+        constexpr int KT = decltype(kt)::value;
+        auto kernel = over_all ? route_backward_columns_kernel<T, true, KT> : route_backward_columns_kernel<T, false, KT>;
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, scores, (int64_t)expert_stride, n, experts, top_k, largest != 0,
+                           scale, d_experts, d_weights, d_dweights, dscores, (int64_t)dexpert_stride);
+        return launched();
+      };
+      return top_k <= 2 ? columns(Int<2>()) : top_k <= 4 ? columns(Int<4>()) : columns(Int<8>());
+    }
+    auto kernel = over_all ? route_backward_kernel<T, true> : route_backward_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 3) / 4)), dim3(256), 0, s, scores, (int64_t)row_stride,
+                       (int64_t)expert_stride, n, experts, top_k, largest != 0, scale, d_experts, d_weights, d_dweights,
+                       dscores, (int64_t)drow_stride, (int64_t)dexpert_stride);
     return launched();
   });
 }
 
 KM_API size_t h2o4gpu_experts_sort_workspace(size_t slots, int experts) {
   if (!experts_ok(experts) || slots > MOST_ROWS) return 0;
-  const int blocks = sort_blocks(slots);
-  return blocks > 1 ? (size_t)blocks * (experts + 1) * sizeof(int) : 0;
+  const int blocks = sort_shape(slots, experts).blocks;
+  return blocks > 1 ? (size_t)(blocks + 1) * (experts + 1) * sizeof(int) : 0;
 }
 
 KM_API int h2o4gpu_experts_sort(size_t slots, int experts, const int *d_experts, int *d_order, int *d_position,
@@ -383,24 +944,28 @@ KM_API int h2o4gpu_experts_sort(size_t slots, int experts, const int *d_experts,
   if (need > 0 && (!ints_ok(d_workspace) || workspace_bytes < need)) return H2O4GPU_KMEANS_EARG;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int buckets = experts + 1;
-  const int blocks = sort_blocks(slots) > 0 ? sort_blocks(slots) : 1;
+  const SortShape shape = sort_shape(slots, experts);
   int *hist = static_cast<int *>(d_workspace);
-  // as many wavefronts as counters of their own fit (128 KB): 16 up to 2047 experts, 2 for the most
-  int waves = 16;
-  while (waves > 1 && (size_t)waves * buckets * sizeof(int) > (128u << 10)) waves >>= 1;
+  // (with very many buckets there is no room for what is added up)
+  const bool scanned = shape.blocks > SORT_SCAN || (shape.blocks > 1 && shape.waves == 1);
   int bits = 0;
   while ((experts >> bits) != 0) bits++;
-  if (blocks > 1) {
+  if (shape.blocks > 1) {
     const size_t lds = (size_t)buckets * sizeof(int);
     KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(expert_count_kernel), lds));
-    hipLaunchKernelGGL(expert_count_kernel, dim3(blocks), dim3(1024), lds, s, d_experts, (int64_t)slots, experts,
-                       hist);
+    hipLaunchKernelGGL(expert_count_kernel, dim3(shape.blocks), dim3(512), lds, s, d_experts, (int64_t)slots, experts,
+                       shape.chunk, hist);
     KM_TRY(launched());
+    if (scanned) {
+      hipLaunchKernelGGL(expert_scan_kernel, dim3((buckets + 3) / 4), dim3(256), 0, s, hist, shape.blocks, buckets);
+      KM_TRY(launched());
+    }
   }
-  const size_t lds = ((size_t)waves * buckets + (size_t)waves * WAVE) * sizeof(int);
+  const size_t lds = ((size_t)shape.waves * (buckets + 1) + (shape.blocks > 1 && !scanned ? 2 * buckets : 0)) * sizeof(int);
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(expert_place_kernel), lds));
-  hipLaunchKernelGGL(expert_place_kernel, dim3(blocks), dim3(waves * WAVE), lds, s, d_experts, (int64_t)slots,
-                     experts, bits, hist, blocks, d_order, d_position, d_offsets);
+  hipLaunchKernelGGL(expert_place_kernel, dim3(shape.blocks), dim3(shape.waves * WAVE), lds, s, d_experts,
+                     (int64_t)slots, experts, bits, shape.chunk, hist, shape.blocks, scanned, d_order, d_position,
+                     d_offsets);
   return launched();
 }
 
@@ -414,9 +979,11 @@ KM_API int h2o4gpu_experts_dispatch(int dtype, size_t tokens, int top_k, size_t 
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    hipLaunchKernelGGL(send_rows_kernel<T>, dim3(grid_of(tokens)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T *>(d_x), (int64_t)x_stride, d_position, (int64_t)tokens, top_k, (int)cols,
-                       static_cast<T *>(d_rows), (int64_t)rows_stride);
+    dim3 grid;
+    const RowShare a = share_rows<T>(tokens, top_k, cols, 4, &grid);
+    hipLaunchKernelGGL((send_rows_kernel<T, 4>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const T *>(d_x), (int64_t)x_stride, d_position, a, static_cast<T *>(d_rows),
+                       (int64_t)rows_stride);
     return launched();
   });
 }
@@ -431,10 +998,12 @@ static int join_rows(int dtype, size_t tokens, int top_k, size_t cols, const voi
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    auto kernel = weighted ? join_rows_kernel<T, true> : join_rows_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid_of(tokens)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T *>(src), (int64_t)src_stride, w, position, (int64_t)tokens, top_k,
-                       (int)cols, static_cast<T *>(dst), (int64_t)dst_stride);
+    dim3 grid;
+    const RowShare a = share_rows<T>(tokens, top_k, cols, 2, &grid);
+    if (tokens >= 4096) grid.y = 1;  // (enough rows for every wavefront to have whole ones)
+    auto kernel = weighted ? join_rows_kernel<T, 2, true> : join_rows_kernel<T, 2, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(src),
+                       (int64_t)src_stride, w, position, a, static_cast<T *>(dst), (int64_t)dst_stride);
     return launched();
   });
 }
@@ -465,10 +1034,15 @@ KM_API int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k,
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    hipLaunchKernelGGL(join_backward_kernel<T>, dim3(grid_of(tokens)), dim3(256), 0,
+    dim3 grid;
+    const RowShare a = share_rows<T>(tokens, top_k, cols, 2, &grid);
+    const bool split = tokens < 1024 && grid.y > 1;  // few long rows
+    auto kernel = top_k <= 2 ? (split ? join_backward_kernel<T, 2, 2, true> : join_backward_kernel<T, 2, 2, false>)
+                             : (split ? join_backward_kernel<T, 2, 4, true> : join_backward_kernel<T, 2, 4, false>);
+    hipLaunchKernelGGL(kernel, dim3(split ? (unsigned)tokens : grid.x), dim3(256), 0,
                        static_cast<hipStream_t>(stream), static_cast<const T *>(d_dout), (int64_t)dout_stride,
-                       static_cast<const T *>(d_rows), (int64_t)rows_stride, d_weights, d_position, (int64_t)tokens,
-                       top_k, (int)cols, static_cast<T *>(d_drows), (int64_t)drows_stride, d_dweights);
+                       static_cast<const T *>(d_rows), (int64_t)rows_stride, d_weights, d_position, a,
+                       static_cast<T *>(d_drows), (int64_t)drows_stride, d_dweights);
     return launched();
   });
 }
