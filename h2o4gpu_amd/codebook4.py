@@ -57,7 +57,7 @@ class Codebook4:
         if tuple(codebook.shape) != (16,) and not (lead and tuple(codebook.shape) == (codes.shape[0], 16)):
             raise ValueError("codebook must have 16 values%s, got shape %s" % (
                 " (or 16 for each expert)" if lead else "", tuple(codebook.shape)))
-        codes, scales, device = codes.contiguous(), scales.contiguous(), codes.device
+        codes, scales, device = codes.contiguous(), scales.contiguous(), codes.device.index
         self.codebook, self.cols, self.group, self.out = codebook.contiguous(), cols, group, codes.shape[-2]
         self.n_experts = codes.shape[0] if lead else 0
         count, lib = max(1, self.n_experts), experts_hip.lib()
@@ -65,9 +65,9 @@ class Codebook4:
         nbytes = lib.h2o4gpu_codebook4_codes_bytes(count, self.out, cols)
         if nbytes == 0:
             raise ValueError("a matrix of %d x %d is beyond what the products take" % (self.out, cols))
-        self.laid_codes = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.laid_codes = codes.new_empty(nbytes)
         nbytes = lib.h2o4gpu_codebook4_scales_bytes(count, self.out, cols, group, kind)
-        self.laid_scales = torch.empty(nbytes // scales.element_size(), dtype=scales.dtype, device=device)
+        self.laid_scales = scales.new_empty(nbytes // scales.element_size())
         _call(device, "h2o4gpu_codebook4_layout", count, self.out, cols, group, codes.data_ptr(), codes.shape[-1],
               kind, scales.data_ptr(), self.laid_codes.data_ptr(), self.laid_scales.data_ptr())
         self._args = (self.laid_codes.data_ptr(), kind, self.laid_scales.data_ptr(), self.codebook.data_ptr())
@@ -159,7 +159,7 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
     codes = torch.empty((flat.shape[0], pitch), dtype=torch.uint8, device=flat.device)
     scales = torch.empty((flat.shape[0], groups), dtype=scale_dtype or weights.dtype, device=flat.device)
     ptr, stride = _rows("weights", flat)
-    _call(flat.device, "h2o4gpu_codebook4_quantize", code, flat.shape[0], cols, group, top, ptr, stride,
+    _call(flat.device.index, "h2o4gpu_codebook4_quantize", code, flat.shape[0], cols, group, top, ptr, stride,
           codebook.data_ptr(), codes.data_ptr(), pitch, _type_of("scales", scales), scales.data_ptr())
     lead = tuple(weights.shape[:-1])
     return Codebook4(codes.reshape(lead + (pitch,)), scales.reshape(lead + (groups,)), codebook, cols, group)
@@ -182,9 +182,10 @@ def product(x, weights):
     ptr, stride = _tokens(x, weights)
     if weights.n_experts:
         raise ValueError("weights hold a matrix per expert: experts_product multiplies with those")
-    y = torch.empty((x.shape[0], weights.out), dtype=x.dtype, device=x.device)
-    _call(x.device, "h2o4gpu_codebook4_product", _TYPES[x.dtype], x.shape[0], weights.out, weights.cols,
-          weights.group, ptr, stride, *weights._args, y.data_ptr(), weights.out)
+    rows, out = x.shape[0], weights.out
+    y = x.new_empty((rows, out))
+    _call(x.device.index, "h2o4gpu_codebook4_product", _TYPES[x.dtype], rows, out, weights.cols, weights.group, ptr,
+          stride, *weights._args, y.data_ptr(), out)
     return y
 
 
@@ -198,8 +199,8 @@ def experts_product(x, weights, order):
         raise ValueError("order has %d experts, weights %d" % (order.n_experts, weights.n_experts))
     if x.shape[0] != order.tokens:
         raise ValueError("x must be (%d, %d), got %s" % (order.tokens, weights.cols, tuple(x.shape)))
-    y = torch.empty((order.tokens * order.top_k, weights.out), dtype=x.dtype, device=x.device)
-    _call(x.device, "h2o4gpu_codebook4_experts_product", _TYPES[x.dtype], order.tokens, order.top_k,
+    y = x.new_empty((order.tokens * order.top_k, weights.out))
+    _call(x.device.index, "h2o4gpu_codebook4_experts_product", _TYPES[x.dtype], order.tokens, order.top_k,
           weights.n_experts, weights.out, weights.cols, weights.group, ptr, stride, *weights._args,
           16 if weights.codebook.dim() == 2 else 0, order.order.data_ptr(), order.offsets.data_ptr(), y.data_ptr(),
           weights.out)

@@ -421,14 +421,21 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 4 : 2) void product4_few_kern
 
 // 16 * MT rows of y at a time, a row of x in each of a product's 16. Rows of x behind the last one are read from
 // the last: their results are not written.
+// A product wants 8 columns of 16 different rows from 16 neighbouring lanes. Loaded like that, x costs an access
+// to the cache for every lane (58 for a load, and they are what bounds 33 x 8192 x 8192 at 26 us); so 16 lanes
+// load 128 columns of one row, and a wavefront's own 16 x 128 corner of LDS turns them. Piece c of row r lies at
+// place c ^ r of its row there, so that 16 rows' pieces c lie in different banks.
 template <typename T, typename S, int MT, int NT, int R, int PER>
 __global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  typedef unsigned XFrag[MT][4][2 * sizeof(T)];
+  constexpr int W = 2 * sizeof(T), SZ = 8 * sizeof(T);  // words and bytes of a piece: 8 values
+  typedef unsigned Piece __attribute__((ext_vector_type(W)));
+  typedef unsigned Piece_u __attribute__((ext_vector_type(W), aligned(sizeof(T))));
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  float *red = reinterpret_cast<float *>(lds + TABLE_BYTES);
+  char *turn = lds + TABLE_BYTES + wave * (256 * SZ);
+  float *red = reinterpret_cast<float *>(lds + TABLE_BYTES);  // (in the same place, when the corners are done with)
   const int teams = waves / a.splits, team = wave / a.splits, part = wave % a.splits;
   const int tiles16 = (int)((a.m.out + 15) >> 4), subs = (a.m.cols + 127) >> 7;
   const Share share = share_of(a, reinterpret_cast<int *>(red), y);
@@ -445,30 +452,53 @@ __global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product
     const bool mine = tile < tiles16;
     reader.move_to(tile, tiles16, subs);
     for (int64_t lo = begin; lo < hi; lo += (int64_t)gridDim.z * (16 * MT)) {
-      const T *row[MT];
+      // load j of 16 rows: row 4 j + q, its piece r ^ (4 j + q)
+      const T *from[MT][4];
 #pragma unroll
-      for (int t = 0; t < MT; t++) row[t] = x_row(x, a, lo + 16 * t + r < hi ? lo + 16 * t + r : hi - 1) + 8 * q;
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int64_t p = lo + 16 * m + 4 * j + q;
+          from[m][j] = x_row(x, a, p < hi ? p : hi - 1) + 8 * (r ^ (4 * j + q));
+        }
       floatx4 acc[MT][NT] = {};
       Tiles<S, NT, PER> held[R];
-      XFrag xf[R];
-      const auto fetch = [&](int j, int sub) {
-        reader.fetch(held[j], sub);
+      Piece raw[R][MT][4];
+      const auto fetch = [&](int k, int sub) {
+        reader.fetch(held[k], sub);
 #pragma unroll
-        for (int t = 0; t < MT; t++)
+        for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) load_x8<T>(row[t] + ((int64_t)sub * 128 + 32 * i), xf[j][t][i]);
+          for (int j = 0; j < 4; j++) raw[k][m][j] = *reinterpret_cast<const Piece_u *>(from[m][j] + (int64_t)sub * 128);
       };
-      const auto multiply = [&](int st, int t) {
-        unsigned b[4][2 * sizeof(T)];
-        decode<T>(held[st].words[t], lane_at, b);
+      unsigned xf[MT][4][W];
+      const auto turn_x = [&](int k) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) *reinterpret_cast<Piece *>(turn + (64 * j + lane) * SZ) = raw[k][m][j];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const Piece v = *reinterpret_cast<const Piece *>(turn + (16 * r + ((4 * i + q) ^ r)) * SZ);
+            __builtin_memcpy(xf[m][i], &v, SZ);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
+      };
+      const auto multiply = [&](const Tiles<S, NT, PER> &h, int t) {
+        unsigned b[4][W];
+        decode<T>(h.words[t], lane_at, b);
         floatx4 sum[MT] = {};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
 #pragma unroll
           for (int m = 0; m < MT; m++) {
-            sum[m] = Mfma4<T>::mma(xf[st][m][i], b[i], sum[m]);
+            sum[m] = Mfma4<T>::mma(xf[m][i], b[i], sum[m]);
             if ((i + 1) % (4 / PER) == 0) {
-              const float sc = (float)held[st].scale[t].v[i * PER / 4];
+              const float sc = (float)h.scale[t].v[i * PER / 4];
 #pragma unroll
               for (int v = 0; v < 4; v++) acc[m][t][v] = fmaf(sc, sum[m][v], acc[m][t][v]);
               sum[m] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -478,32 +508,35 @@ __global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product
       };
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < R; j++)
-          if (j < count) fetch(j, first + j);
+        for (int k = 0; k < R; k++)
+          if (k < count) fetch(k, first + k);
       }
       if (!have_table) make_table<T>(lds, a.m, share.expert);
       have_table = true;
       if (mine) {
         for (int b = 0; b < count; b += R) {
 #pragma unroll
-          for (int j = 0; j < R; j++) {
-            if (b + j >= count) break;
+          for (int k = 0; k < R; k++) {
+            if (b + k >= count) break;
+            turn_x(k);
 #pragma unroll
-            for (int t = 0; t < NT; t++) multiply(j, t);
-            if (b + R + j < count) fetch(j, first + b + R + j);
+            for (int n = 0; n < NT; n++) multiply(held[k], n);
+            if (b + R + k < count) fetch(k, first + b + R + k);
           }
         }
         if ((cols & 127) && part == 0) {  // the columns behind the last whole 128 (part 0 has the fewest before)
           reader.fetch(held[0], full);
 #pragma unroll
-          for (int t = 0; t < MT; t++)
+          for (int m = 0; m < MT; m++) {
+            const T *row = x_row(x, a, lo + 16 * m + r < hi ? lo + 16 * m + r : hi - 1) + 8 * q;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
               const int k = full * 128 + 32 * i;
-              load_x8_end<T>(row[t] + k, cols - k - 8 * q, xf[0][t][i]);
+              load_x8_end<T>(row + k, cols - k - 8 * q, xf[m][i]);
             }
+          }
 #pragma unroll
-          for (int t = 0; t < NT; t++) multiply(0, t);
+          for (int t = 0; t < NT; t++) multiply(held[0], t);
         }
       }
       // the sums of a tile's wavefronts, in their order
@@ -536,14 +569,15 @@ __global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product
           const int token = i / (16 * NT), c = i % (16 * NT);
           const int64_t n = 16 * (int64_t)tile + c;
           if (n < a.m.out) {
-            const float *from = red + team * a.splits * (4 * NT * 64) + (4 * (c >> 4) + (token & 3)) * 64 +
-                                (token >> 2) * 16 + (c & 15);
-            float sum = 0.f;
-            for (int w = 0; w < a.splits; w++) sum += from[w * (4 * NT * 64)];
-            y[(lo + 16 * m + token) * a.ys + n] = (T)sum;
+            const float *at = red + team * a.splits * (4 * NT * 64) + (4 * (c >> 4) + (token & 3)) * 64 +
+                              (token >> 2) * 16 + (c & 15);
+            float total = 0.f;
+            for (int w = 0; w < a.splits; w++) total += at[w * (4 * NT * 64)];
+            y[(lo + 16 * m + token) * a.ys + n] = (T)total;
           }
         }
       }
+      if (a.splits > 1) __syncthreads();  // (before the corners are used again)
     }
   }
 }
@@ -613,7 +647,9 @@ static unsigned blocks_for(size_t items) { return (unsigned)((items + 255) / 256
 template <typename T>
 static int launch_product4(void (*kernel)(const T *, T *, Product4Args), int rows, int tile, const T *x, T *y,
                            Product4Args a, int waves, int splits, hipStream_t s) {
-  const size_t lds = TABLE_BYTES + (size_t)waves * 64 * (tile / 16) * (rows < 4 ? rows : 4) * sizeof(float);
+  const size_t sums = (size_t)waves * 64 * (tile / 16) * (rows < 4 ? rows : 4) * sizeof(float);
+  const size_t corners = rows >= 16 ? (size_t)waves * 256 * 8 * sizeof(T) : 0;
+  const size_t lds = TABLE_BYTES + (sums > corners ? sums : corners);
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
   a.splits = splits;
   const int teams = waves / splits;
@@ -644,16 +680,17 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
   // rows that a matrix has, about, and matrices (or workgroups along the rows of one)
   const int64_t shares = !src.offsets ? 1 : src.rows < src.experts ? src.rows : src.experts;
   const int64_t rows = (src.rows + shares - 1) / shares;
-  // Rows of y at a time, in 16s. x is read once for every 16 * NT columns of y, from an L2 that gives some
-  // 13 TB/s, so with many rows wide tiles pay: 64 x 8192 x 8192 takes 26 us with 2 x 4 tiles, 42 with 2 x 2, 37 with
-  // 4 x 2; 33 rows 25 with 3 x 2, 26 with 2 x 4, 32 with 2 x 2.
-  const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 ? 3 : 2;
+  const bool few = rows <= (src.offsets ? 2 : 4), two_bytes = dtype != H2O4GPU_EXPERTS_FLOAT32;
+  // Rows of y at a time, in 16s, and columns, in 16s. x is read once for every 16 * NT columns of y and a matrix
+  // once for every 16 * MT rows, so both are as large as there are registers for (a float takes twice as many, and
+  // so do four scales for 128 columns) while every CU has a workgroup. 33 x 8192 x 8192: 22 us with 3 x 2, 29 with
+  // 2 x 2, 33 with 1 x 2; 64 rows 23 with 2 x 4, 31 with 2 x 2, 38 with 3 x 2; 16 rows 14 with 1 x 2, 18 with 1 x 4,
+  // 21 with 1 x 1; 64 experts of 2048 x 4096 with four rows each 59 with 1 x 4, 97 with 1 x 2.
+  const int mt = rows <= 16 ? 1 : rows > 32 && rows <= 48 && two_bytes && m.per < 4 ? 3 : 2;
   const int64_t steps = src.offsets ? 1 : (src.rows + 16 * mt - 1) / (16 * mt);
-  // Columns of y at a time: as wide as leaves a workgroup for every CU (16 rows x 8192 x 8192: 15 us with 32, 20
-  // with 16, 18 with 64; 64 experts of 2048 x 4096: 53 us with 64, 80 with 32, 101 with 16).
   const int64_t all = tiles * shares * steps;
-  const bool few = rows <= (src.offsets ? 2 : 4);
-  const int nt = few ? 1 : all >= 1024 && mt < 3 && (mt == 1 || m.per < 4) ? 4 : all >= 512 ? 2 : 1;
+  const bool wide = two_bytes && (mt == 1 ? m.per < 4 : mt == 2 && m.per == 1);
+  const int nt = few ? 1 : all >= 1024 && wide ? 4 : all >= 512 && (two_bytes || mt == 1) ? 2 : 1;
   // Wavefronts that share a tile: as few as give every CU two workgroups of eight.
   const int waves = 8;
   int splits = 8;
@@ -679,15 +716,20 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
       if (few) return FEW(4);
       // (a float takes twice the registers: no more than 2 x 2)
       if constexpr (sizeof(T) == 2) {
-        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : nt == 2 ? MANY(1, 2, 2) : MANY(1, 4, 2);
-        if (mt == 3) return nt == 1 ? MANY(3, 1, 1) : MANY(3, 2, 1);
-        if (nt == 4)  // (four scales for 128 columns take too many registers here)
-          return launch_product4(m.per == 1 ? product4_kernel<T, S, 2, 4, 1, 1> : product4_kernel<T, S, 2, 4, 1, 2>, 32,
-                                 64, tx, ty, a, waves, splits, s);
-        return nt == 1 ? MANY(2, 1, 2) : MANY(2, 2, 1);
-      } else {
-        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : MANY(1, 2, 2);
+        if (mt == 3)
+          return nt == 1 ? launch_product4(m.per == 1 ? product4_kernel<T, S, 3, 1, 1, 1> : product4_kernel<T, S, 3, 1, 1, 2>,
+                                           48, 16, tx, ty, a, waves, splits, s)
+                         : launch_product4(m.per == 1 ? product4_kernel<T, S, 3, 2, 1, 1> : product4_kernel<T, S, 3, 2, 1, 2>,
+                                           48, 32, tx, ty, a, waves, splits, s);
+        if (nt == 4)
+          return mt == 1 ? launch_product4(m.per == 1 ? product4_kernel<T, S, 1, 4, 2, 1> : product4_kernel<T, S, 1, 4, 2, 2>,
+                                           16, 64, tx, ty, a, waves, splits, s)
+                         : launch_product4(product4_kernel<T, S, 2, 4, 1, 1>, 32, 64, tx, ty, a, waves, splits, s);
+        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : MANY(1, 2, 1);
         return nt == 1 ? MANY(2, 1, 1) : MANY(2, 2, 1);
+      } else {
+        if (mt == 1) return nt == 1 ? MANY(1, 1, 1) : MANY(1, 2, 1);
+        return MANY(2, 1, 1);
       }
 #undef FEW
 #undef MANY

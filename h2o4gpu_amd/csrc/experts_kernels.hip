@@ -594,11 +594,19 @@ typedef unsigned uintx4_u __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 struct Row {
   static constexpr int N = 16 / sizeof(T);
+  // ONCE: past the caches (see moves_once)
+  template <bool ONCE>
   static __device__ __forceinline__ uintx4 load(const T *row, int piece) {
-    return *reinterpret_cast<const uintx4_u *>(row + (int64_t)piece * N);
+    const uintx4_u *at = reinterpret_cast<const uintx4_u *>(row + (int64_t)piece * N);
+    return ONCE ? __builtin_nontemporal_load(at) : *at;
   }
+  template <bool ONCE>
   static __device__ __forceinline__ void store(T *row, int piece, uintx4 v) {
-    *reinterpret_cast<uintx4_u *>(row + (int64_t)piece * N) = v;
+    uintx4_u *at = reinterpret_cast<uintx4_u *>(row + (int64_t)piece * N);
+    if (ONCE)
+      __builtin_nontemporal_store((uintx4_u)v, at);
+    else
+      *at = v;
   }
   static __device__ __forceinline__ void unpack(uintx4 v, float (&f)[N]) {
     T e[N];
@@ -625,7 +633,7 @@ struct RowShare {
 };
 
 // dst[place(t, j)] = src[t], zeros where the slot has no expert. A row is read once for its top_k places.
-template <typename T, int U>
+template <typename T, int U, bool ONCE>
 __global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss, const int *position, RowShare a,
                                                         T *dst, int64_t ds) {
   constexpr int N = Row<T>::N;
@@ -637,13 +645,13 @@ __global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss
     uintx4 p[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (first + u * lanes < whole) p[u] = Row<T>::load(row, first + u * lanes);
+      if (first + u * lanes < whole) p[u] = Row<T>::template load<ONCE>(row, first + u * lanes);
     for (int j = 0; j < a.K; j++) {
       const int at = position[t * a.K + j];
       T *to = dst + (int64_t)(at < 0 ? ~at : at) * ds;
 #pragma unroll
       for (int u = 0; u < U; u++)
-        if (first + u * lanes < whole) Row<T>::store(to, first + u * lanes, at < 0 ? uintx4{0, 0, 0, 0} : p[u]);
+        if (first + u * lanes < whole) Row<T>::template store<false>(to, first + u * lanes, at < 0 ? uintx4{0, 0, 0, 0} : p[u]);
     }
     if (blockIdx.y == 0)
       for (int c = whole * N + lane; c < a.d; c += lanes) {
@@ -657,7 +665,7 @@ __global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss
 }
 
 // dst[t] = sum over j of (w[t][j] *) src[place(t, j)], j ascending; four rows of them on their way at a time.
-template <typename T, int U, bool WEIGHTED>
+template <typename T, int U, bool WEIGHTED, bool ONCE, bool PUT_ONCE>
 __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss, const float *w, const int *position,
                                                         RowShare a, T *dst, int64_t ds) {
   constexpr int N = Row<T>::N;
@@ -681,7 +689,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss
 #pragma unroll
           for (int u = 0; u < U; u++)
             if (at[j] >= 0 && i0 + u * lanes < whole)
-              p[j][u] = Row<T>::load(src + (int64_t)at[j] * ss, i0 + u * lanes);
+              p[j][u] = Row<T>::template load<ONCE>(src + (int64_t)at[j] * ss, i0 + u * lanes);
 #pragma unroll
         for (int j = 0; j < 4; j++)
           if (at[j] >= 0) {
@@ -696,7 +704,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss
       }
 #pragma unroll
       for (int u = 0; u < U; u++)
-        if (i0 + u * lanes < whole) Row<T>::store(dst + t * ds, i0 + u * lanes, Row<T>::pack(acc[u]));
+        if (i0 + u * lanes < whole) Row<T>::template store<PUT_ONCE>(dst + t * ds, i0 + u * lanes, Row<T>::pack(acc[u]));
     }
     if (blockIdx.y == 0)
       for (int c = whole * N + lane; c < a.d; c += lanes) {
@@ -714,7 +722,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss
 
 // Both gradients of the weighted sum in one pass over the rows: J of a token's places at a time. SPLIT: the
 // four wavefronts of a workgroup share a token's row, otherwise each has tokens of its own.
-template <typename T, int U, int J, bool SPLIT>
+template <typename T, int U, int J, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64_t os, const T *rows, int64_t rs,
                                                             const float *w, const int *position, RowShare a,
                                                             T *drows, int64_t drs, float *dw) {
@@ -738,12 +746,12 @@ __global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64
         uintx4 g[U], y[J][U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-          if (i0 + u * stride < whole) g[u] = Row<T>::load(g_row, i0 + u * stride);
+          if (i0 + u * stride < whole) g[u] = Row<T>::template load<ONCE>(g_row, i0 + u * stride);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
           for (int u = 0; u < U; u++)
-            if (at[j] >= 0 && i0 + u * stride < whole) y[j][u] = Row<T>::load(rows + (int64_t)at[j] * rs, i0 + u * stride);
+            if (at[j] >= 0 && i0 + u * stride < whole) y[j][u] = Row<T>::template load<ONCE>(rows + (int64_t)at[j] * rs, i0 + u * stride);
 #pragma unroll
         for (int u = 0; u < U; u++) {
           if (i0 + u * stride >= whole) break;
@@ -759,9 +767,9 @@ __global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64
                 dot[j] = fmaf(gv[e], yv[e], dot[j]);
                 out[e] = by[j] * gv[e];
               }
-              Row<T>::store(drows + (int64_t)at[j] * drs, i0 + u * stride, Row<T>::pack(out));
+              Row<T>::template store<false>(drows + (int64_t)at[j] * drs, i0 + u * stride, Row<T>::pack(out));
             } else if (j0 + j < a.K) {
-              Row<T>::store(drows + (int64_t)~at[j] * drs, i0 + u * stride, uintx4{0, 0, 0, 0});
+              Row<T>::template store<false>(drows + (int64_t)~at[j] * drs, i0 + u * stride, uintx4{0, 0, 0, 0});
             }
           }
         }
@@ -795,6 +803,16 @@ __global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64
       }
     }
   }
+}
+
+// Whether rows are read (and a joined row is written) past the caches: with more than the L2s hold they are not read
+// again before they have left them, and keeping them costs (16384 x 2048 bfloat16, four places: joined 57 us against
+// 94, sent 55 against 58, both gradients 106 against 111). Rows that are no whole cache lines share some with their
+// neighbours and are read better through the caches (100003 x 101 float: 46 us against 49, sent 45 against 53;
+// 200000 x 32 float16, eight places, both gradients: 63 us against 85).
+static bool moves_once(size_t rows, size_t cols, size_t elem) { return rows * cols * elem > (size_t)(32 << 20); }
+static bool whole_lines(const void *p, size_t stride, size_t elem) {
+  return aligned_to(p, 128) && stride * elem % 128 == 0;
 }
 
 // The share of rows of d elements of T, U pieces to a lane, and its grid.
@@ -981,9 +999,10 @@ KM_API int h2o4gpu_experts_dispatch(int dtype, size_t tokens, int top_k, size_t 
     typedef typename decltype(tag)::type T;
     dim3 grid;
     const RowShare a = share_rows<T>(tokens, top_k, cols, 4, &grid);
-    hipLaunchKernelGGL((send_rows_kernel<T, 4>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T *>(d_x), (int64_t)x_stride, d_position, a, static_cast<T *>(d_rows),
-                       (int64_t)rows_stride);
+    const bool once = moves_once(tokens * top_k, cols, sizeof(T)) && whole_lines(d_x, x_stride, sizeof(T));
+    hipLaunchKernelGGL((once ? send_rows_kernel<T, 4, true> : send_rows_kernel<T, 4, false>), grid, dim3(256), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const T *>(d_x), (int64_t)x_stride, d_position, a,
+                       static_cast<T *>(d_rows), (int64_t)rows_stride);
     return launched();
   });
 }
@@ -999,9 +1018,22 @@ static int join_rows(int dtype, size_t tokens, int top_k, size_t cols, const voi
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
     dim3 grid;
-    const RowShare a = share_rows<T>(tokens, top_k, cols, 2, &grid);
+    // short rows: a piece a lane (60000 x 515 bfloat16, three places: 61 us against 71 with two); long ones: four
+    // (16384 x 2048, four places: 81 against 85)
+    const bool short_rows = cols <= 128 * Row<T>::N;
+    const RowShare a = share_rows<T>(tokens, top_k, cols, short_rows ? 1 : 4, &grid);
     if (tokens >= 4096) grid.y = 1;  // (enough rows for every wavefront to have whole ones)
-    auto kernel = weighted ? join_rows_kernel<T, 2, true> : join_rows_kernel<T, 2, false>;
+    const bool put_once = moves_once(tokens * top_k, cols, sizeof(T));
+    const bool once = put_once && whole_lines(src, src_stride, sizeof(T));
+    const auto pick = [&](auto u, auto by_weight) {
+      constexpr int U = decltype(u)::value;
+      constexpr bool W = decltype(by_weight)::value != 0;
+      return once       ? join_rows_kernel<T, U, W, true, true>
+             : put_once ? join_rows_kernel<T, U, W, false, true>
+                        : join_rows_kernel<T, U, W, false, false>;
+    };
+    auto kernel = short_rows ? (weighted ? pick(Int<1>(), Int<1>()) : pick(Int<1>(), Int<0>()))
+                             : (weighted ? pick(Int<4>(), Int<1>()) : pick(Int<4>(), Int<0>()));
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(src),
                        (int64_t)src_stride, w, position, a, static_cast<T *>(dst), (int64_t)dst_stride);
     return launched();
@@ -1037,8 +1069,15 @@ KM_API int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k,
     dim3 grid;
     const RowShare a = share_rows<T>(tokens, top_k, cols, 2, &grid);
     const bool split = tokens < 1024 && grid.y > 1;  // few long rows
-    auto kernel = top_k <= 2 ? (split ? join_backward_kernel<T, 2, 2, true> : join_backward_kernel<T, 2, 2, false>)
-                             : (split ? join_backward_kernel<T, 2, 4, true> : join_backward_kernel<T, 2, 4, false>);
+    const bool once = moves_once(tokens * top_k, cols, sizeof(T)) && whole_lines(d_rows, rows_stride, sizeof(T)) &&
+                      whole_lines(d_dout, dout_stride, sizeof(T));
+    const auto pick = [&](auto j) {
+      constexpr int J = decltype(j)::value;
+      return split ? join_backward_kernel<T, 2, J, true, false>
+             : once ? join_backward_kernel<T, 2, J, false, true>
+                    : join_backward_kernel<T, 2, J, false, false>;
+    };
+    auto kernel = top_k <= 2 ? pick(Int<2>()) : pick(Int<4>());
     hipLaunchKernelGGL(kernel, dim3(split ? (unsigned)tokens : grid.x), dim3(256), 0,
                        static_cast<hipStream_t>(stream), static_cast<const T *>(d_dout), (int64_t)dout_stride,
                        static_cast<const T *>(d_rows), (int64_t)rows_stride, d_weights, d_position, a,

@@ -17,27 +17,27 @@ operation, and an ExpertOrder used on another stream than it was made on likewis
 the same bits. The kernels are the library's (include/h2o4gpu_experts.h); there is no CPU path.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from .libs import experts_hip
 
 _TYPES = {torch.float32: experts_hip.FLOAT32, torch.bfloat16: experts_hip.BFLOAT16,
           torch.float16: experts_hip.FLOAT16}
-_lib = None
+_functions = {}
+# (the raw handle directly where torch offers it: building a Stream object takes longer than queueing a kernel)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(device, name, *args):
-    """Calls a function of the library with `args` and the current stream of `device`."""
-    global _lib
-    if _lib is None:
-        _lib = experts_hip.lib()
-    fn = getattr(_lib, name)
-    index = device.index
+def _call(index, name, *args):
+    """Calls a function of the library with `args` and the current stream of device `index`."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(experts_hip.lib(), name)
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         experts_hip.check(name, rc)
 
@@ -75,7 +75,10 @@ def _rows(name, t):
 
 
 def _gradient(t):
-    """An incoming gradient with contiguous rows (autograd hands out expanded and transposed ones)."""
+    """An incoming gradient with contiguous rows (autograd hands out expanded and transposed ones). There
+    is no gradient of a gradient."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the gradients of expert layers cannot be differentiated again")
     if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
@@ -88,31 +91,32 @@ class _Route(torch.autograd.Function):
     def forward(ctx, scores, top_k, largest, scale, over_all):
         chosen, weights = _route(scores, top_k, largest, scale, over_all)
         ctx.mark_non_differentiable(chosen)
+        ctx.set_materialize_grads(False)  # (a tensor of zeros for the choice, otherwise)
         ctx.save_for_backward(scores, chosen, weights)
         ctx.how = (top_k, largest, scale, over_all)
         return chosen, weights
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _, dweights):
+        if dweights is None:
+            return None, None, None, None, None
         scores, chosen, weights = ctx.saved_tensors
         top_k, largest, scale, over_all = ctx.how
         dscores = torch.empty_like(scores)
-        dweights = dweights.contiguous()
-        _call(scores.device, "h2o4gpu_experts_route_backward", _TYPES[scores.dtype], scores.shape[0],
-              scores.shape[1], top_k, largest, over_all, scale, scores.data_ptr(), scores.stride(0),
-              scores.stride(1), chosen.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dscores.data_ptr(),
-              dscores.stride(0), dscores.stride(1))
+        dweights = _gradient(dweights).contiguous()
+        rows, n_experts = scores.shape
+        _call(scores.device.index, "h2o4gpu_experts_route_backward", _TYPES[scores.dtype], rows, n_experts, top_k,
+              largest, over_all, scale, scores.data_ptr(), *scores.stride(), chosen.data_ptr(), weights.data_ptr(),
+              dweights.data_ptr(), dscores.data_ptr(), *dscores.stride())
         return dscores, None, None, None, None
 
 
 def _route(scores, top_k, largest, scale, over_all):
-    rows = scores.shape[0]
-    chosen = torch.empty((rows, top_k), dtype=torch.int32, device=scores.device)
-    weights = torch.empty((rows, top_k), dtype=torch.float32, device=scores.device)
-    _call(scores.device, "h2o4gpu_experts_route", _TYPES[scores.dtype], rows, scores.shape[1], top_k, largest,
-          over_all, scale, scores.data_ptr(), scores.stride(0), scores.stride(1), chosen.data_ptr(),
-          weights.data_ptr())
+    rows, n_experts = scores.shape
+    chosen = scores.new_empty((rows, top_k), dtype=torch.int32)
+    weights = torch.empty_like(chosen, dtype=torch.float32)
+    _call(scores.device.index, "h2o4gpu_experts_route", _TYPES[scores.dtype], rows, n_experts, top_k, largest,
+          over_all, scale, scores.data_ptr(), *scores.stride(), chosen.data_ptr(), weights.data_ptr())
     return chosen, weights
 
 
@@ -173,13 +177,11 @@ def sort_by_expert(experts, n_experts):
         raise ValueError("experts must have 1 to %d choices a token, got %d" % (experts_hip.MAX_TOP_K,
                                                                                  experts.shape[1]))
     experts = experts.contiguous()
-    device, slots = experts.device, experts.numel()
-    order = torch.empty(slots, dtype=torch.int32, device=device)
-    position = torch.empty(experts.shape, dtype=torch.int32, device=device)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
+    slots = experts.numel()
+    order, position, offsets = experts.new_empty(slots), torch.empty_like(experts), experts.new_empty(n_experts + 1)
     need = experts_hip.lib().h2o4gpu_experts_sort_workspace(slots, n_experts)
-    work = torch.empty(need // 4, dtype=torch.int32, device=device) if need else None
-    _call(device, "h2o4gpu_experts_sort", slots, n_experts, experts.data_ptr(), order.data_ptr(),
+    work = experts.new_empty(need // 4) if need else None
+    _call(experts.device.index, "h2o4gpu_experts_sort", slots, n_experts, experts.data_ptr(), order.data_ptr(),
           position.data_ptr(), offsets.data_ptr(), work.data_ptr() if need else None, need)
     return ExpertOrder(order, position, offsets, n_experts)
 
@@ -194,10 +196,11 @@ def _order_of(order, device):
 # ---- rows out and back ---------------------------------------------------------------------------
 
 def _dispatch(x, order):
-    rows = torch.empty((order.tokens * order.top_k, x.shape[1]), dtype=x.dtype, device=x.device)
     ptr, stride = _rows("x", x)
-    _call(x.device, "h2o4gpu_experts_dispatch", _TYPES[x.dtype], order.tokens, order.top_k, x.shape[1], ptr,
-          stride, order.position.data_ptr(), rows.data_ptr(), x.shape[1])
+    cols = x.shape[1]
+    rows = x.new_empty((order.tokens * order.top_k, cols))
+    _call(x.device.index, "h2o4gpu_experts_dispatch", _TYPES[x.dtype], order.tokens, order.top_k, cols, ptr, stride,
+          order.position.data_ptr(), rows.data_ptr(), cols)
     return rows
 
 
@@ -208,14 +211,14 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, order)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, drows):
         order = ctx.order
         drows = _gradient(drows)
         ptr, stride = _rows("drows", drows)
-        dx = torch.empty((order.tokens, drows.shape[1]), dtype=drows.dtype, device=drows.device)
-        _call(drows.device, "h2o4gpu_experts_dispatch_backward", _TYPES[drows.dtype], order.tokens, order.top_k,
-              drows.shape[1], ptr, stride, order.position.data_ptr(), dx.data_ptr(), drows.shape[1])
+        cols = drows.shape[1]
+        dx = drows.new_empty((order.tokens, cols))
+        _call(drows.device.index, "h2o4gpu_experts_dispatch_backward", _TYPES[drows.dtype], order.tokens, order.top_k,
+              cols, ptr, stride, order.position.data_ptr(), dx.data_ptr(), cols)
         return dx, None
 
 
@@ -234,10 +237,11 @@ def dispatch(x, order):
 
 
 def _combine(rows, weights, order):
-    out = torch.empty((order.tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
     ptr, stride = _rows("rows", rows)
-    _call(rows.device, "h2o4gpu_experts_combine", _TYPES[rows.dtype], order.tokens, order.top_k, rows.shape[1],
-          ptr, stride, weights.data_ptr(), order.position.data_ptr(), out.data_ptr(), rows.shape[1])
+    cols = rows.shape[1]
+    out = rows.new_empty((order.tokens, cols))
+    _call(rows.device.index, "h2o4gpu_experts_combine", _TYPES[rows.dtype], order.tokens, order.top_k, cols, ptr,
+          stride, weights.data_ptr(), order.position.data_ptr(), out.data_ptr(), cols)
     return out
 
 
@@ -249,16 +253,14 @@ class _Combine(torch.autograd.Function):
         return _combine(rows, weights, order)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
         order = ctx.order
         rows, weights = ctx.saved_tensors
         dout = _gradient(dout)
         gptr, gstride = _rows("dout", dout)
         rptr, rstride = _rows("rows", rows)
-        drows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
-        dweights = torch.empty(weights.shape, dtype=torch.float32, device=rows.device)
-        _call(rows.device, "h2o4gpu_experts_combine_backward", _TYPES[rows.dtype], order.tokens, order.top_k,
+        drows, dweights = rows.new_empty(rows.shape), torch.empty_like(weights)
+        _call(rows.device.index, "h2o4gpu_experts_combine_backward", _TYPES[rows.dtype], order.tokens, order.top_k,
               rows.shape[1], gptr, gstride, rptr, rstride, weights.data_ptr(), order.position.data_ptr(),
               drows.data_ptr(), rows.shape[1], dweights.data_ptr())
         return drows, dweights, None
