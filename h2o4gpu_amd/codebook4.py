@@ -28,10 +28,11 @@ class Codebook4:
     multiple of 32. codebook: (16,) or (experts, 16) finite values in the type of the tokens.
 
     Codes and scales are copied once into the order that the products read them in (`laid_codes`,
-    `laid_scales`); those passed in are not needed afterwards.
+    `laid_scales`); those passed in are not needed afterwards. `dtype` is that of the tokens.
     """
 
-    __slots__ = ("laid_codes", "laid_scales", "codebook", "cols", "group", "out", "n_experts", "_args")
+    __slots__ = ("laid_codes", "laid_scales", "codebook", "cols", "group", "out", "n_experts", "dtype",
+                 "device", "_args")
 
     def __init__(self, codes, scales, codebook, cols, group):
         lead = codes.dim() - 2 if isinstance(codes, torch.Tensor) else 0
@@ -60,6 +61,7 @@ class Codebook4:
         codes, scales, device = codes.contiguous(), scales.contiguous(), codes.device.index
         self.codebook, self.cols, self.group, self.out = codebook.contiguous(), cols, group, codes.shape[-2]
         self.n_experts = codes.shape[0] if lead else 0
+        self.dtype, self.device = codebook.dtype, codes.device
         count, lib = max(1, self.n_experts), experts_hip.lib()
         kind = _TYPES[scales.dtype]
         nbytes = lib.h2o4gpu_codebook4_codes_bytes(count, self.out, cols)
@@ -89,11 +91,6 @@ class Codebook4:
         laid = laid.reshape(count, tiles * 16, subs * per)[:, :self.out]
         laid = laid[..., ::self.group * per // 128].contiguous()[..., :-(-self.cols // self.group)]
         return laid if self.n_experts else laid[0]
-
-    @property
-    def dtype(self):
-        """The type of the tokens that this matrix multiplies."""
-        return self.codebook.dtype
 
     def dequantize(self):
         """The matrix as a float32 tensor (for checks and for training on)."""
@@ -168,7 +165,8 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
 def _tokens(x, weights):
     if not isinstance(weights, Codebook4):
         raise TypeError("weights must be a Codebook4, got %s" % type(weights).__name__)
-    _tensor("x", x, 2, weights.laid_codes.device, weights.dtype)
+    if not (isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == weights.dtype and x.device == weights.device):
+        _tensor("x", x, 2, weights.device, weights.dtype)
     if x.shape[1] != weights.cols:
         raise ValueError("x must be (tokens, %d), got %s" % (weights.cols, tuple(x.shape)))
     if x.requires_grad and torch.is_grad_enabled():

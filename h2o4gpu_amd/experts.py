@@ -16,6 +16,8 @@ read on that stream: one that another stream writes has to be waited for, as wit
 operation, and an ExpertOrder used on another stream than it was made on likewise. Same inputs give
 the same bits. The kernels are the library's (include/h2o4gpu_experts.h); there is no CPU path.
 """
+import functools
+
 import torch
 
 from .libs import experts_hip
@@ -132,8 +134,9 @@ def route(scores, top_k, largest=True, scale=1.0, over_all=False):
     scale * score (scale * -score for distances) over the chosen experts, or with over_all over every
     available one. They have a gradient with respect to the scores, the choice held fixed.
     """
-    _tensor("scores", scores, 2)
-    _type_of("scores", scores)
+    if not (isinstance(scores, torch.Tensor) and scores.is_cuda and scores.dim() == 2 and scores.dtype in _TYPES):
+        _tensor("scores", scores, 2)
+        _type_of("scores", scores)
     top_k, largest, scale, over_all = int(top_k), int(bool(largest)), float(scale), int(bool(over_all))
     if not 1 <= scores.shape[1] <= experts_hip.MAX_EXPERTS:
         raise ValueError("scores must have 1 to %d experts, got %d" % (experts_hip.MAX_EXPERTS, scores.shape[1]))
@@ -164,6 +167,11 @@ class ExpertOrder:
         self.tokens, self.top_k = position.shape
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(slots, n_experts):
+    return experts_hip.lib().h2o4gpu_experts_sort_workspace(slots, n_experts)
+
+
 def sort_by_expert(experts, n_experts):
     """ExpertOrder of the (tokens, top_k) int32 choices of `route` (or of (tokens,) labels).
     A value that is none of 0 .. n_experts - 1 is a slot without an expert."""
@@ -179,7 +187,7 @@ def sort_by_expert(experts, n_experts):
     experts = experts.contiguous()
     slots = experts.numel()
     order, position, offsets = experts.new_empty(slots), torch.empty_like(experts), experts.new_empty(n_experts + 1)
-    need = experts_hip.lib().h2o4gpu_experts_sort_workspace(slots, n_experts)
+    need = _workspace(slots, n_experts)
     work = experts.new_empty(need // 4) if need else None
     _call(experts.device.index, "h2o4gpu_experts_sort", slots, n_experts, experts.data_ptr(), order.data_ptr(),
           position.data_ptr(), offsets.data_ptr(), work.data_ptr() if need else None, need)
@@ -226,8 +234,9 @@ def dispatch(x, order):
     """Rows in expert order, (tokens * top_k, cols): the token of every slot of `order`, zeros in the
     places behind offsets[-1]. x: (tokens, cols) with contiguous rows. Its gradient is the sum of a
     token's rows' gradients."""
-    _tensor("x", x, 2)
-    _type_of("x", x)
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.dtype in _TYPES):
+        _tensor("x", x, 2)
+        _type_of("x", x)
     _order_of(order, x.device)
     if x.shape[0] != order.tokens or x.shape[1] < 1:
         raise ValueError("x must be (%d, cols), got %s" % (order.tokens, tuple(x.shape)))
@@ -270,8 +279,9 @@ def combine(rows, weights, order):
     """(tokens, cols): the weighted sum of every token's rows, summed in float32 and rounded once.
     rows: (tokens * top_k, cols) in expert order; weights: (tokens, top_k) float32. Slots without an
     expert add nothing, whatever lies in their places. Gradients for rows and weights."""
-    _tensor("rows", rows, 2)
-    _type_of("rows", rows)
+    if not (isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _TYPES):
+        _tensor("rows", rows, 2)
+        _type_of("rows", rows)
     _order_of(order, rows.device)
     _tensor("weights", weights, 2, rows.device, torch.float32)
     if rows.shape[0] != order.tokens * order.top_k or rows.shape[1] < 1:
