@@ -597,14 +597,18 @@ __global__ __launch_bounds__(256) void layout4_codes_kernel(const uint8_t *codes
     const int64_t tile = (i >> 6) / subs, e = tile / tiles16, n = (tile % tiles16) * 16 + r;
     const uint8_t *row = codes + (e * out + n) * pitch;
     unsigned w[4] = {0, 0, 0, 0};
-    if (n < out)
-      for (int j = 0; j < 4; j++)
-        for (int b = 0; b < 4; b++) {
-          const int k = sub * 128 + 32 * j + 8 * q + 2 * b;
-          unsigned v = k < cols ? row[k / 2] : 0;
-          if (k + 1 >= cols) v &= 15;
-          w[j] |= v << (8 * b);
+    if (n < out) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int k0 = sub * 128 + 32 * j + 8 * q;
+        if (k0 + 8 <= cols) {
+          __builtin_memcpy(&w[j], row + k0 / 2, 4);
+        } else {
+          for (int b = 0; b < 4 && k0 + 2 * b < cols; b++)
+            w[j] |= (row[k0 / 2 + b] & (k0 + 2 * b + 1 < cols ? 255u : 15u)) << (8 * b);
         }
+      }
+    }
     to[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
