@@ -68,7 +68,7 @@ def main(argv=None):
         adam.zero_grad()
         loss.backward()
         adam.step()
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
         if not a.quiet and step % 10 == 0:
             print("step %d: loss %.4f" % (step, losses[-1]))
 

@@ -200,6 +200,6 @@ def experts_product(x, weights, order):
     y = x.new_empty((order.tokens * order.top_k, weights.out))
     _call(x.device.index, "h2o4gpu_codebook4_experts_product", _TYPES[x.dtype], order.tokens, order.top_k,
           weights.n_experts, weights.out, weights.cols, weights.group, ptr, stride, *weights._args,
-          16 if weights.codebook.dim() == 2 else 0, order.order.data_ptr(), order.offsets.data_ptr(), y.data_ptr(),
+          16 if weights.codebook.dim() == 2 else 0, order._order_ptr, order._offsets_ptr, y.data_ptr(),
           weights.out)
     return y

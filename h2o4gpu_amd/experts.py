@@ -152,19 +152,34 @@ def route(scores, top_k, largest=True, scale=1.0, over_all=False):
 # ---- order by expert ----------------------------------------------------------------------------
 
 class ExpertOrder:
-    """Slots ordered by expert; token t's j-th choice is slot t * top_k + j.
+    """Slots ordered by expert, as sort_by_expert makes it; token t's j-th choice is slot t * top_k + j.
 
     order (tokens * top_k,): the slots of expert 0, then of expert 1, ..., each in ascending order, then
     those without an expert. position (tokens, top_k): a slot's place in it, as ~place (negative) where
     it has no expert. offsets (n_experts + 1,): where each expert's rows begin; the last is how many
-    slots have one. All int32, on the GPU.
+    slots have one. All int32, on the GPU, in one allocation.
     """
 
-    __slots__ = ("order", "position", "offsets", "n_experts", "tokens", "top_k")
+    __slots__ = ("n_experts", "tokens", "top_k", "device", "_buffer", "_order_ptr", "_position_ptr", "_offsets_ptr")
 
-    def __init__(self, order, position, offsets, n_experts):
-        self.order, self.position, self.offsets, self.n_experts = order, position, offsets, n_experts
-        self.tokens, self.top_k = position.shape
+    def __init__(self, buffer, tokens, top_k, n_experts):
+        slots = tokens * top_k
+        self.n_experts, self.tokens, self.top_k, self.device, self._buffer = n_experts, tokens, top_k, buffer.device, buffer
+        self._order_ptr = buffer.data_ptr()
+        self._position_ptr = self._order_ptr + 4 * slots
+        self._offsets_ptr = self._position_ptr + 4 * slots
+
+    @property
+    def order(self):
+        return self._buffer.as_strided((self.tokens * self.top_k,), (1,), 0)
+
+    @property
+    def position(self):
+        return self._buffer.as_strided((self.tokens, self.top_k), (self.top_k, 1), self.tokens * self.top_k)
+
+    @property
+    def offsets(self):
+        return self._buffer.as_strided((self.n_experts + 1,), (1,), 2 * self.tokens * self.top_k)
 
 
 @functools.lru_cache(maxsize=256)
@@ -179,26 +194,26 @@ def sort_by_expert(experts, n_experts):
         experts = experts.unsqueeze(1)
     _tensor("experts", experts, 2, dtype=torch.int32)
     n_experts = int(n_experts)
+    tokens, top_k = experts.shape
     if not 1 <= n_experts <= experts_hip.MAX_EXPERTS:
         raise ValueError("n_experts must be 1 to %d, got %d" % (experts_hip.MAX_EXPERTS, n_experts))
-    if not 1 <= experts.shape[1] <= experts_hip.MAX_TOP_K:
-        raise ValueError("experts must have 1 to %d choices a token, got %d" % (experts_hip.MAX_TOP_K,
-                                                                                 experts.shape[1]))
+    if not 1 <= top_k <= experts_hip.MAX_TOP_K:
+        raise ValueError("experts must have 1 to %d choices a token, got %d" % (experts_hip.MAX_TOP_K, top_k))
     experts = experts.contiguous()
-    slots = experts.numel()
-    order, position, offsets = experts.new_empty(slots), torch.empty_like(experts), experts.new_empty(n_experts + 1)
+    slots = tokens * top_k
     need = _workspace(slots, n_experts)
     work = experts.new_empty(need // 4) if need else None
-    _call(experts.device.index, "h2o4gpu_experts_sort", slots, n_experts, experts.data_ptr(), order.data_ptr(),
-          position.data_ptr(), offsets.data_ptr(), work.data_ptr() if need else None, need)
-    return ExpertOrder(order, position, offsets, n_experts)
+    order = ExpertOrder(experts.new_empty(2 * slots + n_experts + 1), tokens, top_k, n_experts)
+    _call(order.device.index, "h2o4gpu_experts_sort", slots, n_experts, experts.data_ptr(), order._order_ptr,
+          order._position_ptr, order._offsets_ptr, work.data_ptr() if need else None, need)
+    return order
 
 
 def _order_of(order, device):
     if not isinstance(order, ExpertOrder):
         raise TypeError("order must be an ExpertOrder (sort_by_expert), got %s" % type(order).__name__)
-    if order.position.device != device:
-        raise ValueError("order is on %s, expected %s" % (order.position.device, device))
+    if order.device != device:
+        raise ValueError("order is on %s, expected %s" % (order.device, device))
 
 
 # ---- rows out and back ---------------------------------------------------------------------------
@@ -208,7 +223,7 @@ def _dispatch(x, order):
     cols = x.shape[1]
     rows = x.new_empty((order.tokens * order.top_k, cols))
     _call(x.device.index, "h2o4gpu_experts_dispatch", _TYPES[x.dtype], order.tokens, order.top_k, cols, ptr, stride,
-          order.position.data_ptr(), rows.data_ptr(), cols)
+          order._position_ptr, rows.data_ptr(), cols)
     return rows
 
 
@@ -226,7 +241,7 @@ class _Dispatch(torch.autograd.Function):
         cols = drows.shape[1]
         dx = drows.new_empty((order.tokens, cols))
         _call(drows.device.index, "h2o4gpu_experts_dispatch_backward", _TYPES[drows.dtype], order.tokens, order.top_k,
-              cols, ptr, stride, order.position.data_ptr(), dx.data_ptr(), cols)
+              cols, ptr, stride, order._position_ptr, dx.data_ptr(), cols)
         return dx, None
 
 
@@ -250,7 +265,7 @@ def _combine(rows, weights, order):
     cols = rows.shape[1]
     out = rows.new_empty((order.tokens, cols))
     _call(rows.device.index, "h2o4gpu_experts_combine", _TYPES[rows.dtype], order.tokens, order.top_k, cols, ptr,
-          stride, weights.data_ptr(), order.position.data_ptr(), out.data_ptr(), cols)
+          stride, weights.data_ptr(), order._position_ptr, out.data_ptr(), cols)
     return out
 
 
@@ -270,7 +285,7 @@ class _Combine(torch.autograd.Function):
         rptr, rstride = _rows("rows", rows)
         drows, dweights = rows.new_empty(rows.shape), torch.empty_like(weights)
         _call(rows.device.index, "h2o4gpu_experts_combine_backward", _TYPES[rows.dtype], order.tokens, order.top_k,
-              rows.shape[1], gptr, gstride, rptr, rstride, weights.data_ptr(), order.position.data_ptr(),
+              rows.shape[1], gptr, gstride, rptr, rstride, weights.data_ptr(), order._position_ptr,
               drows.data_ptr(), rows.shape[1], dweights.data_ptr())
         return drows, dweights, None
 
