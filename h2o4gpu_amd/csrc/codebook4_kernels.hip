@@ -672,6 +672,58 @@ static int launch_product4(void (*kernel)(const T *, T *, Product4Args), int row
   return launched();
 }
 
+// Rows of y that a workgroup has at a time and columns that a team of its eight wavefronts has, both in 16s, and
+// the wavefronts of a team, which share the columns of the matrix.
+struct Tiling4 {
+  int mt, nt, splits;
+};
+
+// As few wavefronts to a team as give every CU two workgroups (of `all` tiles of 16 x 16 * mt).
+static Tiling4 with_splits(int mt, int nt, int64_t all, int subs) {
+  int splits = 8;
+  while (splits > 1 && (splits / 2 >= subs || (all + nt - 1) / nt * (splits / 2) >= 4096)) splits /= 2;
+  return Tiling4{mt, nt, splits};
+}
+
+// With experts, whose rows are not known here. x is read once for every 16 * nt columns of y and a matrix once for
+// every 16 * mt rows, so both are as large as there are registers for (a float takes twice as many, and so do four
+// scales for 128 columns) while every CU has a workgroup. 64 experts of 2048 x 4096 with four rows each: 59 us with
+// 1 x 4, 97 with 1 x 2.
+static Tiling4 experts_tiling(int64_t rows, int64_t tiles, int subs, int per, bool two_bytes) {
+  const int mt = rows <= 16 ? 1 : rows > 32 && rows <= 48 && two_bytes && per < 4 ? 3 : 2;
+  const bool wide = two_bytes && (mt == 1 ? per < 4 : mt == 2 && per == 1);
+  const int nt = tiles >= 1024 && wide ? 4 : tiles >= 512 && (two_bytes || mt == 1) ? 2 : 1;
+  return with_splits(mt, nt, tiles, subs);
+}
+
+// Without: the least of what was found to describe the kernel's time, workgroups on 256 CUs in turns (a CU has
+// registers for one), each with a start and an end that take as long as 20 steps of 1 x 1, and a step of 128 columns
+// that takes one more for every tile and two for every 16 rows after the first. 8192 columns: 16 rows x 8192 take
+// 14.6 us with 1 x 2, 16.1 with 1 x 3, 18.5 with 1 x 4; x 11000, 24.9, 16.8 and 19.9. 33 rows x 8192: 21.6 with
+// 3 x 2, 29.9 with 2 x 2; x 11008, 38.1 with 3 x 2 and 32.8 with 2 x 3 and half the teams.
+static Tiling4 product_tiling(int64_t rows, int64_t tiles, int subs, int per, bool two_bytes) {
+  static const int halves[][3] = {{3, 2, 2}, {2, 4, 1}, {2, 3, 2}, {1, 4, 2}, {1, 3, 4}, {2, 2, 4}, {1, 2, 4}, {1, 1, 4}};
+  static const int floats[][3] = {{2, 1, 4}, {1, 2, 4}, {1, 1, 4}};
+  Tiling4 best{1, 1, 8};
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < (two_bytes ? 8 : 3); i++) {
+    const int *shape = two_bytes ? halves[i] : floats[i];
+    const int mt = shape[0], nt = shape[1];
+    if (per > shape[2] || (mt > 1 && rows <= 16 * (mt - 1))) continue;
+    const int64_t steps = (rows + 16 * mt - 1) / (16 * mt), wide = (tiles + nt - 1) / nt;
+    for (int splits = 8; splits >= 1; splits /= 2) {
+      if (splits > 1 && splits / 2 >= subs) continue;
+      const int64_t turns = ((wide + 8 / splits - 1) / (8 / splits) * steps + 255) / 256;
+      const int64_t time = turns * (20 + (int64_t)((subs + splits - 1) / splits) * (nt + 2 * (mt - 1)));
+      if (time < least) {
+        least = time;
+        best = Tiling4{mt, nt, splits};
+      }
+    }
+  }
+  return best;
+}
+
 static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m, int scale_dtype,
                     const RowSource &src, void *y, size_t y_stride, hipStream_t s) {
   Product4Args a;
@@ -688,21 +740,11 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
   // Few rows: the kernel that loads x least. Experts' rows are not spread evenly, and where there are tiles for
   // every wavefront wide ones are better still (64 experts of 2048 x 4096, 128 rows: 53 us against 82; 16 rows: 18
   // against 15).
-  const bool few = src.offsets ? rows <= 2 && tiles * shares < 4096 : rows <= 4;
-  // Rows of y at a time, in 16s, and columns, in 16s. x is read once for every 16 * NT columns of y and a matrix
-  // once for every 16 * MT rows, so both are as large as there are registers for (a float takes twice as many, and
-  // so do four scales for 128 columns) while every CU has a workgroup. 33 x 8192 x 8192: 22 us with 3 x 2, 29 with
-  // 2 x 2, 33 with 1 x 2; 64 rows 23 with 2 x 4, 31 with 2 x 2, 38 with 3 x 2; 16 rows 14 with 1 x 2, 18 with 1 x 4,
-  // 21 with 1 x 1; 64 experts of 2048 x 4096 with four rows each 59 with 1 x 4, 97 with 1 x 2.
-  const int mt = rows <= 16 ? 1 : rows > 32 && rows <= 48 && two_bytes && m.per < 4 ? 3 : 2;
-  const int64_t steps = src.offsets ? 1 : (src.rows + 16 * mt - 1) / (16 * mt);
-  const int64_t all = tiles * shares * steps;
-  const bool wide = two_bytes && (mt == 1 ? m.per < 4 : mt == 2 && m.per == 1);
-  const int nt = few ? 1 : all >= 1024 && wide ? 4 : all >= 512 && (two_bytes || mt == 1) ? 2 : 1;
-  // Wavefronts that share a tile: as few as give every CU two workgroups of eight.
-  const int waves = 8;
-  int splits = 8;
-  while (splits > 1 && (splits / 2 >= subs || (all + nt - 1) / nt * (splits / 2) >= 4096)) splits /= 2;
+  const bool few = src.rows == 1 || (src.offsets ? rows <= 2 && tiles * shares < 4096 : rows <= 4);
+  const Tiling4 t = few           ? with_splits(1, 1, tiles * shares, subs)
+                    : src.offsets ? experts_tiling(rows, tiles * shares, subs, m.per, two_bytes)
+                                  : product_tiling(src.rows, tiles, subs, m.per, two_bytes);
+  const int waves = 8, mt = t.mt, nt = t.nt, splits = t.splits;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
     const T *tx = static_cast<const T *>(x);
@@ -714,33 +756,30 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
                   : m.per == 2 ? product4_few_kernel<T, S, MP, 2>                                            \
                                : product4_few_kernel<T, S, MP, 4>,                                           \
                   MP, 16, tx, ty, a, waves, splits, s)
+#define MOST2(MT, NT, R)                                                                                     \
+  launch_product4(m.per == 1 ? product4_kernel<T, S, MT, NT, R, 1> : product4_kernel<T, S, MT, NT, R, 2>,    \
+                  16 * MT, 16 * NT, tx, ty, a, waves, splits, s)
 #define MANY(MT, NT, R)                                                                                      \
   launch_product4(m.per == 1   ? product4_kernel<T, S, MT, NT, R, 1>                                         \
                   : m.per == 2 ? product4_kernel<T, S, MT, NT, R, 2>                                         \
                                : product4_kernel<T, S, MT, NT, R, 4>,                                        \
                   16 * MT, 16 * NT, tx, ty, a, waves, splits, s)
-      // PROBE HERE
       if (src.rows == 1) return FEW(1);
       if (few) return FEW(4);
-      // (a float takes twice the registers: no more than 2 x 2)
+      // (a shape that was not chosen for four scales has no kernel for them, nor 2 x 4 for two)
       if constexpr (sizeof(T) == 2) {
-        if (mt == 3)
-          return nt == 1 ? launch_product4(m.per == 1 ? product4_kernel<T, S, 3, 1, 1, 1> : product4_kernel<T, S, 3, 1, 1, 2>,
-                                           48, 16, tx, ty, a, waves, splits, s)
-                         : launch_product4(m.per == 1 ? product4_kernel<T, S, 3, 2, 1, 1> : product4_kernel<T, S, 3, 2, 1, 2>,
-                                           48, 32, tx, ty, a, waves, splits, s);
-        if (nt == 4)
-          return mt == 1 ? launch_product4(m.per == 1 ? product4_kernel<T, S, 1, 4, 2, 1> : product4_kernel<T, S, 1, 4, 2, 2>,
-                                           16, 64, tx, ty, a, waves, splits, s)
-                         : launch_product4(product4_kernel<T, S, 2, 4, 1, 1>, 32, 64, tx, ty, a, waves, splits, s);
-        if (mt == 1) return nt == 1 ? MANY(1, 1, 2) : MANY(1, 2, 1);
-        return nt == 1 ? MANY(2, 1, 1) : MANY(2, 2, 1);
+        if (mt == 3) return nt == 1 ? MOST2(3, 1, 1) : MOST2(3, 2, 1);
+        if (mt == 2 && nt == 4)
+          return launch_product4(product4_kernel<T, S, 2, 4, 1, 1>, 32, 64, tx, ty, a, waves, splits, s);
+        if (mt == 2) return nt == 1 ? MANY(2, 1, 1) : nt == 2 ? MANY(2, 2, 1) : MOST2(2, 3, 1);
+        return nt == 1 ? MANY(1, 1, 2) : nt == 2 ? MANY(1, 2, 1) : nt == 3 ? MANY(1, 3, 1) : MOST2(1, 4, 2);
       } else {
-        if (mt == 1) return nt == 1 ? MANY(1, 1, 1) : MANY(1, 2, 1);
-        return MANY(2, 1, 1);
+        if (mt == 2) return MANY(2, 1, 1);
+        return nt == 1 ? MANY(1, 1, 1) : MANY(1, 2, 1);
       }
 #undef FEW
 #undef MANY
+#undef MOST2
     });
   });
 }
