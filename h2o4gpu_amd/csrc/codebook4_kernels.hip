@@ -197,7 +197,7 @@ __device__ __forceinline__ Share share_of(const Product4Args &a, int *found, T *
   if (!a.src.offsets) return s;
   const int E = a.src.experts;
   if (blockIdx.y == gridDim.y - 1) {
-    for (int64_t p = a.src.offsets[E] + blockIdx.x; p < s.hi; p += gridDim.x)
+    for (int64_t p = a.src.offsets[E] + blockIdx.z * gridDim.x + blockIdx.x; p < s.hi; p += gridDim.x * gridDim.z)
       for (int64_t n = threadIdx.x; n < a.m.out; n += blockDim.x) y[p * a.ys + n] = (T)0.f;
     s.hi = 0;
     return s;
@@ -421,10 +421,11 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 4 : 2) void product4_few_kern
 
 // 16 * MT rows of y at a time, a row of x in each of a product's 16. Rows of x behind the last one are read from
 // the last: their results are not written.
-// A product wants 8 columns of 16 different rows from 16 neighbouring lanes. Loaded like that, x costs an access
-// to the cache for every lane (58 for a load, and they are what bounds 33 x 8192 x 8192 at 26 us); so 16 lanes
-// load 128 columns of one row, and a wavefront's own 16 x 128 corner of LDS turns them. Piece c of row r lies at
-// place c ^ r of its row there, so that 16 rows' pieces c lie in different banks.
+// A product wants 8 columns of 16 different rows from 16 neighbouring lanes. x is not loaded like that: 16 lanes load
+// 128 columns of one row, and a wavefront's own 16 x 128 corner of LDS turns them (33 x 8192 x 8192: 25.4 -> 21.8
+// us). Piece c of row r lies at place c ^ r of its row there, so that 16 rows' pieces c lie in different banks.
+// What bounds it at that size: every workgroup reads all of x, from L2; without these loads 16.5 us, with the loads
+// and without the turn 20.1, and a step's x on its way a step earlier 21.7. 16 x 8192 x 8192: 14.6 us, 64: 23.7.
 template <typename T, typename S, int MT, int NT, int R, int PER>
 __global__ __launch_bounds__(512) void product4_kernel(const T *x, T *y, Product4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -647,10 +648,11 @@ static size_t subs_of(size_t cols) { return (cols + 127) / 128; }
 static int scales_per_sub(int group) { return group % 128 == 0 ? 1 : group % 64 == 0 ? 2 : 4; }
 static unsigned blocks_for(size_t items) { return (unsigned)((items + 255) / 256 < 65536 ? (items + 255) / 256 : 65536); }
 
-// rows: of y that a workgroup has at a time, tile: columns of y a team of wavefronts has.
+// rows: of y that a workgroup has at a time, tile: columns of y a team of wavefronts has, share_rows: rows of y
+// that a matrix has, about.
 template <typename T>
 static int launch_product4(void (*kernel)(const T *, T *, Product4Args), int rows, int tile, const T *x, T *y,
-                           Product4Args a, int waves, int splits, hipStream_t s) {
+                           Product4Args a, int64_t share_rows, int waves, int splits, hipStream_t s) {
   const size_t sums = (size_t)waves * 64 * (tile / 16) * (rows < 4 ? rows : 4) * sizeof(float);
   const size_t corners = rows >= 16 ? (size_t)waves * 256 * 8 * sizeof(T) : 0;
   const size_t lds = TABLE_BYTES + (sums > corners ? sums : corners);
@@ -658,13 +660,10 @@ static int launch_product4(void (*kernel)(const T *, T *, Product4Args), int row
   a.splits = splits;
   const int teams = waves / splits;
   const unsigned tiles = (unsigned)((a.m.out + tile - 1) / tile);
-  unsigned gx = (tiles + teams - 1) / teams, gy = 1, gz = 1;
-  if (a.src.offsets) {
-    gy = (unsigned)(a.src.rows < a.src.experts ? a.src.rows : a.src.experts) + 1;
-  } else {
-    const int64_t steps = (a.src.rows + rows - 1) / rows;
-    gz = (unsigned)(steps < 256 ? steps : 256);
-  }
+  unsigned gx = (tiles + teams - 1) / teams;
+  const unsigned gy = a.src.offsets ? (unsigned)(a.src.rows < a.src.experts ? a.src.rows : a.src.experts) + 1 : 1;
+  const int64_t steps = (share_rows + rows - 1) / rows;
+  const unsigned gz = (unsigned)(steps < 256 ? steps : 256);
   // no more workgroups than run at once, twice over: one that has several tiles makes its table once
   const unsigned most = 1024 / (gy * gz) > 0 ? 1024 / (gy * gz) : 1;
   if (gx > most) gx = most;
@@ -685,24 +684,28 @@ static Tiling4 with_splits(int mt, int nt, int64_t all, int subs) {
   return Tiling4{mt, nt, splits};
 }
 
-// With experts, whose rows are not known here. x is read once for every 16 * nt columns of y and a matrix once for
-// every 16 * mt rows, so both are as large as there are registers for (a float takes twice as many, and so do four
-// scales for 128 columns) while every CU has a workgroup. 64 experts of 2048 x 4096 with four rows each: 59 us with
-// 1 x 4, 97 with 1 x 2.
+// Many experts, whose rows are not known here: with this many tiles, counting turns by their average is worse (64
+// experts of 2048 x 4096 with four rows each: 84 us; with 32 rows 206 against 190; 16 of 3000 x 3000 in float with
+// six rows 74 against 67), with fewer it is better (8 experts of 3000 x 4096 with four rows: 18 against 26, with 32
+// rows 35 against 44). x is read once for every 16 * nt columns of y and a matrix once for every 16 * mt rows, so both
+// are as large as there are registers for (a float takes twice as many, and so do four scales for 128 columns).
+// 64 experts of 2048 x 4096 with four rows each: 59 us with 1 x 4, 97 with 1 x 2.
 static Tiling4 experts_tiling(int64_t rows, int64_t tiles, int subs, int per, bool two_bytes) {
-  const int mt = rows <= 16 ? 1 : rows > 32 && rows <= 48 && two_bytes && per < 4 ? 3 : 2;
-  const bool wide = two_bytes && (mt == 1 ? per < 4 : mt == 2 && per == 1);
-  const int nt = tiles >= 1024 && wide ? 4 : tiles >= 512 && (two_bytes || mt == 1) ? 2 : 1;
-  return with_splits(mt, nt, tiles, subs);
+  if (rows <= 16) return with_splits(1, two_bytes && per < 4 ? 4 : 2, tiles, subs);
+  // (640 tokens, four choices: 224 us with 2 x 4, 244 with 3 x 2; groups of 64: 246 with 2 x 3, 227 with 3 x 2)
+  if (two_bytes && per == 2 && rows > 32 && rows <= 48) return with_splits(3, 2, tiles, subs);
+  return with_splits(2, !two_bytes ? 1 : per == 1 ? 4 : per == 2 ? 3 : 2, tiles, subs);
 }
 
-// Without: the least of what was found to describe the kernel's time, workgroups on 256 CUs in turns (a CU has
-// registers for one), each with a start and an end that take as long as 20 steps of 1 x 1, and a step of 128 columns
-// that takes one more for every tile and two for every 16 rows after the first. 8192 columns: 16 rows x 8192 take
+// A matrix, or a few: the least of what was found to describe the kernel's time, workgroups on 256 CUs in turns (a
+// CU has registers for one), each with a start and an end that take as long as 20 steps of 1 x 1, and a step of 128
+// columns that takes one more for every tile and two for every 16 rows after the first. 8192 columns: 16 rows x 8192 take
 // 14.6 us with 1 x 2, 16.1 with 1 x 3, 18.5 with 1 x 4; x 11000, 24.9, 16.8 and 19.9. 33 rows x 8192: 21.6 with
 // 3 x 2, 29.9 with 2 x 2; x 11008, 38.1 with 3 x 2 and 32.8 with 2 x 3 and half the teams.
-static Tiling4 product_tiling(int64_t rows, int64_t tiles, int subs, int per, bool two_bytes) {
-  static const int halves[][3] = {{3, 2, 2}, {2, 4, 1}, {2, 3, 2}, {1, 4, 2}, {1, 3, 4}, {2, 2, 4}, {1, 2, 4}, {1, 1, 4}};
+static Tiling4 product_tiling(int64_t rows, int64_t tiles, int64_t shares, int subs, int per, bool two_bytes) {
+  // mt, nt, and for how many scales of 128 columns there are registers
+  static const int halves[][3] = {{3, 2, 2}, {2, 4, 1}, {2, 3, 2}, {1, 4, 2},
+                                  {1, 3, 4}, {2, 2, 4}, {1, 2, 4}, {1, 1, 4}};
   static const int floats[][3] = {{2, 1, 4}, {1, 2, 4}, {1, 1, 4}};
   Tiling4 best{1, 1, 8};
   int64_t least = INT64_MAX;
@@ -713,7 +716,7 @@ static Tiling4 product_tiling(int64_t rows, int64_t tiles, int subs, int per, bo
     const int64_t steps = (rows + 16 * mt - 1) / (16 * mt), wide = (tiles + nt - 1) / nt;
     for (int splits = 8; splits >= 1; splits /= 2) {
       if (splits > 1 && splits / 2 >= subs) continue;
-      const int64_t turns = ((wide + 8 / splits - 1) / (8 / splits) * steps + 255) / 256;
+      const int64_t turns = ((wide + 8 / splits - 1) / (8 / splits) * steps * shares + 255) / 256;
       const int64_t time = turns * (20 + (int64_t)((subs + splits - 1) / splits) * (nt + 2 * (mt - 1)));
       if (time < least) {
         least = time;
@@ -733,7 +736,7 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
   a.ys = (int64_t)y_stride;
   const int subs = (int)subs_of(m.cols);
   const int64_t tiles = (int64_t)tiles_of(m.out);
-  // rows that a matrix has, about, and matrices (or workgroups along the rows of one)
+  // rows that a matrix has, about, and matrices (or workgroups for a row each)
   const int64_t shares = !src.offsets ? 1 : src.rows < src.experts ? src.rows : src.experts;
   const int64_t rows = (src.rows + shares - 1) / shares;
   const bool two_bytes = dtype != H2O4GPU_EXPERTS_FLOAT32;
@@ -741,9 +744,10 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
   // every wavefront wide ones are better still (64 experts of 2048 x 4096, 128 rows: 53 us against 82; 16 rows: 18
   // against 15).
   const bool few = src.rows == 1 || (src.offsets ? rows <= 2 && tiles * shares < 4096 : rows <= 4);
-  const Tiling4 t = few           ? with_splits(1, 1, tiles * shares, subs)
-                    : src.offsets ? experts_tiling(rows, tiles * shares, subs, m.per, two_bytes)
-                                  : product_tiling(src.rows, tiles, subs, m.per, two_bytes);
+  const Tiling4 t = few ? with_splits(1, 1, tiles * shares, subs)
+                    : src.offsets && tiles * shares >= (two_bytes ? 4096 : 1024)
+                        ? experts_tiling(rows, tiles * shares, subs, m.per, two_bytes)
+                        : product_tiling(rows, tiles, shares, subs, m.per, two_bytes);
   const int waves = 8, mt = t.mt, nt = t.nt, splits = t.splits;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
@@ -755,23 +759,23 @@ static int product4(int dtype, const void *x, size_t x_stride, const Matrix4 &m,
   launch_product4(m.per == 1   ? product4_few_kernel<T, S, MP, 1>                                            \
                   : m.per == 2 ? product4_few_kernel<T, S, MP, 2>                                            \
                                : product4_few_kernel<T, S, MP, 4>,                                           \
-                  MP, 16, tx, ty, a, waves, splits, s)
+                  MP, 16, tx, ty, a, rows, waves, splits, s)
 #define MOST2(MT, NT, R)                                                                                     \
   launch_product4(m.per == 1 ? product4_kernel<T, S, MT, NT, R, 1> : product4_kernel<T, S, MT, NT, R, 2>,    \
-                  16 * MT, 16 * NT, tx, ty, a, waves, splits, s)
+                  16 * MT, 16 * NT, tx, ty, a, rows, waves, splits, s)
 #define MANY(MT, NT, R)                                                                                      \
   launch_product4(m.per == 1   ? product4_kernel<T, S, MT, NT, R, 1>                                         \
                   : m.per == 2 ? product4_kernel<T, S, MT, NT, R, 2>                                         \
                                : product4_kernel<T, S, MT, NT, R, 4>,                                        \
-                  16 * MT, 16 * NT, tx, ty, a, waves, splits, s)
+                  16 * MT, 16 * NT, tx, ty, a, rows, waves, splits, s)
       if (src.rows == 1) return FEW(1);
       if (few) return FEW(4);
-      // (a shape that was not chosen for four scales has no kernel for them, nor 2 x 4 for two)
+      // (a shape that is not chosen for four scales has no kernel for them, nor 2 x 4 for two)
       if constexpr (sizeof(T) == 2) {
-        if (mt == 3) return nt == 1 ? MOST2(3, 1, 1) : MOST2(3, 2, 1);
+        if (mt == 3) return MOST2(3, 2, 1);
         if (mt == 2 && nt == 4)
-          return launch_product4(product4_kernel<T, S, 2, 4, 1, 1>, 32, 64, tx, ty, a, waves, splits, s);
-        if (mt == 2) return nt == 1 ? MANY(2, 1, 1) : nt == 2 ? MANY(2, 2, 1) : MOST2(2, 3, 1);
+          return launch_product4(product4_kernel<T, S, 2, 4, 1, 1>, 32, 64, tx, ty, a, rows, waves, splits, s);
+        if (mt == 2) return nt == 2 ? MANY(2, 2, 1) : MOST2(2, 3, 1);
         return nt == 1 ? MANY(1, 1, 2) : nt == 2 ? MANY(1, 2, 1) : nt == 3 ? MANY(1, 3, 1) : MOST2(1, 4, 2);
       } else {
         if (mt == 2) return MANY(2, 1, 1);
