@@ -131,8 +131,8 @@ __device__ __forceinline__ float sum_of(float v) {
 
 // Rows whose scores lie side by side, at most LANES * NV of them: LANES lanes have a row in registers, W scores in
 // a row each at a time. Every round takes the best that is left (a lane's own best, then across the lanes) and
-// strikes it out. Lane j ends with choice j. 16384 rows of 256 bfloat16, eight chosen of all: 10 us (40 with
-// the kernel above).
+// strikes it out. Lane j ends with choice j. What bounds it is the rounds' comparisons: 16384 rows of 256 bfloat16,
+// eight chosen of all, take 14 us (40 with the kernel above), reading them 2. 64000 x 1000 floats, eight: 167.
 template <typename T, bool ALL, int LANES, int NV>
 __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_t rs, int64_t rows, int E, int K,
                                                          bool largest, float scale, int *experts, float *weights) {
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_
 // Scores of one expert side by side (row stride 1, the distances of transform): a lane has a row and walks down
 // its experts with its best KT in order. The wavefronts of a workgroup each walk a stretch of
 // the experts, and the first joins their lists (a later stretch's equal score stays behind). 1M rows x 64, two
-// chosen: 60 us.
+// chosen: 51 us, 5.3 TB/s, what a copy reaches.
 template <typename T, bool ALL, int KT>
 __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, int64_t es, int64_t rows, int E, int K,
                                                              bool largest, float scale, int *experts, float *weights) {
@@ -289,7 +289,8 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
 }
 
 // One wavefront a row, any strides: inner = sum of w g over the chosen, then every expert's gradient, in LDS 1024 at
-// a time where the chosen ones' are put in their places.
+// a time where the chosen ones' are put in their places. 16384 x 256 bfloat16: 11 us, the writes alone 2; 64000 x
+// 1000 floats: 140.
 template <typename T, bool ALL>
 __global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, int64_t rs, int64_t es, int64_t rows,
                                                              int E, int K, bool largest, float scale,
@@ -422,7 +423,8 @@ __global__ __launch_bounds__(256) void route_backward_columns_kernel(const T *sc
 
 // A workgroup of up to 8 wavefronts has a chunk of slots, each wavefront a stretch of it, 64 slots at a time and at
 // most SORT_STEPS times. Two slots of a wavefront find that they name the same expert by comparing a bit of
-// all 64 numbers at a time, so that no order depends on when an addition happens.
+// all 64 numbers at a time, so that no order depends on when an addition happens. 16384 x 4 slots of 64 experts: 4 us
+// to count and 7 to place; 100003 x 3 of 1000: 5, 5 to add up and 9 to place; 32 slots: 3, one launch.
 static const int SORT_STEPS = 4, SORT_WAVES = 8;
 static const size_t SORT_LDS = 150u << 10;
 
@@ -632,7 +634,8 @@ struct RowShare {
   int K, d, lanes_log2;
 };
 
-// dst[place(t, j)] = src[t], zeros where the slot has no expert. A row is read once for its top_k places.
+// dst[place(t, j)] = src[t], zeros where the slot has no expert. A row is read once for its top_k places. Memory
+// bounds it: 16384 x 2048 bfloat16, four places, 54 us, 6.2 TB/s, mostly writes.
 template <typename T, int U, bool ONCE>
 __global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss, const int *position, RowShare a,
                                                         T *dst, int64_t ds) {
@@ -665,6 +668,7 @@ __global__ __launch_bounds__(256) void send_rows_kernel(const T *src, int64_t ss
 }
 
 // dst[t] = sum over j of (w[t][j] *) src[place(t, j)], j ascending; four rows of them on their way at a time.
+// Memory bounds it: 16384 x 2048 bfloat16, four places, 57 us, 5.9 TB/s.
 template <typename T, int U, bool WEIGHTED, bool ONCE, bool PUT_ONCE>
 __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss, const float *w, const int *position,
                                                         RowShare a, T *dst, int64_t ds) {
@@ -721,7 +725,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const T *src, int64_t ss
 }
 
 // Both gradients of the weighted sum in one pass over the rows: J of a token's places at a time. SPLIT: the
-// four wavefronts of a workgroup share a token's row, otherwise each has tokens of its own.
+// four wavefronts of a workgroup share a token's row, otherwise each has tokens of its own. 16384 x 2048 bfloat16,
+// four places: 94 us, 6.4 TB/s.
 template <typename T, int U, int J, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(256) void join_backward_kernel(const T *dout, int64_t os, const T *rows, int64_t rs,
                                                             const float *w, const int *position, RowShare a,

@@ -88,11 +88,59 @@ def _quantize():
             for data in ("normal", "zeros", "huge", "nan")]
 
 
+# (rows, out, cols, group): together every shape that a product's tiles take, with teams of one to eight wavefronts.
+PRODUCTS = (
+    (10, 259, 258, 128), (5, 268, 517, 128), (15, 258, 518, 64), (6, 264, 525, 32), (336, 1548, 37, 128),
+    (401, 625, 155, 128), (230, 276, 513, 128), (373, 1309, 55, 64), (379, 321, 259, 64),
+    (243, 261, 518, 64), (472, 1039, 37, 32), (293, 419, 270, 32), (211, 303, 517, 32),
+    (463, 2115, 83, 128), (401, 1183, 130, 128), (369, 333, 515, 128), (474, 2110, 46, 64),
+    (475, 544, 277, 64), (305, 390, 524, 64), (405, 2320, 42, 32), (453, 515, 336, 32), (470, 264, 517, 32),
+    (401, 2590, 38, 128), (455, 527, 279, 128), (425, 2331, 36, 64), (465, 1028, 171, 64),
+    (353, 1418, 131, 32), (456, 3276, 40, 128), (398, 1924, 139, 128), (405, 439, 787, 128),
+    (451, 3171, 34, 64), (468, 780, 409, 64), (411, 449, 780, 64), (313, 6155, 43, 128),
+    (338, 1424, 284, 128), (408, 596, 518, 128), (473, 4173, 41, 64), (452, 2084, 206, 64),
+    (469, 517, 536, 64), (451, 3081, 64, 32), (414, 1846, 142, 32), (382, 665, 519, 32),
+    (436, 4609, 34, 128), (408, 2554, 134, 128), (413, 615, 561, 128), (327, 6305, 35, 64),
+    (500, 1049, 261, 64), (370, 677, 547, 64), (400, 7545, 47, 128), (404, 1957, 284, 128),
+    (393, 949, 680, 128), (331, 9143, 130, 128), (178, 8083, 158, 128), (428, 871, 747, 128),
+    (419, 6915, 359, 64), (367, 2038, 281, 64), (417, 867, 730, 64),
+)
+
+# (tokens, top_k, experts, out, cols, group): the same, and the last ones with more tiles than are counted.
+EXPERTS_PRODUCTS = (
+    (8, 1, 2, 266, 533, 128), (9, 1, 2, 259, 298, 32), (270, 1, 2, 277, 527, 128), (301, 2, 3, 815, 33, 64),
+    (129, 3, 2, 318, 281, 32), (437, 1, 3, 270, 713, 128), (280, 3, 2, 1033, 49, 64),
+    (225, 3, 2, 340, 331, 32), (196, 3, 2, 270, 530, 128), (193, 3, 2, 403, 283, 32),
+    (162, 3, 2, 409, 806, 128), (412, 2, 2, 1575, 38, 64), (425, 2, 2, 280, 578, 128),
+    (358, 3, 2, 1627, 67, 64), (280, 3, 2, 428, 419, 32), (251, 3, 2, 381, 564, 128),
+    (424, 3, 3, 1671, 50, 64), (458, 3, 3, 260, 535, 128), (399, 2, 3, 447, 765, 128),
+    (485, 2, 3, 3000, 47, 64), (300, 3, 100, 700, 130, 128), (310, 2, 200, 350, 300, 64),
+    (500, 2, 25, 2640, 200, 64), (400, 2, 40, 1700, 260, 64), (600, 3, 70, 1000, 130, 128),
+    (600, 3, 70, 1000, 264, 32), (700, 1, 100, 690, 33, 32), (300, 2, 300, 230, 70, 64),
+)
+
+
+def _shapes():
+    out = []
+    for rows, n, cols, group in PRODUCTS:
+        for dtype in TYPES:
+            out.append(dict(op="product", rows=rows, out=n, cols=cols, group=group, dtype=dtype,
+                            scale_dtype=TYPES[(rows + cols + n) % 3] if n % 2 else dtype,
+                            layout=("plain", "strided", "unaligned")[(rows + n) % 3]))
+    for i, (tokens, top_k, experts, n, cols, group) in enumerate(EXPERTS_PRODUCTS):
+        for dtype in TYPES:
+            out.append(dict(op="experts_product", tokens=tokens, top_k=top_k, experts=experts, out=n, cols=cols,
+                            group=group, dtype=dtype, dropped=(0.0, 0.3)[i % 2], books=(tokens + n) % 2 == 0,
+                            layout=("plain", "strided", "unaligned")[(tokens + top_k) % 3]))
+    return out
+
+
 def all_cases():
     cases = _sort() + _route() + _rows() + _product() + _experts_product() + _quantize()
     cases += [dict(op=name) for name in ("differences_route", "differences_rows", "refusals", "graph", "other_stream",
                                          "broadcast_gradients", "unwanted_places", "fitted_codebook", "far_rows",
                                          "repeats", "long_cache", "c_refusals", "example")]
+    cases += _shapes()
     for i, c in enumerate(cases):
         c["name"] = "%03d_%s" % (i, "_".join(str(v) for v in c.values()))
     return cases
