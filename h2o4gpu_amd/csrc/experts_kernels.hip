@@ -26,6 +26,13 @@ __device__ __forceinline__ float softmax_term(float k, float best, float scale) 
   return k == best || scale == 0.f ? 1.0f : expf(scale * (k - best));
 }
 
+// The same of a score that is not chosen: its exponent x is rounded to |x| 2^-23, which moves a term by at most 0.4 of
+// that of the largest (1). scale2: scale * log2(e), of which exp2 is one instruction.
+__device__ __forceinline__ float other_term(float k, float best, float scale2) {
+  return k == best || scale2 == 0.f ? 1.0f : __builtin_amdgcn_exp2f(scale2 * (k - best));
+}
+static const float LOG2E = 1.44269504088896341f;
+
 __device__ __forceinline__ bool comes_before(float ka, int ia, float kb, int ib) {
   return ka > kb || (ka == kb && ia < ib);
 }
@@ -111,16 +118,16 @@ __device__ __forceinline__ float key_of(unsigned rank) {
   return __uint_as_float((int)rank < 0 ? rank & 0x7fffffffu : ~rank);
 }
 
-// The better of (rank, index) and that of the lane a step away, over LANES lanes.
+// The largest (and the least) of LANES lanes' values, in all of them.
 template <int LANES, int STEP = 0>
-__device__ __forceinline__ void best_of(unsigned &rank, unsigned &index) {
-  if constexpr ((1 << STEP) < LANES) {
-    const unsigned r = from_step<STEP>(rank), i = from_step<STEP>(index);
-    const bool take = r > rank || (r == rank && i < index);
-    rank = take ? r : rank;
-    index = take ? i : index;
-    best_of<LANES, STEP + 1>(rank, index);
-  }
+__device__ __forceinline__ unsigned most_of(unsigned v) {
+  if constexpr ((1 << STEP) < LANES) return most_of<LANES, STEP + 1>(max(v, from_step<STEP>(v)));
+  return v;
+}
+template <int LANES, int STEP = 0>
+__device__ __forceinline__ unsigned least_of(unsigned v) {
+  if constexpr ((1 << STEP) < LANES) return least_of<LANES, STEP + 1>(min(v, from_step<STEP>(v)));
+  return v;
 }
 template <int LANES, int STEP = 0>
 __device__ __forceinline__ float sum_of(float v) {
@@ -129,10 +136,44 @@ __device__ __forceinline__ float sum_of(float v) {
   return v;
 }
 
+// What a row's kernel compares. A 16-bit score's rank and its expert fit into one number, of which the largest is the
+// best with the lowest index; a float's rank fills one by itself (and its expert is looked for).
+template <typename T>
+struct Key {
+  static const bool WITH_EXPERT = false;
+  static __device__ __forceinline__ unsigned of(T s, bool largest, unsigned) { return rank_of(s, largest); }
+  static __device__ __forceinline__ float score(unsigned key) { return key_of(key); }
+};
+template <>
+struct Key<bfloat16_t> {
+  static const bool WITH_EXPERT = true;
+  static __device__ __forceinline__ unsigned of(bfloat16_t s, bool largest, unsigned e) {
+    const unsigned rank = rank_of((float)s, largest);
+    return rank ? (rank & 0xffff0000u) | (0xffff - e) : 0;
+  }
+  static __device__ __forceinline__ float score(unsigned key) {
+    return key_of((int)key < 0 ? key & 0xffff0000u : key | 0xffffu);
+  }
+};
+template <>
+struct Key<float16_t> {
+  static const bool WITH_EXPERT = true;
+  static __device__ __forceinline__ unsigned of(float16_t s, bool largest, unsigned e) {
+    const float16_t k = largest ? s : -s;
+    const unsigned u = k == (float16_t)0 ? 0 : __builtin_bit_cast(unsigned short, k);
+    return (float)k > -__builtin_huge_valf() ? (u & 0x8000 ? 0xffff - u : u | 0x8000) << 16 | (0xffff - e) : 0;
+  }
+  static __device__ __forceinline__ float score(unsigned key) {
+    const unsigned rank = key >> 16;
+    return (float)__builtin_bit_cast(float16_t, (unsigned short)(rank & 0x8000 ? rank & 0x7fff : 0xffff - rank));
+  }
+};
+
 // Rows whose scores lie side by side, at most LANES * NV of them: LANES lanes have a row in registers, W scores in
 // a row each at a time. Every round takes the best that is left (a lane's own best, then across the lanes) and
-// strikes it out. Lane j ends with choice j. What bounds it is the rounds' comparisons: 16384 rows of 256 bfloat16,
-// eight chosen of all, take 14 us (40 with the kernel above), reading them 2. 64000 x 1000 floats, eight: 167.
+// strikes it out, without a branch. Lane j ends with choice j. What bounds it are the rounds: 16384 rows of 256
+// bfloat16, eight chosen of all, take 10 us (40 with the kernel above), reading them 2; 200000 x 100, four: 36 and 8;
+// 64000 x 1000 floats, eight of all: 134 and 49.
 template <typename T, bool ALL, int LANES, int NV>
 __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_t rs, int64_t rows, int E, int K,
                                                          bool largest, float scale, int *experts, float *weights) {
@@ -141,7 +182,7 @@ __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_
   const int64_t step = (int64_t)gridDim.x * (256 / LANES);
   for (int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
     const T *s = scores + row * rs;
-    unsigned rank[NV];
+    unsigned key[NV];
 #pragma unroll
     for (int c = 0; c < NV / W; c++) {
       const int e = (c * LANES + lane) * W;
@@ -151,49 +192,50 @@ __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_
       if (e + W <= E) {
         some = *reinterpret_cast<const Some *>(s + e);
 #pragma unroll
-        for (int i = 0; i < W; i++) rank[c * W + i] = rank_of((float)some.v[i], largest);
+        for (int i = 0; i < W; i++) key[c * W + i] = Key<T>::of(some.v[i], largest, e + i);
       } else {
 #pragma unroll
-        for (int i = 0; i < W; i++) rank[c * W + i] = e + i < E ? rank_of((float)s[e + i], largest) : 0;
+        for (int i = 0; i < W; i++) key[c * W + i] = e + i < E ? Key<T>::of(s[e + i], largest, e + i) : 0;
       }
     }
-    unsigned all[NV];
-    if (ALL) {
-#pragma unroll
-      for (int i = 0; i < NV; i++) all[i] = rank[i];
-    }
-    unsigned mine = 0, first = 0;
+    unsigned mine = 0;
     int mine_e = -1;
-    float total = 0.f;
+    float first = 0.f, total = 0.f;
     for (int j = 0; j < K; j++) {
-      unsigned r = 0, at = 0;
+      unsigned best = key[0];
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const bool better = rank[i] > r;
-        r = better ? rank[i] : r;
-        at = better ? (i / W * LANES * W + i % W) : at;
+      for (int i = 1; i < NV; i++) best = max(best, key[i]);
+      best = most_of<LANES>(best);
+      if (best == 0) break;
+      if (j == 0) {
+        first = Key<T>::score(best);
+        if (ALL) {
+#pragma unroll
+          for (int i = 0; i < NV; i++) total += key[i] ? other_term(Key<T>::score(key[i]), first, scale * LOG2E) : 0.f;
+          total = sum_of<LANES>(total);
+        }
       }
-      at += lane * W;
-      const unsigned own = at;
-      best_of<LANES>(r, at);
-      if (r == 0) break;
-      if (j == 0) first = r;
-      if (!ALL) total += softmax_term(key_of(r), key_of(first), scale);
-      mine = lane == j ? r : mine;
-      mine_e = lane == j ? (int)at : mine_e;
-      if (own == at) {
+      if constexpr (Key<T>::WITH_EXPERT) {
+        mine_e = lane == j ? 0xffff - (int)(best & 0xffff) : mine_e;
 #pragma unroll
-        for (int i = 0; i < NV; i++) rank[i] = i / W * LANES * W + i % W + lane * W == at ? 0 : rank[i];
+        for (int i = 0; i < NV; i++) key[i] = key[i] == best ? 0 : key[i];
+      } else {  // the first of its expert's, and that one struck out
+        unsigned at = 1u << 30;
+#pragma unroll
+        for (int i = NV - 1; i >= 0; i--) at = key[i] == best ? i / W * LANES * W + i % W : at;
+        at = least_of<LANES>(at + lane * W);
+        mine_e = lane == j ? (int)at : mine_e;
+        const unsigned here = at - lane * W;
+#pragma unroll
+        for (int i = 0; i < NV; i++) key[i] = here == (unsigned)(i / W * LANES * W + i % W) ? 0 : key[i];
       }
+      mine = lane == j ? best : mine;
     }
-    if (ALL) {
-#pragma unroll
-      for (int i = 0; i < NV; i++) total += all[i] ? softmax_term(key_of(all[i]), key_of(first), scale) : 0.f;
-      total = sum_of<LANES>(total);
-    }
+    const float weight = mine ? softmax_term(Key<T>::score(mine), first, scale) : 0.f;
+    if (!ALL) total = sum_of<LANES>(weight);
     if (lane < K) {
       experts[row * K + lane] = mine_e;
-      weights[row * K + lane] = mine ? softmax_term(key_of(mine), key_of(first), scale) / total : 0.f;
+      weights[row * K + lane] = mine ? weight / total : 0.f;
     }
   }
 }
@@ -289,8 +331,7 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
 }
 
 // One wavefront a row, any strides: inner = sum of w g over the chosen, then every expert's gradient, in LDS 1024 at
-// a time where the chosen ones' are put in their places. 16384 x 256 bfloat16: 11 us, the writes alone 2; 64000 x
-// 1000 floats: 140.
+// a time where the chosen ones' are put in their places.
 template <typename T, bool ALL>
 __global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, int64_t rs, int64_t es, int64_t rows,
                                                              int E, int K, bool largest, float scale,
@@ -332,6 +373,79 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const T *scores, in
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       for (int i = lane; i < end; i += WAVE) dscores[row * drs + (base + i) * des] = (T)mine[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
+// The same of rows whose scores, and gradients, lie side by side: LANES lanes have a row, four experts in a row each
+// at a time. 16384 x 256 bfloat16, eight of all: 9 us (11 with the kernel above); 64000 x 1000 floats: 108 (140);
+// 500000 x 8 float16, two of all, and the choice itself: 23 us with four lanes, 50 with 16 (136).
+template <typename T, bool ALL, int LANES>
+__global__ __launch_bounds__(256) void route_backward_rows_kernel(const T *scores, int64_t rs, int64_t rows, int E,
+                                                                  int K, bool largest, float scale,
+                                                                  const int *experts, const float *weights,
+                                                                  const float *dweights, T *dscores, int64_t drs) {
+  __shared__ float4 held[256];
+  struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T v[4];
+  };
+  const int lane = threadIdx.x & (LANES - 1);
+  float4 *four = held + threadIdx.x;
+  float *mine = reinterpret_cast<float *>(held + (threadIdx.x - lane));
+  const float sign = largest ? scale : -scale, ninf = -__builtin_huge_valf();
+  const int64_t step = (int64_t)gridDim.x * (256 / LANES);
+  for (int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
+    const T *s = scores + row * rs;
+    T *ds = dscores + row * drs;
+    int e_mine = -1;
+    float w = 0.f, g = 0.f;
+    if (lane < K) {
+      e_mine = experts[row * K + lane];
+      w = weights[row * K + lane];
+      g = dweights[row * K + lane];
+    }
+    if (e_mine < 0) g = 0.f;
+    const float inner = sum_of<LANES>(w != 0.f ? w * g : 0.f);
+    const int e0 = __shfl(e_mine, 0, LANES);
+    const float w0 = __shfl(w, 0, LANES);
+    float top = 0.f;
+    if (ALL && e0 >= 0) top = (largest ? 1.f : -1.f) * (float)s[e0];
+    const float own = w != 0.f ? sign * w * (g - inner) : 0.f, rest = ALL && e0 >= 0 ? -sign * w0 * inner : 0.f;
+    for (int base = 0; base < E; base += 4 * LANES) {
+      const int at = base + 4 * lane, left = E - at;
+      float d[4] = {};
+      if (ALL && rest != 0.f && left > 0) {
+        Four some;
+        if (left >= 4) {
+          some = *reinterpret_cast<const Four *>(s + at);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) some.v[i] = s[at + (i < left ? i : 0)];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float k = largest ? (float)some.v[i] : -(float)some.v[i];
+          const float p = k > ninf ? other_term(k, top, scale * LOG2E) : 0.f;
+          d[i] = p != 0.f ? rest * p : 0.f;
+        }
+      }
+      *four = float4{d[0], d[1], d[2], d[3]};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (e_mine >= base && e_mine < base + 4 * LANES) mine[e_mine - base] = own;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const float4 f = *four;
+      const Four out{{(T)f.x, (T)f.y, (T)f.z, (T)f.w}};
+      if (left >= 4) {
+        *reinterpret_cast<Four *>(ds + at) = out;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+          if (i < left) ds[at + i] = out.v[i];
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
@@ -944,6 +1058,19 @@ KM_API int h2o4gpu_experts_route_backward(int dtype, size_t rows, int experts, i
         return launched();
       };
       return top_k <= 2 ? columns(Int<2>()) : top_k <= 4 ? columns(Int<4>()) : columns(Int<8>());
+    }
+    if (expert_stride == 1 && dexpert_stride == 1) {
+      const auto in_rows = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        auto kernel = over_all ? route_backward_rows_kernel<T, true, L> : route_backward_rows_kernel<T, false, L>;
+        hipLaunchKernelGGL(kernel, dim3(grid_of((rows * L + 255) / 256)), dim3(256), 0, s, scores, (int64_t)row_stride, n,
+                           experts, top_k, largest != 0, scale, d_experts, d_weights, d_dweights, dscores,
+                           (int64_t)drow_stride);
+        return launched();
+      };
+      return experts <= 16 && top_k <= 4    ? in_rows(Int<4>())
+             : experts <= 64 && top_k <= 16 ? in_rows(Int<16>())
+                                            : in_rows(Int<64>());
     }
     auto kernel = over_all ? route_backward_kernel<T, true> : route_backward_kernel<T, false>;
     hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 3) / 4)), dim3(256), 0, s, scores, (int64_t)row_stride,
