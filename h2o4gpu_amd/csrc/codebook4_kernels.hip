@@ -2,8 +2,6 @@
 #include "experts_common.h"
 #include "mfma_traits.h"
 
-#include <type_traits>
-
 namespace kmhip {
 
 // ---------------------------------------------------------------------------

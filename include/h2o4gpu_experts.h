@@ -113,7 +113,8 @@ int h2o4gpu_codebook4_layout(size_t experts, size_t out, size_t cols, int group,
                              size_t codes_pitch, int scale_dtype, const void *d_scales, void *d_laid_codes,
                              void *d_laid_scales, void *stream);
 /* d_y [rows][out] = d_x [rows][cols] times the matrix's transpose; products and sums in float, one
- * rounding at the end. */
+ * rounding at the end. (Both products: the first call of a type and size sets its kernel's limit of shared
+ * memory, and is to be outside a capture.) */
 int h2o4gpu_codebook4_product(int dtype, size_t rows, size_t out, size_t cols, int group, const void *d_x,
                               size_t x_stride, const void *d_laid_codes, int scale_dtype, const void *d_laid_scales,
                               const void *d_codebook, void *d_y, size_t y_stride, void *stream);
