@@ -242,14 +242,15 @@ __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_
 
 // Scores of one expert side by side (row stride 1, the distances of transform): a lane has a row and walks down
 // its experts with its best KT in order. The wavefronts of a workgroup each walk a stretch of
-// the experts, and the first joins their lists (a later stretch's equal score stays behind). 1M rows x 64, two
-// chosen: 51 us, 5.3 TB/s, what a copy reaches.
+// the experts, and their lists are joined in pairs (a later stretch's equal score stays behind). 1M rows x 64, two
+// chosen: 51 us, 5.3 TB/s, what a copy reaches. 1000 x 1000, two of all: 20 (30 with the lists joined one after
+// another).
 template <typename T, bool ALL, int KT>
 __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, int64_t es, int64_t rows, int E, int K,
                                                              bool largest, float scale, int *experts, float *weights) {
   extern __shared__ float lists[];  // [parts][2 KT + 1][64]: keys, experts, sums over all
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, parts = blockDim.x >> 6;
-  const float ninf = -__builtin_huge_valf();
+  const float ninf = -__builtin_huge_valf(), scale2 = scale * LOG2E;
   const int lo = (int)((int64_t)E * part / parts), hi = (int)((int64_t)E * (part + 1) / parts);
   for (int64_t row0 = (int64_t)blockIdx.x * 64; row0 < rows; row0 += (int64_t)gridDim.x * 64) {
     const int64_t row = row0 + lane < rows ? row0 + lane : rows - 1;
@@ -278,40 +279,43 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
         if (e0 + i >= hi) break;
         const float f = largest ? (float)v[i] : -(float)v[i];
         if (ALL && f > ninf) {  // (sums are of terms against the best so far)
-          if (f > key[0])
-            sum = key[0] > ninf ? sum * softmax_term(key[0], f, scale) + 1.f : 1.f;
-          else
-            sum += softmax_term(f, key[0], scale);
+          const float term = key[0] > ninf ? other_term(fminf(f, key[0]), fmaxf(f, key[0]), scale2) : 0.f;
+          sum = f > key[0] ? sum * term + 1.f : sum + term;
         }
         if (f > key[KT - 1]) insert(f, e0 + i);
       }
     }
-    if (parts > 1) {
-      __syncthreads();
+    if (parts > 1) {  // (a power of two)
       float *mine = lists + (size_t)part * (2 * KT + 1) * 64 + lane;
+      const auto put = [&] {
 #pragma unroll
-      for (int j = 0; j < KT; j++) {
-        mine[2 * j * 64] = key[j];
-        mine[(2 * j + 1) * 64] = __int_as_float(id[j]);
-      }
-      mine[2 * KT * 64] = sum;
+        for (int j = 0; j < KT; j++) {
+          mine[2 * j * 64] = key[j];
+          mine[(2 * j + 1) * 64] = __int_as_float(id[j]);
+        }
+        mine[2 * KT * 64] = sum;
+      };
       __syncthreads();
-      if (part > 0) continue;
-      for (int p = 1; p < parts; p++) {
-        const float *other = lists + (size_t)p * (2 * KT + 1) * 64 + lane;
+      put();
+      for (int apart = 1; apart < parts; apart *= 2) {
+        __syncthreads();
+        if (part & (2 * apart - 1)) continue;
+        const float *other = mine + (size_t)apart * (2 * KT + 1) * 64;
         if (ALL) {
           const float top = other[0], its = other[2 * KT * 64];
           if (top > key[0])
-            sum = (key[0] > ninf ? sum * softmax_term(key[0], top, scale) : 0.f) + its;
+            sum = (key[0] > ninf ? sum * other_term(key[0], top, scale2) : 0.f) + its;
           else if (top > ninf)
-            sum += its * softmax_term(top, key[0], scale);
+            sum += its * other_term(top, key[0], scale2);
         }
 #pragma unroll
         for (int j = 0; j < KT; j++) {
           const float k = other[2 * j * 64];
           if (k > key[KT - 1]) insert(k, __float_as_int(other[(2 * j + 1) * 64]));
         }
+        if (2 * apart < parts) put();
       }
+      if (part > 0) continue;
     }
     if (row0 + lane >= rows) continue;
     float p[KT], total = 0.f;
@@ -513,7 +517,7 @@ __global__ __launch_bounds__(256) void route_backward_columns_kernel(const T *sc
         float out = 0.f;
         if (ALL) {
           const float k = largest ? (float)v[i] : -(float)v[i];
-          const float p = k > ninf ? softmax_term(k, top, scale) : 0.f;
+          const float p = k > ninf ? other_term(k, top, scale * LOG2E) : 0.f;
           out = p != 0.f && rest != 0.f ? rest * p : 0.f;
         }
         if (u0 + i == id[0]) {
