@@ -102,12 +102,21 @@ class Codebook4:
         return values * self.scales().float().repeat_interleave(self.group, -1)[..., :self.cols]
 
 
+def _spread(n, m, device=None):
+    """m ascending places of n (m <= n), one in each of m equal stretches. Where in its stretch a place lies goes
+    by multiples of the golden ratio, so that every column of a matrix is met as often as any other. (A stretch is
+    n / m long, no whole number: below 1.6, an end and a start that share a place may both name it.)"""
+    i = torch.arange(m, dtype=torch.float64, device=device)
+    return ((i + (i * 0.6180339887498949).frac()) * (n / m)).long().clamp_(max=n - 1)
+
+
 def fit_codebook(values, sample=1 << 20, seed=0):
-    """The 16 centroids k-means finds for `values` (a GPU tensor, any shape), ascending, float32."""
+    """The 16 centroids k-means finds for `values` (a GPU tensor, any shape; of more than `sample`, that many
+    spread over all of them), ascending, float32."""
     from .solvers.kmeans import KMeans
     flat = values.reshape(-1)
-    if flat.numel() > sample:  # evenly spaced: repeatable, and every part of the matrix is in it
-        flat = flat[torch.arange(sample, device=flat.device) * (flat.numel() // sample)]
+    if flat.numel() > sample:
+        flat = flat[_spread(flat.numel(), sample, flat.device)]
     flat = flat.float()
     flat = flat[torch.isfinite(flat)]
     if flat.numel() < 16:
@@ -144,8 +153,8 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
     if codebook is None:
         if top != 1.0:
             raise ValueError("top goes with a given codebook; one that is fitted has 1")
-        part = flat[torch.arange(min(flat.shape[0], 4096), device=flat.device) *
-                    (flat.shape[0] // min(flat.shape[0], 4096))].float()
+        part = flat if flat.shape[0] <= 4096 else flat[_spread(flat.shape[0], 4096, flat.device)]
+        part = part.float()
         padded = torch.nn.functional.pad(part, (0, groups * group - cols)).reshape(part.shape[0], groups, group)
         scaled = padded / padded.abs().amax(2, keepdim=True).clamp_min(1e-38)
         codebook = fit_codebook(scaled.reshape(part.shape[0], -1)[:, :cols])

@@ -1,0 +1,35 @@
+"""Host-side pieces of the expert layers and 4-bit products that need no GPU. They run in a child process:
+PyTorch's copy of the HIP runtime is never loaded beside the library's in this one."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def run(code):
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+# n values (or rows) of which m are taken, and how many neighbours make a row
+@pytest.mark.parametrize("n,m,cols", [(5, 5, 1), (8193, 4096, 1), (8000, 4096, 1), (8191, 4096, 1), (4097, 4096, 1),
+                                      ((1 << 20) + 1, 1 << 20, 7), (4096 * 320, 1 << 20, 320), (4096 * 640, 1 << 20, 640),
+                                      (4096 * 4096, 1 << 20, 4096), (4096 * 1024, 1 << 20, 1024), (10 ** 9, 1000, 64)])
+def test_a_sample_is_spread_over_all(n, m, cols):
+    run("""
+import torch
+from h2o4gpu_amd.codebook4 import _spread
+n, m, cols = %d, %d, %d
+at = _spread(n, m)
+stretch = -(-n // m)
+assert at.dtype == torch.int64 and at.numel() == m
+gaps = at[1:] - at[:-1]
+assert int(gaps.min()) >= (1 if n >= 2 * m or n == m else 0) and int(gaps.max()) <= 2 * stretch
+assert 0 <= int(at[0]) < stretch and n - stretch <= int(at[-1]) < n
+if m >= 64 * cols:  # every column about as often as any other
+    share = torch.bincount(at %% cols, minlength=cols).double() * cols / m
+    assert 0.8 <= float(share.min()) and float(share.max()) <= 1.2, share
+""" % (n, m, cols))
