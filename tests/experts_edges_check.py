@@ -3,6 +3,7 @@ line for each. Not collected by pytest.
 
 Oracles are the formulas in 64 bits; U32 is the largest relative error of one float32 rounding."""
 import json
+import math
 import os
 import sys
 import traceback
@@ -11,7 +12,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
-from h2o4gpu_amd import codebook4  # noqa: E402
+from h2o4gpu_amd import codebook4, experts  # noqa: E402
 
 U32 = 2.0 ** -24
 
@@ -40,6 +41,68 @@ def codebook_of_all_experts():
     # sixteen entries of a mixture by halves: a third of the error at most (about an eighth, were they those of
     # Lloyd's fixed point on the whole matrices)
     assert joint < alone / 3, (joint, alone)
+
+
+def softmax_over_all(s, K, largest, scale):
+    """Choice, softmax over all experts and its exponents in 64 bits; no score is masked."""
+    key = s.double() if largest else -s.double()
+    chosen = torch.argsort(key, dim=1, descending=True, stable=True)[:, :K]
+    x = scale * (key - key.amax(1, keepdim=True))
+    return chosen, torch.softmax(x, 1), x
+
+
+def check_over_all(s, K, largest, scale, place, chain, g, same_rows=None):
+    """route over all experts and its gradient, each number against its own size. s: float32 scores on the host,
+    place(s): them on the GPU; same_rows: which row of s each row of place(s) is (all of them, one after another).
+
+    Roundings, in U32: an exponent x is the product of two rounded factors and rounded itself, so e^x is off by
+    3 |x|, and by 4 for the exponential. A sum over all is off by its terms' errors, each by its share p of the sum,
+    and by `chain`, the additions one after another (and what moves the sum to another best score). A weight: its
+    term, the sum, a division. A gradient: scale * p * (g - inner), inner a sum of K products."""
+    rows, E = s.shape
+    chosen, p, x = softmax_over_all(s, K, largest, scale)
+    d = place(s).requires_grad_()
+    got, weights = experts.route(d, K, largest=largest, scale=scale, over_all=True)
+    ds, = torch.autograd.grad(weights, d, g[same_rows].cuda() if same_rows is not None else g.cuda())
+    if same_rows is not None:
+        for t in (got, weights, ds):
+            for lo in range(rows, t.shape[0], rows):
+                part = t[lo:lo + rows]
+                assert torch.equal(part, t[:part.shape[0]]), "equal rows, other results"
+        got, weights, ds = got[:rows], weights[:rows], ds[:rows]
+    assert torch.equal(got.cpu().long(), chosen), "choice"
+    total = 3 * (p * -x).sum(1, keepdim=True) + 4 + chain
+    pick = p.gather(1, chosen)
+    c = 3 * -x.gather(1, chosen) + 4 + total + 2
+    off = (weights.detach().cpu().double() - pick).abs() / pick / U32
+    assert bool((off <= c).all()), "weights off by %.0f, %.0f allowed" % (float((off / c).max() * c.max()), float(c.max()))
+    full = torch.zeros_like(p).scatter_(1, chosen, g.double())
+    inner = (pick * g.double()).sum(1, keepdim=True)
+    sign = scale if largest else -scale
+    want = sign * p * (full - inner)
+    size = scale * p * (full.abs() + (pick * g.double().abs()).sum(1, keepdim=True))
+    bound = U32 * size * (2 * c.amax(1, keepdim=True) + 3 * -x + 4 + K + 6) + 2.0 ** -126
+    off = (ds.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), "gradient off by %.3g times what is allowed" % float((off / bound).max())
+    # zeros in place of the gradients of experts that are not chosen would be seen
+    others = torch.ones_like(p).scatter_(1, chosen, 0.0).bool()
+    assert bool((want.abs() > 8 * bound)[others & (p > 2.0 ** -100)].all())
+
+
+def long_sums_of_distances():
+    """So many rows that one lane has all of a row's distances. Rows whose other experts all have one term, for
+    which roundings do not even out, and rows that get better, or worse, by equal steps."""
+    K, scale = 2, 0.7
+    for E in (1000, 4096):
+        term = torch.linspace(0.01, 0.9, 90, dtype=torch.float64)
+        s = (-torch.log(term) / scale)[:, None].repeat(1, E).float() + 1
+        s.scatter_(1, torch.randint(0, E, (90, 1), generator=gen(80)), 1.0)
+        steps = torch.arange(E).float()[None] * torch.tensor([0.001, 0.01, 0.1])[:, None]
+        s = torch.cat([s, steps, steps.flip(1), 3 * torch.rand(30, E, generator=gen(81))])
+        at = torch.arange(131072 + 77) % s.shape[0]
+        g = 0.5 + torch.rand(s.shape[0], K, generator=gen(82))
+        # a lane's sum: pairs of eight (3), an addition (2), moves of the sum (8 each, every one a factor e less)
+        check_over_all(s, K, False, scale, lambda s: s.t().cuda()[:, at.cuda()].t(), 3 + 2 + 13 + 5, g, at)
 
 
 def main():
