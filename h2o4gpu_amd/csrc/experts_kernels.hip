@@ -26,12 +26,23 @@ __device__ __forceinline__ float softmax_term(float k, float best, float scale) 
   return k == best || scale == 0.f ? 1.0f : expf(scale * (k - best));
 }
 
-// The same of a score that is not chosen: its exponent x is rounded to |x| 2^-23, which moves a term by at most 0.4 of
-// that of the largest (1). scale2: scale * log2(e), of which exp2 is one instruction.
-__device__ __forceinline__ float other_term(float k, float best, float scale2) {
+// The same as a term of a sum over all. Its exponent x is a product of two rounded factors and rounded itself, so
+// that the term is off by up to 1.5 |x| 2^-23 of it: 0.6 * 2^-23 of the largest one (1), 1.5 ln(E) 2^-23 of the sum.
+// scale2: scale * log2(e), of which exp2 is one instruction.
+__device__ __forceinline__ float summed_term(float k, float best, float scale2) {
   return k == best || scale2 == 0.f ? 1.0f : __builtin_amdgcn_exp2f(scale2 * (k - best));
 }
 static const float LOG2E = 1.44269504088896341f;
+
+// The same where it is a result's factor (the gradient of a score that is not chosen, whose own size counts), in a few
+// instructions: exp2 has the rounded x log2(e), and a product what that is off by. Terms below 2^-126 are 0.
+__device__ __forceinline__ float other_term(float k, float best, float scale) {
+  if (k == best || scale == 0.f) return 1.0f;
+  const float high = 1.44269504f, low = 1.92596299e-8f;  // log2(e) is their sum
+  const float x = fmaxf(scale * (k - best), -200.f), y = x * high;
+  const float p = __builtin_amdgcn_exp2f(y), rest = fmaf(x, low, fmaf(x, high, -y));
+  return fmaf(p, rest * 0.693147181f, p);
+}
 
 __device__ __forceinline__ bool comes_before(float ka, int ia, float kb, int ib) {
   return ka > kb || (ka == kb && ia < ib);
@@ -211,7 +222,7 @@ __global__ __launch_bounds__(256) void route_rows_kernel(const T *scores, int64_
         first = Key<T>::score(best);
         if (ALL) {
 #pragma unroll
-          for (int i = 0; i < NV; i++) total += key[i] ? other_term(Key<T>::score(key[i]), first, scale * LOG2E) : 0.f;
+          for (int i = 0; i < NV; i++) total += key[i] ? summed_term(Key<T>::score(key[i]), first, scale * LOG2E) : 0.f;
           total = sum_of<LANES>(total);
         }
       }
@@ -287,13 +298,13 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
 #pragma unroll
         for (int i = 1; i < 8; i++) most = fmaxf(most, f[i]);
         if (scale * (most - ref) > 1.f) {
-          const float by = other_term(ref, most, scale2);
+          const float by = summed_term(ref, most, scale2);
           sum *= by;
           over *= by;
           ref = most;
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = f[i] > ninf ? other_term(f[i], ref, scale2) : 0.f;
+        for (int i = 0; i < 8; i++) t[i] = f[i] > ninf ? summed_term(f[i], ref, scale2) : 0.f;
         const float add = (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]))) - over;
         const float next = sum + add;
         over = (next - sum) - add;
@@ -303,7 +314,7 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
       for (int i = 0; i < 8; i++)
         if (f[i] > key[KT - 1]) insert(f[i], e0 + i);
     }
-    if (ALL) sum = key[0] > ninf ? (sum - over) * other_term(ref, key[0], scale2) : 0.f;
+    if (ALL) sum = key[0] > ninf ? (sum - over) * summed_term(ref, key[0], scale2) : 0.f;
     if (parts > 1) {  // (a power of two)
       float *mine = lists + (size_t)part * (2 * KT + 1) * 64 + lane;
       const auto put = [&] {
@@ -323,9 +334,9 @@ __global__ __launch_bounds__(1024) void route_columns_kernel(const T *scores, in
         if (ALL) {
           const float top = other[0], its = other[2 * KT * 64];
           if (top > key[0])
-            sum = (key[0] > ninf ? sum * other_term(key[0], top, scale2) : 0.f) + its;
+            sum = (key[0] > ninf ? sum * summed_term(key[0], top, scale2) : 0.f) + its;
           else if (top > ninf)
-            sum += its * other_term(top, key[0], scale2);
+            sum += its * summed_term(top, key[0], scale2);
         }
 #pragma unroll
         for (int j = 0; j < KT; j++) {
@@ -450,7 +461,7 @@ __global__ __launch_bounds__(256) void route_backward_rows_kernel(const T *score
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float k = largest ? (float)some.v[i] : -(float)some.v[i];
-          const float p = k > ninf ? other_term(k, top, scale * LOG2E) : 0.f;
+          const float p = k > ninf ? other_term(k, top, scale) : 0.f;
           d[i] = p != 0.f ? rest * p : 0.f;
         }
       }
@@ -536,7 +547,7 @@ __global__ __launch_bounds__(256) void route_backward_columns_kernel(const T *sc
         float out = 0.f;
         if (ALL) {
           const float k = largest ? (float)v[i] : -(float)v[i];
-          const float p = k > ninf ? other_term(k, top, scale * LOG2E) : 0.f;
+          const float p = k > ninf ? other_term(k, top, scale) : 0.f;
           out = p != 0.f && rest != 0.f ? rest * p : 0.f;
         }
         if (u0 + i == id[0]) {

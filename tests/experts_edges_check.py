@@ -105,6 +105,31 @@ def long_sums_of_distances():
         check_over_all(s, K, False, scale, lambda s: s.t().cuda()[:, at.cuda()].t(), 3 + 2 + 13 + 5, g, at)
 
 
+def small_gradients():
+    """Gradients of scores far below the best one, against each other: they are one factor of the row times their
+    terms e^x. Scores are multiples of a sixteenth, so that x is exact; a term is off by 4 U32 (exponential) and one
+    for each of three products, its neighbour likewise."""
+    rows, E, K = 64, 300, 2
+    x = -5 - torch.randint(0, 1200, (rows, E), generator=gen(90)).float() / 16
+    x[:, :2] = -5
+    x[:, 7] = 0
+    g = 0.5 + torch.rand(rows, K, generator=gen(91))
+    for largest in (True, False):
+        s = x if largest else -x
+        wide = torch.zeros(2 * rows, 3 * E, device="cuda")[::2, ::3]
+        wide.copy_(s)
+        for d in (s.cuda(), s.t().contiguous().cuda().t(), wide):
+            d = d.detach().requires_grad_()
+            chosen, weights = experts.route(d, K, largest=largest, over_all=True)
+            assert bool((chosen.cpu()[:, 0] == 7).all() and (chosen.cpu()[:, 1] == 0).all())
+            ds, = torch.autograd.grad(weights, d, g.cuda())
+            ratio = ds.cpu().double() / ds.cpu().double()[:, 1:2]
+            want = torch.exp(x.double() - x.double()[:, 1:2])
+            off = (ratio / want - 1).abs() / U32
+            off[:, 0] = off[:, 7] = 0  # (the chosen ones)
+            assert float(off.max()) <= 14, "strides %s: off by %.1f" % (d.stride(), float(off.max()))
+
+
 def main():
     for name in sys.argv[1:]:
         print("# " + name, flush=True)
