@@ -14,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CHECKS = [
     "codebook_of_all_experts",
     "long_sums_of_distances",
+    "every_number_by_its_size",
     "small_gradients",
 ]
 
