@@ -12,6 +12,9 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "examples"))
+from experts_device_check import _order, choices, matrix, near, order_oracle, product_bound  # noqa: E402
 from h2o4gpu_amd import codebook4, experts  # noqa: E402
 
 U32 = 2.0 ** -24
@@ -158,6 +161,74 @@ def small_gradients():
             off = (ratio / want - 1).abs() / U32
             off[:, 0] = off[:, 7] = 0  # (the chosen ones)
             assert float(off.max()) <= 14, "strides %s: off by %.1f" % (d.stride(), float(off.max()))
+
+
+def tokens_that_are_not_finite():
+    """A NaN or an infinity in one token's row is in that token's results, as multiplying would have it, and in no
+    other's, though few rows share a matrix instruction and are multiplied with more than their own columns."""
+    def spoiled(rows, cols, dt, seed):
+        x = torch.randn(rows, cols, generator=gen(seed)).to(dt)
+        x[0, cols // 2] = float("nan")
+        if rows > 1:
+            x[1, 0] = float("inf")
+        if rows > 3:
+            x[2, cols - 1] = -float("inf")
+        if rows > 15:
+            x[-2, cols // 3] = float("inf")
+            x[-2, cols // 2] = -float("inf")
+        return x
+
+    for dtype in ("float32", "bfloat16", "float16"):
+        for rows in (1, 2, 3, 4, 5, 16, 33, 70):
+            for n, cols, group in ((40, 300, 32), (33, 2047, 64), (200, 1024, 128)):
+                w, W = matrix(dict(out=n, cols=cols, group=group, dtype=dtype, layout="plain"), ())
+                x = spoiled(rows, cols, getattr(torch, dtype), 95)
+                near(codebook4.product(x.cuda(), w), x.double() @ W.t(), product_bound(x, W), "y")
+        for tokens, top_k, E in ((1, 2, 8), (4, 2, 3), (40, 3, 4)):
+            c = dict(tokens=tokens, top_k=top_k, experts=E, out=40, cols=300, group=64, dtype=dtype, layout="plain")
+            e, o, pos = _order(c)
+            w, W = matrix(c, (E,))
+            x = spoiled(tokens, 300, getattr(torch, dtype), 96)
+            want, bound = torch.zeros(tokens * top_k, 40, dtype=torch.float64), torch.zeros(tokens * top_k, 40, dtype=torch.float64)
+            for t in range(tokens):
+                for j in range(top_k):
+                    want[pos[t, j]] = W[e[t, j]] @ x[t].double()
+                    bound[pos[t, j]] = product_bound(x[t:t + 1], W[e[t, j]])[0]
+            near(codebook4.experts_product(x.cuda(), w, o), want, bound, "rows")
+
+
+def a_token_served_alone():
+    """The example's serving path: tokens one by one and all at once, both against the formula."""
+    from cluster_experts import serve
+    rows, E, K, d, n, scale = 60, 7, 2, 96, 50, 0.3
+    x, near_by = torch.randn(rows, d, generator=gen(100)), torch.rand(rows, E, generator=gen(101)) * 9
+    distances = near_by.t().contiguous().cuda().t()
+    packed = codebook4.quantize(torch.randn(E, n, d, generator=gen(102)).cuda(), 32)
+    W = packed.dequantize().cpu().double()
+    key = -near_by.double()
+    chosen = torch.argsort(key, dim=1, descending=True, stable=True)[:, :K]
+    w = torch.softmax(scale * key.gather(1, chosen), 1)
+    want, bound = torch.zeros(rows, n, dtype=torch.float64), torch.zeros(rows, n, dtype=torch.float64)
+    for t in range(rows):
+        for j in range(K):
+            e = int(chosen[t, j])
+            y = W[e] @ x[t].double()
+            want[t] += w[t, j] * y
+            # a weight: exponent (2 * 3 at most here), exponential, sum, division; the join
+            bound[t] += w[t, j] * (product_bound(x[t:t + 1], W[e])[0] + (2 * 3 + 4 + K + 2 + K + 1) * U32 * y.abs())
+    near(serve(x.cuda(), distances, packed, K, scale), want, bound, "all")
+    for t in (0, 1, 31, rows - 1):
+        near(serve(x[t:t + 1].cuda(), distances[t:t + 1], packed, K, scale), want[t:t + 1], bound[t:t + 1], "token %d" % t)
+
+
+def labels_in_order():
+    """Labels, one a row, in place of choices."""
+    for rows, E in ((0, 3), (1, 1), (1000, 7), (70_000, 300)):
+        labels = choices(rows, 1, E, "dropped")
+        order, position, offsets = order_oracle(labels, E)
+        o = experts.sort_by_expert(torch.from_numpy(labels[:, 0].copy()).cuda(), E)
+        for got, want in ((o.order, order), (o.position, position), (o.offsets, offsets)):
+            assert torch.equal(got.cpu(), torch.from_numpy(want)), (rows, E)
 
 
 def main():

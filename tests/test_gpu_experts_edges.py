@@ -16,6 +16,9 @@ CHECKS = [
     "long_sums_of_distances",
     "every_number_by_its_size",
     "small_gradients",
+    "tokens_that_are_not_finite",
+    "a_token_served_alone",
+    "labels_in_order",
 ]
 
 
