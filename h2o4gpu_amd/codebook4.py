@@ -16,7 +16,7 @@ The products are for serving and have no gradient. Streams and graphs as in h2o4
 import numpy as np
 import torch
 
-from .experts import _TYPES, _call, _order_of, _rows, _tensor, _type_of
+from .experts import _TYPES, _call, _no_tangents, _order_of, _rows, _tensor, _type_of
 from .libs import experts_hip
 
 
@@ -180,6 +180,7 @@ def _tokens(x, weights):
         raise ValueError("x must be (tokens, %d), got %s" % (weights.cols, tuple(x.shape)))
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("products with 4-bit matrices have no gradient: detach x, or multiply with dequantize()")
+    _no_tangents(x)
     return _rows("x", x)
 
 

@@ -10,7 +10,7 @@ centroids or scores, and the results come back and are joined by weight.
     Y = experts.combine(rows, weights, order)
 
 `route`, `dispatch` and `combine` have gradients (with respect to the scores, the tokens, the rows
-and the weights). All work is queued on the current stream of the tensors' device, nothing waits
+and the weights); forward-mode derivatives are refused. All work is queued on the current stream of the tensors' device, nothing waits
 for it and nothing is copied to the host, so the calls can be recorded into a graph. Tensors are
 read on that stream: one that another stream writes has to be waited for, as with any torch
 operation, and an ExpertOrder used on another stream than it was made on likewise. Same inputs give
@@ -19,6 +19,7 @@ the same bits. The kernels are the library's (include/h2o4gpu_experts.h); there 
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .libs import experts_hip
 
@@ -74,6 +75,14 @@ def _rows(name, t):
     elif stride < t.shape[1]:
         raise ValueError("the rows of %s overlap (strides %s)" % (name, t.stride()))
     return t.data_ptr(), stride
+
+
+def _no_tangents(*tensors):
+    """Refuses tensors of a forward-mode derivative: their tangents would be left out without a word."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (outside of any dual_level, this is all that is looked at)
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("expert layers and 4-bit products have no forward-mode derivative")
 
 
 def _gradient(t):
@@ -144,6 +153,7 @@ def route(scores, top_k, largest=True, scale=1.0, over_all=False):
         raise ValueError("top_k must be 1 to %d, got %d" % (min(scores.shape[1], experts_hip.MAX_TOP_K), top_k))
     if not 0.0 <= scale <= 3.4e38:
         raise ValueError("scale must be finite and not negative, got %r" % scale)
+    _no_tangents(scores)
     if scores.requires_grad and torch.is_grad_enabled():
         return _Route.apply(scores, top_k, largest, scale, over_all)
     return _route(scores, top_k, largest, scale, over_all)
@@ -255,6 +265,7 @@ def dispatch(x, order):
     _order_of(order, x.device)
     if x.shape[0] != order.tokens or x.shape[1] < 1:
         raise ValueError("x must be (%d, cols), got %s" % (order.tokens, tuple(x.shape)))
+    _no_tangents(x)
     if x.requires_grad and torch.is_grad_enabled():
         return _Dispatch.apply(x, order)
     return _dispatch(x, order)
@@ -303,6 +314,7 @@ def combine(rows, weights, order):
         raise ValueError("rows must be (%d, cols), got %s" % (order.tokens * order.top_k, tuple(rows.shape)))
     if tuple(weights.shape) != (order.tokens, order.top_k):
         raise ValueError("weights must be (%d, %d), got %s" % (order.tokens, order.top_k, tuple(weights.shape)))
+    _no_tangents(rows, weights)
     weights = weights.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _Combine.apply(rows, weights, order)

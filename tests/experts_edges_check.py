@@ -231,6 +231,40 @@ def labels_in_order():
             assert torch.equal(got.cpu(), torch.from_numpy(want)), (rows, E)
 
 
+def refuses(kind, f, *args, **kw):
+    try:
+        f(*args, **kw)
+    except kind:
+        return
+    raise AssertionError("%s was not refused with %s" % (f.__name__, kind.__name__))
+
+
+def forward_mode_is_refused():
+    """A tangent is refused, not dropped; tensors without one are taken inside of a dual level as well."""
+    from torch.autograd import forward_ad
+    T, K, E, d = 6, 2, 4, 64
+    s, x, y = (torch.randn(T, E, device="cuda"), torch.randn(T, d, device="cuda"), torch.randn(T * K, d, device="cuda"))
+    w = torch.rand(T, K, device="cuda")
+    o = experts.sort_by_expert(experts.route(s, K)[0], E)
+    W = torch.randn(E, 20, d, device="cuda")
+    book = torch.linspace(-1, 1, 16, device="cuda")
+    one, many = codebook4.quantize(W[0], 32, book), codebook4.quantize(W, 32, book)
+    calls = ((experts.route, (s, K), 1), (experts.dispatch, (x, o), 1), (experts.combine, (y, w, o), 2),
+             (codebook4.product, (x, one), 1), (codebook4.experts_product, (x, many, o), 1))
+    for f, args, tensors in calls:
+        want = f(*args)
+        with forward_ad.dual_level():
+            for at in range(tensors):
+                for given in (args[at], args[at].clone().requires_grad_()):
+                    if f.__module__.endswith("codebook4") and given.requires_grad:
+                        continue  # (refused for its gradient)
+                    dual = forward_ad.make_dual(given, torch.ones_like(given))
+                    refuses(NotImplementedError, f, *(args[:at] + (dual,) + args[at + 1:]))
+            got = f(*args)
+        for a, b in zip(got, want) if isinstance(got, tuple) else ((got, want),):
+            assert torch.equal(a, b)
+
+
 def main():
     for name in sys.argv[1:]:
         print("# " + name, flush=True)

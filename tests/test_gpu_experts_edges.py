@@ -19,6 +19,7 @@ CHECKS = [
     "tokens_that_are_not_finite",
     "a_token_served_alone",
     "labels_in_order",
+    "forward_mode_is_refused",
 ]
 
 
