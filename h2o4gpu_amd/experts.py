@@ -85,11 +85,28 @@ def _no_tangents(*tensors):
                 raise NotImplementedError("expert layers and 4-bit products have no forward-mode derivative")
 
 
-def _gradient(t):
-    """An incoming gradient with contiguous rows (autograd hands out expanded and transposed ones). There
-    is no gradient of a gradient."""
-    if torch.is_grad_enabled():
+class _Once(torch.autograd.Function):
+    """A gradient as it is, behind which nothing can be differentiated with respect to what it was made of."""
+
+    @staticmethod
+    def forward(ctx, gradient, *sources):
+        return gradient.view_as(gradient)
+
+    @staticmethod
+    def backward(ctx, _):
         raise RuntimeError("the gradients of expert layers cannot be differentiated again")
+
+
+def _once(gradient, *sources):
+    """What a backward pass returns for a gradient that the kernels made of `sources`. Under create_graph it
+    belongs to a graph, in which others' gradients may be differentiated again and this one is an error."""
+    if torch.is_grad_enabled() and any(s.requires_grad for s in sources):
+        return _Once.apply(gradient, *sources)
+    return gradient
+
+
+def _gradient(t):
+    """An incoming gradient with contiguous rows (autograd hands out expanded and transposed ones)."""
     if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
@@ -119,7 +136,7 @@ class _Route(torch.autograd.Function):
         _call(scores.device.index, "h2o4gpu_experts_route_backward", _TYPES[scores.dtype], rows, n_experts, top_k,
               largest, over_all, scale, scores.data_ptr(), *scores.stride(), chosen.data_ptr(), weights.data_ptr(),
               dweights.data_ptr(), dscores.data_ptr(), *dscores.stride())
-        return dscores, None, None, None, None
+        return _once(dscores, scores, dweights), None, None, None, None
 
 
 def _route(scores, top_k, largest, scale, over_all):
@@ -252,7 +269,7 @@ class _Dispatch(torch.autograd.Function):
         dx = drows.new_empty((order.tokens, cols))
         _call(drows.device.index, "h2o4gpu_experts_dispatch_backward", _TYPES[drows.dtype], order.tokens, order.top_k,
               cols, ptr, stride, order._position_ptr, dx.data_ptr(), cols)
-        return dx, None
+        return _once(dx, drows), None
 
 
 def dispatch(x, order):
@@ -298,7 +315,7 @@ class _Combine(torch.autograd.Function):
         _call(rows.device.index, "h2o4gpu_experts_combine_backward", _TYPES[rows.dtype], order.tokens, order.top_k,
               rows.shape[1], gptr, gstride, rptr, rstride, weights.data_ptr(), order._position_ptr,
               drows.data_ptr(), rows.shape[1], dweights.data_ptr())
-        return drows, dweights, None
+        return _once(drows, weights, dout), _once(dweights, rows, dout), None
 
 
 def combine(rows, weights, order):

@@ -265,6 +265,45 @@ def forward_mode_is_refused():
             assert torch.equal(a, b)
 
 
+def second_derivatives():
+    """create_graph: gradients come as without it, those of other layers can be differentiated again, and what
+    needs a second derivative of an expert layer is an error, also where the incoming gradient is a constant."""
+    T, K, E, d = 6, 2, 4, 64
+    o = experts.sort_by_expert(experts.route(torch.randn(T, E, device="cuda"), K)[0], E)
+
+    def leaf(*shape):
+        return torch.randn(*shape, device="cuda", requires_grad=True)
+
+    s, x, y, w = leaf(T, E), leaf(T, d), leaf(T * K, d), leaf(T, K)
+    by = torch.randn(T, K, device="cuda")
+    layers = (([s], lambda: (experts.route(s, K)[1] * by).sum(), [True]),
+              ([s], lambda: experts.route(s, K, over_all=True)[1].square().sum(), [True]),
+              ([x], lambda: experts.dispatch(x, o).square().sum(), [True]),
+              ([x], lambda: experts.dispatch(x, o).sum(), [False]),  # (the gradient is top_k, whatever x is)
+              ([y, w], lambda: experts.combine(y, w, o).sum(), [True, True]),
+              ([y, w], lambda: experts.combine(y, w, o).square().sum(), [True, True]))
+    for leaves, f, depends in layers:
+        want = torch.autograd.grad(f(), leaves)
+        scale = leaf(1)
+        got = torch.autograd.grad(f() * 1 + scale.pow(3).sum(), leaves + [scale], create_graph=True)
+        for a, b, on in zip(got, want, depends):
+            assert torch.equal(a, b) and a.requires_grad == on
+            if on:
+                refuses(RuntimeError, torch.autograd.grad, a.square().sum(), leaves, retain_graph=True, allow_unused=True)
+        # a penalty on another layer's gradient
+        second, = torch.autograd.grad(got[-1].square().sum(), scale)
+        assert torch.allclose(second, 36 * scale.detach() ** 3)
+        # gradients added up in place, twice
+        for t in leaves:
+            t.grad = None
+        for k in (1, 2):
+            f().backward(create_graph=True)
+            for t, b in zip(leaves, want):
+                assert torch.allclose(t.grad, k * b, rtol=1e-6)
+        for t in leaves:
+            t.grad = None
+
+
 def main():
     for name in sys.argv[1:]:
         print("# " + name, flush=True)

@@ -20,6 +20,7 @@ CHECKS = [
     "a_token_served_alone",
     "labels_in_order",
     "forward_mode_is_refused",
+    "second_derivatives",
 ]
 
 
