@@ -1029,8 +1029,10 @@ KM_API int h2o4gpu_experts_route(int dtype, size_t rows, int experts, int top_k,
         constexpr int KT = decltype(kt)::value;
         int parts = 1;  // until there are some 2048 wavefronts, or a stretch is as short as a load's eight
         while (parts < 16 && (n + 63) / 64 * parts < 2048 && experts / (parts * 2) >= 8) parts *= 2;
-        hipLaunchKernelGGL((route_columns_kernel<T, decltype(all)::value, KT>), dim3(grid_of((rows + 63) / 64)),
-                           dim3(64 * parts), parts > 1 ? sizeof(float) * parts * (2 * KT + 1) * 64 : 0, s, scores,
+        auto kernel = route_columns_kernel<T, decltype(all)::value, KT>;
+        const size_t lds = parts > 1 ? sizeof(float) * parts * (2 * KT + 1) * 64 : 0;  // (68 KB for 16 lists of eight)
+        KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
+        hipLaunchKernelGGL(kernel, dim3(grid_of((rows + 63) / 64)), dim3(64 * parts), lds, s, scores,
                            (int64_t)expert_stride, n, experts, top_k, largest != 0, scale, d_experts, d_weights);
         return launched();
       };

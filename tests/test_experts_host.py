@@ -1,6 +1,7 @@
 """Host-side pieces of the expert layers and 4-bit products that need no GPU. They run in a child process:
 PyTorch's copy of the HIP runtime is never loaded beside the library's in this one."""
 import os
+import re
 import subprocess
 import sys
 
@@ -33,3 +34,30 @@ if m >= 64 * cols:  # every column about as often as any other
     share = torch.bincount(at %% cols, minlength=cols).double() * cols / m
     assert 0.8 <= float(share.min()) and float(share.max()) <= 1.2, share
 """ % (n, m, cols))
+
+
+def launches(text):
+    """(kernel, bytes of dynamic LDS, what precedes) of every launch in a source."""
+    for at in (m.end() for m in re.finditer(r"hipLaunchKernelGGL\(", text)):
+        depth, args, start = 0, [], at
+        for i in range(at, len(text)):
+            if text[i] == "," and depth == 0:
+                args.append(text[start:i].strip())
+                start = i + 1
+            depth += (text[i] in "({[") - (text[i] in ")}]")
+            if depth < 0:
+                break
+        yield args[0], args[3], text[:at]
+
+
+@pytest.mark.parametrize("name", ["experts_kernels.hip", "codebook4_kernels.hip"])
+def test_launches_with_dynamic_lds_raise_their_kernel_s_limit(name):
+    """The limit is 64 KB unless it is raised: every launch whose bytes are not a constant goes by the helper."""
+    text = open(os.path.join(ROOT, "h2o4gpu_amd", "csrc", name)).read()
+    found = list(launches(text))
+    assert len(found) >= 4
+    for kernel, lds, before in found:
+        if lds == "0":
+            continue
+        asked = "KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(%s), %s));" % (kernel, lds)
+        assert asked in before[-1200:], "%s is launched with %s bytes" % (kernel, lds)
