@@ -8,8 +8,11 @@
  *
  * Every pointer named d_* is device memory of the CURRENT device. Work is queued on `stream` (a
  * hipStream_t, NULL = the default stream) and the call returns without waiting; no function
- * allocates, copies to the host or keeps anything between calls, so all of them can be recorded
- * into a graph. Strides count elements. A call that returns an error has queued nothing, but for
+ * allocates, copies to the host or keeps data or a workspace between calls, so all of them can be
+ * recorded into a graph. What stays is a kernel's limit of shared memory on a device: a call that
+ * needs more than 64 KB and more than any before it raises it, and is to be outside a capture, so
+ * make one of the same type and sizes before recording. That may be route (distances), sort and
+ * both products. Strides count elements. A call that returns an error has queued nothing, but for
  * H2O4GPU_KMEANS_EDEVICE. Sizes of 0 rows are a success that queues nothing (but for the offsets
  * of experts_sort). Same inputs give the same bits in every call.
  * Status codes are those of h2o4gpu_kmeans.h.
@@ -113,8 +116,7 @@ int h2o4gpu_codebook4_layout(size_t experts, size_t out, size_t cols, int group,
                              size_t codes_pitch, int scale_dtype, const void *d_scales, void *d_laid_codes,
                              void *d_laid_scales, void *stream);
 /* d_y [rows][out] = d_x [rows][cols] times the matrix's transpose; products and sums in float, one
- * rounding at the end. (Both products: the first call of a type and size sets its kernel's limit of shared
- * memory, and is to be outside a capture.) */
+ * rounding at the end. */
 int h2o4gpu_codebook4_product(int dtype, size_t rows, size_t out, size_t cols, int group, const void *d_x,
                               size_t x_stride, const void *d_laid_codes, int scale_dtype, const void *d_laid_scales,
                               const void *d_codebook, void *d_y, size_t y_stride, void *stream);
