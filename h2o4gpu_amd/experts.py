@@ -10,12 +10,13 @@ centroids or scores, and the results come back and are joined by weight.
     Y = experts.combine(rows, weights, order)
 
 `route`, `dispatch` and `combine` have gradients (with respect to the scores, the tokens, the rows
-and the weights); forward-mode derivatives are refused. All work is queued on the current stream of the tensors' device, nothing waits
-for it and nothing is copied to the host, so the calls can be recorded into a graph (after a call of
-the same type and sizes outside of one, which may raise a kernel's limit of shared memory). Tensors are
-read on that stream: one that another stream writes has to be waited for, as with any torch
-operation, and an ExpertOrder used on another stream than it was made on likewise. Same inputs give
-the same bits. The kernels are the library's (include/h2o4gpu_experts.h); there is no CPU path.
+and the weights); forward-mode derivatives are refused. All work is queued on the current stream of
+the tensors' device, nothing waits for it and nothing is copied to the host, so the calls can be
+recorded into a graph (after a call of the same type and sizes outside of one, which may raise a
+kernel's limit of shared memory). Tensors are read on that stream: one that another stream writes has
+to be waited for, as with any torch operation, and an ExpertOrder used on another stream than it was
+made on likewise. Same inputs give the same bits. The kernels are the library's
+(include/h2o4gpu_experts.h); there is no CPU path.
 """
 import functools
 
