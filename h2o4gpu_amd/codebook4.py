@@ -20,12 +20,20 @@ from .experts import _TYPES, _call, _no_tangents, _order_of, _rows, _tensor, _ty
 from .libs import experts_hip
 
 
+def _group_of(group):
+    group = int(group)
+    if group < 32 or group % 32 or group > experts_hip.MAX_GROUP:
+        raise ValueError("group must be a multiple of 32, at most %d, got %d" % (experts_hip.MAX_GROUP, group))
+    return group
+
+
 class Codebook4:
     """A 4-bit matrix (out, cols), or one per expert (experts, out, cols).
 
     codes: uint8 (..., out, bytes), two columns a byte, the even one in the low half; bytes is at least
     cols / 2 rounded up. scales: (..., out, ceil(cols / group)), float32, bfloat16 or float16; group is a
-    multiple of 32. codebook: (16,) or (experts, 16) finite values in the type of the tokens.
+    multiple of 32 (longer than a row: one scale a row). codebook: (16,) or (experts, 16) finite values in
+    the type of the tokens.
 
     Codes and scales are copied once into the order that the products read them in (`laid_codes`,
     `laid_scales`); those passed in are not needed afterwards. `dtype` is that of the tokens.
@@ -43,9 +51,7 @@ class Codebook4:
         _type_of("scales", scales)
         _tensor("codebook", codebook, codebook.dim() if isinstance(codebook, torch.Tensor) else 1, codes.device)
         _type_of("codebook", codebook)
-        cols, group = int(cols), int(group)
-        if group < 32 or group % 32:
-            raise ValueError("group must be a multiple of 32, got %d" % group)
+        cols, group = int(cols), _group_of(group)
         if cols < 1 or codes.shape[-1] < (cols + 1) // 2:
             raise ValueError("%d bytes a row do not hold %d columns" % (codes.shape[-1], cols))
         if codes.shape[-2] < 1 or (lead and not 1 <= codes.shape[0] <= experts_hip.MAX_EXPERTS):
@@ -99,7 +105,7 @@ class Codebook4:
             values = table[torch.arange(self.n_experts, device=codes.device)[:, None, None], codes]
         else:
             values = table[codes]
-        return values * self.scales().float().repeat_interleave(self.group, -1)[..., :self.cols]
+        return values * self.scales().float()[..., torch.arange(self.cols, device=codes.device) // self.group]
 
 
 def _spread(n, m, device=None):
@@ -138,9 +144,7 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
     """
     _tensor("weights", weights, weights.dim() if isinstance(weights, torch.Tensor) and weights.dim() == 3 else 2)
     code = _type_of("weights", weights)
-    group, top = int(group), float(top)
-    if group < 32 or group % 32:
-        raise ValueError("group must be a multiple of 32, got %d" % group)
+    group, top = _group_of(group), float(top)
     if min(weights.shape) < 1:
         raise ValueError("weights are empty: %s" % (tuple(weights.shape),))
     if not 0.0 < top <= 3.4e38:
@@ -155,7 +159,8 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
             raise ValueError("top goes with a given codebook; one that is fitted has 1")
         part = flat if flat.shape[0] <= 4096 else flat[_spread(flat.shape[0], 4096, flat.device)]
         part = part.float()
-        padded = torch.nn.functional.pad(part, (0, groups * group - cols)).reshape(part.shape[0], groups, group)
+        width = min(group, cols)  # (a longer group is a row)
+        padded = torch.nn.functional.pad(part, (0, groups * width - cols)).reshape(part.shape[0], groups, width)
         scaled = padded / padded.abs().amax(2, keepdim=True).clamp_min(1e-38)
         codebook = fit_codebook(scaled.reshape(part.shape[0], -1)[:, :cols])
     _tensor("codebook", codebook, 1, weights.device)

@@ -630,7 +630,7 @@ static const size_t MOST_OUT = 1 << 24, MOST_COLS4 = 1000000, MOST_ROWS4 = 21474
 
 static bool sizes_ok(size_t experts, size_t out, size_t cols, int group) {
   return experts >= 1 && experts <= H2O4GPU_EXPERTS_MAX_EXPERTS && out >= 1 && out <= MOST_OUT && cols >= 1 &&
-         cols <= MOST_COLS4 && group >= 32 && group % 32 == 0;
+         cols <= MOST_COLS4 && group >= 32 && group % 32 == 0 && group <= H2O4GPU_CODEBOOK4_MAX_GROUP;
 }
 
 static bool strided_ok(int dtype, const void *p, size_t stride, size_t cols) {

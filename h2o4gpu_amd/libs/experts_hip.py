@@ -16,6 +16,7 @@ c_void_p = ctypes.c_void_p
 FLOAT32, BFLOAT16, FLOAT16 = 0, 1, 2
 MAX_EXPERTS = 16384
 MAX_TOP_K = 64
+MAX_GROUP = 1 << 30
 
 # every symbol include/h2o4gpu_experts.h declares: name -> (restype, argtypes)
 PROTOTYPES = {

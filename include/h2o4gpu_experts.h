@@ -35,6 +35,7 @@ extern "C" {
 
 #define H2O4GPU_EXPERTS_MAX_EXPERTS 16384
 #define H2O4GPU_EXPERTS_MAX_TOP_K 64
+#define H2O4GPU_CODEBOOK4_MAX_GROUP (1 << 30)
 
 /* The top_k best experts of every row and their weights.
  * d_scores: rows x experts of `dtype`; element (t, e) lies at t * row_stride + e * expert_stride,
@@ -93,7 +94,7 @@ int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k, size_t
 
 /* A 4-bit matrix [out][cols]: codes are 4 bits each, the even column in a byte's low half, rows
  * codes_pitch bytes apart (at least cols / 2, rounded up); scales [out][ceil(cols / group)] of
- * `scale_dtype`, group a multiple of 32; codebook: 16 finite values of `dtype`. Element (n, k) is
+ * `scale_dtype`, group a multiple of 32 (up to MAX_GROUP); codebook: 16 finite values of `dtype`. Element (n, k) is
  * codebook[code(n, k)] * scales[n][k / group].
  *
  * quantize: codes and scales of a matrix d_w of `dtype`. A group's scale is its largest magnitude

@@ -304,6 +304,27 @@ def second_derivatives():
             t.grad = None
 
 
+def groups_longer_than_a_row():
+    """One scale a row, with groups of any length; a length that the library's int would cut off is refused (its
+    rows of scales would be other ones than those that were allocated)."""
+    W = torch.randn(40, 100, generator=gen(110)).cuda()
+    book = torch.linspace(-1, 1, 16, device="cuda")
+    x = torch.randn(3, 100, generator=gen(111)).cuda()
+    want = codebook4.quantize(W, 128, book)
+    fitted = codebook4.quantize(W, 128)
+    for group in (256, 32 * 1001, 1 << 30):
+        q = codebook4.quantize(W, group, book)
+        assert torch.equal(q.codes(), want.codes()) and torch.equal(q.scales(), want.scales())
+        assert torch.equal(q.dequantize(), want.dequantize())
+        near(codebook4.product(x, q), x.cpu().double() @ q.dequantize().cpu().double().t(),
+             product_bound(x.cpu(), q.dequantize().cpu().double()), "y")
+        assert torch.equal(codebook4.quantize(W, group).codebook, fitted.codebook)
+    codes, scales = torch.zeros(40, 50, dtype=torch.uint8, device="cuda"), torch.ones(40, 1, device="cuda")
+    for group in ((1 << 30) + 32, 2 ** 31 - 32, 2 ** 31, 2 ** 32 + 32, 2 ** 40):
+        refuses(ValueError, codebook4.quantize, W, group, book)
+        refuses(ValueError, codebook4.Codebook4, codes, scales, book, 100, group)
+
+
 def main():
     for name in sys.argv[1:]:
         print("# " + name, flush=True)

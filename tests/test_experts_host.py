@@ -36,6 +36,23 @@ if m >= 64 * cols:  # every column about as often as any other
 """ % (n, m, cols))
 
 
+def test_the_library_refuses_groups_that_its_counts_do_not_hold():
+    """cols + group is an int in the kernels."""
+    run(r"""
+from h2o4gpu_amd.libs import experts_hip as e
+lib = e.lib()
+for group, fine in ((32, True), (e.MAX_GROUP, True), (e.MAX_GROUP + 32, False), (2 ** 31 - 32, False)):
+    assert (lib.h2o4gpu_codebook4_scales_bytes(1, 4, 100, group, 0) > 0) == fine, group
+    if not fine:
+        assert lib.h2o4gpu_codebook4_quantize(0, 4, 100, group, 1.0, 16, 100, 16, 16, 50, 0, 16, None) == -2
+        assert lib.h2o4gpu_codebook4_layout(1, 4, 100, group, 16, 50, 0, 16, 16, 16, None) == -2
+        assert lib.h2o4gpu_codebook4_product(0, 1, 4, 100, group, 16, 100, 16, 0, 16, 16, 16, 4, None) == -2
+import re
+assert re.search(r"#define H2O4GPU_CODEBOOK4_MAX_GROUP \(1 << 30\)", open("include/h2o4gpu_experts.h").read())
+assert e.MAX_GROUP == 1 << 30
+""")
+
+
 def launches(text):
     """(kernel, bytes of dynamic LDS, what precedes) of every launch in a source."""
     for at in (m.end() for m in re.finditer(r"hipLaunchKernelGGL\(", text)):

@@ -21,6 +21,7 @@ CHECKS = [
     "labels_in_order",
     "forward_mode_is_refused",
     "second_derivatives",
+    "groups_longer_than_a_row",
 ]
 
 
