@@ -140,7 +140,9 @@ def quantize(weights, group=128, codebook=None, top=1.0, scale_dtype=None):
     A group's scale is its largest magnitude over `top`, and every element gets the code of the entry
     nearest to element / scale. codebook: 16 values (top: the one that a group's largest magnitude
     stands for, e.g. 7 for the integers -8 .. 7); None fits it to the scaled elements with k-means.
-    It is rounded to the weights' type before the codes are chosen. scale_dtype defaults to that type.
+    It is rounded to the weights' type before the codes are chosen. scale_dtype defaults to that type; a
+    scale that is 0 or no finite number of it (a float32 matrix beyond float16's 65504, say) becomes 1,
+    and what is larger than the codebook's largest value then is that value. NaN and infinities get code 0.
     """
     _tensor("weights", weights, weights.dim() if isinstance(weights, torch.Tensor) and weights.dim() == 3 else 2)
     code = _type_of("weights", weights)

@@ -154,7 +154,8 @@ def route(scores, top_k, largest=True, scale=1.0, over_all=False):
     """The `top_k` best experts of every row, best first, and their weights.
 
     scores: (rows, experts), any strides: a model's scores (largest=True) or squared distances as
-    KMeans.transform gives them (largest=False: the nearest are the best). Equal scores go to the
+    KMeans.transform gives them for float32 rows (largest=False: the nearest are the best; up to eight
+    of them are found in one pass over the distances, more in one for each). Equal scores go to the
     lowest index. NaN and the worst infinity mark experts that are not available; where none is left
     the expert is -1 and its weight 0. Scores of the best infinity share the weight equally.
 
@@ -218,7 +219,10 @@ def _workspace(slots, n_experts):
 
 def sort_by_expert(experts, n_experts):
     """ExpertOrder of the (tokens, top_k) int32 choices of `route` (or of (tokens,) labels).
-    A value that is none of 0 .. n_experts - 1 is a slot without an expert."""
+    A value that is none of 0 .. n_experts - 1 is a slot without an expert.
+
+    While it runs, many slots take a workspace: n_experts / 512 bytes a slot up to some 3200 experts, and
+    as a workgroup then has fewer slots, 20 bytes at 5000 and 256 at 16384."""
     if isinstance(experts, torch.Tensor) and experts.dim() == 1:
         experts = experts.unsqueeze(1)
     _tensor("experts", experts, 2, dtype=torch.int32)

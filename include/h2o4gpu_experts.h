@@ -100,7 +100,7 @@ int h2o4gpu_experts_combine_backward(int dtype, size_t tokens, int top_k, size_t
  * quantize: codes and scales of a matrix d_w of `dtype`. A group's scale is its largest magnitude
  * over `top` (> 0: the codebook's value that this magnitude stands for), rounded to scale_dtype (1
  * where that gives 0 or no finite number); an element's code is the entry nearest to element / scale,
- * ties to the lowest (0 for a NaN). A row's bytes behind column cols are written as 0. */
+ * ties to the lowest (0 for a NaN and an infinity). A row's bytes behind column cols are written as 0. */
 int h2o4gpu_codebook4_quantize(int dtype, size_t out, size_t cols, int group, float top, const void *d_w,
                                size_t w_stride, const void *d_codebook, void *d_codes, size_t codes_pitch,
                                int scale_dtype, void *d_scales, void *stream);
