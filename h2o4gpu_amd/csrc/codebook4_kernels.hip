@@ -704,7 +704,7 @@ static Tiling4 experts_tiling(int64_t rows, int64_t tiles, int subs, int per, bo
 // 3 x 2, 29.9 with 2 x 2; x 11008, 38.1 with 3 x 2 and 32.8 with 2 x 3 and half the teams.
 static Tiling4 product_tiling(int64_t rows, int64_t tiles, int64_t shares, int subs, int per, bool two_bytes) {
   // mt, nt, and for how many scales of 128 columns there are registers. (Two float scales beside 16-bit rows are more
-  // than there is room for with 3 x 2 and 1 x 4, by 3 and 6 registers: 48 rows x 8192 x 8192, groups of 64, take 23.2
+  // than there is room for with 3 x 2 and 1 x 4, by 12 and 24 bytes a lane: 48 rows x 8192 x 8192, groups of 64, take 23.2
   // us so and 22.0 with scales of 16 bits, of which 6 % fewer bytes are loaded; 64 experts of 2048 x 4096 with four
   // rows each 76 and 74.)
   static const int halves[][3] = {{3, 2, 2}, {2, 4, 1}, {2, 3, 2}, {1, 4, 2},
