@@ -3,7 +3,6 @@ line for each. Not collected by pytest.
 
 Oracles are the formulas in 64 bits; U32 is the largest relative error of one float32 rounding."""
 import json
-import math
 import os
 import sys
 import traceback
@@ -318,7 +317,8 @@ def groups_longer_than_a_row():
         assert torch.equal(q.dequantize(), want.dequantize())
         near(codebook4.product(x, q), x.cpu().double() @ q.dequantize().cpu().double().t(),
              product_bound(x.cpu(), q.dequantize().cpu().double()), "y")
-        assert torch.equal(codebook4.quantize(W, group).codebook, fitted.codebook)
+        # (means of at most 4000 values, whose order of addition is the fit's own)
+        assert float((codebook4.quantize(W, group).codebook - fitted.codebook).abs().max()) <= 4000 * U32
     codes, scales = torch.zeros(40, 50, dtype=torch.uint8, device="cuda"), torch.ones(40, 1, device="cuda")
     for group in ((1 << 30) + 32, 2 ** 31 - 32, 2 ** 31, 2 ** 32 + 32, 2 ** 40):
         refuses(ValueError, codebook4.quantize, W, group, book)
