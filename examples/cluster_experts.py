@@ -4,8 +4,9 @@
 
 k-means finds clusters of the tokens; every token goes to the linear models of its two nearest
 centres, whose results are joined by a softmax over the distances. The models learn by gradient
-descent through combine and dispatch. Then each is compressed to 4-bit codes of a codebook that
-k-means finds for its values, and single tokens are served from those.
+descent through combine, product and dispatch. Then each is compressed to 4-bit codes of a codebook
+that k-means finds for its values, and single tokens are served from those; and to microscaled 4-bit
+numbers, which are multiplied with tokens in such numbers.
 """
 import argparse
 import os
@@ -14,23 +15,25 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from h2o4gpu_amd import KMeans, codebook4, experts  # noqa: E402
+from h2o4gpu_amd import KMeans, codebook4, experts, microscale4  # noqa: E402
 
 
 def forward(x, distances, W, top_k, scale):
     chosen, weights = experts.route(distances, top_k, largest=False, scale=scale)
     order = experts.sort_by_expert(chosen, W.shape[0])
-    rows = experts.dispatch(x, order)
-    at = order.offsets.tolist()  # the training loop waits here for the rows' counts
-    y = torch.cat([rows[at[e]:at[e + 1]] @ W[e].t() for e in range(W.shape[0])])
-    return experts.combine(y, weights, order)
+    rows = experts.product(experts.dispatch(x, order), W, order)
+    return experts.combine(rows, weights, order)
 
 
 def serve(x, distances, packed, top_k, scale):
-    """The same with 4-bit models: nothing waits, so it can be recorded into a graph."""
+    """The same with 4-bit models: a codebook's, or microscaled ones and the tokens in 4 bits too."""
     chosen, weights = experts.route(distances, top_k, largest=False, scale=scale)
     order = experts.sort_by_expert(chosen, packed.n_experts)
-    return experts.combine(codebook4.experts_product(x, packed, order), weights, order)
+    if isinstance(packed, microscale4.Microscale4):
+        rows = microscale4.experts_product(microscale4.quantize(x), packed, order)
+    else:
+        rows = codebook4.experts_product(x, packed, order)
+    return experts.combine(rows, weights, order)
 
 
 def main(argv=None):
@@ -79,10 +82,13 @@ def main(argv=None):
         error = float((small - full).norm() / full.norm())
         one = serve(x[:1], distances[:1], packed, a.top_k, scale)
         same = float((one - small[:1]).abs().max() / small[:1].abs().max())
+        four = serve(x, distances, microscale4.quantize(W.detach()), a.top_k, scale)
+        four_error = float((four - full).norm() / full.norm())
     if not a.quiet:
-        print("loss %.4f -> %.4f; served with 4 bits: %.2f%% from the trained models" % (losses[0], losses[-1],
-                                                                                       100 * error))
-    return dict(loss_first=losses[0], loss_last=losses[-1], served_error=error, single_token=same)
+        print("loss %.4f -> %.4f; served with 4 bits: %.2f%% from the trained models, %.2f%% with the tokens in 4 bits"
+              % (losses[0], losses[-1], 100 * error, 100 * four_error))
+    return dict(loss_first=losses[0], loss_last=losses[-1], served_error=error, single_token=same,
+                served_four_error=four_error)
 
 
 if __name__ == "__main__":

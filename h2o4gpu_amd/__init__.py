@@ -7,7 +7,8 @@ The compute path is libh2o4gpu_kmeans_hip.so (hand-written HIP kernels behind th
 declared in include/h2o4gpu_kmeans.h); build it with `python -m h2o4gpu_amd.build`.
 
 On PyTorch-ROCm tensors, imported by themselves: h2o4gpu_amd.experts (rows to the models of their
-clusters and back, with gradients) and h2o4gpu_amd.codebook4 (4-bit matrices and their products).
+clusters, through them and back, with gradients), h2o4gpu_amd.codebook4 (4-bit matrices and their products) and
+h2o4gpu_amd.microscale4 (both operands of a product in microscaled 4 bits).
 """
 from .solvers.kmeans import KMeans, KMeansH2O  # noqa: F401
 

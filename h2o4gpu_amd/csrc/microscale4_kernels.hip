@@ -1,0 +1,399 @@
+// Microscaled 4-bit numbers: blocks of 32 elements with one sign, two exponent and one mantissa bit (0, 0.5, 1,
+// 1.5, 2, 3, 4, 6) share a power of two, 2^(byte - 127). Numbers into them and back, and products of two such
+// matrices on the scaled matrix instructions, which multiply 128 columns of both in the time of 32 in 16 bits.
+//
+// A matrix lies in memory in rows: codes two to a byte, the even column in the low half, 128 bytes (256 columns)
+// or a multiple to a row; scales 16 bytes for 512 columns, the byte of the block b of these 16 at 4 * (b % 4) + b / 4:
+// lane group g of a matrix instruction multiplies block g of its 128 columns, and has the scales of four
+// instructions in one word. Behind a row's last column lie zeros (codes and scales).
+#include "product_tiles.h"
+
+namespace kmhip {
+namespace {
+
+constexpr size_t MAX_SIDE = (size_t)1 << 30;
+
+__host__ __device__ inline size_t codes_pitch(size_t cols) { return (cols + 255) / 256 * 128; }
+__host__ __device__ inline size_t scales_pitch(size_t cols) { return (cols + 511) / 512 * 16; }
+__host__ __device__ inline unsigned scale_place(unsigned block) {
+  return block / 16 * 16 + block % 4 * 4 + block % 16 / 4;
+}
+// The element a code's low four bits stand for: sign, two bits of exponent, one of mantissa. The bits of 2 m, 2 m + 1
+// halves put where a float has its own make 2^-126 times as much (and 0.5 a denormal number that the product mends).
+__device__ __forceinline__ float element(unsigned code) {
+  const float m = __uint_as_float((code & 7) << 22) * 0x1p126f;
+  return __uint_as_float(__float_as_uint(m) | (code & 8) << 28);
+}
+__device__ __forceinline__ float power_of(unsigned byte) {
+  return byte == 255 ? __builtin_nanf("") : __uint_as_float(byte ? byte << 23 : 0x400000u);
+}
+
+// One thread: eight columns, a word of codes; four threads a block, which share its largest magnitude. A block's
+// power of two is that of the largest magnitude over 4, so that it lands in [4, 8), where 6 is the largest element
+// and what is beyond stays 6. Magnitudes are compared as their bits, in which NaN and infinities are the largest:
+// their block's scale is 255, not a number. Bound by memory: 512 bytes of 16-bit elements in, 136 out a wavefront.
+template <typename T, int UNROLL>
+__global__ __launch_bounds__(256) void quantize_kernel(const T *x, size_t x_stride, unsigned cols, size_t words,
+                                                       unsigned row_words, unsigned *codes, unsigned char *scales,
+                                                       unsigned scales_row) {
+  const size_t base = (size_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+  u32x4 in[UNROLL][sizeof(T) / 2];
+  size_t row[UNROLL];
+  unsigned word[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const size_t at = base + u * 256;
+    row[u] = at / row_words;
+    word[u] = (unsigned)(at - row[u] * row_words);
+    const int left = at < words ? (int)cols - (int)word[u] * 8 : 0;
+    const T *p = x + row[u] * x_stride + word[u] * 8;
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+      in[u][h] = load_piece(p + h * (16 / sizeof(T)), left - h * (int)(16 / sizeof(T)));
+  }
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(in[u][i / 4][i % 4]);
+      } else {
+        const unsigned short bits = (unsigned short)(in[u][0][i / 2] >> (16 * (i & 1)));
+        v[i] = (float)__builtin_bit_cast(T, bits);
+      }
+    }
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned m = __float_as_uint(v[i]) & 0x7fffffffu;
+      most = m > most ? m : most;
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+      const unsigned other = __shfl_xor(most, d);
+      most = other > most ? other : most;
+    }
+    const unsigned e = most >> 23, byte = e == 255 ? 255 : e > 2 ? e - 2 : 0;
+    unsigned out = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+    // rounds to the nearest, a tie to the even mantissa, and saturates
+    const float power = __uint_as_float(byte ? byte << 23 : 0x400000u);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[0], v[1], power, 0);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[2], v[3], power, 1);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[4], v[5], power, 2);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[6], v[7], power, 3);
+#endif
+    if (byte == 255) out = 0;
+    if (base + u * 256 < words) {
+      codes[base + u * 256] = out;
+      if ((word[u] & 3) == 0) {
+        unsigned char *s = scales + row[u] * scales_row + scale_place(word[u] / 4);
+        s[0] = (unsigned char)byte;
+        // the last 256 columns of a row that is no multiple of 512: the other half's bytes
+        if ((word[u] & 63) < 32 && (word[u] | 31) == row_words - 1) s[2] = 0;
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dequantize_kernel(const unsigned *codes, const unsigned char *scales, unsigned cols,
+                                                         size_t words, unsigned row_words, unsigned scales_row, T *out,
+                                                         size_t out_stride, int aligned) {
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= words) return;
+  const size_t row = at / row_words;
+  const unsigned word = (unsigned)(at - row * row_words);
+  if (word * 8 >= cols) return;
+  const unsigned code = codes[row * (codes_pitch(cols) / 4) + word];
+  const float power = power_of(scales[row * scales_row + scale_place(word / 4)]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = element(code >> (4 * i)) * power;
+  T *o = out + row * out_stride + word * 8;
+  const int left = (int)cols - (int)word * 8;
+  store_four(o, f32x4{v[0], v[1], v[2], v[3]}, left, aligned);
+  store_four(o + 4, f32x4{v[4], v[5], v[6], v[7]}, left - 4, aligned);
+}
+
+// Codes and scales that come in plain rows, into the layout above.
+__global__ __launch_bounds__(256) void layout_kernel(const unsigned char *in, size_t in_pitch, const unsigned char *in_scales,
+                                                     unsigned cols, size_t words, unsigned row_words, unsigned *codes,
+                                                     unsigned char *scales, unsigned scales_row) {
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= words) return;
+  const size_t row = at / row_words;
+  const unsigned word = (unsigned)(at - row * row_words);
+  unsigned out = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned col = word * 8 + 2 * i;
+    if (col < cols) {
+      unsigned two = in[row * in_pitch + col / 2];
+      if (col + 1 == cols) two &= 15;
+      out |= two << (8 * i);
+    }
+  }
+  codes[at] = out;
+  if ((word & 3) == 0) {
+    const unsigned block = word / 4, blocks = (cols + 31) / 32;
+    unsigned char *s = scales + row * scales_row + scale_place(block);
+    s[0] = block < blocks ? in_scales[row * blocks + block] : 0;
+    if ((word & 63) < 32 && (word | 31) == row_words - 1) s[2] = 0;
+  }
+}
+
+struct FourArgs {
+  const unsigned char *x, *x_scales, *w, *w_scales;
+  void *y;
+  size_t y_stride;
+  const int *order, *offsets;  // with experts only; order: x's row of y's row p is order[p] / top_k (none: p)
+  int top_k, experts;          // experts 0: one matrix
+  int rows, out, cols, y_aligned;
+};
+
+__device__ __forceinline__ void to_lds_16(const void *from, char *lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)(lds), 16, 0, 0);
+#else
+  (void)from;
+  (void)lds;
+#endif
+}
+
+template <int STEP>
+__device__ __forceinline__ void mfma_four(f32x4 &acc, u32x4 w, u32x4 x, unsigned sw, unsigned sx) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef int i32x8 __attribute__((ext_vector_type(8)));
+  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, STEP, (int)sw, STEP, (int)sx);
+#endif
+}
+
+// Stages of 256 columns go straight to LDS, two of them: the next is on its way while one is multiplied.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
+  typedef OperandTile<bfloat16_t, BM, false> TX;  // (bytes are bytes: a stage is 128 of each row)
+  typedef OperandTile<bfloat16_t, BN, false> TW;
+  constexpr int THREADS = WM * WN * 64;
+  constexpr int PX = TX::SLOTS / THREADS, PW = TW::SLOTS / THREADS;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr int STAGE = (BM + BN) * 128;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n_tiles = (a.out + BN - 1) / BN;
+  const int n0 = (int)(blockIdx.x % n_tiles) * BN, number = (int)(blockIdx.x / n_tiles);
+  int expert = 0, first = number * BM, m_here = a.rows - first < BM ? a.rows - first : BM;
+  int stages = (a.cols + 255) / 256;
+  if (a.experts) {
+    if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here)) return;
+    if (expert == a.experts) stages = 0, expert = 0;
+  }
+  const int n_here = a.out - n0 < BN ? a.out - n0 : BN;
+  const size_t pitch = codes_pitch(a.cols), spitch = scales_pitch(a.cols);
+  const size_t w_row = (size_t)expert * a.out + n0;
+  auto x_row = [&](int m) -> size_t {
+    m = first + (m < m_here ? m : m_here - 1);
+    return a.order ? (size_t)(a.order[m] / a.top_k) : (size_t)m;
+  };
+  const unsigned char *gx[PX], *gw[PW];
+  const int wm = wave / WN, wn = wave % WN;
+  const unsigned char *sx_at[FM], *sw_at[FN];
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (stages) {
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      int r, k;
+      TX::place(i * THREADS + tid, r, k);
+      gx[i] = a.x + x_row(r) * pitch + k * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      int r, k;
+      TW::place(i * THREADS + tid, r, k);
+      gw[i] = a.w + (w_row + (r < n_here ? r : n_here - 1)) * pitch + k * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      sx_at[i] = a.x_scales + x_row((wm * FM + i) * 16 + (lane & 15)) * spitch + 4 * (lane >> 4);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int r = (wn * FN + j) * 16 + (lane & 15);
+      sw_at[j] = a.w_scales + (w_row + (r < n_here ? r : n_here - 1)) * spitch + 4 * (lane >> 4);
+    }
+  }
+  auto load = [&](int t) {
+    char *at = lds + (t & 1) * STAGE + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < PX; ++i) to_lds_16(gx[i] + (size_t)t * 128, at + i * THREADS * 16);
+#pragma unroll
+    for (int i = 0; i < PW; ++i) to_lds_16(gw[i] + (size_t)t * 128, at + BM * 128 + i * THREADS * 16);
+  };
+  if (stages) load(0);
+  for (int t = 0; t < stages; ++t) {
+    unsigned sx[FM], sw[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      sx[i] = *reinterpret_cast<const unsigned *>(sx_at[i] + (size_t)(t / 2) * 16) >> (16 * (t & 1));
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      sw[j] = *reinterpret_cast<const unsigned *>(sw_at[j] + (size_t)(t / 2) * 16) >> (16 * (t & 1));
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the stage has arrived
+    __syncthreads();
+    if (t + 1 < stages) load(t + 1);
+    const char *at = lds + (t & 1) * STAGE;
+    auto step = [&](auto number) {
+      constexpr int STEP = decltype(number)::value;
+      u32x4 fx[FM], fw[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, wm * FM + i, STEP);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fw[j] = TW::fragment(at + BM * 128, lane, wn * FN + j, STEP);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) mfma_four<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
+    };
+    step(Int<0>());
+    step(Int<1>());
+    __syncthreads();
+  }
+  T *y = static_cast<T *>(a.y) + (size_t)first * a.y_stride + n0;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = (wm * FM + i) * 16 + (lane & 15);
+    if (m >= m_here) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
+      store_four(y + (size_t)m * a.y_stride + n, acc[i][j], n_here - n, a.y_aligned);
+    }
+  }
+}
+
+template <typename T>
+int launch_four(const FourArgs &a, hipStream_t stream) {
+  constexpr int BM = 128, BN = 128;
+  const size_t m_tiles = a.experts ? ragged_tiles(a.experts, a.rows, BM) : ((size_t)a.rows + BM - 1) / BM;
+  const size_t n_tiles = ((size_t)a.out + BN - 1) / BN;
+  hipLaunchKernelGGL((four_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(m_tiles * n_tiles)), dim3(256), 0, stream, a);
+  return launched();
+}
+
+bool sized(size_t rows, size_t cols) { return cols >= 1 && cols <= MAX_SIDE && rows <= ((size_t)1 << 40) / codes_pitch(cols); }
+
+}  // namespace
+}  // namespace kmhip
+
+using namespace kmhip;
+
+KM_API size_t h2o4gpu_microscale4_codes_pitch(size_t cols) { return cols < 1 || cols > MAX_SIDE ? 0 : codes_pitch(cols); }
+KM_API size_t h2o4gpu_microscale4_scales_pitch(size_t cols) {
+  return cols < 1 || cols > MAX_SIDE ? 0 : scales_pitch(cols);
+}
+
+KM_API int h2o4gpu_microscale4_quantize(int dtype, size_t rows, size_t cols, const void *d_x, size_t x_stride,
+                                        void *d_codes, void *d_scales, void *stream) {
+  if (!known_type(dtype) || !sized(rows, cols)) return H2O4GPU_KMEANS_EARG;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_x || !d_codes || !d_scales || (rows > 1 && x_stride < cols) || !aligned_to(d_codes, 16) ||
+      !aligned_to(d_scales, 16))
+    return H2O4GPU_KMEANS_EARG;
+  return with_type(dtype, [&](auto tag) {
+    typedef typename decltype(tag)::type T;
+    constexpr int UNROLL = 2;
+    const unsigned row_words = (unsigned)(codes_pitch(cols) / 4);
+    const size_t words = rows * row_words, blocks = (words + 256 * UNROLL - 1) / (256 * UNROLL);
+    hipLaunchKernelGGL((quantize_kernel<T, UNROLL>), dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const T *>(d_x), x_stride, (unsigned)cols, words, row_words,
+                       static_cast<unsigned *>(d_codes), static_cast<unsigned char *>(d_scales),
+                       (unsigned)scales_pitch(cols));
+    return launched();
+  });
+}
+
+KM_API int h2o4gpu_microscale4_dequantize(int dtype, size_t rows, size_t cols, const void *d_codes, const void *d_scales,
+                                          void *d_out, size_t out_stride, void *stream) {
+  if (!known_type(dtype) || !sized(rows, cols)) return H2O4GPU_KMEANS_EARG;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_out || !d_codes || !d_scales || (rows > 1 && out_stride < cols) || !aligned_to(d_codes, 16) ||
+      !aligned_to(d_scales, 16))
+    return H2O4GPU_KMEANS_EARG;
+  return with_type(dtype, [&](auto tag) {
+    typedef typename decltype(tag)::type T;
+    const unsigned row_words = (unsigned)((cols + 7) / 8);
+    const size_t words = rows * row_words;
+    const int aligned = out_stride % 4 == 0 && aligned_to(d_out, 4 * sizeof(T));
+    hipLaunchKernelGGL((dequantize_kernel<T>), dim3((unsigned)((words + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const unsigned *>(d_codes),
+                       static_cast<const unsigned char *>(d_scales), (unsigned)cols, words, row_words,
+                       (unsigned)scales_pitch(cols), static_cast<T *>(d_out), out_stride, aligned);
+    return launched();
+  });
+}
+
+KM_API int h2o4gpu_microscale4_layout(size_t rows, size_t cols, const void *d_codes, size_t codes_stride,
+                                      const void *d_scales, void *d_laid_codes, void *d_laid_scales, void *stream) {
+  if (!sized(rows, cols)) return H2O4GPU_KMEANS_EARG;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_codes || !d_scales || !d_laid_codes || !d_laid_scales || codes_stride < (cols + 1) / 2 ||
+      !aligned_to(d_laid_codes, 16) || !aligned_to(d_laid_scales, 16))
+    return H2O4GPU_KMEANS_EARG;
+  const unsigned row_words = (unsigned)(codes_pitch(cols) / 4);
+  const size_t words = rows * row_words;
+  hipLaunchKernelGGL(layout_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const unsigned char *>(d_codes), codes_stride,
+                     static_cast<const unsigned char *>(d_scales), (unsigned)cols, words, row_words,
+                     static_cast<unsigned *>(d_laid_codes), static_cast<unsigned char *>(d_laid_scales),
+                     (unsigned)scales_pitch(cols));
+  return launched();
+}
+
+namespace {
+int four_product(int dtype, FourArgs a, size_t rows, size_t out, size_t cols, void *stream) {
+  if (!known_type(dtype) || !sized(rows, cols) || out < 1 || out > MAX_SIDE || rows > (size_t)INT_MAX - 65536)
+    return H2O4GPU_KMEANS_EARG;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!a.x || !a.x_scales || !a.w || !a.w_scales || !a.y || (rows > 1 && a.y_stride < out)) return H2O4GPU_KMEANS_EARG;
+  for (const void *p : {a.x, a.x_scales, a.w, a.w_scales})
+    if (!aligned_to(p, 16)) return H2O4GPU_KMEANS_EARG;
+  a.rows = (int)rows, a.out = (int)out, a.cols = (int)cols;
+  a.y_aligned = a.y_stride % 4 == 0 && aligned_to(a.y, 4 * type_size(dtype));
+  return with_type(dtype, [&](auto tag) {
+    return launch_four<typename decltype(tag)::type>(a, static_cast<hipStream_t>(stream));
+  });
+}
+}  // namespace
+
+KM_API int h2o4gpu_microscale4_product(int dtype, size_t rows, size_t out, size_t cols, const void *d_x,
+                                       const void *d_x_scales, const void *d_w, const void *d_w_scales, void *d_y,
+                                       size_t y_stride, void *stream) {
+  FourArgs a = {};
+  a.x = static_cast<const unsigned char *>(d_x), a.x_scales = static_cast<const unsigned char *>(d_x_scales);
+  a.w = static_cast<const unsigned char *>(d_w), a.w_scales = static_cast<const unsigned char *>(d_w_scales);
+  a.y = d_y, a.y_stride = y_stride;
+  return four_product(dtype, a, rows, out, cols, stream);
+}
+
+KM_API int h2o4gpu_microscale4_experts_product(int dtype, size_t tokens, int top_k, int experts, size_t out, size_t cols,
+                                               const void *d_x, const void *d_x_scales, const void *d_w,
+                                               const void *d_w_scales, const int *d_order, const int *d_offsets, void *d_y,
+                                               size_t y_stride, void *stream) {
+  if (experts < 1 || experts > H2O4GPU_EXPERTS_MAX_EXPERTS || top_k < 1 || top_k > H2O4GPU_EXPERTS_MAX_TOP_K ||
+      tokens > (size_t)INT_MAX)
+    return H2O4GPU_KMEANS_EARG;
+  if (tokens && !d_offsets) return H2O4GPU_KMEANS_EARG;
+  FourArgs a = {};
+  a.x = static_cast<const unsigned char *>(d_x), a.x_scales = static_cast<const unsigned char *>(d_x_scales);
+  a.w = static_cast<const unsigned char *>(d_w), a.w_scales = static_cast<const unsigned char *>(d_w_scales);
+  a.y = d_y, a.y_stride = y_stride;
+  a.order = d_order, a.offsets = d_offsets, a.top_k = top_k, a.experts = experts;
+  return four_product(dtype, a, tokens * top_k, out, cols, stream);
+}

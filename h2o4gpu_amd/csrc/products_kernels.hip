@@ -1,0 +1,211 @@
+// Products grouped by expert: rows in expert order times each expert's matrix, and the two gradients.
+//
+//   product:          y[p] = W[e] x[p]                     p in [offsets[e], offsets[e + 1])
+//   product_drows:    dx[p] = W[e]^T dy[p]
+//   product_dweights: dW[e] = sum over p of dy[p] x[p]^T
+//
+// Sums are float32, in an order that depends on the sizes alone; one rounding at the end.
+#include "product_tiles.h"
+
+namespace kmhip {
+namespace {
+
+enum Kind { FORWARD, DROWS, DWEIGHTS };
+
+struct ProductArgs {
+  const void *x;  // m's operand: rows in expert order (dy of DWEIGHTS)
+  const void *w;  // n's operand: the matrices (x of DWEIGHTS)
+  void *c;
+  size_t x_stride, w_stride, w_expert, c_stride, c_expert;
+  const int *offsets;
+  int experts, rows, n, k;  // DWEIGHTS: n = cols, k = out, which is C's m
+  int c_aligned;            // four elements of C may be stored at once
+};
+
+// Any strides and alignment: pieces come through registers, masked at the edges. Two stages in LDS.
+template <typename T, Kind KIND, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
+  constexpr bool XC = KIND == DWEIGHTS, WC = KIND != FORWARD;
+  typedef OperandTile<T, BM, XC> TX;
+  typedef OperandTile<T, BN, WC> TW;
+  constexpr int THREADS = WM * WN * 64, KS = TX::KS;
+  constexpr int PX = TX::SLOTS / THREADS, PW = TW::SLOTS / THREADS;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr int STAGE = (BM + BN) * 128;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * BN;
+  int expert, first, m_here;
+  const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
+  T *c = static_cast<T *>(a.c);
+  int k_end = a.k;
+  if (KIND == DWEIGHTS) {
+    const int tiles = (a.k + BM - 1) / BM;
+    expert = blockIdx.y / tiles;
+    first = (blockIdx.y % tiles) * BM;
+    m_here = a.k - first < BM ? a.k - first : BM;
+    const int begin = a.offsets[expert];
+    k_end = a.offsets[expert + 1] - begin;
+    x += (size_t)begin * a.x_stride + first;
+    w += (size_t)begin * a.w_stride;
+    c += (size_t)expert * a.c_expert + (size_t)first * a.c_stride;
+  } else {
+    if (!ragged_tile(a.offsets, a.experts, a.rows, BM, blockIdx.y, expert, first, m_here)) return;
+    x += (size_t)first * a.x_stride;
+    c += (size_t)first * a.c_stride;
+    w += (size_t)expert * a.w_expert;
+    if (expert == a.experts) k_end = 0;  // rows without an expert: zeros
+  }
+  const int n_here = a.n - n0 < BN ? a.n - n0 : BN;
+  w += WC ? (size_t)n0 : (size_t)n0 * a.w_stride;
+
+  u32x4 px[PX], pw[PW];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      int r, k;
+      TX::place(i * THREADS + tid, r, k);
+      k += k0;
+      if (XC)
+        px[i] = load_piece(x + (size_t)k * a.x_stride + r, k < k_end ? m_here - r : 0);
+      else
+        px[i] = load_piece(x + (size_t)r * a.x_stride + k, r < m_here ? k_end - k : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      int r, k;
+      TW::place(i * THREADS + tid, r, k);
+      k += k0;
+      if (WC)
+        pw[i] = load_piece(w + (size_t)k * a.w_stride + r, k < k_end ? n_here - r : 0);
+      else
+        pw[i] = load_piece(w + (size_t)r * a.w_stride + k, r < n_here ? k_end - k : 0);
+    }
+  };
+  auto put = [&](char *at) {
+#pragma unroll
+    for (int i = 0; i < PX; ++i) *reinterpret_cast<u32x4 *>(at + (i * THREADS + tid) * 16) = px[i];
+#pragma unroll
+    for (int i = 0; i < PW; ++i) *reinterpret_cast<u32x4 *>(at + BM * 128 + (i * THREADS + tid) * 16) = pw[i];
+  };
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wm = wave / WN, wn = wave % WN;
+  const int stages = (k_end + KS - 1) / KS;
+  if (stages > 0) {
+    load(0);
+    put(lds);
+  }
+  __syncthreads();
+  for (int t = 0; t < stages; ++t) {
+    const char *at = lds + (t & 1) * STAGE;
+    if (t + 1 < stages) load((t + 1) * KS);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      u32x4 fx[FM], fw[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, wm * FM + i, step);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fw[j] = TW::fragment(at + BM * 128, lane, wn * FN + j, step);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) mfma_piece(acc[i][j], fw[j], fx[i], Tag<T>());
+    }
+    if (t + 1 < stages) put(lds + ((t + 1) & 1) * STAGE);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = (wm * FM + i) * 16 + (lane & 15);
+    if (m >= m_here) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
+      store_four(c + (size_t)m * a.c_stride + n0 + n, acc[i][j], n_here - n, a.c_aligned);
+    }
+  }
+}
+
+template <typename T, Kind KIND>
+int launch_product(const ProductArgs &a, hipStream_t stream) {
+  constexpr int BM = 128, BN = 128;
+  const size_t m_tiles =
+      KIND == DWEIGHTS ? (size_t)a.experts * ((a.k + BM - 1) / BM) : ragged_tiles(a.experts, a.rows, BM);
+  const size_t n_tiles = ((size_t)a.n + BN - 1) / BN;
+  hipLaunchKernelGGL((product_kernel<T, KIND, BM, BN, 2, 2>), dim3((unsigned)n_tiles, (unsigned)m_tiles), dim3(256), 0,
+                     stream, a);
+  return launched();
+}
+
+// Strides of rows of `cols` elements, each row apart from the next.
+bool fits(size_t rows, size_t cols, size_t stride) { return rows < 2 || stride >= cols; }
+
+constexpr size_t MAX_SIDE = (size_t)1 << 30;
+
+// What all three have in common. > 0: go on, else the status to return.
+int check(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *offsets) {
+  if (!known_type(dtype) || experts < 1 || experts > H2O4GPU_EXPERTS_MAX_EXPERTS) return H2O4GPU_KMEANS_EARG;
+  if (out < 1 || cols < 1 || out > MAX_SIDE || cols > MAX_SIDE || rows > (size_t)INT_MAX - 65536 || !offsets)
+    return H2O4GPU_KMEANS_EARG;
+  return 1;
+}
+
+}  // namespace
+}  // namespace kmhip
+
+using namespace kmhip;
+
+KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
+                                   size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
+                                   const int *d_offsets, void *d_y, size_t y_stride, void *stream) {
+  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "");
+      rc <= 0)
+    return rc;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_rows || !d_weights || !d_y || !fits(rows, cols, rows_stride) || !fits(out, cols, w_stride) ||
+      !fits(rows, out, y_stride))
+    return H2O4GPU_KMEANS_EARG;
+  ProductArgs a = {d_rows, d_weights, d_y, rows_stride, w_stride, expert_stride, y_stride, 0, d_offsets, experts, (int)rows,
+                   (int)out, (int)cols, 0};
+  a.c_aligned = y_stride % 4 == 0 && aligned_to(d_y, 4 * type_size(dtype));
+  return with_type(dtype, [&](auto tag) {
+    return launch_product<typename decltype(tag)::type, FORWARD>(a, static_cast<hipStream_t>(stream));
+  });
+}
+
+KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
+                                         size_t dy_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
+                                         const int *d_offsets, void *d_drows, size_t drows_stride, void *stream) {
+  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : ""); rc <= 0) return rc;
+  if (rows == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_dy || !d_weights || !d_drows || !fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
+      !fits(rows, cols, drows_stride))
+    return H2O4GPU_KMEANS_EARG;
+  ProductArgs a = {d_dy, d_weights, d_drows, dy_stride, w_stride, expert_stride, drows_stride, 0, d_offsets, experts,
+                   (int)rows, (int)cols, (int)out, 0};
+  a.c_aligned = drows_stride % 4 == 0 && aligned_to(d_drows, 4 * type_size(dtype));
+  return with_type(dtype, [&](auto tag) {
+    return launch_product<typename decltype(tag)::type, DROWS>(a, static_cast<hipStream_t>(stream));
+  });
+}
+
+KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols,
+                                            const void *d_dy, size_t dy_stride, const void *d_rows, size_t rows_stride,
+                                            const int *d_offsets, void *d_dweights, void *stream) {
+  if (int rc = check(dtype, rows, experts, out, cols, d_offsets); rc <= 0) return rc;
+  if (!d_dweights || (rows && (!d_dy || !d_rows)) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
+    return H2O4GPU_KMEANS_EARG;
+  ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
+                   (int)cols, (int)out, 0};
+  a.c_aligned = cols % 4 == 0 && aligned_to(d_dweights, 4 * type_size(dtype));
+  return with_type(dtype, [&](auto tag) {
+    return launch_product<typename decltype(tag)::type, DWEIGHTS>(a, static_cast<hipStream_t>(stream));
+  });
+}

@@ -6,11 +6,11 @@ centroids or scores, and the results come back and are joined by weight.
     chosen, weights = experts.route(model.transform(X), top_k=2, largest=False)
     order = experts.sort_by_expert(chosen, 64)
     rows = experts.dispatch(X, order)              # rows of expert 0, then of expert 1, ...
-    ...                                            # every expert works on its rows
+    rows = experts.product(rows, W, order)         # W (64, out, cols): a matrix per expert
     Y = experts.combine(rows, weights, order)
 
-`route`, `dispatch` and `combine` have gradients (with respect to the scores, the tokens, the rows
-and the weights); forward-mode derivatives are refused. All work is queued on the current stream of
+`route`, `dispatch`, `product` and `combine` have gradients (with respect to the scores, the tokens, the
+rows, the matrices and the weights); forward-mode derivatives are refused. All work is queued on the current stream of
 the tensors' device, nothing waits for it and nothing is copied to the host, so the calls can be
 recorded into a graph (after a call of the same type and sizes outside of one, which may raise a
 kernel's limit of shared memory). Tensors are read on that stream: one that another stream writes has
@@ -69,7 +69,7 @@ def _tensor(name, t, dims, device=None, dtype=None):
 
 def _rows(name, t):
     """(pointer, elements between rows) of a matrix whose rows are contiguous."""
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if t.stride(1) != 1 and t.shape[1] > 1 and t.shape[0] > 0:
         raise ValueError("the rows of %s must be contiguous (strides %s)" % (name, t.stride()))
     stride = t.stride(0)
     if t.shape[0] < 2:
@@ -342,3 +342,78 @@ def combine(rows, weights, order):
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _Combine.apply(rows, weights, order)
     return _combine(rows, weights, order)
+
+
+# ---- the experts' own products ----------------------------------------------------------------------
+
+def _matrices(weights):
+    """(pointer, elements between experts, elements between rows) of (experts, out, cols) with contiguous rows."""
+    n_experts, out, cols = weights.shape
+    expert_stride, stride, inner = weights.stride()
+    if inner != 1 and cols > 1:
+        raise ValueError("the rows of weights must be contiguous (strides %s)" % (weights.stride(),))
+    if out < 2:
+        stride = cols
+    elif stride < cols:
+        raise ValueError("the rows of weights overlap (strides %s)" % (weights.stride(),))
+    return weights.data_ptr(), expert_stride, stride
+
+
+def _product(rows, weights, order):
+    ptr, stride = _rows("rows", rows)
+    n_experts, out, cols = weights.shape
+    y = rows.new_empty((rows.shape[0], out))
+    _call(rows.device.index, "h2o4gpu_experts_product", _TYPES[rows.dtype], rows.shape[0], n_experts, out, cols, ptr,
+          stride, *_matrices(weights), order._offsets_ptr, y.data_ptr(), out)
+    return y
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, order):
+        ctx.order = order
+        ctx.save_for_backward(rows, weights)
+        return _product(rows, weights, order)
+
+    @staticmethod
+    def backward(ctx, dy):
+        order = ctx.order
+        rows, weights = ctx.saved_tensors
+        dy = _gradient(dy)
+        ptr, stride = _rows("dy", dy)
+        n_experts, out, cols = weights.shape
+        code, count = _TYPES[dy.dtype], dy.shape[0]
+        drows = dweights = None
+        if ctx.needs_input_grad[0]:
+            drows = rows.new_empty(rows.shape)
+            _call(dy.device.index, "h2o4gpu_experts_product_drows", code, count, n_experts, out, cols, ptr, stride,
+                  *_matrices(weights), order._offsets_ptr, drows.data_ptr(), cols)
+            drows = _once(drows, weights, dy)
+        if ctx.needs_input_grad[1]:
+            dweights = weights.new_empty(weights.shape)
+            _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols, ptr, stride,
+                  *_rows("rows", rows), order._offsets_ptr, dweights.data_ptr())
+            dweights = _once(dweights, rows, dy)
+        return drows, dweights, None
+
+
+def product(rows, weights, order):
+    """(tokens * top_k, out): every row times the transpose of its expert's matrix, zeros in the places
+    behind order.offsets[-1] (what lies there in `rows` is not read). rows: (tokens * top_k, cols) in
+    expert order, as `dispatch` gives them; weights: (experts, out, cols) of the same type, rows of both
+    contiguous. Sums are float32, rounded once. Gradients for rows and weights; an expert without
+    rows has a gradient of zeros."""
+    if not (isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _TYPES):
+        _tensor("rows", rows, 2)
+        _type_of("rows", rows)
+    _order_of(order, rows.device)
+    _tensor("weights", weights, 3, rows.device, rows.dtype)
+    if weights.shape[0] != order.n_experts or weights.shape[1] < 1:
+        raise ValueError("weights must be (%d, out, cols), got %s" % (order.n_experts, tuple(weights.shape)))
+    if rows.shape[0] != order.tokens * order.top_k or rows.shape[1] != weights.shape[2] or rows.shape[1] < 1:
+        raise ValueError("rows must be (%d, %d), got %s" % (order.tokens * order.top_k, weights.shape[2],
+                                                            tuple(rows.shape)))
+    _no_tangents(rows, weights)
+    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return _Product.apply(rows, weights, order)
+    return _product(rows, weights, order)

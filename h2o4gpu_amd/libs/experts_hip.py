@@ -1,7 +1,7 @@
 """ctypes binding of include/h2o4gpu_experts.h: expert layers and 4-bit products on device pointers.
 
-Same library as kmeans_hip; the torch-facing functions are h2o4gpu_amd.experts and
-h2o4gpu_amd.codebook4.
+Same library as kmeans_hip; the torch-facing functions are h2o4gpu_amd.experts, h2o4gpu_amd.codebook4
+and h2o4gpu_amd.microscale4.
 """
 import ctypes
 
@@ -48,6 +48,25 @@ PROTOTYPES = {
     "h2o4gpu_codebook4_experts_product": (c_int, [c_int, c_size_t, c_int, c_int, c_size_t, c_size_t, c_int,
                                                   c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_size_t,
                                                   c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "h2o4gpu_experts_product": (c_int, [c_int, c_size_t, c_int, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p,
+                                        c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "h2o4gpu_experts_product_drows": (c_int, [c_int, c_size_t, c_int, c_size_t, c_size_t, c_void_p, c_size_t,
+                                              c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "h2o4gpu_experts_product_dweights": (c_int, [c_int, c_size_t, c_int, c_size_t, c_size_t, c_void_p, c_size_t,
+                                                 c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "h2o4gpu_microscale4_codes_pitch": (c_size_t, [c_size_t]),
+    "h2o4gpu_microscale4_scales_pitch": (c_size_t, [c_size_t]),
+    "h2o4gpu_microscale4_quantize": (c_int, [c_int, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p,
+                                             c_void_p]),
+    "h2o4gpu_microscale4_dequantize": (c_int, [c_int, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p, c_size_t,
+                                               c_void_p]),
+    "h2o4gpu_microscale4_layout": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p,
+                                           c_void_p]),
+    "h2o4gpu_microscale4_product": (c_int, [c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_void_p, c_size_t, c_void_p]),
+    "h2o4gpu_microscale4_experts_product": (c_int, [c_int, c_size_t, c_int, c_int, c_size_t, c_size_t, c_void_p,
+                                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                    c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -131,6 +131,54 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
                                       size_t codebook_stride, const int *d_order, const int *d_offsets, void *d_y,
                                       size_t y_stride, void *stream);
 
+/* The experts' own products, rows in expert order: d_y[p] = W_e d_rows[p] for the rows p in
+ * [d_offsets[e], d_offsets[e + 1]) of each expert e, zeros for those behind d_offsets[experts] (what
+ * lies there is not read). d_offsets [experts + 1] as experts_sort writes it: from 0, ascending, at
+ * most rows. W_e: [out][cols], rows w_stride elements apart, at d_weights + e * expert_stride (0: one
+ * matrix for all). Products and sums in float, one rounding at the end.
+ * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
+ * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none). */
+int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
+                            size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
+                            const int *d_offsets, void *d_y, size_t y_stride, void *stream);
+int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
+                                  size_t dy_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
+                                  const int *d_offsets, void *d_drows, size_t drows_stride, void *stream);
+int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
+                                     size_t dy_stride, const void *d_rows, size_t rows_stride, const int *d_offsets,
+                                     void *d_dweights, void *stream);
+
+/* Microscaled 4-bit matrices: every 32 columns of a row share a power of two, 2^(byte - 127), and an
+ * element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 .. 7, the sign is 8) times it. A
+ * scale byte of 255 is not a number, and neither is its block.
+ * In memory: rows of codes_pitch(cols) bytes, two codes a byte, the even column in the low half; rows of
+ * scales_pitch(cols) bytes of scales, block b of every 16 at byte 4 * (b % 4) + b / 4. Both start at a
+ * multiple of 16 bytes; behind a row's last column lie zeros. Pitches are 0 for bad arguments.
+ *
+ * quantize: the scale of a block is 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; elements
+ * are rounded to the nearest, a tie to the even code, those beyond 6 are 6. A block with a NaN or an
+ * infinity is not a number; a block of zeros has scale byte 0. dequantize: the reverse, rounded to dtype.
+ * layout: from codes in rows codes_stride bytes apart and scales [rows][ceil(cols / 32)]. */
+size_t h2o4gpu_microscale4_codes_pitch(size_t cols);
+size_t h2o4gpu_microscale4_scales_pitch(size_t cols);
+int h2o4gpu_microscale4_quantize(int dtype, size_t rows, size_t cols, const void *d_x, size_t x_stride, void *d_codes,
+                                 void *d_scales, void *stream);
+int h2o4gpu_microscale4_dequantize(int dtype, size_t rows, size_t cols, const void *d_codes, const void *d_scales,
+                                   void *d_out, size_t out_stride, void *stream);
+int h2o4gpu_microscale4_layout(size_t rows, size_t cols, const void *d_codes, size_t codes_stride,
+                               const void *d_scales, void *d_laid_codes, void *d_laid_scales, void *stream);
+/* d_y [rows][out] of dtype = x [rows][cols] times the transpose of w [out][cols], both microscaled;
+ * sums in float, one rounding at the end. experts_product: w [experts][out][cols], rows in expert
+ * order: row p of d_y is x's row d_order[p] / top_k (d_order NULL: x's row p, x then has
+ * tokens * top_k rows) times the matrix of the expert whose rows p is among; zeros for the rows
+ * behind d_offsets[experts]. */
+int h2o4gpu_microscale4_product(int dtype, size_t rows, size_t out, size_t cols, const void *d_x, const void *d_x_scales,
+                                const void *d_w, const void *d_w_scales, void *d_y, size_t y_stride, void *stream);
+int h2o4gpu_microscale4_experts_product(int dtype, size_t tokens, int top_k, int experts, size_t out, size_t cols,
+                                        const void *d_x, const void *d_x_scales, const void *d_w,
+                                        const void *d_w_scales, const int *d_order, const int *d_offsets, void *d_y,
+                                        size_t y_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
