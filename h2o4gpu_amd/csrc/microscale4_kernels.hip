@@ -6,7 +6,7 @@
 // or a multiple to a row; scales 16 bytes for 512 columns, the byte of the block b of these 16 at 4 * (b % 4) + b / 4:
 // lane group g of a matrix instruction multiplies block g of its 128 columns, and has the scales of four
 // instructions in one word. Behind a row's last column lie zeros (codes and scales).
-#include "product_tiles.h"
+#include "product_pipe.h"
 
 namespace kmhip {
 namespace {
@@ -153,17 +153,14 @@ struct FourArgs {
   int rows, out, cols, y_aligned;
 };
 
-__device__ __forceinline__ void to_lds_16(const void *from, char *lds) {
+__device__ __forceinline__ void to_lds(const void *from, char *lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)(lds), 16, 0, 0);
-#else
-  (void)from;
-  (void)lds;
 #endif
 }
 
 template <int STEP>
-__device__ __forceinline__ void mfma_four(f32x4 &acc, u32x4 w, u32x4 x, unsigned sw, unsigned sx) {
+__device__ __forceinline__ void mfma_four_builtin(f32x4 &acc, u32x4 w, u32x4 x, unsigned sw, unsigned sx) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef int i32x8 __attribute__((ext_vector_type(8)));
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -232,9 +229,9 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
   auto load = [&](int t) {
     char *at = lds + (t & 1) * STAGE + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < PX; ++i) to_lds_16(gx[i] + (size_t)t * 128, at + i * THREADS * 16);
+    for (int i = 0; i < PX; ++i) to_lds(gx[i] + (size_t)t * 128, at + i * THREADS * 16);
 #pragma unroll
-    for (int i = 0; i < PW; ++i) to_lds_16(gw[i] + (size_t)t * 128, at + BM * 128 + i * THREADS * 16);
+    for (int i = 0; i < PW; ++i) to_lds(gw[i] + (size_t)t * 128, at + BM * 128 + i * THREADS * 16);
   };
   if (stages) load(0);
   for (int t = 0; t < stages; ++t) {
@@ -259,7 +256,7 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) mfma_four<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
+        for (int j = 0; j < FN; ++j) mfma_four_builtin<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
     };
     step(Int<0>());
     step(Int<1>());
@@ -279,7 +276,19 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 }
 
 template <typename T>
-int launch_four(const FourArgs &a, hipStream_t stream) {
+int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
+  const size_t pitch = codes_pitch(a.cols);
+  if (x_rows * pitch < BUFFER_BYTES && pitch < BUFFER_BYTES / 512 && a.out >= 128 &&
+      a.rows / (a.experts ? a.experts : 1) >= 128) {
+    PipeArgs p = {};
+    p.x = (const char *)a.x, p.w = (const char *)a.w, p.x_scales = a.x_scales, p.w_scales = a.w_scales, p.c = a.y;
+    p.x_stride = p.w_stride = pitch, p.w_expert = pitch * a.out, p.scales_stride = scales_pitch(a.cols);
+    p.c_stride = a.y_stride, p.c_aligned = a.y_aligned, p.x_bytes = x_rows * pitch;
+    p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
+    p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
+    return a.order ? launch_pipe<Four, T, FORWARD, true, 256, 256, 2, 4>(p, stream)
+                   : launch_pipe<Four, T, FORWARD, false, 256, 256, 2, 4>(p, stream);
+  }
   constexpr int BM = 128, BN = 128;
   const size_t m_tiles = a.experts ? ragged_tiles(a.experts, a.rows, BM) : ((size_t)a.rows + BM - 1) / BM;
   const size_t n_tiles = ((size_t)a.out + BN - 1) / BN;
@@ -357,7 +366,7 @@ KM_API int h2o4gpu_microscale4_layout(size_t rows, size_t cols, const void *d_co
 }
 
 namespace {
-int four_product(int dtype, FourArgs a, size_t rows, size_t out, size_t cols, void *stream) {
+int four_product(int dtype, FourArgs a, size_t x_rows, size_t rows, size_t out, size_t cols, void *stream) {
   if (!known_type(dtype) || !sized(rows, cols) || out < 1 || out > MAX_SIDE || rows > (size_t)INT_MAX - 65536)
     return H2O4GPU_KMEANS_EARG;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
@@ -367,7 +376,7 @@ int four_product(int dtype, FourArgs a, size_t rows, size_t out, size_t cols, vo
   a.rows = (int)rows, a.out = (int)out, a.cols = (int)cols;
   a.y_aligned = a.y_stride % 4 == 0 && aligned_to(a.y, 4 * type_size(dtype));
   return with_type(dtype, [&](auto tag) {
-    return launch_four<typename decltype(tag)::type>(a, static_cast<hipStream_t>(stream));
+    return launch_four<typename decltype(tag)::type>(a, x_rows, static_cast<hipStream_t>(stream));
   });
 }
 }  // namespace
@@ -379,7 +388,7 @@ KM_API int h2o4gpu_microscale4_product(int dtype, size_t rows, size_t out, size_
   a.x = static_cast<const unsigned char *>(d_x), a.x_scales = static_cast<const unsigned char *>(d_x_scales);
   a.w = static_cast<const unsigned char *>(d_w), a.w_scales = static_cast<const unsigned char *>(d_w_scales);
   a.y = d_y, a.y_stride = y_stride;
-  return four_product(dtype, a, rows, out, cols, stream);
+  return four_product(dtype, a, rows, rows, out, cols, stream);
 }
 
 KM_API int h2o4gpu_microscale4_experts_product(int dtype, size_t tokens, int top_k, int experts, size_t out, size_t cols,
@@ -395,5 +404,5 @@ KM_API int h2o4gpu_microscale4_experts_product(int dtype, size_t tokens, int top
   a.w = static_cast<const unsigned char *>(d_w), a.w_scales = static_cast<const unsigned char *>(d_w_scales);
   a.y = d_y, a.y_stride = y_stride;
   a.order = d_order, a.offsets = d_offsets, a.top_k = top_k, a.experts = experts;
-  return four_product(dtype, a, tokens * top_k, out, cols, stream);
+  return four_product(dtype, a, d_order ? tokens : tokens * top_k, tokens * top_k, out, cols, stream);
 }

@@ -5,12 +5,10 @@
 //   product_dweights: dW[e] = sum over p of dy[p] x[p]^T
 //
 // Sums are float32, in an order that depends on the sizes alone; one rounding at the end.
-#include "product_tiles.h"
+#include "product_pipe.h"
 
 namespace kmhip {
 namespace {
-
-enum Kind { FORWARD, DROWS, DWEIGHTS };
 
 struct ProductArgs {
   const void *x;  // m's operand: rows in expert order (dy of DWEIGHTS)
@@ -133,8 +131,29 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   }
 }
 
+// Whether every piece of 16 bytes of both operands lies at a multiple of 16 and within the reach of a buffer.
+template <typename T, Kind KIND>
+bool pieces_aligned(const ProductArgs &a) {
+  constexpr size_t EPP = 16 / sizeof(T);
+  const size_t m = KIND == DWEIGHTS ? a.k : 0, k = KIND == DWEIGHTS ? 0 : a.k, n = KIND == FORWARD ? 0 : a.n;
+  return aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % EPP == 0 && a.w_stride % EPP == 0 &&
+         a.w_expert % EPP == 0 && m % EPP == 0 && k % EPP == 0 && n % EPP == 0 &&
+         a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
+}
+
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (pieces_aligned<T, KIND>(a)) {
+      PipeArgs p = {};
+      p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
+      p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
+      p.c_stride = a.c_stride, p.c_expert = a.c_expert, p.c_aligned = a.c_aligned;
+      p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
+      const size_t rows = KIND == DWEIGHTS ? (size_t)a.k : a.rows / a.experts;
+      if (rows >= 128 && a.n >= 128) return launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream);
+    }
+  }
   constexpr int BM = 128, BN = 128;
   const size_t m_tiles =
       KIND == DWEIGHTS ? (size_t)a.experts * ((a.k + BM - 1) / BM) : ragged_tiles(a.experts, a.rows, BM);
