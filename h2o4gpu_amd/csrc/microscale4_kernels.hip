@@ -283,7 +283,7 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
     PipeArgs p = {};
     p.x = (const char *)a.x, p.w = (const char *)a.w, p.x_scales = a.x_scales, p.w_scales = a.w_scales, p.c = a.y;
     p.x_stride = p.w_stride = pitch, p.w_expert = pitch * a.out, p.scales_stride = scales_pitch(a.cols);
-    p.c_stride = a.y_stride, p.c_aligned = a.y_aligned, p.x_bytes = x_rows * pitch;
+    p.c_stride = a.y_stride, p.c_aligned = a.y_stride % (16 / sizeof(T)) == 0 && aligned_to(a.y, 16), p.x_bytes = x_rows * pitch;
     p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
     p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
     return a.order ? launch_pipe<Four, T, FORWARD, true, 256, 256, 2, 4>(p, stream)

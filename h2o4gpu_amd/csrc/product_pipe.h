@@ -28,8 +28,8 @@ struct PipeArgs {
   const int *order, *offsets;  // order: x's row of C's row p is order[p] / top_k (none: p)
   int top_k, experts;          // experts 0: one matrix and `rows` rows
   int rows, n, k;              // k in elements (Four: in groups of four columns); DWEIGHTS: k is C's m
-  int m_tiles, n_tiles;
-  int c_aligned;               // four elements of C may be stored at once
+  int m_tiles, n_tiles, band;
+  int c_aligned;               // C's rows begin at multiples of 16 bytes
 };
 
 template <typename T>
@@ -39,6 +39,11 @@ struct PipeElement {
 template <>
 struct PipeElement<Four> {
   typedef bfloat16_t type;
+};
+
+template <typename T>
+struct Pieces {
+  T v[16 / sizeof(T)];
 };
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -66,12 +71,17 @@ __device__ __forceinline__ const char *same_in_all(const char *p) {
   const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((size_t)p >> 32));
   return (const char *)((size_t)hi << 32 | lo);
 }
-// 16 bytes at each lane's own offset from `base` to 64 consecutive places from `lds` on (base and lds are the same in
-// every lane). What lies `size` bytes and more behind base is not read.
-__device__ __forceinline__ void to_lds_16(const char *base, unsigned size, unsigned offset, unsigned lds) {
+// 16 bytes at each lane's own offset behind a buffer's start to 64 consecutive places from `lds` on (the same in every
+// lane); nothing is read behind the buffer's size. Written out, because the compiler would wait for all of these before
+// a read of LDS that it cannot tell from where they write; who reads there waits for vmcnt by hand.
+__device__ __forceinline__ u32x4 buffer_of(const char *start, unsigned size) {
+  return u32x4{(unsigned)(size_t)start, (unsigned)((size_t)start >> 32) & 0xffffu, size, 0x00020000u};
+}
+__device__ __forceinline__ void to_lds_16(u32x4 buffer, unsigned offset, unsigned lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)size, 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(size_t)lds, 16, (int)offset, 0, 0, 0);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(offset), "s"(buffer));
 #endif
 }
 
@@ -150,6 +160,58 @@ struct PipeOperand {
   }
 };
 
+// A wavefront's part of a tile to memory: through its own LDS, so that a row's numbers go out side by side, 16 bytes a
+// lane. (The lanes of a sum hold four numbers of 16 rows each; stored as they are, 8192^3 took 100 us longer.)
+template <typename OUT, int FM, int FN, int BYTES>
+__device__ __forceinline__ void store_tile(char *mine, int lane, f32x4 (&acc)[FM][FN], OUT *c, size_t stride, int m0,
+                                           int n0, int m_here, int n_here, bool aligned) {
+  constexpr int LINE = FN * 16 * (int)sizeof(OUT), PIECES = LINE / 16, EPP = 16 / (int)sizeof(OUT);
+  constexpr int PASS = BYTES / (LINE * 16) < FM ? BYTES / (LINE * 16) : FM;  // blocks of 16 rows at a time
+  static_assert(PASS >= 1 && FM % PASS == 0 && PIECES >= 8 && 64 % PIECES == 0, "");
+  if (!aligned) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = m0 + i * 16 + (lane & 15);
+      if (m >= m_here) continue;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = n0 + j * 16 + 4 * (lane >> 4);
+        store_four(c + (size_t)m * stride + n, acc[i][j], n_here - n, false);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int p = 0; p < FM / PASS; ++p) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int m = i * 16 + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int byte = (j * 16 + 4 * (lane >> 4)) * (int)sizeof(OUT);
+        char *at = mine + m * LINE + (byte / 16 ^ (m & 7)) * 16 + byte % 16;
+        store_four(reinterpret_cast<OUT *>(at), acc[p * PASS + i][j], 4, true);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < PASS * 16 * PIECES / 64; ++r) {
+      const int m = r * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + m * LINE + (piece ^ (m & 7)) * 16);
+      const int row = m0 + p * PASS * 16 + m, n = n0 + piece * EPP;
+      if (row < m_here && n < n_here) {
+        OUT *to = c + (size_t)row * stride + n;
+        if (n + EPP <= n_here) {
+          *reinterpret_cast<u32x4 *>(to) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < EPP; ++e)
+            if (n + e < n_here) to[e] = __builtin_bit_cast(Pieces<OUT>, v).v[e];
+        }
+      }
+    }
+  }
+}
+
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   typedef typename PipeElement<ELEMENT>::type T;
@@ -171,8 +233,8 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   {
     const unsigned total = (unsigned)a.m_tiles * a.n_tiles, id = blockIdx.x, most = total & ~7u;
     const unsigned at = id < most ? (id & 7) * (most >> 3) + (id >> 3) : id;
-    const unsigned band = 8u * a.n_tiles, m0 = at / band * 8;
-    const unsigned high = (unsigned)a.m_tiles - m0 < 8 ? (unsigned)a.m_tiles - m0 : 8;
+    const unsigned band = (unsigned)a.band * a.n_tiles, m0 = at / band * a.band;
+    const unsigned high = (unsigned)a.m_tiles - m0 < (unsigned)a.band ? (unsigned)a.m_tiles - m0 : a.band;
     const unsigned in = at % band;
     number = (int)(m0 + in % high), n_tile = (int)(in / high);
   }
@@ -261,37 +323,46 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
         const unsigned s = to + 2 * STAGE + (pair & 1) * SCALES;
 #pragma unroll
         for (int i = 0; i < PS; ++i) {
-          to_lds_16(s_from[i] + (size_t)pair * 16, pair * 2 < stages ? s_size[i] : 0, s_off[i], s + i * THREADS * 16);
+          to_lds_16(buffer_of(s_from[i] + (size_t)pair * 16, pair * 2 < stages ? s_size[i] : 0), s_off[i], s + i * THREADS * 16);
         }
       }
     };
+    // The stage that is loaded next, and how much of it there is.
     struct Stage {
       const char *x, *w;
       unsigned x_size, w_size, to;
+    } next;
+    const auto x_size_of = [&](int k_here) {
+      return XC ? (unsigned)((k_here - 1) * a.x_stride) + m_here * SIZE : (unsigned)((m_here - 1) * a.x_stride) + k_here * SIZE;
     };
-    auto stage_of = [&](int t) {
-      const int k_here = k_end - t * KS < KS ? k_end - t * KS : KS;
-      Stage s;
-      s.x = x + t * x_step, s.w = w + t * w_step;
-      s.x_size = GATHER ? (unsigned)(a.x_bytes - t * x_step)
-                 : XC   ? (unsigned)((k_here - 1) * a.x_stride) + m_here * SIZE
-                        : (unsigned)((m_here - 1) * a.x_stride) + k_here * SIZE;
-      s.w_size = WC ? (unsigned)((k_here - 1) * a.w_stride) + n_here * SIZE
-                    : (unsigned)((n_here - 1) * a.w_stride) + k_here * SIZE;
-      if (t >= stages) s.x_size = s.w_size = 0;  // nothing is read
-      s.to = to + (t & 1) * STAGE;
-      return s;
+    const auto w_size_of = [&](int k_here) {
+      return WC ? (unsigned)((k_here - 1) * a.w_stride) + n_here * SIZE : (unsigned)((n_here - 1) * a.w_stride) + k_here * SIZE;
     };
-    auto load_one = [&](const Stage &s, int i) {
+    const unsigned x_full = x_size_of(KS), w_full = w_size_of(KS);
+    const unsigned x_last = x_size_of(k_end - full * KS), w_last = w_size_of(k_end - full * KS);
+    unsigned x_left = GATHER ? (unsigned)a.x_bytes : 0;
+    auto size_next = [&](int t) {
+      next.x_size = t < full ? (GATHER ? x_left : x_full) : t < stages ? x_last : 0;
+      next.w_size = t < full ? w_full : t < stages ? w_last : 0;
+    };
+    next.x = x, next.w = w, next.to = to;
+    size_next(0);
+    auto advance = [&](int t) {  // to stage t
+      next.x += x_step, next.w += w_step, next.to ^= STAGE;
+      if (GATHER) x_left -= 128;
+      size_next(t);
+    };
+    auto load_one = [&](int i) {
       if (i < X::P)
-        to_lds_16(s.x, s.x_size, GATHER ? x_off[GATHER ? i : 0] : x_off[0] + i * x_next, s.to + i * THREADS * 16);
+        to_lds_16(buffer_of(next.x, next.x_size), GATHER ? x_off[GATHER ? i : 0] : x_off[0] + i * x_next,
+                  next.to + i * THREADS * 16);
       else
-        to_lds_16(s.w, s.w_size, w_off + (i - X::P) * w_next, s.to + BM * 128 + (i - X::P) * THREADS * 16);
+        to_lds_16(buffer_of(next.w, next.w_size), w_off + (i - X::P) * w_next,
+                  next.to + BM * 128 + (i - X::P) * THREADS * 16);
     };
-    auto load = [&](int t) {
-      const Stage s = stage_of(t);
+    auto load = [&]() {
 #pragma unroll
-      for (int i = 0; i < X::P + W::P; ++i) load_one(s, i);
+      for (int i = 0; i < X::P + W::P; ++i) load_one(i);
     };
     X fx;
     W fw;
@@ -332,19 +403,22 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       else
         mfma_piece(acc[i][j], f[S].w[j], f[S].x[i], Tag<T>());
     };
-    // A step's products with `ops` other instructions between them, as evenly as they go.
-    auto multiply = [&](auto step, auto odd, auto ops, auto other) {
-      constexpr int OPS = decltype(ops)::value, EACH = FM * FN / (OPS ? OPS : 1);
-      static_assert(EACH >= 1, "more loads than products");
+    // A step's products, with `reads` LDS reads spread between the first 3/4 of them and `loads` loads between all. (A
+    // load takes its turn in the CU's address unit; a wavefront that has to wait for that issues nothing else.)
+    auto multiply = [&](auto step, auto odd, auto reads, auto read_it, auto loads, auto load_it) {
+      constexpr int R = decltype(reads)::value, L = decltype(loads)::value, Q = FM * FN, SPAN = Q * 3 / 4;
 #pragma unroll
-      for (int r = 0; r < OPS; ++r) {
-        other(r);
+      for (int q = 0; q < Q; ++q) {
+        // (the r-th goes before product r * SPAN / R)
 #pragma unroll
-        for (int q = r * EACH; q < (r + 1) * EACH; ++q) multiply_one(step, odd, q);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int r = 0; r < R; ++r)
+          if (r * SPAN / (R ? R : 1) == q) read_it(r);
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+          if (l * Q / (L ? L : 1) == q) load_it(l);
+        multiply_one(step, odd, q);
+        if (R || L) __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int q = OPS * EACH; q < FM * FN; ++q) multiply_one(step, odd, q);
     };
     // everything this wavefront has asked for is there; then everybody's is
     auto meet = [&]() {
@@ -372,25 +446,23 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       }
     };
 
-    load(0);
+    load();
     load_scales(0);
     meet();
-    load(1);
+    advance(1);
+    load();
     read(Int<0>());
     read_scales(0);
     constexpr int LOADS = X::P + W::P, READS = FM + FN;
     auto stage = [&](int t, auto odd) {
-      multiply(Int<0>(), odd, Int<READS>(), [&](int r) { read_one(Int<1>(), r); });
+      multiply(Int<0>(), odd, Int<READS>(), [&](int r) { read_one(Int<1>(), r); }, Int<0>(), [](int) {});
+      advance(t + 2);
       meet();
-      const Stage s = stage_of(t + 2);
       if (!decltype(odd)::value) load_scales((t >> 1) + 1);
       fx.swap(STAGE), fw.swap(STAGE);
-      multiply(Int<1>(), odd, Int<LOADS + READS>(), [&](int r) {
-        if (r < LOADS)
-          load_one(s, r);
-        else
-          read_one(Int<0>(), r - LOADS);
-      });
+      multiply(
+          Int<1>(), odd, Int<READS>(), [&](int r) { read_one(Int<0>(), r); }, Int<LOADS>(),
+          [&](int l) { load_one(l); });
       if (decltype(odd)::value) read_scales((t >> 1) + 1);
     };
     if constexpr (FOUR) {
@@ -407,23 +479,17 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     if (!FOUR && full < stages) {
       read(Int<1>());
       mask(Int<0>());
-      multiply(Int<0>(), Int<0>(), Int<0>(), [](int) {});
+      multiply(Int<0>(), Int<0>(), Int<0>(), [](int) {}, Int<0>(), [](int) {});
       mask(Int<1>());
-      multiply(Int<1>(), Int<0>(), Int<0>(), [](int) {});
+      multiply(Int<1>(), Int<0>(), Int<0>(), [](int) {}, Int<0>(), [](int) {});
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads that read nothing end before the LDS is another's)
   }
+  // loads that read nothing end, and everybody's reads, before the LDS is used again
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
 
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = (wm * FM + i) * 16 + (lane & 15);
-    if (m >= m_here) continue;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
-      store_four(c + (size_t)m * a.c_stride + n0 + n, acc[i][j], n_here - n, a.c_aligned);
-    }
-  }
+  store_tile<OUT, FM, FN, STAGE * 2 / (WM * WN)>(lds + wave * (STAGE * 2 / (WM * WN)), lane, acc, c + n0, a.c_stride,
+                                                 wm * FM * 16, wn * FN * 16, m_here, n_here, a.c_aligned);
 }
 
 constexpr size_t BUFFER_BYTES = (size_t)1 << 32;  // what a buffer's offsets reach
@@ -434,6 +500,7 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
                          : a.experts      ? ragged_tiles(a.experts, a.rows, BM)
                                           : ((size_t)a.rows + BM - 1) / BM;
   a.m_tiles = (int)m_tiles, a.n_tiles = (a.n + BN - 1) / BN;
+  a.band = a.n_tiles >= 8 ? 4 : a.n_tiles >= 4 ? 8 : 16;
   const size_t blocks = m_tiles * a.n_tiles;
   if (m_tiles > (size_t)INT_MAX || blocks > (size_t)1 << 22) return H2O4GPU_KMEANS_EARG;
   const size_t lds = (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0));

@@ -148,7 +148,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
       PipeArgs p = {};
       p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
       p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
-      p.c_stride = a.c_stride, p.c_expert = a.c_expert, p.c_aligned = a.c_aligned;
+      p.c_stride = a.c_stride, p.c_expert = a.c_expert, p.c_aligned = a.c_stride % (16 / sizeof(T)) == 0 && a.c_expert % (16 / sizeof(T)) == 0 && aligned_to(a.c, 16);
       p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
       const size_t rows = KIND == DWEIGHTS ? (size_t)a.k : a.rows / a.experts;
       if (rows >= 128 && a.n >= 128) return launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream);
