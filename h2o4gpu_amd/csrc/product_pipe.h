@@ -75,7 +75,9 @@ __device__ __forceinline__ const char *same_in_all(const char *p) {
 // lane); nothing is read behind the buffer's size. Written out, because the compiler would wait for all of these before
 // a read of LDS that it cannot tell from where they write; who reads there waits for vmcnt by hand.
 __device__ __forceinline__ u32x4 buffer_of(const char *start, unsigned size) {
-  return u32x4{(unsigned)(size_t)start, (unsigned)((size_t)start >> 32) & 0xffffu, size, 0x00020000u};
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(size_t)start),
+               (unsigned)__builtin_amdgcn_readfirstlane((unsigned)((size_t)start >> 32) & 0xffffu),
+               (unsigned)__builtin_amdgcn_readfirstlane(size), 0x00020000u};
 }
 __device__ __forceinline__ void to_lds_16(u32x4 buffer, unsigned offset, unsigned lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -160,6 +162,62 @@ struct PipeOperand {
   }
 };
 
+constexpr int PIPE_TABLE = 2046;  // experts + 2 numbers of 4 bytes fit 8 KB of LDS
+
+// table[e]: how many tiles of BM rows the experts before e have; [experts + 1]: all, those without an expert included.
+template <int BM, int THREADS>
+__device__ __forceinline__ void tile_table(int *table, const int *offsets, int experts, int rows) {
+  constexpr int EACH = (PIPE_TABLE + 1 + THREADS - 1) / THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int mine[EACH], sum = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = tid * EACH + i;
+    mine[i] = 0;
+    if (e <= experts) mine[i] = ((e < experts ? offsets[e + 1] : rows) - offsets[e] + BM - 1) / BM;
+    sum += mine[i];
+  }
+  int before = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int other = __shfl_up(before, d);
+    if (lane >= d) before += other;
+  }
+  // (the sums of whole wavefronts lie behind the table)
+  int *sums = table + PIPE_TABLE + 2;
+  if (lane == 63) sums[wave] = before;
+  __syncthreads();
+  before -= sum;
+  for (int w = 0; w < wave; ++w) before += sums[w];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = tid * EACH + i;
+    if (e <= experts) table[e] = before;
+    before += mine[i];
+    if (e == experts) table[e + 1] = before;
+  }
+  __syncthreads();
+}
+
+template <int BM>
+__device__ __forceinline__ void listed_tile(const int *table, const int *offsets, int experts, int rows, int number,
+                                            int &stretch, int &first, int &rows_here) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = experts + 1;  // the last e with table[e] <= number
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const bool below = lane * step < n && table[lo + lane * step] <= number;
+    const int skip = (__popcll(__ballot(below)) - 1) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int begin = offsets[lo], end = lo == experts ? rows : offsets[lo + 1];
+  stretch = lo;
+  first = begin + (number - __builtin_amdgcn_readfirstlane(table[lo])) * BM;
+  rows_here = end - first < BM ? end - first : BM;
+}
+
 // A wavefront's part of a tile to memory: through its own LDS, so that a row's numbers go out side by side, 16 bytes a
 // lane. (The lanes of a sum hold four numbers of 16 rows each; stored as they are, 8192^3 took 100 us longer.)
 template <typename OUT, int FM, int FN, int BYTES>
@@ -226,16 +284,32 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   static_assert((STAGE & (STAGE - 1)) == 0, "the buffers are told apart by one bit");
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // Neighbours of a tile run at the same time on the same chiplet (workgroups go round the eight): eight tiles
-  // of m by as many of n as it holds.
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Tiles of m, numbered without gaps: those of expert 0, of expert 1, ..., of the rows without an expert. A table in
+  // LDS says where each expert's begin; beyond PIPE_TABLE experts the numbers have gaps (ragged_tile).
+  int *table = reinterpret_cast<int *>(lds + 2 * STAGE + (FOUR ? 2 * (BM + BN) * 16 : 0));
+  const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = ragged && a.experts < PIPE_TABLE;
+  unsigned m_tiles = (unsigned)a.m_tiles;
+  if (listed) {
+    tile_table<BM, THREADS>(table, a.offsets, a.experts, a.rows);
+    m_tiles = __builtin_amdgcn_readfirstlane(table[a.experts + 1]);
+  }
+  // Workgroups go round the eight chiplets; each of these takes a stretch of the tiles, and its workgroups neighbours
+  // of that at the same time: `band` tiles of m by as many of n as there are workgroups.
+  const unsigned total = m_tiles * (unsigned)a.n_tiles, die = blockIdx.x & 7;
+  const unsigned last_tile = (unsigned)((unsigned long long)total * (die + 1) / 8);
+  for (unsigned tile = (unsigned)((unsigned long long)total * die / 8) + (blockIdx.x >> 3); tile < last_tile;
+       tile += gridDim.x >> 3) {
+  // (what follows from a thread's number is made anew for each tile and each part of it: kept, it would take the
+  // registers of the sums)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63;
   int number, n_tile;
   {
-    const unsigned total = (unsigned)a.m_tiles * a.n_tiles, id = blockIdx.x, most = total & ~7u;
-    const unsigned at = id < most ? (id & 7) * (most >> 3) + (id >> 3) : id;
-    const unsigned band = (unsigned)a.band * a.n_tiles, m0 = at / band * a.band;
-    const unsigned high = (unsigned)a.m_tiles - m0 < (unsigned)a.band ? (unsigned)a.m_tiles - m0 : a.band;
-    const unsigned in = at % band;
+    const unsigned band = (unsigned)a.band * a.n_tiles, m0 = tile / band * a.band;
+    const unsigned high = m_tiles - m0 < (unsigned)a.band ? m_tiles - m0 : a.band;
+    const unsigned in = tile % band;
     number = (int)(m0 + in % high), n_tile = (int)(in / high);
   }
   const int n0 = n_tile * BN, n_here = a.n - n0 < BN ? a.n - n0 : BN;
@@ -253,8 +327,11 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     c += (size_t)expert * a.c_expert + (size_t)first * a.c_stride;
   } else {
     m_here = a.rows - first < BM ? a.rows - first : BM;
-    if (a.experts) {
-      if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here)) return;
+    if (ragged) {
+      if (listed)
+        listed_tile<BM>(table, a.offsets, a.experts, a.rows, number, expert, first, m_here);
+      else if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here))
+        continue;
       if (expert == a.experts) k_end = 0, expert = 0;  // rows without an expert: zeros
     }
     if (!GATHER) x += (size_t)first * a.x_stride;
@@ -488,10 +565,15 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
 
-  store_tile<OUT, FM, FN, STAGE * 2 / (WM * WN)>(lds + wave * (STAGE * 2 / (WM * WN)), lane, acc, c + n0, a.c_stride,
+  int tid2 = threadIdx.x;
+  asm volatile("" : "+v"(tid2));
+  store_tile<OUT, FM, FN, STAGE * 2 / (WM * WN)>(lds + wave * (STAGE * 2 / (WM * WN)), tid2 & 63, acc, c + n0, a.c_stride,
                                                  wm * FM * 16, wn * FN * 16, m_here, n_here, a.c_aligned);
+  __syncthreads();
+  }
 }
 
+constexpr size_t PIPE_WORKGROUPS = 256;    // one to a CU, as many as the LDS allows
 constexpr size_t BUFFER_BYTES = (size_t)1 << 32;  // what a buffer's offsets reach
 
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
@@ -501,11 +583,12 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
                                           : ((size_t)a.rows + BM - 1) / BM;
   a.m_tiles = (int)m_tiles, a.n_tiles = (a.n + BN - 1) / BN;
   a.band = a.n_tiles >= 8 ? 4 : a.n_tiles >= 4 ? 8 : 16;
-  const size_t blocks = m_tiles * a.n_tiles;
-  if (m_tiles > (size_t)INT_MAX || blocks > (size_t)1 << 22) return H2O4GPU_KMEANS_EARG;
-  const size_t lds = (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0));
+  const size_t tiles = m_tiles * a.n_tiles;
+  if (m_tiles > (size_t)INT_MAX || tiles > (size_t)INT_MAX) return H2O4GPU_KMEANS_EARG;
+  const size_t lds = (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (PIPE_TABLE + 2 + WM * WN) * 4;
   const auto kernel = pipe_kernel<ELEMENT, OUT, KIND, GATHER, BM, BN, WM, WN>;
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
+  const size_t blocks = tiles < PIPE_WORKGROUPS ? (tiles + 7) / 8 * 8 : PIPE_WORKGROUPS;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WM * WN * 64), lds, stream, a);
   return launched();
 }
