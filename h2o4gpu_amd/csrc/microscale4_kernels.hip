@@ -159,16 +159,6 @@ __device__ __forceinline__ void to_lds(const void *from, char *lds) {
 #endif
 }
 
-template <int STEP>
-__device__ __forceinline__ void mfma_four_builtin(f32x4 &acc, u32x4 w, u32x4 x, unsigned sw, unsigned sx) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  typedef int i32x8 __attribute__((ext_vector_type(8)));
-  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-  const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, STEP, (int)sw, STEP, (int)sx);
-#endif
-}
-
 // Stages of 256 columns go straight to LDS, two of them: the next is on its way while one is multiplied.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
@@ -256,7 +246,7 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) mfma_four_builtin<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
+        for (int j = 0; j < FN; ++j) mfma_four<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
     };
     step(Int<0>());
     step(Int<1>());

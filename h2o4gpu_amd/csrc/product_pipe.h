@@ -56,6 +56,13 @@ __device__ __forceinline__ u32x4 lds_read_16(unsigned at) {
 __device__ __forceinline__ unsigned lds_read_4(unsigned at) {
   return *(__attribute__((address_space(3))) const unsigned *)(size_t)at;
 }
+__device__ __forceinline__ unsigned lds_read_2(unsigned at) {
+  return *(__attribute__((address_space(3))) const unsigned short *)(size_t)at;
+}
+// the other one of two places `apart` bytes apart, the first at `start`
+__device__ __forceinline__ unsigned scales_swapped(unsigned at, unsigned apart, unsigned start) {
+  return at >= start + apart ? at - apart : at + apart;
+}
 __device__ __forceinline__ u32x2 lds_read_turned(unsigned at) {
   u32x2 out = {at, at};
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -87,35 +94,16 @@ __device__ __forceinline__ void to_lds_16(u32x4 buffer, unsigned offset, unsigne
 #endif
 }
 
-// The scales' bytes are number SELECT of their words. Written out, because only so the sum stays in its registers (the
-// compiler gives the builtin's result others, and spills where all are taken). It knows no waits for it: a sum is
-// touched by nothing but these until sums_done(), and again by one only 15 others later.
+// The scales' bytes are number SELECT of their words.
 template <int SELECT>
 __device__ __forceinline__ void mfma_four(f32x4 &acc, u32x4 w, u32x4 x, unsigned sw, unsigned sx) {
 #if defined(__HIP_DEVICE_COMPILE__)
-#define KM_MFMA_FOUR(MORE)                                                                               \
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " MORE " cbsz:4 blgp:4" \
-               : "+v"(acc)                                                                               \
-               : "v"(w), "v"(x), "v"(sw), "v"(sx))
-  if constexpr (SELECT == 0) KM_MFMA_FOUR("op_sel_hi:[0,0,0]");
-  if constexpr (SELECT == 1) KM_MFMA_FOUR("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
-  if constexpr (SELECT == 2) KM_MFMA_FOUR("op_sel_hi:[1,1,0]");
-  if constexpr (SELECT == 3) KM_MFMA_FOUR("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
-#undef KM_MFMA_FOUR
+  typedef int i32x8 __attribute__((ext_vector_type(8)));
+  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, SELECT, (int)sw, SELECT, (int)sx);
 #endif
 }
-// The matrix instructions before it have written their sums.
-template <int FM, int FN>
-__device__ __forceinline__ void sums_done(f32x4 (&acc)[FM][FN]) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));
-#endif
-}
-
 // One operand of a tile of R rows in a workgroup of THREADS: where its pieces come from, where fragments lie.
 template <typename T, int R, bool COLUMNS, int THREADS, int F>
 struct PipeOperand {
@@ -218,58 +206,57 @@ __device__ __forceinline__ void listed_tile(const int *table, const int *offsets
   rows_here = end - first < BM ? end - first : BM;
 }
 
-// A wavefront's part of a tile to memory: through its own LDS, so that a row's numbers go out side by side, 16 bytes a
-// lane. (The lanes of a sum hold four numbers of 16 rows each; stored as they are, 8192^3 took 100 us longer.)
-template <typename OUT, int FM, int FN, int BYTES>
-__device__ __forceinline__ void store_tile(char *mine, int lane, f32x4 (&acc)[FM][FN], OUT *c, size_t stride, int m0,
-                                           int n0, int m_here, int n_here, bool aligned) {
-  constexpr int LINE = FN * 16 * (int)sizeof(OUT), PIECES = LINE / 16, EPP = 16 / (int)sizeof(OUT);
-  constexpr int PASS = BYTES / (LINE * 16) < FM ? BYTES / (LINE * 16) : FM;  // blocks of 16 rows at a time
-  static_assert(PASS >= 1 && FM % PASS == 0 && PIECES >= 8 && 64 % PIECES == 0, "");
-  if (!aligned) {
+// A wavefront's part of a tile to memory, 16 bytes a lane and 64 of a row side by side. A lane has four numbers of a row;
+// of 2-byte ones, the quarters of the wavefront (16 lanes) that hold neighbours exchange halves of two blocks: what bit 0
+// of the block's number and the two of the quarter's say (b; q1 q0) lies after the first exchange at (q1; b q0), after
+// the second at (q0; b q1). (Stored as they are, eight bytes a lane, 8192^3 took 100 us longer.)
+template <typename OUT, int FM, int FN>
+__device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN], OUT *c, size_t stride, int m0, int n0,
+                                           int m_here, int n_here, bool aligned) {
+  constexpr int EPP = 16 / (int)sizeof(OUT);
+  const int i = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int m = m0 + i * 16 + (lane & 15);
-      if (m >= m_here) continue;
+  for (int b = 0; b < FM; ++b) {
+    const int m = m0 + b * 16 + i;
+    OUT *row = c + (size_t)m * stride;
+    if constexpr (sizeof(OUT) == 4) {
+      if (m < m_here) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int n = n0 + j * 16 + 4 * (lane >> 4);
-        store_four(c + (size_t)m * stride + n, acc[i][j], n_here - n, false);
+        for (int j = 0; j < FN; ++j) store_four(row + n0 + j * 16 + 4 * q, acc[b][j], n_here - (n0 + j * 16 + 4 * q), aligned);
       }
-    }
-    return;
-  }
+    } else {
 #pragma unroll
-  for (int p = 0; p < FM / PASS; ++p) {
+      for (int j = 0; j < FN; j += 2) {
+        typedef OUT four __attribute__((ext_vector_type(4)));
+        u32x2 lo = __builtin_bit_cast(u32x2, four{(OUT)acc[b][j][0], (OUT)acc[b][j][1], (OUT)acc[b][j][2], (OUT)acc[b][j][3]});
+        u32x2 hi = __builtin_bit_cast(
+            u32x2, four{(OUT)acc[b][j + 1][0], (OUT)acc[b][j + 1][1], (OUT)acc[b][j + 1][2], (OUT)acc[b][j + 1][3]});
+#if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-    for (int i = 0; i < PASS; ++i) {
-      const int m = i * 16 + (lane & 15);
+        for (int w = 0; w < 2; ++w) {
+          const auto far = __builtin_amdgcn_permlane32_swap(lo[w], hi[w], false, false);
+          const auto near = __builtin_amdgcn_permlane16_swap(far[0], far[1], false, false);
+          lo[w] = near[0], hi[w] = near[1];
+        }
+#endif
+        const u32x4 piece = {lo[0], lo[1], hi[0], hi[1]};
+        const int n = n0 + j * 16 + 8 * q;
+        if (m < m_here && n < n_here) {
+          if (aligned && n + EPP <= n_here) {
+            *reinterpret_cast<u32x4 *>(row + n) = piece;
+          } else {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int byte = (j * 16 + 4 * (lane >> 4)) * (int)sizeof(OUT);
-        char *at = mine + m * LINE + (byte / 16 ^ (m & 7)) * 16 + byte % 16;
-        store_four(reinterpret_cast<OUT *>(at), acc[p * PASS + i][j], 4, true);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < PASS * 16 * PIECES / 64; ++r) {
-      const int m = r * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + m * LINE + (piece ^ (m & 7)) * 16);
-      const int row = m0 + p * PASS * 16 + m, n = n0 + piece * EPP;
-      if (row < m_here && n < n_here) {
-        OUT *to = c + (size_t)row * stride + n;
-        if (n + EPP <= n_here) {
-          *reinterpret_cast<u32x4 *>(to) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < EPP; ++e)
-            if (n + e < n_here) to[e] = __builtin_bit_cast(Pieces<OUT>, v).v[e];
+            for (int e = 0; e < EPP; ++e)
+              if (n + e < n_here) row[n + e] = __builtin_bit_cast(Pieces<OUT>, piece).v[e];
+          }
         }
       }
     }
   }
 }
 
+// One stage after another, of one tile after another: what is loaded is two stages ahead of what is multiplied, and may
+// be the next tile's, so that a tile's first stages arrive while the one before ends and goes out.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   typedef typename PipeElement<ELEMENT>::type T;
@@ -280,14 +267,18 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   typedef PipeOperand<T, BM, XC, THREADS, FM> X;
   typedef PipeOperand<T, BN, WC, THREADS, FN> W;
   constexpr int SIZE = (int)sizeof(T), EPP = 16 / SIZE, KS = 8 * EPP;
-  constexpr int STAGE = (BM + BN) * 128;
+  constexpr int STAGE = (BM + BN) * 128, SCALES = (BM + BN) * 16;
   static_assert((STAGE & (STAGE - 1)) == 0, "the buffers are told apart by one bit");
+  static_assert(!FOUR || BM + BN == THREADS, "a lane loads one row's scales");
+  // stages, two of them | Four: scales of two stages, two of these | GATHER: where x's rows lie | table of tiles
   extern __shared__ __attribute__((aligned(16))) char lds[];
+  unsigned *gathered = reinterpret_cast<unsigned *>(lds + 2 * STAGE + (FOUR ? 2 * SCALES : 0));
+  int *table = reinterpret_cast<int *>(gathered + (GATHER ? BM : 0));
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const unsigned base = lds_address(lds), to = base + wave * 1024;
   // Tiles of m, numbered without gaps: those of expert 0, of expert 1, ..., of the rows without an expert. A table in
   // LDS says where each expert's begin; beyond PIPE_TABLE experts the numbers have gaps (ragged_tile).
-  int *table = reinterpret_cast<int *>(lds + 2 * STAGE + (FOUR ? 2 * (BM + BN) * 16 : 0));
   const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = ragged && a.experts < PIPE_TABLE;
   unsigned m_tiles = (unsigned)a.m_tiles;
   if (listed) {
@@ -297,280 +288,272 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   // Workgroups go round the eight chiplets; each of these takes a stretch of the tiles, and its workgroups neighbours
   // of that at the same time: `band` tiles of m by as many of n as there are workgroups.
   const unsigned total = m_tiles * (unsigned)a.n_tiles, die = blockIdx.x & 7;
-  const unsigned last_tile = (unsigned)((unsigned long long)total * (die + 1) / 8);
-  for (unsigned tile = (unsigned)((unsigned long long)total * die / 8) + (blockIdx.x >> 3); tile < last_tile;
-       tile += gridDim.x >> 3) {
-  // (what follows from a thread's number is made anew for each tile and each part of it: kept, it would take the
-  // registers of the sums)
-  int tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));
-  const int lane = tid & 63;
-  int number, n_tile;
+  const unsigned tiles_end = (unsigned)((unsigned long long)total * (die + 1) / 8);
+  unsigned tile = (unsigned)((unsigned long long)total * die / 8) + (blockIdx.x >> 3);
+
+  struct Tile {
+    int n0, n_here, m_here, first, expert, k_end;  // m_here 0: there is none
+  };
+  // the next tile of this workgroup
+  auto locate = [&]() {
+    Tile r = {0, 0, 0, 0, 0, 0};
+    for (; tile < tiles_end && r.m_here <= 0; tile += gridDim.x >> 3) {
+      const unsigned band = (unsigned)a.band * a.n_tiles, m0 = tile / band * a.band;
+      const unsigned high = m_tiles - m0 < (unsigned)a.band ? m_tiles - m0 : a.band;
+      const unsigned in = tile % band;
+      const int number = (int)(m0 + in % high), n_tile = (int)(in / high);
+      r.n0 = n_tile * BN, r.n_here = a.n - r.n0 < BN ? a.n - r.n0 : BN;
+      r.k_end = a.k;
+      if constexpr (KIND == DWEIGHTS) {
+        const int tiles = (a.k + BM - 1) / BM;
+        r.expert = number / tiles, r.first = number % tiles * BM;
+        r.m_here = a.k - r.first < BM ? a.k - r.first : BM;
+        r.k_end = a.offsets[r.expert + 1] - a.offsets[r.expert];
+      } else if (ragged) {
+        if (listed)
+          listed_tile<BM>(table, a.offsets, a.experts, a.rows, number, r.expert, r.first, r.m_here);
+        else
+          ragged_tile(a.offsets, a.experts, a.rows, BM, number, r.expert, r.first, r.m_here);
+        if (r.expert == a.experts) r.k_end = 0, r.expert = 0;  // rows without an expert: zeros
+      } else {
+        r.first = number * BM, r.m_here = a.rows - r.first < BM ? a.rows - r.first : BM;
+      }
+    }
+    r.m_here = __builtin_amdgcn_readfirstlane(r.m_here > 0 ? r.m_here : 0);
+    r.first = __builtin_amdgcn_readfirstlane(r.first);
+    r.k_end = __builtin_amdgcn_readfirstlane(r.k_end);
+    return r;
+  };
+  // x's rows of a tile, for the lanes that load them later
+  auto order_of = [&](const Tile &r) -> int {
+    const int m = (int)threadIdx.x % BM;
+    return GATHER && r.m_here > 0 ? a.order[r.first + (m < r.m_here ? m : r.m_here - 1)] : 0;
+  };
+  auto put_order = [&](int slot) {
+    if (GATHER && threadIdx.x < BM) gathered[threadIdx.x] = (unsigned)(slot / a.top_k);
+  };
+  auto stages_of = [&](int k_end) { return k_end <= KS ? 2 : (k_end + KS - 1) / KS; };
+
+  // ---- what is loaded
+  // Where a lane's pieces lie behind a stage's start. No piece is clamped: what lies behind the operand's last byte of
+  // the stage is not read, and a piece of a row or column that does not exist is multiplied into what is not stored, or
+  // masked. From one of a lane's pieces to its next, THREADS slots on, are so many rows or k, turned alike.
+  unsigned x_off[GATHER ? X::P : 1], w_off, s_off = 0;
+  const unsigned x_next = (unsigned)((XC ? THREADS / X::Tile::PER_K : THREADS / 8) * a.x_stride);
+  const unsigned w_next = (unsigned)((WC ? THREADS / W::Tile::PER_K : THREADS / 8) * a.w_stride);
   {
-    const unsigned band = (unsigned)a.band * a.n_tiles, m0 = tile / band * a.band;
-    const unsigned high = m_tiles - m0 < (unsigned)a.band ? m_tiles - m0 : a.band;
-    const unsigned in = tile % band;
-    number = (int)(m0 + in % high), n_tile = (int)(in / high);
+    int r, k;
+    W::Tile::place(threadIdx.x, r, k);
+    w_off = WC ? (unsigned)(k * a.w_stride) + r * SIZE : (unsigned)(r * a.w_stride) + k * SIZE;
+    X::Tile::place(threadIdx.x, r, k);
+    if (!GATHER) x_off[0] = XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE;
+    if (FOUR) s_off = (unsigned)((threadIdx.x % BM) * a.scales_stride);
   }
-  const int n0 = n_tile * BN, n_here = a.n - n0 < BN ? a.n - n0 : BN;
-  int expert = 0, first = number * BM, m_here, k_end = a.k;
-  const char *x = a.x, *w = a.w;
-  OUT *c = static_cast<OUT *>(a.c);
-  if constexpr (KIND == DWEIGHTS) {
-    const int tiles = (a.k + BM - 1) / BM;
-    expert = number / tiles, first = number % tiles * BM;
-    m_here = a.k - first < BM ? a.k - first : BM;
-    const int begin = a.offsets[expert];
-    k_end = a.offsets[expert + 1] - begin;
-    x += (size_t)begin * a.x_stride + (size_t)first * SIZE;
-    w += (size_t)begin * a.w_stride + (size_t)n0 * SIZE;
-    c += (size_t)expert * a.c_expert + (size_t)first * a.c_stride;
-  } else {
-    m_here = a.rows - first < BM ? a.rows - first : BM;
-    if (ragged) {
-      if (listed)
-        listed_tile<BM>(table, a.offsets, a.experts, a.rows, number, expert, first, m_here);
-      else if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here))
-        continue;
-      if (expert == a.experts) k_end = 0, expert = 0;  // rows without an expert: zeros
-    }
-    if (!GATHER) x += (size_t)first * a.x_stride;
-    w += (size_t)expert * a.w_expert + (WC ? (size_t)n0 * SIZE : (size_t)n0 * a.w_stride);
-    c += (size_t)first * a.c_stride;
-  }
-  const int stages = (k_end + KS - 1) / KS, full = k_end / KS;
-
-  f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int wm = wave / WN, wn = wave % WN;
-
-  if (stages > 0) {
-    // Where a lane's pieces lie behind a stage's start. No piece is clamped: what lies behind the operand's last byte
-    // of the stage is not read, and a piece of a row or column that does not exist is multiplied into what is not
-    // stored, or masked.
-    unsigned x_off[GATHER ? X::P : 1], w_off;
-    {
-      int r, k;
-      W::Tile::place(tid, r, k);
-      w_off = WC ? (unsigned)(k * a.w_stride) + r * SIZE : (unsigned)(r * a.w_stride) + k * SIZE;
-#pragma unroll
-      for (int i = 0; i < (GATHER ? X::P : 1); ++i) {
-        X::Tile::place(i * THREADS + tid, r, k);
-        if (GATHER) {
-          const int p = first + (r < m_here ? r : m_here - 1);
-          x_off[i] = (unsigned)((a.order[p] / a.top_k) * a.x_stride) + k * SIZE;
-        } else {
-          x_off[i] = XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE;
-        }
-      }
-    }
-    // from one of a lane's pieces to its next: THREADS slots on are so many rows or k on, turned alike
-    const unsigned x_next = (unsigned)((XC ? THREADS / X::Tile::PER_K : THREADS / 8) * a.x_stride);
-    const unsigned w_next = (unsigned)((WC ? THREADS / W::Tile::PER_K : THREADS / 8) * a.w_stride);
-    const size_t x_step = XC ? KS * a.x_stride : 128, w_step = WC ? KS * a.w_stride : 128;
-    // Scales of two stages (512 columns), 16 bytes a row: the first BM lanes of the workgroup load x's, BN others w's.
-    constexpr int SCALES = (BM + BN) * 16;
-    static_assert(!FOUR || BM + BN == THREADS || BM + BN == 2 * THREADS, "a lane loads one or two rows' scales");
-    constexpr int PS = FOUR ? (BM + BN) / THREADS : 1;
-    unsigned s_off[PS], s_size[PS];
-    const char *s_from[PS];
-    if constexpr (FOUR) {
-#pragma unroll
-      for (int i = 0; i < PS; ++i) {
-        const bool of_x = i * THREADS + wave * 64 < BM;
-        const size_t row = of_x ? (GATHER ? 0 : (size_t)first) : (size_t)expert * a.n + n0;
-        const unsigned rows = of_x ? (GATHER ? (unsigned)(a.x_bytes / a.x_stride) : (unsigned)m_here) : (unsigned)n_here;
-        s_from[i] = same_in_all((const char *)(of_x ? a.x_scales : a.w_scales) + row * a.scales_stride);
-        s_size[i] = __builtin_amdgcn_readfirstlane((rows - 1) * (unsigned)a.scales_stride + 16);
-        const int r = i * THREADS + tid;
-        if (GATHER && r < BM) {
-          const int m = r < m_here ? r : m_here - 1;
-          s_off[i] = (unsigned)((a.order[first + m] / a.top_k) * a.scales_stride);
-        } else {
-          s_off[i] = (unsigned)((r < BM ? r : r - BM) * a.scales_stride);
-        }
-      }
-    }
-    const unsigned base = lds_address(lds), to = base + wave * 1024;
-    auto load_scales = [&](int pair) {
-      if constexpr (FOUR) {
-        const unsigned s = to + 2 * STAGE + (pair & 1) * SCALES;
-#pragma unroll
-        for (int i = 0; i < PS; ++i) {
-          to_lds_16(buffer_of(s_from[i] + (size_t)pair * 16, pair * 2 < stages ? s_size[i] : 0), s_off[i], s + i * THREADS * 16);
-        }
-      }
-    };
-    // The stage that is loaded next, and how much of it there is.
-    struct Stage {
-      const char *x, *w;
-      unsigned x_size, w_size, to;
-    } next;
-    const auto x_size_of = [&](int k_here) {
-      return XC ? (unsigned)((k_here - 1) * a.x_stride) + m_here * SIZE : (unsigned)((m_here - 1) * a.x_stride) + k_here * SIZE;
-    };
-    const auto w_size_of = [&](int k_here) {
-      return WC ? (unsigned)((k_here - 1) * a.w_stride) + n_here * SIZE : (unsigned)((n_here - 1) * a.w_stride) + k_here * SIZE;
-    };
-    const unsigned x_full = x_size_of(KS), w_full = w_size_of(KS);
-    const unsigned x_last = x_size_of(k_end - full * KS), w_last = w_size_of(k_end - full * KS);
-    unsigned x_left = GATHER ? (unsigned)a.x_bytes : 0;
-    auto size_next = [&](int t) {
-      next.x_size = t < full ? (GATHER ? x_left : x_full) : t < stages ? x_last : 0;
-      next.w_size = t < full ? w_full : t < stages ? w_last : 0;
-    };
-    next.x = x, next.w = w, next.to = to;
-    size_next(0);
-    auto advance = [&](int t) {  // to stage t
-      next.x += x_step, next.w += w_step, next.to ^= STAGE;
-      if (GATHER) x_left -= 128;
-      size_next(t);
-    };
-    auto load_one = [&](int i) {
-      if (i < X::P)
-        to_lds_16(buffer_of(next.x, next.x_size), GATHER ? x_off[GATHER ? i : 0] : x_off[0] + i * x_next,
-                  next.to + i * THREADS * 16);
-      else
-        to_lds_16(buffer_of(next.w, next.w_size), w_off + (i - X::P) * w_next,
-                  next.to + BM * 128 + (i - X::P) * THREADS * 16);
-    };
-    auto load = [&]() {
-#pragma unroll
-      for (int i = 0; i < X::P + W::P; ++i) load_one(i);
-    };
-    X fx;
-    W fw;
-    fx.init(base, lane, wm * FM);
-    fw.init(base + BM * 128, lane, wn * FN);
-    const unsigned s_at = base + 2 * STAGE + (lane & 15) * 16 + 4 * (lane >> 4);
-
-    struct Fragments {
-      u32x4 x[FM], w[FN];
-    } f[2];
-    auto read_one = [&](auto step, int r) {
-      constexpr int S = decltype(step)::value;
-      if (r < FN)
-        f[S].w[r] = fw.template fragment<S>(r);
-      else
-        f[S].x[r - FN] = fx.template fragment<S>(r - FN);
-    };
-    auto read = [&](auto step) {
-#pragma unroll
-      for (int r = 0; r < FN + FM; ++r) read_one(step, r);
-    };
-    unsigned sx[FOUR ? FM : 1], sw[FOUR ? FN : 1];
-    auto read_scales = [&](int pair) {
-      if constexpr (FOUR) {
-        const unsigned s = s_at + (pair & 1) * SCALES;
-#pragma unroll
-        for (int i = 0; i < FM; ++i) sx[i] = lds_read_4(s + (wm * FM + i) * 256);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) sw[j] = lds_read_4(s + BM * 16 + (wn * FN + j) * 256);
-      }
-    };
-    // product q of a step of a stage of even (ODD 0) or odd number
-    auto multiply_one = [&](auto step, auto odd, int q) {
-      constexpr int S = decltype(step)::value, ODD = decltype(odd)::value;
-      const int i = q / FN, j = q % FN;
-      if constexpr (FOUR)
-        mfma_four<2 * ODD + S>(acc[i][j], f[S].w[j], f[S].x[i], sw[j], sx[i]);
-      else
-        mfma_piece(acc[i][j], f[S].w[j], f[S].x[i], Tag<T>());
-    };
-    // A step's products, with `reads` LDS reads spread between the first 3/4 of them and `loads` loads between all. (A
-    // load takes its turn in the CU's address unit; a wavefront that has to wait for that issues nothing else.)
-    auto multiply = [&](auto step, auto odd, auto reads, auto read_it, auto loads, auto load_it) {
-      constexpr int R = decltype(reads)::value, L = decltype(loads)::value, Q = FM * FN, SPAN = Q * 3 / 4;
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        // (the r-th goes before product r * SPAN / R)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (r * SPAN / (R ? R : 1) == q) read_it(r);
-#pragma unroll
-        for (int l = 0; l < L; ++l)
-          if (l * Q / (L ? L : 1) == q) load_it(l);
-        multiply_one(step, odd, q);
-        if (R || L) __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    // everything this wavefront has asked for is there; then everybody's is
-    auto meet = [&]() {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    // A step that reaches behind the last k: what lies there is no part of the sum, and may be anything.
-    auto mask = [&](auto step) {
-      constexpr int S = decltype(step)::value;
-      const int left = k_end - full * KS - S * (KS / 2) - EPP * (lane >> 4);
-      if (left < EPP) {
-        u32x4 keep;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int bytes = (left * SIZE) - 4 * i;
-          keep[i] = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : 0xffffu;
-        }
-#pragma unroll
-        for (int i = 0; i < FM; ++i) f[S].x[i] &= keep;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) f[S].w[j] &= keep;
-      }
-    };
-
-    load();
-    load_scales(0);
-    meet();
-    advance(1);
-    load();
-    read(Int<0>());
-    read_scales(0);
-    constexpr int LOADS = X::P + W::P, READS = FM + FN;
-    auto stage = [&](int t, auto odd) {
-      multiply(Int<0>(), odd, Int<READS>(), [&](int r) { read_one(Int<1>(), r); }, Int<0>(), [](int) {});
-      advance(t + 2);
-      meet();
-      if (!decltype(odd)::value) load_scales((t >> 1) + 1);
-      fx.swap(STAGE), fw.swap(STAGE);
-      multiply(
-          Int<1>(), odd, Int<READS>(), [&](int r) { read_one(Int<0>(), r); }, Int<LOADS>(),
-          [&](int l) { load_one(l); });
-      if (decltype(odd)::value) read_scales((t >> 1) + 1);
-    };
-    if constexpr (FOUR) {
-      for (int t = 0;;) {
-        stage(t, Int<0>());
-        if (++t == stages) break;
-        stage(t, Int<1>());
-        if (++t == stages) break;
-      }
-      sums_done(acc);
+  const size_t x_step = XC ? KS * a.x_stride : 128, w_step = WC ? KS * a.w_stride : 128;
+  Tile in;  // the tile that is loaded
+  const char *in_x = nullptr, *in_w = nullptr, *in_s = nullptr;
+  unsigned in_s_size = 0;
+  int in_left = 0, in_stages = 0, in_stage = 0;  // k and stages that are left, and the number of the next one
+  auto enter = [&](const Tile &r) {
+    in = r;
+    in_x = a.x, in_w = a.w;
+    if constexpr (KIND == DWEIGHTS) {
+      const int begin = a.offsets[r.expert];
+      in_x += (size_t)begin * a.x_stride + (size_t)r.first * SIZE;
+      in_w += (size_t)begin * a.w_stride + (size_t)r.n0 * SIZE;
     } else {
-      for (int t = 0; t < full; ++t) stage(t, Int<0>());
+      if (!GATHER) in_x += (size_t)r.first * a.x_stride;
+      in_w += (size_t)r.expert * a.w_expert + (WC ? (size_t)r.n0 * SIZE : (size_t)r.n0 * a.w_stride);
     }
-    if (!FOUR && full < stages) {
-      read(Int<1>());
-      mask(Int<0>());
-      multiply(Int<0>(), Int<0>(), Int<0>(), [](int) {}, Int<0>(), [](int) {});
-      mask(Int<1>());
-      multiply(Int<1>(), Int<0>(), Int<0>(), [](int) {}, Int<0>(), [](int) {});
+    in_x = same_in_all(in_x), in_w = same_in_all(in_w);
+    in_left = r.k_end, in_stages = r.m_here ? stages_of(r.k_end) : 0x7fffffff, in_stage = 0;
+    if (r.m_here == 0) in_left = 0;
+    if constexpr (GATHER) {
+#pragma unroll
+      for (int i = 0; i < X::P; ++i) {
+        int m, k;
+        X::Tile::place(i * THREADS + threadIdx.x, m, k);
+        x_off[i] = gathered[m] * (unsigned)a.x_stride + k * SIZE;
+      }
     }
-  }
-  // loads that read nothing end, and everybody's reads, before the LDS is used again
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __syncthreads();
+    if constexpr (FOUR) {
+      const bool of_x = wave * 64 < BM;
+      const size_t row = of_x ? (GATHER ? 0 : (size_t)r.first) : (size_t)r.expert * a.n + r.n0;
+      const unsigned rows = of_x ? (GATHER ? (unsigned)(a.x_bytes / a.x_stride) : (unsigned)r.m_here) : (unsigned)r.n_here;
+      in_s = same_in_all((const char *)(of_x ? a.x_scales : a.w_scales) + row * a.scales_stride);
+      in_s_size = (rows - 1) * (unsigned)a.scales_stride + 16;
+      if (GATHER && of_x) s_off = gathered[threadIdx.x % BM] * (unsigned)a.scales_stride;
+    }
+  };
+  unsigned x_size = 0, w_size = 0;
+  auto size_up = [&]() {  // of the stage that is loaded now
+    const int k_here = in_left < KS ? in_left : KS;
+    x_size = k_here <= 0 ? 0
+             : GATHER    ? (unsigned)(a.x_bytes - (size_t)in_stage * 128)
+             : XC        ? (unsigned)((k_here - 1) * a.x_stride) + in.m_here * SIZE
+                         : (unsigned)((in.m_here - 1) * a.x_stride) + k_here * SIZE;
+    w_size = k_here <= 0 ? 0
+             : WC        ? (unsigned)((k_here - 1) * a.w_stride) + in.n_here * SIZE
+                         : (unsigned)((in.n_here - 1) * a.w_stride) + k_here * SIZE;
+  };
+  unsigned buffer = 0;  // of the stage that is loaded now: 0 or STAGE
+  auto load_one = [&](int i) {
+    if (i < X::P)
+      to_lds_16(buffer_of(in_x, x_size), GATHER ? x_off[GATHER ? i : 0] : x_off[0] + i * x_next,
+                to + buffer + i * THREADS * 16);
+    else
+      to_lds_16(buffer_of(in_w, w_size), w_off + (i - X::P) * w_next, to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
+  };
+  unsigned scales_in = 0;  // 0 or SCALES
+  auto load_scales = [&]() {  // of this stage and the next, 512 columns, at every even stage of a tile
+    if constexpr (FOUR) {
+      if (!(in_stage & 1)) {
+        to_lds_16(buffer_of(in_s + (size_t)in_stage * 8, in_left > 0 ? in_s_size : 0), s_off, to + 2 * STAGE + scales_in);
+        scales_in ^= SCALES;
+      }
+    }
+  };
+  auto loaded = [&]() {
+    in_x += x_step, in_w += w_step, in_left -= KS, ++in_stage, buffer ^= STAGE;
+  };
 
-  int tid2 = threadIdx.x;
-  asm volatile("" : "+v"(tid2));
-  store_tile<OUT, FM, FN, STAGE * 2 / (WM * WN)>(lds + wave * (STAGE * 2 / (WM * WN)), tid2 & 63, acc, c + n0, a.c_stride,
-                                                 wm * FM * 16, wn * FN * 16, m_here, n_here, a.c_aligned);
+  // ---- what is multiplied
+  f32x4 acc[FM][FN];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  X fx;
+  W fw;
+  fx.init(base, threadIdx.x & 63, wm * FM);
+  fw.init(base + BM * 128, threadIdx.x & 63, wn * FN);
+  unsigned s_at = base + 2 * STAGE + (threadIdx.x & 15) * 16 + (threadIdx.x & 48) / 4;
+
+  struct Fragments {
+    u32x4 x[FM], w[FN];
+  } f[2];
+  auto read_one = [&](auto step, int r) {
+    constexpr int S = decltype(step)::value;
+    if (r < FN)
+      f[S].w[r] = fw.template fragment<S>(r);
+    else
+      f[S].x[r - FN] = fx.template fragment<S>(r - FN);
+  };
+  unsigned sx[FOUR ? FM : 1], sw[FOUR ? FN : 1];
+  auto read_scales = [&](int t) {  // two bytes: those of the stage's two steps
+    if constexpr (FOUR) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) sw[j] = lds_read_2(s_at + (t & 1) * 2 + BM * 16 + (wn * FN + j) * 256);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) sx[i] = lds_read_2(s_at + (t & 1) * 2 + (wm * FM + i) * 256);
+    }
+  };
+  auto multiply_one = [&](auto step, int q) {
+    constexpr int S = decltype(step)::value;
+    const int i = q / FN, j = q % FN;
+    if constexpr (FOUR)
+      mfma_four<S>(acc[i][j], f[S].w[j], f[S].x[i], sw[j], sx[i]);
+    else
+      mfma_piece(acc[i][j], f[S].w[j], f[S].x[i], Tag<T>());
+  };
+  // A step's products, with the LDS reads of the next step spread between the first 3/4 of them and `loads` loads between
+  // all. (A load takes its turn in the CU's address unit; a wavefront that has to wait for that issues nothing else.)
+  auto multiply = [&](auto step, auto loads, auto load_it) {
+    constexpr int S = decltype(step)::value, R = FM + FN, L = decltype(loads)::value, Q = FM * FN, SPAN = Q * 3 / 4;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r * SPAN / R == q) read_one(Int<1 - S>(), r);
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        if (l * Q / (L ? L : 1) == q) load_it(l);
+      multiply_one(step, q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // everything this wavefront has asked for is there; then everybody's is
+  auto meet = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step that reaches behind the last k (`left` are there): what lies there is no part of the sum, and may be anything.
+  auto mask = [&](auto step, int left) {
+    constexpr int S = decltype(step)::value;
+    left -= S * (KS / 2) + EPP * ((threadIdx.x & 63) >> 4);
+    u32x4 keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bytes = left * SIZE - 4 * i;
+      keep[i] = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : 0xffffu;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) f[S].x[i] &= keep;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) f[S].w[j] &= keep;
+  };
+
+  Tile now = locate();  // the tile that is multiplied
+  if (now.m_here == 0) return;
+  put_order(order_of(now));
   __syncthreads();
+  enter(now);
+  for (int s = 0; s < 2; ++s) {  // (a tile has two stages at least)
+    size_up();
+#pragma unroll
+    for (int i = 0; i < X::P + W::P; ++i) load_one(i);
+    load_scales();
+    loaded();
+    if (s == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
+  Tile ahead = locate();
+  __syncthreads();
+  put_order(order_of(ahead));
+  clear();
+#pragma unroll
+  for (int r = 0; r < FM + FN; ++r) read_one(Int<0>(), r);
+  read_scales(0);
+  for (int t = 0, left = now.k_end;;) {
+    if (!FOUR && left < KS) mask(Int<0>(), left);
+    multiply(Int<0>(), Int<0>(), [](int) {});
+    meet();
+    if (in_stage == in_stages) enter(ahead);
+    size_up();
+    if (!FOUR && left < KS) mask(Int<1>(), left);
+    fx.swap(STAGE), fw.swap(STAGE);
+    multiply(Int<1>(), Int<X::P + W::P>(), load_one);
+    load_scales();
+    loaded();
+    ++t, left -= KS;
+    if (FOUR && !(t & 1)) s_at = scales_swapped(s_at, SCALES, base + 2 * STAGE);
+    if (t == stages_of(now.k_end)) {
+      if (FOUR) {
+        if (t & 1) s_at = scales_swapped(s_at, SCALES, base + 2 * STAGE);
+        if (now.k_end == 0) clear();
+      }
+      // `in` is the tile that comes now; the one after it is looked for while this one goes out
+      const Tile next = in;
+      ahead = locate();
+      const int slot = order_of(ahead);
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));  // (what follows from it is not kept over the stages)
+      OUT *c = static_cast<OUT *>(a.c) + (KIND == DWEIGHTS ? (size_t)now.expert * a.c_expert : 0) +
+               (size_t)now.first * a.c_stride + now.n0;
+      store_tile<OUT, FM, FN>(tid & 63, acc, c, a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here, a.c_aligned);
+      put_order(slot);
+      now = next;
+      if (now.m_here == 0) break;
+      t = 0, left = now.k_end;
+      clear();
+    }
+    read_scales(t);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads that read nothing end before the LDS is another's)
 }
 
 constexpr size_t PIPE_WORKGROUPS = 256;    // one to a CU, as many as the LDS allows
@@ -585,7 +568,8 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
   a.band = a.n_tiles >= 8 ? 4 : a.n_tiles >= 4 ? 8 : 16;
   const size_t tiles = m_tiles * a.n_tiles;
   if (m_tiles > (size_t)INT_MAX || tiles > (size_t)INT_MAX) return H2O4GPU_KMEANS_EARG;
-  const size_t lds = (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (PIPE_TABLE + 2 + WM * WN) * 4;
+  const size_t lds =
+      (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (GATHER ? BM * 4 : 0) + (PIPE_TABLE + 2 + WM * WN) * 4;
   const auto kernel = pipe_kernel<ELEMENT, OUT, KIND, GATHER, BM, BN, WM, WN>;
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
   const size_t blocks = tiles < PIPE_WORKGROUPS ? (tiles + 7) / 8 * 8 : PIPE_WORKGROUPS;
