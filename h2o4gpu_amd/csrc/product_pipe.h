@@ -56,9 +56,6 @@ __device__ __forceinline__ u32x4 lds_read_16(unsigned at) {
 __device__ __forceinline__ unsigned lds_read_4(unsigned at) {
   return *(__attribute__((address_space(3))) const unsigned *)(size_t)at;
 }
-__device__ __forceinline__ unsigned lds_read_2(unsigned at) {
-  return *(__attribute__((address_space(3))) const unsigned short *)(size_t)at;
-}
 // the other one of two places `apart` bytes apart, the first at `start`
 __device__ __forceinline__ unsigned scales_swapped(unsigned at, unsigned apart, unsigned start) {
   return at >= start + apart ? at - apart : at + apart;
@@ -102,6 +99,7 @@ __device__ __forceinline__ void mfma_four(f32x4 &acc, u32x4 w, u32x4 x, unsigned
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
   const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, SELECT, (int)sw, SELECT, (int)sx);
+  asm volatile("" : "+v"(acc));  // (stays where it is written, between the loads around it)
 #endif
 }
 // One operand of a tile of R rows in a workgroup of THREADS: where its pieces come from, where fragments lie.
@@ -152,9 +150,10 @@ struct PipeOperand {
 
 constexpr int PIPE_TABLE = 2046;  // experts + 2 numbers of 4 bytes fit 8 KB of LDS
 
-// table[e]: how many tiles of BM rows the experts before e have; [experts + 1]: all, those without an expert included.
-template <int BM, int THREADS>
-__device__ __forceinline__ void tile_table(int *table, const int *offsets, int experts, int rows) {
+// table[e]: the sum of count(rows of an expert) over the experts before e; [experts + 1]: over all, and over the rows
+// without an expert.
+template <int THREADS, typename COUNT>
+__device__ __forceinline__ void tile_table(int *table, const int *offsets, int experts, int rows, COUNT count) {
   constexpr int EACH = (PIPE_TABLE + 1 + THREADS - 1) / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int mine[EACH], sum = 0;
@@ -162,7 +161,7 @@ __device__ __forceinline__ void tile_table(int *table, const int *offsets, int e
   for (int i = 0; i < EACH; ++i) {
     const int e = tid * EACH + i;
     mine[i] = 0;
-    if (e <= experts) mine[i] = ((e < experts ? offsets[e + 1] : rows) - offsets[e] + BM - 1) / BM;
+    if (e <= experts) mine[i] = count((e < experts ? offsets[e + 1] : rows) - offsets[e]);
     sum += mine[i];
   }
   int before = sum;
@@ -187,11 +186,10 @@ __device__ __forceinline__ void tile_table(int *table, const int *offsets, int e
   __syncthreads();
 }
 
-template <int BM>
-__device__ __forceinline__ void listed_tile(const int *table, const int *offsets, int experts, int rows, int number,
-                                            int &stretch, int &first, int &rows_here) {
+// The last e of the first `n` with table[e] <= number.
+__device__ __forceinline__ int last_below(const int *table, int n, int number) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = experts + 1;  // the last e with table[e] <= number
+  int lo = 0;
   while (n > 1) {
     const int step = (n + 63) / 64;
     const bool below = lane * step < n && table[lo + lane * step] <= number;
@@ -199,7 +197,13 @@ __device__ __forceinline__ void listed_tile(const int *table, const int *offsets
     lo += skip;
     n = n - skip < step ? n - skip : step;
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <int BM>
+__device__ __forceinline__ void listed_tile(const int *table, const int *offsets, int experts, int rows, int number,
+                                            int &stretch, int &first, int &rows_here) {
+  const int lo = last_below(table, experts + 1, number);
   const int begin = offsets[lo], end = lo == experts ? rows : offsets[lo + 1];
   stretch = lo;
   first = begin + (number - __builtin_amdgcn_readfirstlane(table[lo])) * BM;
@@ -270,26 +274,43 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   constexpr int STAGE = (BM + BN) * 128, SCALES = (BM + BN) * 16;
   static_assert((STAGE & (STAGE - 1)) == 0, "the buffers are told apart by one bit");
   static_assert(!FOUR || BM + BN == THREADS, "a lane loads one row's scales");
-  // stages, two of them | Four: scales of two stages, two of these | GATHER: where x's rows lie | table of tiles
+  // stages, two of them | Four: scales of two stages, two of these | GATHER: which rows of x, of two tiles | table of tiles
   extern __shared__ __attribute__((aligned(16))) char lds[];
   unsigned *gathered = reinterpret_cast<unsigned *>(lds + 2 * STAGE + (FOUR ? 2 * SCALES : 0));
-  int *table = reinterpret_cast<int *>(gathered + (GATHER ? BM : 0));
+  int *table = reinterpret_cast<int *>(gathered + (GATHER ? 2 * BM : 0));
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const unsigned base = lds_address(lds), to = base + wave * 1024;
-  // Tiles of m, numbered without gaps: those of expert 0, of expert 1, ..., of the rows without an expert. A table in
+  // Tiles of m are numbered without gaps: those of expert 0, of expert 1, ..., of the rows without an expert. A table in
   // LDS says where each expert's begin; beyond PIPE_TABLE experts the numbers have gaps (ragged_tile).
-  const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = ragged && a.experts < PIPE_TABLE;
+  const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = a.experts > 0 && a.experts < PIPE_TABLE;
+  auto stages_of = [](int k) { return k <= KS ? 2 : (k + KS - 1) / KS; };
   unsigned m_tiles = (unsigned)a.m_tiles;
-  if (listed) {
-    tile_table<BM, THREADS>(table, a.offsets, a.experts, a.rows);
-    m_tiles = __builtin_amdgcn_readfirstlane(table[a.experts + 1]);
-  }
   // Workgroups go round the eight chiplets; each of these takes a stretch of the tiles, and its workgroups neighbours
   // of that at the same time: `band` tiles of m by as many of n as there are workgroups.
-  const unsigned total = m_tiles * (unsigned)a.n_tiles, die = blockIdx.x & 7;
-  const unsigned tiles_end = (unsigned)((unsigned long long)total * (die + 1) / 8);
-  unsigned tile = (unsigned)((unsigned long long)total * die / 8) + (blockIdx.x >> 3);
+  const unsigned die = blockIdx.x & 7;
+  unsigned tile, tiles_end;
+  if (listed && KIND == DWEIGHTS) {
+    // stretches of as many stages, since an expert's tiles have as many as its rows fill
+    tile_table<THREADS>(table, a.offsets, a.experts, a.rows, stages_of);
+    const unsigned long long each = m_tiles / a.experts * (unsigned)a.n_tiles, all = table[a.experts] * each;
+    auto border = [&](unsigned d) {
+      const unsigned long long work = all * d / 8;
+      const int e = last_below(table, a.experts, (int)(work / each));
+      const unsigned stages = table[e + 1] - table[e];
+      const unsigned long long in = (work - table[e] * each) / stages;
+      return (unsigned)__builtin_amdgcn_readfirstlane((int)(e * each + (in < each ? in : each)));
+    };
+    tile = border(die) + (blockIdx.x >> 3), tiles_end = border(die + 1);
+  } else {
+    if (listed) {
+      tile_table<THREADS>(table, a.offsets, a.experts, a.rows, [](int rows) { return (rows + BM - 1) / BM; });
+      m_tiles = __builtin_amdgcn_readfirstlane(table[a.experts + 1]);
+    }
+    const unsigned total = m_tiles * (unsigned)a.n_tiles;
+    tiles_end = (unsigned)((unsigned long long)total * (die + 1) / 8);
+    tile = (unsigned)((unsigned long long)total * die / 8) + (blockIdx.x >> 3);
+  }
 
   struct Tile {
     int n0, n_here, m_here, first, expert, k_end;  // m_here 0: there is none
@@ -329,16 +350,17 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     const int m = (int)threadIdx.x % BM;
     return GATHER && r.m_here > 0 ? a.order[r.first + (m < r.m_here ? m : r.m_here - 1)] : 0;
   };
+  unsigned rows_put = 0, rows_in = BM;  // which of the two is written next, and which is read
   auto put_order = [&](int slot) {
-    if (GATHER && threadIdx.x < BM) gathered[threadIdx.x] = (unsigned)(slot / a.top_k);
+    if (GATHER && threadIdx.x < BM) gathered[rows_put + threadIdx.x] = (unsigned)(slot / a.top_k);
+    rows_put ^= BM;
   };
-  auto stages_of = [&](int k_end) { return k_end <= KS ? 2 : (k_end + KS - 1) / KS; };
 
   // ---- what is loaded
   // Where a lane's pieces lie behind a stage's start. No piece is clamped: what lies behind the operand's last byte of
   // the stage is not read, and a piece of a row or column that does not exist is multiplied into what is not stored, or
   // masked. From one of a lane's pieces to its next, THREADS slots on, are so many rows or k, turned alike.
-  unsigned x_off[GATHER ? X::P : 1], w_off, s_off = 0;
+  unsigned x_off, w_off;
   const unsigned x_next = (unsigned)((XC ? THREADS / X::Tile::PER_K : THREADS / 8) * a.x_stride);
   const unsigned w_next = (unsigned)((WC ? THREADS / W::Tile::PER_K : THREADS / 8) * a.w_stride);
   {
@@ -346,8 +368,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     W::Tile::place(threadIdx.x, r, k);
     w_off = WC ? (unsigned)(k * a.w_stride) + r * SIZE : (unsigned)(r * a.w_stride) + k * SIZE;
     X::Tile::place(threadIdx.x, r, k);
-    if (!GATHER) x_off[0] = XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE;
-    if (FOUR) s_off = (unsigned)((threadIdx.x % BM) * a.scales_stride);
+    x_off = GATHER ? k * SIZE : XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE;
   }
   const size_t x_step = XC ? KS * a.x_stride : 128, w_step = WC ? KS * a.w_stride : 128;
   Tile in;  // the tile that is loaded
@@ -368,21 +389,13 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     in_x = same_in_all(in_x), in_w = same_in_all(in_w);
     in_left = r.k_end, in_stages = r.m_here ? stages_of(r.k_end) : 0x7fffffff, in_stage = 0;
     if (r.m_here == 0) in_left = 0;
-    if constexpr (GATHER) {
-#pragma unroll
-      for (int i = 0; i < X::P; ++i) {
-        int m, k;
-        X::Tile::place(i * THREADS + threadIdx.x, m, k);
-        x_off[i] = gathered[m] * (unsigned)a.x_stride + k * SIZE;
-      }
-    }
+    rows_in ^= BM;
     if constexpr (FOUR) {
       const bool of_x = wave * 64 < BM;
       const size_t row = of_x ? (GATHER ? 0 : (size_t)r.first) : (size_t)r.expert * a.n + r.n0;
       const unsigned rows = of_x ? (GATHER ? (unsigned)(a.x_bytes / a.x_stride) : (unsigned)r.m_here) : (unsigned)r.n_here;
       in_s = same_in_all((const char *)(of_x ? a.x_scales : a.w_scales) + row * a.scales_stride);
       in_s_size = (rows - 1) * (unsigned)a.scales_stride + 16;
-      if (GATHER && of_x) s_off = gathered[threadIdx.x % BM] * (unsigned)a.scales_stride;
     }
   };
   unsigned x_size = 0, w_size = 0;
@@ -397,9 +410,18 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
                          : (unsigned)((in.n_here - 1) * a.w_stride) + k_here * SIZE;
   };
   unsigned buffer = 0;  // of the stage that is loaded now: 0 or STAGE
+  unsigned row_off[GATHER ? X::P : 1];
+  auto find_rows = [&]() {  // (kept over a stage only, for want of registers)
+    if constexpr (GATHER) {
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+#pragma unroll
+      for (int i = 0; i < X::P; ++i) row_off[i] = gathered[rows_in + i * (THREADS / 8) + tid / 8] * (unsigned)a.x_stride;
+    }
+  };
   auto load_one = [&](int i) {
     if (i < X::P)
-      to_lds_16(buffer_of(in_x, x_size), GATHER ? x_off[GATHER ? i : 0] : x_off[0] + i * x_next,
+      to_lds_16(buffer_of(in_x, x_size), x_off + (GATHER ? row_off[GATHER ? i : 0] : i * x_next),
                 to + buffer + i * THREADS * 16);
     else
       to_lds_16(buffer_of(in_w, w_size), w_off + (i - X::P) * w_next, to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
@@ -408,7 +430,11 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   auto load_scales = [&]() {  // of this stage and the next, 512 columns, at every even stage of a tile
     if constexpr (FOUR) {
       if (!(in_stage & 1)) {
-        to_lds_16(buffer_of(in_s + (size_t)in_stage * 8, in_left > 0 ? in_s_size : 0), s_off, to + 2 * STAGE + scales_in);
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const unsigned row = GATHER && wave * 64 < BM ? gathered[rows_in + tid % BM] : tid % BM;
+        to_lds_16(buffer_of(in_s + (size_t)in_stage * 8, in_left > 0 ? in_s_size : 0), row * (unsigned)a.scales_stride,
+                  to + 2 * STAGE + scales_in);
         scales_in ^= SCALES;
       }
     }
@@ -442,12 +468,19 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       f[S].x[r - FN] = fx.template fragment<S>(r - FN);
   };
   unsigned sx[FOUR ? FM : 1], sw[FOUR ? FN : 1];
-  auto read_scales = [&](int t) {  // two bytes: those of the stage's two steps
+  auto read_scales = [&](int t) {  // words of the four steps of two stages: their low halves count
     if constexpr (FOUR) {
+      if (t & 1) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) sw[j] = lds_read_2(s_at + (t & 1) * 2 + BM * 16 + (wn * FN + j) * 256);
+        for (int j = 0; j < FN; ++j) sw[j] >>= 16;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) sx[i] = lds_read_2(s_at + (t & 1) * 2 + (wm * FM + i) * 256);
+        for (int i = 0; i < FM; ++i) sx[i] >>= 16;
+      } else {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sw[j] = lds_read_4(s_at + BM * 16 + (wn * FN + j) * 256);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sx[i] = lds_read_4(s_at + (wm * FM + i) * 256);
+      }
     }
   };
   auto multiply_one = [&](auto step, int q) {
@@ -505,6 +538,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   enter(now);
   for (int s = 0; s < 2; ++s) {  // (a tile has two stages at least)
     size_up();
+    find_rows();
 #pragma unroll
     for (int i = 0; i < X::P + W::P; ++i) load_one(i);
     load_scales();
@@ -524,6 +558,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     meet();
     if (in_stage == in_stages) enter(ahead);
     size_up();
+    find_rows();
     if (!FOUR && left < KS) mask(Int<1>(), left);
     fx.swap(STAGE), fw.swap(STAGE);
     multiply(Int<1>(), Int<X::P + W::P>(), load_one);
@@ -569,7 +604,7 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
   const size_t tiles = m_tiles * a.n_tiles;
   if (m_tiles > (size_t)INT_MAX || tiles > (size_t)INT_MAX) return H2O4GPU_KMEANS_EARG;
   const size_t lds =
-      (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (GATHER ? BM * 4 : 0) + (PIPE_TABLE + 2 + WM * WN) * 4;
+      (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (GATHER ? BM * 8 : 0) + (PIPE_TABLE + 2 + WM * WN) * 4;
   const auto kernel = pipe_kernel<ELEMENT, OUT, KIND, GATHER, BM, BN, WM, WN>;
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
   const size_t blocks = tiles < PIPE_WORKGROUPS ? (tiles + 7) / 8 * 8 : PIPE_WORKGROUPS;
