@@ -6,7 +6,7 @@
 // or a multiple to a row; scales 16 bytes for 512 columns, the byte of the block b of these 16 at 4 * (b % 4) + b / 4:
 // lane group g of a matrix instruction multiplies block g of its 128 columns, and has the scales of four
 // instructions in one word. Behind a row's last column lie zeros (codes and scales).
-#include "product_pipe.h"
+#include "product_thin.h"
 
 namespace kmhip {
 namespace {
@@ -151,6 +151,8 @@ struct FourArgs {
   const int *order, *offsets;  // with experts only; order: x's row of y's row p is order[p] / top_k (none: p)
   int top_k, experts;          // experts 0: one matrix
   int rows, out, cols, y_aligned;
+  unsigned first_block;
+  int n_tiles;
 };
 
 __device__ __forceinline__ void to_lds(const void *from, char *lds) {
@@ -171,8 +173,8 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n_tiles = (a.out + BN - 1) / BN;
-  const int n0 = (int)(blockIdx.x % n_tiles) * BN, number = (int)(blockIdx.x / n_tiles);
+  const unsigned block = a.first_block + blockIdx.x;
+  const int n0 = (int)(block % (unsigned)a.n_tiles) * BN, number = (int)(block / (unsigned)a.n_tiles);
   int expert = 0, first = number * BM, m_here = a.rows - first < BM ? a.rows - first : BM;
   int stages = (a.cols + 255) / 256;
   if (a.experts) {
@@ -268,6 +270,14 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 template <typename T>
 int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   const size_t pitch = codes_pitch(a.cols);
+  if (a.rows / (a.experts ? a.experts : 1) <= 64) {
+    ThinArgs t = {};
+    t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
+    t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);
+    t.c_stride = a.y_stride, t.c_aligned = a.y_aligned, t.order = a.order, t.offsets = a.offsets, t.top_k = a.top_k;
+    t.experts = a.experts, t.rows = a.rows, t.n = a.out, t.k = (int)((a.cols + 127) / 128 * 32);
+    return launch_thin<Four, T, true>(t, stream);
+  }
   if (x_rows * pitch < BUFFER_BYTES && pitch < BUFFER_BYTES / 512 && a.out >= 128 &&
       a.rows / (a.experts ? a.experts : 1) >= 128) {
     PipeArgs p = {};
@@ -281,9 +291,13 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   }
   constexpr int BM = 128, BN = 128;
   const size_t m_tiles = a.experts ? ragged_tiles(a.experts, a.rows, BM) : ((size_t)a.rows + BM - 1) / BM;
-  const size_t n_tiles = ((size_t)a.out + BN - 1) / BN;
-  hipLaunchKernelGGL((four_kernel<T, BM, BN, 2, 2>), dim3((unsigned)(m_tiles * n_tiles)), dim3(256), 0, stream, a);
-  return launched();
+  FourArgs f = a;
+  f.n_tiles = (a.out + BN - 1) / BN;
+  return in_launches(m_tiles * f.n_tiles, [&](unsigned first, unsigned blocks) {
+    f.first_block = first;
+    hipLaunchKernelGGL((four_kernel<T, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, f);
+    return launched();
+  });
 }
 
 bool sized(size_t rows, size_t cols) { return cols >= 1 && cols <= MAX_SIDE && rows <= ((size_t)1 << 40) / codes_pitch(cols); }

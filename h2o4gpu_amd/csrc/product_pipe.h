@@ -8,8 +8,6 @@
 // buffer is free for stage t + 2 from there, and what arrives there is stage t + 1, half a stage before it is needed.
 #pragma once
 
-#include <limits.h>
-
 #include "product_tiles.h"
 
 namespace kmhip {

@@ -1,0 +1,147 @@
+// Products of few rows: the matrices are read once, straight into the registers of the matrix instructions' operand, and
+// that is what bounds them. A workgroup has 16 NB rows of a matrix and MB blocks of 16 rows of x; its wavefronts share
+// the columns and add up their sums in LDS.
+#pragma once
+
+#include "product_pipe.h"
+
+namespace kmhip {
+
+struct ThinArgs {
+  const char *x, *w;
+  const unsigned char *x_scales, *w_scales;            // Four only, rows of `scales_stride` bytes
+  void *c;
+  size_t x_stride, w_stride, w_expert, scales_stride;  // bytes
+  size_t c_stride;                                     // elements
+  const int *order, *offsets;                          // as in PipeArgs
+  int top_k, experts, rows, n, k;                      // k in elements (Four: in groups of four columns)
+  unsigned first_block;
+  int n_tiles, c_aligned;                              // c_aligned: four elements of C may be stored at once
+};
+
+// ALIGNED: every piece lies at a multiple of 16 bytes, and k is whole pieces.
+template <typename ELEMENT, typename OUT, int MB, int NB, int WAVES, bool ALIGNED>
+__global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
+  typedef typename PipeElement<ELEMENT>::type T;
+  constexpr bool FOUR = __is_same(ELEMENT, Four);
+  constexpr int SIZE = (int)sizeof(T), EPP = 16 / SIZE, STEP = 4 * EPP, U = 4;  // k of a step; steps of a turn
+  __shared__ f32x4 sums[WAVES][MB * NB][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const unsigned block = a.first_block + blockIdx.x;
+  const int n0 = (int)(block % (unsigned)a.n_tiles) * (16 * NB), number = (int)(block / (unsigned)a.n_tiles);
+  int expert = 0, first = number * (16 * MB), m_here = a.rows - first < 16 * MB ? a.rows - first : 16 * MB, k = a.k;
+  if (a.experts) {
+    if (!ragged_tile(a.offsets, a.experts, a.rows, 16 * MB, number, expert, first, m_here)) return;
+    if (expert == a.experts) k = 0, expert = 0;  // rows without an expert: zeros
+  }
+  const int n_here = a.n - n0 < 16 * NB ? a.n - n0 : 16 * NB;
+
+  f32x4 acc[MB][NB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // rows that do not exist are read at the last one that does
+  const char *x[MB], *w[NB];
+  const unsigned char *xs[FOUR ? MB : 1], *ws[FOUR ? NB : 1];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const int p = first + (m * 16 + i < m_here ? m * 16 + i : m_here - 1);
+    const size_t row = a.order && k ? (size_t)(a.order[p] / a.top_k) : (size_t)p;
+    x[m] = a.x + row * a.x_stride + g * 16;
+    if constexpr (FOUR) xs[m] = a.x_scales + row * a.scales_stride + 4 * g;
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int r = n0 + (n * 16 + i < n_here ? n * 16 + i : n_here - 1);
+    w[n] = a.w + (size_t)expert * a.w_expert + (size_t)r * a.w_stride + g * 16;
+    if constexpr (FOUR) ws[n] = a.w_scales + ((size_t)expert * a.n + r) * a.scales_stride + 4 * g;
+  }
+  const int turns = (k + U * STEP - 1) / (U * STEP);
+  // a wavefront's turns lie side by side
+  const int each = (turns + WAVES - 1) / WAVES, begin = wave * each, end = begin + each < turns ? begin + each : turns;
+  u32x4 fx[U][MB], fw[U][NB];
+  unsigned sx[FOUR ? MB : 1], sw[FOUR ? NB : 1];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t at = ((size_t)t * U + u) * 64;
+      const int left = k - ((t * U + u) * STEP + g * EPP);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (ALIGNED)
+          fw[u][n] = left > 0 ? *reinterpret_cast<const u32x4 *>(w[n] + at) : u32x4{0, 0, 0, 0};
+        else
+          fw[u][n] = load_piece(reinterpret_cast<const T *>(w[n] + at), left);
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        if constexpr (ALIGNED)
+          fx[u][m] = left > 0 ? *reinterpret_cast<const u32x4 *>(x[m] + at) : u32x4{0, 0, 0, 0};
+        else
+          fx[u][m] = load_piece(reinterpret_cast<const T *>(x[m] + at), left);
+      }
+    }
+    if constexpr (FOUR) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sw[n] = *reinterpret_cast<const unsigned *>(ws[n] + (size_t)t * 16);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) sx[m] = *reinterpret_cast<const unsigned *>(xs[m] + (size_t)t * 16);
+    }
+  };
+  for (int t = begin; t < end; ++t) {
+    load(t);
+    auto step = [&](auto number) {
+      constexpr int S = decltype(number)::value;
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if constexpr (FOUR)
+            mfma_four<S>(acc[m][n], fw[S][n], fx[S][m], sw[n], sx[m]);
+          else
+            mfma_piece(acc[m][n], fw[S][n], fx[S][m], Tag<T>());
+        }
+    };
+    step(Int<0>());
+    step(Int<1>());
+    step(Int<2>());
+    step(Int<3>());
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sums[wave][m * NB + n][lane] = acc[m][n];
+  __syncthreads();
+  for (int b = wave; b < MB * NB; b += WAVES) {
+    f32x4 s = sums[0][b][lane];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) s += sums[v][b][lane];
+    const int m = b / NB * 16 + i, n = b % NB * 16 + 4 * g;
+    if (m < m_here)
+      store_four(static_cast<OUT *>(a.c) + (size_t)(first + m) * a.c_stride + n0 + n, s, n_here - n, a.c_aligned);
+  }
+}
+
+template <typename ELEMENT, typename OUT, bool ALIGNED>
+int launch_thin(ThinArgs &a, hipStream_t stream) {
+  const int each = a.experts ? a.rows / a.experts : a.rows;  // rows of an expert, on average
+  auto launch = [&](auto mb, auto nb) {
+    constexpr int MB = decltype(mb)::value, NB = decltype(nb)::value, WAVES = 8;
+    const size_t m_tiles =
+        a.experts ? ragged_tiles(a.experts, a.rows, 16 * MB) : ((size_t)a.rows + 16 * MB - 1) / (16 * MB);
+    a.n_tiles = (a.n + 16 * NB - 1) / (16 * NB);
+    return in_launches(m_tiles * a.n_tiles, [&](unsigned first, unsigned blocks) {
+      a.first_block = first;
+      hipLaunchKernelGGL((thin_kernel<ELEMENT, OUT, MB, NB, WAVES, ALIGNED>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+      return launched();
+    });
+  };
+  if (each <= 16) return launch(Int<1>(), Int<1>());
+  if (each <= 32) return launch(Int<2>(), Int<2>());
+  if (each <= 48) return launch(Int<3>(), Int<2>());
+  return launch(Int<4>(), Int<2>());
+}
+
+}  // namespace kmhip

@@ -6,6 +6,8 @@
 // and a stage of an operand tile is 128 bytes of k for each of its rows, in either order.
 #pragma once
 
+#include <limits.h>
+
 #include "experts_common.h"
 
 namespace kmhip {
@@ -145,6 +147,15 @@ __device__ __forceinline__ bool ragged_tile(const int *offsets, int count, int r
   return rows_here > 0;
 }
 inline size_t ragged_tiles(int count, int rows, int tile) { return (size_t)(rows / tile) + count + 1; }
+
+// launch(first block, blocks) until all of them are; a launch has at most 2^32 threads.
+template <typename F>
+inline int in_launches(size_t blocks, F launch) {
+  constexpr size_t MOST = (size_t)1 << 22;
+  if (blocks > UINT_MAX) return H2O4GPU_KMEANS_EARG;
+  for (size_t b = 0; b < blocks; b += MOST) KM_TRY(launch((unsigned)b, (unsigned)(blocks - b < MOST ? blocks - b : MOST)));
+  return H2O4GPU_KMEANS_OK;
+}
 
 // f's four values of consecutive n to row m of C; `full`: all four exist and the address is aligned to four.
 template <typename T>

@@ -5,7 +5,7 @@
 //   product_dweights: dW[e] = sum over p of dy[p] x[p]^T
 //
 // Sums are float32, in an order that depends on the sizes alone; one rounding at the end.
-#include "product_pipe.h"
+#include "product_thin.h"
 
 namespace kmhip {
 namespace {
@@ -18,6 +18,8 @@ struct ProductArgs {
   const int *offsets;
   int experts, rows, n, k;  // DWEIGHTS: n = cols, k = out, which is C's m
   int c_aligned;            // four elements of C may be stored at once
+  unsigned first_block;
+  int n_tiles;
 };
 
 // Any strides and alignment: pieces come through registers, masked at the edges. Two stages in LDS.
@@ -33,15 +35,16 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = blockIdx.x * BN;
+  const unsigned block = a.first_block + blockIdx.x, number = block / (unsigned)a.n_tiles;
+  const int n0 = (int)(block % (unsigned)a.n_tiles) * BN;
   int expert, first, m_here;
   const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
   T *c = static_cast<T *>(a.c);
   int k_end = a.k;
   if (KIND == DWEIGHTS) {
     const int tiles = (a.k + BM - 1) / BM;
-    expert = blockIdx.y / tiles;
-    first = (blockIdx.y % tiles) * BM;
+    expert = number / tiles;
+    first = (number % tiles) * BM;
     m_here = a.k - first < BM ? a.k - first : BM;
     const int begin = a.offsets[expert];
     k_end = a.offsets[expert + 1] - begin;
@@ -49,7 +52,7 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
     w += (size_t)begin * a.w_stride;
     c += (size_t)expert * a.c_expert + (size_t)first * a.c_stride;
   } else {
-    if (!ragged_tile(a.offsets, a.experts, a.rows, BM, blockIdx.y, expert, first, m_here)) return;
+    if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here)) return;
     x += (size_t)first * a.x_stride;
     c += (size_t)first * a.c_stride;
     w += (size_t)expert * a.w_expert;
@@ -143,6 +146,16 @@ bool pieces_aligned(const ProductArgs &a) {
 
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
+  if constexpr (KIND == FORWARD) {
+    if (a.rows / a.experts <= 64) {
+      ThinArgs t = {};
+      t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
+      t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
+      t.c_stride = a.c_stride, t.c_aligned = a.c_aligned, t.offsets = a.offsets;
+      t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
+      return pieces_aligned<T, KIND>(a) ? launch_thin<T, T, true>(t, stream) : launch_thin<T, T, false>(t, stream);
+    }
+  }
   if constexpr (sizeof(T) == 2) {
     if (pieces_aligned<T, KIND>(a)) {
       PipeArgs p = {};
@@ -157,10 +170,13 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
   constexpr int BM = 128, BN = 128;
   const size_t m_tiles =
       KIND == DWEIGHTS ? (size_t)a.experts * ((a.k + BM - 1) / BM) : ragged_tiles(a.experts, a.rows, BM);
-  const size_t n_tiles = ((size_t)a.n + BN - 1) / BN;
-  hipLaunchKernelGGL((product_kernel<T, KIND, BM, BN, 2, 2>), dim3((unsigned)n_tiles, (unsigned)m_tiles), dim3(256), 0,
-                     stream, a);
-  return launched();
+  ProductArgs p = a;
+  p.n_tiles = (a.n + BN - 1) / BN;
+  return in_launches(m_tiles * p.n_tiles, [&](unsigned first, unsigned blocks) {
+    p.first_block = first;
+    hipLaunchKernelGGL((product_kernel<T, KIND, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, p);
+    return launched();
+  });
 }
 
 // Strides of rows of `cols` elements, each row apart from the next.
@@ -192,7 +208,7 @@ KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t o
       !fits(rows, out, y_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_rows, d_weights, d_y, rows_stride, w_stride, expert_stride, y_stride, 0, d_offsets, experts, (int)rows,
-                   (int)out, (int)cols, 0};
+                   (int)out, (int)cols, 0, 0, 0};
   a.c_aligned = y_stride % 4 == 0 && aligned_to(d_y, 4 * type_size(dtype));
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, FORWARD>(a, static_cast<hipStream_t>(stream));
@@ -208,7 +224,7 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
       !fits(rows, cols, drows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_weights, d_drows, dy_stride, w_stride, expert_stride, drows_stride, 0, d_offsets, experts,
-                   (int)rows, (int)cols, (int)out, 0};
+                   (int)rows, (int)cols, (int)out, 0, 0, 0};
   a.c_aligned = drows_stride % 4 == 0 && aligned_to(d_drows, 4 * type_size(dtype));
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DROWS>(a, static_cast<hipStream_t>(stream));
@@ -222,7 +238,7 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
   if (!d_dweights || (rows && (!d_dy || !d_rows)) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
-                   (int)cols, (int)out, 0};
+                   (int)cols, (int)out, 0, 0, 0};
   a.c_aligned = cols % 4 == 0 && aligned_to(d_dweights, 4 * type_size(dtype));
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DWEIGHTS>(a, static_cast<hipStream_t>(stream));
