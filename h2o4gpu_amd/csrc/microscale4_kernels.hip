@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *x, size_t x_stri
 template <typename T>
 __global__ __launch_bounds__(256) void dequantize_kernel(const unsigned *codes, const unsigned char *scales, unsigned cols,
                                                          size_t words, unsigned row_words, unsigned scales_row, T *out,
-                                                         size_t out_stride, int aligned) {
+                                                         size_t out_stride) {
   const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= words) return;
   const size_t row = at / row_words;
@@ -113,8 +113,14 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const unsigned *codes, 
   for (int i = 0; i < 8; ++i) v[i] = element(code >> (4 * i)) * power;
   T *o = out + row * out_stride + word * 8;
   const int left = (int)cols - (int)word * 8;
-  store_four(o, f32x4{v[0], v[1], v[2], v[3]}, left, aligned);
-  store_four(o + 4, f32x4{v[4], v[5], v[6], v[7]}, left - 4, aligned);
+  if (left >= 8) {
+    typedef Beside<T, 8> eight;
+    reinterpret_cast<eight *>(o)->v =
+        typename eight::vector{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
+  } else {
+    store_four(o, f32x4{v[0], v[1], v[2], v[3]}, left);
+    store_four(o + 4, f32x4{v[4], v[5], v[6], v[7]}, left - 4);
+  }
 }
 
 // Codes and scales that come in plain rows, into the layout above.
@@ -150,7 +156,7 @@ struct FourArgs {
   size_t y_stride;
   const int *order, *offsets;  // with experts only; order: x's row of y's row p is order[p] / top_k (none: p)
   int top_k, experts;          // experts 0: one matrix
-  int rows, out, cols, y_aligned;
+  int rows, out, cols;
   unsigned first_block;
   int n_tiles;
 };
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
-      store_four(y + (size_t)m * a.y_stride + n, acc[i][j], n_here - n, a.y_aligned);
+      store_four(y + (size_t)m * a.y_stride + n, acc[i][j], n_here - n);
     }
   }
 }
@@ -274,7 +280,7 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);
-    t.c_stride = a.y_stride, t.c_aligned = a.y_aligned, t.order = a.order, t.offsets = a.offsets, t.top_k = a.top_k;
+    t.c_stride = a.y_stride, t.order = a.order, t.offsets = a.offsets, t.top_k = a.top_k;
     t.experts = a.experts, t.rows = a.rows, t.n = a.out, t.k = (int)((a.cols + 127) / 128 * 32);
     return launch_thin<Four, T, true>(t, stream);
   }
@@ -283,7 +289,7 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
     PipeArgs p = {};
     p.x = (const char *)a.x, p.w = (const char *)a.w, p.x_scales = a.x_scales, p.w_scales = a.w_scales, p.c = a.y;
     p.x_stride = p.w_stride = pitch, p.w_expert = pitch * a.out, p.scales_stride = scales_pitch(a.cols);
-    p.c_stride = a.y_stride, p.c_aligned = a.y_stride % (16 / sizeof(T)) == 0 && aligned_to(a.y, 16), p.x_bytes = x_rows * pitch;
+    p.c_stride = a.y_stride, p.x_bytes = x_rows * pitch;
     p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
     p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
     return a.order ? launch_pipe<Four, T, FORWARD, true, 256, 256, 2, 4>(p, stream)
@@ -343,11 +349,10 @@ KM_API int h2o4gpu_microscale4_dequantize(int dtype, size_t rows, size_t cols, c
     typedef typename decltype(tag)::type T;
     const unsigned row_words = (unsigned)((cols + 7) / 8);
     const size_t words = rows * row_words;
-    const int aligned = out_stride % 4 == 0 && aligned_to(d_out, 4 * sizeof(T));
     hipLaunchKernelGGL((dequantize_kernel<T>), dim3((unsigned)((words + 255) / 256)), dim3(256), 0,
                        static_cast<hipStream_t>(stream), static_cast<const unsigned *>(d_codes),
                        static_cast<const unsigned char *>(d_scales), (unsigned)cols, words, row_words,
-                       (unsigned)scales_pitch(cols), static_cast<T *>(d_out), out_stride, aligned);
+                       (unsigned)scales_pitch(cols), static_cast<T *>(d_out), out_stride);
     return launched();
   });
 }
@@ -378,7 +383,6 @@ int four_product(int dtype, FourArgs a, size_t x_rows, size_t rows, size_t out, 
   for (const void *p : {a.x, a.x_scales, a.w, a.w_scales})
     if (!aligned_to(p, 16)) return H2O4GPU_KMEANS_EARG;
   a.rows = (int)rows, a.out = (int)out, a.cols = (int)cols;
-  a.y_aligned = a.y_stride % 4 == 0 && aligned_to(a.y, 4 * type_size(dtype));
   return with_type(dtype, [&](auto tag) {
     return launch_four<typename decltype(tag)::type>(a, x_rows, static_cast<hipStream_t>(stream));
   });

@@ -24,10 +24,11 @@ struct PipeArgs {
   size_t c_stride, c_expert;                           // elements
   size_t x_bytes;              // GATHER: all of x, below 2^32
   const int *order, *offsets;  // order: x's row of C's row p is order[p] / top_k (none: p)
+  int part;                    // DWEIGHTS: rows of a part of an expert's (PartOfRows)
+  float *sums;
   int top_k, experts;          // experts 0: one matrix and `rows` rows
   int rows, n, k;              // k in elements (Four: in groups of four columns); DWEIGHTS: k is C's m
   int m_tiles, n_tiles, band;
-  int c_aligned;               // C's rows begin at multiples of 16 bytes
 };
 
 template <typename T>
@@ -214,7 +215,7 @@ __device__ __forceinline__ void listed_tile(const int *table, const int *offsets
 // the second at (q0; b q1). (Stored as they are, eight bytes a lane, 8192^3 took 100 us longer.)
 template <typename OUT, int FM, int FN>
 __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN], OUT *c, size_t stride, int m0, int n0,
-                                           int m_here, int n_here, bool aligned) {
+                                           int m_here, int n_here) {
   constexpr int EPP = 16 / (int)sizeof(OUT);
   const int i = lane & 15, q = lane >> 4;
 #pragma unroll
@@ -224,7 +225,7 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
     if constexpr (sizeof(OUT) == 4) {
       if (m < m_here) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) store_four(row + n0 + j * 16 + 4 * q, acc[b][j], n_here - (n0 + j * 16 + 4 * q), aligned);
+        for (int j = 0; j < FN; ++j) store_four(row + n0 + j * 16 + 4 * q, acc[b][j], n_here - (n0 + j * 16 + 4 * q));
       }
     } else {
 #pragma unroll
@@ -244,8 +245,8 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
         const u32x4 piece = {lo[0], lo[1], hi[0], hi[1]};
         const int n = n0 + j * 16 + 8 * q;
         if (m < m_here && n < n_here) {
-          if (aligned && n + EPP <= n_here) {
-            *reinterpret_cast<u32x4 *>(row + n) = piece;
+          if (n + EPP <= n_here) {
+            reinterpret_cast<Beside<OUT, EPP> *>(row + n)->v = __builtin_bit_cast(typename Beside<OUT, EPP>::vector, piece);
           } else {
 #pragma unroll
             for (int e = 0; e < EPP; ++e)
@@ -281,7 +282,8 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   const unsigned base = lds_address(lds), to = base + wave * 1024;
   // Tiles of m are numbered without gaps: those of expert 0, of expert 1, ..., of the rows without an expert. A table in
   // LDS says where each expert's begin; beyond PIPE_TABLE experts the numbers have gaps (ragged_tile).
-  const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = a.experts > 0 && a.experts < PIPE_TABLE;
+  const bool in_parts = KIND == DWEIGHTS && a.part < a.rows;
+  const bool ragged = KIND != DWEIGHTS && a.experts > 0, listed = a.experts > 0 && a.experts < PIPE_TABLE && !in_parts;
   auto stages_of = [](int k) { return k <= KS ? 2 : (k + KS - 1) / KS; };
   unsigned m_tiles = (unsigned)a.m_tiles;
   // Workgroups go round the eight chiplets; each of these takes a stretch of the tiles, and its workgroups neighbours
@@ -312,10 +314,11 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
 
   struct Tile {
     int n0, n_here, m_here, first, expert, k_end;  // m_here 0: there is none
+    int begin, sum;                                // DWEIGHTS: the part's first row, and its place among the sums
   };
   // the next tile of this workgroup
   auto locate = [&]() {
-    Tile r = {0, 0, 0, 0, 0, 0};
+    Tile r = {0, 0, 0, 0, 0, 0, 0, -1};
     for (; tile < tiles_end && r.m_here <= 0; tile += gridDim.x >> 3) {
       const unsigned band = (unsigned)a.band * a.n_tiles, m0 = tile / band * a.band;
       const unsigned high = m_tiles - m0 < (unsigned)a.band ? m_tiles - m0 : a.band;
@@ -325,9 +328,17 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       r.k_end = a.k;
       if constexpr (KIND == DWEIGHTS) {
         const int tiles = (a.k + BM - 1) / BM;
-        r.expert = number / tiles, r.first = number % tiles * BM;
+        r.first = number % tiles * BM;
+        PartOfRows part;
+        if (in_parts) {
+          if (!part_of_rows(a.offsets, a.experts, a.rows, a.part, number / tiles, part)) continue;
+        } else {
+          const int begin = a.offsets[number / tiles];
+          part = {number / tiles, begin, a.offsets[number / tiles + 1] - begin, -1};
+        }
+        r.expert = __builtin_amdgcn_readfirstlane(part.expert), r.k_end = part.rows;
+        r.begin = __builtin_amdgcn_readfirstlane(part.first), r.sum = __builtin_amdgcn_readfirstlane(part.sum);
         r.m_here = a.k - r.first < BM ? a.k - r.first : BM;
-        r.k_end = a.offsets[r.expert + 1] - a.offsets[r.expert];
       } else if (ragged) {
         if (listed)
           listed_tile<BM>(table, a.offsets, a.experts, a.rows, number, r.expert, r.first, r.m_here);
@@ -377,9 +388,8 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     in = r;
     in_x = a.x, in_w = a.w;
     if constexpr (KIND == DWEIGHTS) {
-      const int begin = a.offsets[r.expert];
-      in_x += (size_t)begin * a.x_stride + (size_t)r.first * SIZE;
-      in_w += (size_t)begin * a.w_stride + (size_t)r.n0 * SIZE;
+      in_x += (size_t)r.begin * a.x_stride + (size_t)r.first * SIZE;
+      in_w += (size_t)r.begin * a.w_stride + (size_t)r.n0 * SIZE;
     } else {
       if (!GATHER) in_x += (size_t)r.first * a.x_stride;
       in_w += (size_t)r.expert * a.w_expert + (WC ? (size_t)r.n0 * SIZE : (size_t)r.n0 * a.w_stride);
@@ -575,9 +585,14 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       const int slot = order_of(ahead);
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));  // (what follows from it is not kept over the stages)
+      if (KIND == DWEIGHTS && now.sum >= 0)
+        store_tile<float, FM, FN>(tid & 63, acc, a.sums + (size_t)now.sum * a.c_expert + (size_t)now.first * a.c_stride + now.n0,
+                                  a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here);
+      else {
       OUT *c = static_cast<OUT *>(a.c) + (KIND == DWEIGHTS ? (size_t)now.expert * a.c_expert : 0) +
                (size_t)now.first * a.c_stride + now.n0;
-      store_tile<OUT, FM, FN>(tid & 63, acc, c, a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here, a.c_aligned);
+      store_tile<OUT, FM, FN>(tid & 63, acc, c, a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here);
+      }
       put_order(slot);
       now = next;
       if (now.m_here == 0) break;
@@ -594,7 +609,8 @@ constexpr size_t BUFFER_BYTES = (size_t)1 << 32;  // what a buffer's offsets rea
 
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 int launch_pipe(PipeArgs &a, hipStream_t stream) {
-  const size_t m_tiles = KIND == DWEIGHTS ? (size_t)a.experts * ((a.k + BM - 1) / BM)
+  const size_t m_tiles = KIND == DWEIGHTS ? (a.part < a.rows ? ragged_tiles(a.experts, a.rows, a.part) : (size_t)a.experts) *
+                                                ((a.k + BM - 1) / BM)
                          : a.experts      ? ragged_tiles(a.experts, a.rows, BM)
                                           : ((size_t)a.rows + BM - 1) / BM;
   a.m_tiles = (int)m_tiles, a.n_tiles = (a.n + BN - 1) / BN;

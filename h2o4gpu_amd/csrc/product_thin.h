@@ -16,7 +16,7 @@ struct ThinArgs {
   const int *order, *offsets;                          // as in PipeArgs
   int top_k, experts, rows, n, k;                      // k in elements (Four: in groups of four columns)
   unsigned first_block;
-  int n_tiles, c_aligned;                              // c_aligned: four elements of C may be stored at once
+  int n_tiles;
 };
 
 // ALIGNED: every piece lies at a multiple of 16 bytes, and k is whole pieces.
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
     for (int v = 1; v < WAVES; ++v) s += sums[v][b][lane];
     const int m = b / NB * 16 + i, n = b % NB * 16 + 4 * g;
     if (m < m_here)
-      store_four(static_cast<OUT *>(a.c) + (size_t)(first + m) * a.c_stride + n0 + n, s, n_here - n, a.c_aligned);
+      store_four(static_cast<OUT *>(a.c) + (size_t)(first + m) * a.c_stride + n0 + n, s, n_here - n);
   }
 }
 

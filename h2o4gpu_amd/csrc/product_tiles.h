@@ -142,11 +142,38 @@ __device__ __forceinline__ bool ragged_tile(const int *offsets, int count, int r
   lo = __builtin_amdgcn_readfirstlane(lo);
   const int begin = offsets[lo], end = lo == count ? rows : offsets[lo + 1];
   stretch = lo;
-  first = begin + (number - (begin / tile + lo)) * tile;
+  const long long behind = (long long)(number - (begin / tile + lo)) * tile;  // of the stretch's first row
+  if (behind >= end - begin) {
+    first = end, rows_here = 0;
+    return false;
+  }
+  first = begin + (int)behind;
   rows_here = end - first < tile ? end - first : tile;
-  return rows_here > 0;
+  return true;
 }
 inline size_t ragged_tiles(int count, int rows, int tile) { return (size_t)(rows / tile) + count + 1; }
+
+// A product over the rows of each expert may take them in parts of `part` rows, and experts that have more than that as
+// sums of their parts' products, which lie in `sums` until they are added up. Parts are numbered as ragged tiles are;
+// an expert without rows has one (of none). In any `part` rows, at most one part that is not its expert's first begins
+// and at most one that is the first of several: where a part's sum lies follows from where it begins.
+struct PartOfRows {
+  int expert, first, rows;
+  int sum;  // which of `sums`, or -1: the expert's only part
+};
+__device__ __forceinline__ bool part_of_rows(const int *offsets, int experts, int rows, int part, int number,
+                                             PartOfRows &p) {
+  const bool any = ragged_tile(offsets, experts, rows, part, number, p.expert, p.first, p.rows);
+  if (p.expert == experts) return false;
+  const int begin = offsets[p.expert], end = offsets[p.expert + 1];
+  if (!any) {
+    p.rows = 0, p.sum = -1;
+    return begin == end && number == begin / part + p.expert;
+  }
+  p.sum = end - begin > part ? 2 * (p.first / part) + (p.first == begin) : -1;
+  return true;
+}
+inline size_t part_sums(int rows, int part) { return 2 * ((size_t)rows / part + 1); }
 
 // launch(first block, blocks) until all of them are; a launch has at most 2^32 threads.
 template <typename F>
@@ -157,19 +184,19 @@ inline int in_launches(size_t blocks, F launch) {
   return H2O4GPU_KMEANS_OK;
 }
 
-// f's four values of consecutive n to row m of C; `full`: all four exist and the address is aligned to four.
+// N values side by side, at any address that a T may have; the first `valid` of them.
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Beside {
+  typedef T vector __attribute__((ext_vector_type(N)));
+  vector v;
+};
 template <typename T>
-__device__ __forceinline__ void store_four(T *c, f32x4 v, int valid, bool aligned) {
-  if (aligned && valid >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<f32x4 *>(c) = v;
-    } else {
-      typedef T four __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<four *>(c) = four{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    }
+__device__ __forceinline__ void store_four(T *c, f32x4 v, int valid) {
+  if (valid >= 4) {
+    reinterpret_cast<Beside<T, 4> *>(c)->v = typename Beside<T, 4>::vector{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 3; ++j)
       if (j < valid) c[j] = (T)v[j];
   }
 }

@@ -17,7 +17,8 @@ struct ProductArgs {
   size_t x_stride, w_stride, w_expert, c_stride, c_expert;
   const int *offsets;
   int experts, rows, n, k;  // DWEIGHTS: n = cols, k = out, which is C's m
-  int c_aligned;            // four elements of C may be stored at once
+  int part;                 // DWEIGHTS: rows of a part
+  float *sums;              // of experts with several: matrices like C's, float
   unsigned first_block;
   int n_tiles;
 };
@@ -41,16 +42,18 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
   T *c = static_cast<T *>(a.c);
   int k_end = a.k;
+  float *sum = nullptr;  // C is a part's sum
   if (KIND == DWEIGHTS) {
     const int tiles = (a.k + BM - 1) / BM;
-    expert = number / tiles;
+    PartOfRows part;
+    if (!part_of_rows(a.offsets, a.experts, a.rows, a.part, number / tiles, part)) return;
+    expert = part.expert, k_end = part.rows;
     first = (number % tiles) * BM;
     m_here = a.k - first < BM ? a.k - first : BM;
-    const int begin = a.offsets[expert];
-    k_end = a.offsets[expert + 1] - begin;
-    x += (size_t)begin * a.x_stride + first;
-    w += (size_t)begin * a.w_stride;
+    x += (size_t)part.first * a.x_stride + first;
+    w += (size_t)part.first * a.w_stride;
     c += (size_t)expert * a.c_expert + (size_t)first * a.c_stride;
+    if (part.sum >= 0) sum = a.sums + (size_t)part.sum * a.c_expert + (size_t)first * a.c_stride;
   } else {
     if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here)) return;
     x += (size_t)first * a.x_stride;
@@ -96,7 +99,9 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // blocks of 16 go round the wavefronts, so that they have as many each where a tile is not full
   const int wm = wave / WN, wn = wave % WN;
+  const int m_blocks = ((m_here + 15) / 16 - wm + WM - 1) / WM, n_blocks = ((n_here + 15) / 16 - wn + WN - 1) / WN;
   const int stages = (k_end + KS - 1) / KS;
   if (stages > 0) {
     load(0);
@@ -110,13 +115,16 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
     for (int step = 0; step < 2; ++step) {
       u32x4 fx[FM], fw[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, wm * FM + i, step);
+      for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, i * WM + wm, step);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = TW::fragment(at + BM * 128, lane, wn * FN + j, step);
+      for (int j = 0; j < FN; ++j) fw[j] = TW::fragment(at + BM * 128, lane, j * WN + wn, step);
 #pragma unroll
       for (int i = 0; i < FM; ++i)
+        if (i < m_blocks) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) mfma_piece(acc[i][j], fw[j], fx[i], Tag<T>());
+          for (int j = 0; j < FN; ++j)
+            if (j < n_blocks) mfma_piece(acc[i][j], fw[j], fx[i], Tag<T>());
+        }
     }
     if (t + 1 < stages) put(lds + ((t + 1) & 1) * STAGE);
     __syncthreads();
@@ -124,14 +132,46 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
 
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = (wm * FM + i) * 16 + (lane & 15);
+    const int m = (i * WM + wm) * 16 + (lane & 15);
     if (m >= m_here) continue;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
-      store_four(c + (size_t)m * a.c_stride + n0 + n, acc[i][j], n_here - n, a.c_aligned);
+      const int n = (j * WN + wn) * 16 + 4 * (lane >> 4);
+      if (KIND == DWEIGHTS && sum)
+        store_four(sum + (size_t)m * a.c_stride + n0 + n, acc[i][j], n_here - n);
+      else
+        store_four(c + (size_t)m * a.c_stride + n0 + n, acc[i][j], n_here - n);
     }
   }
+}
+
+// The parts' sums of the experts that have several, added up in order: a workgroup has a stretch of the matrix of the
+// expert whose first part begins in its `part` rows.
+template <typename T>
+__global__ __launch_bounds__(256) void join_parts_kernel(const float *sums, const int *offsets, int experts, int part,
+                                                         size_t size, T *c) {
+  const int window = blockIdx.y;
+  int lo = 0, n = experts;  // the last expert that begins within or before these rows
+  while (n > 1) {
+    const int half = n / 2;
+    if ((long long)offsets[lo + half] < (long long)(window + 1) * part)
+      lo += half, n -= half;
+    else
+      n = half;
+  }
+  const int begin = offsets[lo], rows = offsets[lo + 1] - begin;
+  if (begin / part != window || rows <= part) return;
+  const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= size) return;
+  const int valid = size - at < 4 ? (int)(size - at) : 4;
+  f32x4 total = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; (long long)j * part < rows; ++j) {
+    const float *from = sums + (size_t)(2 * (window + j) + (j == 0)) * size + at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < valid) total[i] += from[i];
+  }
+  store_four(c + (size_t)lo * size + at, total, valid);
 }
 
 // Whether every piece of 16 bytes of both operands lies at a multiple of 16 and within the reach of a buffer.
@@ -144,6 +184,28 @@ bool pieces_aligned(const ProductArgs &a) {
          a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
 }
 
+// Rows of a part of a matrix's gradient: so many that all parts together are some four for each CU, and no fewer than
+// 1024, beside which writing and reading a sum is little. An expert's matrix of many tiles needs no parts.
+int rows_of_part(size_t rows, size_t out, size_t cols) {
+  const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
+  if (tiles >= 128) return INT_MAX;
+  const size_t part = rows * tiles / 1024;
+  return (int)((part > 1024 ? part : 1024) + 63) / 64 * 64;
+}
+size_t sums_bytes(size_t rows, size_t out, size_t cols) {
+  const int part = rows_of_part(rows, out, cols);
+  return rows <= (size_t)part ? 0 : part_sums((int)rows, part) * out * cols * sizeof(float);
+}
+
+template <typename T>
+int join_parts(const ProductArgs &a, hipStream_t stream) {
+  if (a.rows <= a.part) return H2O4GPU_KMEANS_OK;
+  const size_t blocks = (a.c_expert + 1023) / 1024;
+  hipLaunchKernelGGL((join_parts_kernel<T>), dim3((unsigned)blocks, (unsigned)(a.rows / a.part + 1)), dim3(256), 0, stream,
+                     a.sums, a.offsets, a.experts, a.part, a.c_expert, static_cast<T *>(a.c));
+  return launched();
+}
+
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
   if constexpr (KIND == FORWARD) {
@@ -151,7 +213,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
       ThinArgs t = {};
       t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
       t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
-      t.c_stride = a.c_stride, t.c_aligned = a.c_aligned, t.offsets = a.offsets;
+      t.c_stride = a.c_stride, t.offsets = a.offsets;
       t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
       return pieces_aligned<T, KIND>(a) ? launch_thin<T, T, true>(t, stream) : launch_thin<T, T, false>(t, stream);
     }
@@ -161,28 +223,33 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
       PipeArgs p = {};
       p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
       p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
-      p.c_stride = a.c_stride, p.c_expert = a.c_expert, p.c_aligned = a.c_stride % (16 / sizeof(T)) == 0 && a.c_expert % (16 / sizeof(T)) == 0 && aligned_to(a.c, 16);
+      p.c_stride = a.c_stride, p.c_expert = a.c_expert;
       p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
       const size_t rows = KIND == DWEIGHTS ? (size_t)a.k : a.rows / a.experts;
-      if (rows >= 128 && a.n >= 128) return launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream);
+      p.part = a.part, p.sums = a.sums;
+      if (rows >= 128 && a.n >= 128) {
+        KM_TRY((launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream)));
+        return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
+      }
     }
   }
   constexpr int BM = 128, BN = 128;
-  const size_t m_tiles =
-      KIND == DWEIGHTS ? (size_t)a.experts * ((a.k + BM - 1) / BM) : ragged_tiles(a.experts, a.rows, BM);
+  const size_t m_tiles = KIND == DWEIGHTS ? ragged_tiles(a.experts, a.rows, a.part) * ((a.k + BM - 1) / BM)
+                                          : ragged_tiles(a.experts, a.rows, BM);
   ProductArgs p = a;
   p.n_tiles = (a.n + BN - 1) / BN;
-  return in_launches(m_tiles * p.n_tiles, [&](unsigned first, unsigned blocks) {
+  KM_TRY(in_launches(m_tiles * p.n_tiles, [&](unsigned first, unsigned blocks) {
     p.first_block = first;
     hipLaunchKernelGGL((product_kernel<T, KIND, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, p);
     return launched();
-  });
+  }));
+  return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
 }
 
 // Strides of rows of `cols` elements, each row apart from the next.
 bool fits(size_t rows, size_t cols, size_t stride) { return rows < 2 || stride >= cols; }
 
-constexpr size_t MAX_SIDE = (size_t)1 << 30;
+constexpr size_t MAX_SIDE = (size_t)1 << 30, MAX_MATRIX = (size_t)1 << 38;
 
 // What all three have in common. > 0: go on, else the status to return.
 int check(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *offsets) {
@@ -208,8 +275,7 @@ KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t o
       !fits(rows, out, y_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_rows, d_weights, d_y, rows_stride, w_stride, expert_stride, y_stride, 0, d_offsets, experts, (int)rows,
-                   (int)out, (int)cols, 0, 0, 0};
-  a.c_aligned = y_stride % 4 == 0 && aligned_to(d_y, 4 * type_size(dtype));
+                   (int)out, (int)cols, 0, nullptr, 0, 0};
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, FORWARD>(a, static_cast<hipStream_t>(stream));
   });
@@ -224,22 +290,29 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
       !fits(rows, cols, drows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_weights, d_drows, dy_stride, w_stride, expert_stride, drows_stride, 0, d_offsets, experts,
-                   (int)rows, (int)cols, (int)out, 0, 0, 0};
-  a.c_aligned = drows_stride % 4 == 0 && aligned_to(d_drows, 4 * type_size(dtype));
+                   (int)rows, (int)cols, (int)out, 0, nullptr, 0, 0};
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DROWS>(a, static_cast<hipStream_t>(stream));
   });
 }
 
+KM_API size_t h2o4gpu_experts_product_dweights_workspace(size_t rows, int experts, size_t out, size_t cols) {
+  return check(0, rows, experts, out, cols, "") <= 0 || out * cols > MAX_MATRIX ? 0 : sums_bytes(rows, out, cols);
+}
+
 KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols,
                                             const void *d_dy, size_t dy_stride, const void *d_rows, size_t rows_stride,
-                                            const int *d_offsets, void *d_dweights, void *stream) {
+                                            const int *d_offsets, void *d_dweights, void *d_workspace,
+                                            size_t workspace_bytes, void *stream) {
   if (int rc = check(dtype, rows, experts, out, cols, d_offsets); rc <= 0) return rc;
+  if (out * cols > MAX_MATRIX) return H2O4GPU_KMEANS_EARG;
+  const size_t need = sums_bytes(rows, out, cols);
+  if (need > workspace_bytes || (need && (!d_workspace || !aligned_to(d_workspace, 16)))) return H2O4GPU_KMEANS_EARG;
   if (!d_dweights || (rows && (!d_dy || !d_rows)) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
-                   (int)cols, (int)out, 0, 0, 0};
-  a.c_aligned = cols % 4 == 0 && aligned_to(d_dweights, 4 * type_size(dtype));
+                   (int)cols, (int)out, 0, nullptr, 0, 0};
+  a.part = rows_of_part(rows, out, cols), a.sums = static_cast<float *>(d_workspace);
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DWEIGHTS>(a, static_cast<hipStream_t>(stream));
   });

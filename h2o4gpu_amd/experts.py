@@ -359,6 +359,11 @@ def _matrices(weights):
     return weights.data_ptr(), expert_stride, stride
 
 
+@functools.lru_cache(maxsize=256)
+def _sums(rows, n_experts, out, cols):
+    return experts_hip.lib().h2o4gpu_experts_product_dweights_workspace(rows, n_experts, out, cols)
+
+
 def _product(rows, weights, order):
     ptr, stride = _rows("rows", rows)
     n_experts, out, cols = weights.shape
@@ -391,8 +396,10 @@ class _Product(torch.autograd.Function):
             drows = _once(drows, weights, dy)
         if ctx.needs_input_grad[1]:
             dweights = weights.new_empty(weights.shape)
+            need = _sums(count, n_experts, out, cols)
+            work = dy.new_empty(need // 4, dtype=torch.float32) if need else None
             _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols, ptr, stride,
-                  *_rows("rows", rows), order._offsets_ptr, dweights.data_ptr())
+                  *_rows("rows", rows), order._offsets_ptr, dweights.data_ptr(), work.data_ptr() if need else None, need)
             dweights = _once(dweights, rows, dy)
         return drows, dweights, None
 

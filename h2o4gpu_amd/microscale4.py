@@ -15,12 +15,24 @@ gives each expert:
 Nothing here has a gradient: train with experts.product, then quantize. Streams and graphs as in
 h2o4gpu_amd.experts. (h2o4gpu_amd.codebook4 keeps the tokens in 16 or 32 bits and takes any 16 values.)
 """
+import functools
+
 import torch
 
 from .experts import _TYPES, _call, _no_tangents, _order_of, _rows, _tensor, _type_of
 from .libs import experts_hip
 
 BLOCK = 32
+
+
+@functools.lru_cache(maxsize=256)
+def _pitches(cols):
+    """Bytes of a row of codes and of a row of scales."""
+    lib = experts_hip.lib()
+    pitch = lib.h2o4gpu_microscale4_codes_pitch(max(0, cols))
+    if pitch == 0:
+        raise ValueError("a matrix must have 1 to 2^30 columns, got %d" % cols)
+    return pitch, lib.h2o4gpu_microscale4_scales_pitch(cols)
 
 
 class Microscale4:
@@ -34,7 +46,7 @@ class Microscale4:
     afterwards. `dtype` is the type of a product whose tokens this matrix is.
     """
 
-    __slots__ = ("laid_codes", "laid_scales", "rows", "cols", "n_experts", "dtype", "device")
+    __slots__ = ("rows", "cols", "n_experts", "dtype", "device", "_buffer", "_codes_ptr", "_scales_ptr")
 
     def __init__(self, codes, scales, cols, dtype=torch.bfloat16):
         lead = codes.dim() - 2 if isinstance(codes, torch.Tensor) else 0
@@ -48,27 +60,42 @@ class Microscale4:
         if tuple(scales.shape) != tuple(codes.shape[:-1]) + (-(-cols // BLOCK),):
             raise ValueError("scales must be %s, got %s" % (tuple(codes.shape[:-1]) + (-(-cols // BLOCK),),
                                                             tuple(scales.shape)))
-        self._allocate(codes.shape[:-1], cols, dtype, codes.device)
-        codes, scales = codes.contiguous(), scales.contiguous()
-        _call(codes.device.index, "h2o4gpu_microscale4_layout", self.rows * max(1, self.n_experts), cols,
-              codes.data_ptr(), codes.shape[-1], scales.data_ptr(), self.laid_codes.data_ptr(),
-              self.laid_scales.data_ptr())
-
-    def _allocate(self, lead, cols, dtype, device):
         if dtype not in _TYPES:
             raise TypeError("dtype must be float32, bfloat16 or float16, got %s" % (dtype,))
-        if len(lead) == 2 and not 1 <= lead[0] <= experts_hip.MAX_EXPERTS:
-            raise ValueError("a matrix for each of 1 to %d experts is wanted, got %s" % (experts_hip.MAX_EXPERTS,
-                                                                                        tuple(lead) + (cols,)))
-        lib = experts_hip.lib()
-        pitch = lib.h2o4gpu_microscale4_codes_pitch(cols)
-        if pitch == 0:
-            raise ValueError("a matrix must have 1 to 2^30 columns, got %d" % cols)
-        self.rows, self.cols, self.n_experts, self.dtype, self.device = (
-            lead[-1], cols, lead[0] if len(lead) == 2 else 0, dtype, device)
-        self.laid_codes = torch.empty(tuple(lead) + (pitch,), dtype=torch.uint8, device=device)
-        self.laid_scales = torch.empty(tuple(lead) + (lib.h2o4gpu_microscale4_scales_pitch(cols),),
-                                       dtype=torch.uint8, device=device)
+        self._allocate(codes, codes.shape[:-1], cols, dtype)
+        codes, scales = codes.contiguous(), scales.contiguous()
+        _call(codes.device.index, "h2o4gpu_microscale4_layout", self.rows * max(1, self.n_experts), cols,
+              codes.data_ptr(), codes.shape[-1], scales.data_ptr(), self._codes_ptr, self._scales_ptr)
+
+    def _allocate(self, like, lead, cols, dtype):
+        self.rows, self.cols, self.dtype, self.device = lead[-1], cols, dtype, like.device
+        rows = self.rows
+        if len(lead) == 2:
+            if not 1 <= lead[0] <= experts_hip.MAX_EXPERTS:
+                raise ValueError("a matrix for each of 1 to %d experts is wanted, got %s" % (
+                    experts_hip.MAX_EXPERTS, tuple(lead) + (cols,)))
+            rows *= lead[0]
+        self.n_experts = lead[0] if len(lead) == 2 else 0
+        pitch, scales_pitch = _pitches(cols)
+        self._buffer = like.new_empty(rows * (pitch + scales_pitch), dtype=torch.uint8)
+        self._codes_ptr = self._buffer.data_ptr()
+        self._scales_ptr = self._codes_ptr + rows * pitch
+
+    def _laid(self, which):
+        pitch = _pitches(self.cols)[which]
+        begin = which * self.rows * max(1, self.n_experts) * _pitches(self.cols)[0]
+        shape = ((self.n_experts,) if self.n_experts else ()) + (self.rows, pitch)
+        return self._buffer[begin:begin + self.rows * max(1, self.n_experts) * pitch].view(shape)
+
+    @property
+    def laid_codes(self):
+        """The codes as the products read them: uint8 (..., rows, a multiple of 128 bytes), zeros behind the last column."""
+        return self._laid(0)
+
+    @property
+    def laid_scales(self):
+        """The scales' bytes as the products read them, 16 for 512 columns."""
+        return self._laid(1)
 
     def codes(self):
         """The codes, one a byte: uint8 (..., rows, cols)."""
@@ -83,9 +110,10 @@ class Microscale4:
         """The numbers that the matrix stands for, (..., rows, cols), rounded to `dtype`."""
         if dtype not in _TYPES:
             raise TypeError("dtype must be float32, bfloat16 or float16, got %s" % (dtype,))
-        out = torch.empty(tuple(self.laid_codes.shape[:-1]) + (self.cols,), dtype=dtype, device=self.device)
+        lead = (self.n_experts,) if self.n_experts else ()
+        out = self._buffer.new_empty(lead + (self.rows, self.cols), dtype=dtype)
         _call(self.device.index, "h2o4gpu_microscale4_dequantize", _TYPES[dtype], self.rows * max(1, self.n_experts),
-              self.cols, self.laid_codes.data_ptr(), self.laid_scales.data_ptr(), out.data_ptr(), self.cols)
+              self.cols, self._codes_ptr, self._scales_ptr, out.data_ptr(), self.cols)
         return out
 
 
@@ -96,26 +124,29 @@ def quantize(values):
     are rounded to the nearest number, a tie to the one of even code, and what is then beyond 6 is 6
     (from 7 times the power on that is a step down by up to a quarter). A block that holds a NaN or an infinity is NaN.
     """
-    _tensor("values", values, values.dim() if isinstance(values, torch.Tensor) and values.dim() == 3 else 2)
-    code = _type_of("values", values)
+    if not (isinstance(values, torch.Tensor) and values.is_cuda and values.dim() in (2, 3) and values.dtype in _TYPES):
+        _tensor("values", values, values.dim() if isinstance(values, torch.Tensor) and values.dim() == 3 else 2)
+        _type_of("values", values)
     if values.requires_grad and torch.is_grad_enabled():
         raise ValueError("microscaled numbers have no gradient: detach values")
     _no_tangents(values)
+    shape = values.shape
     out = object.__new__(Microscale4)
-    out._allocate(values.shape[:-1], values.shape[-1], values.dtype, values.device)
-    flat = values if values.dim() == 2 else values.reshape(-1, values.shape[-1])
-    if values.dim() == 3 and flat.shape[0] > 1 and not (flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1]):
-        flat = flat.contiguous()
-    ptr, stride = _rows("values", flat)
-    _call(values.device.index, "h2o4gpu_microscale4_quantize", code, flat.shape[0], flat.shape[1], ptr, stride,
-          out.laid_codes.data_ptr(), out.laid_scales.data_ptr())
+    out._allocate(values, shape[:-1], shape[-1], values.dtype)
+    if len(shape) == 3:
+        values = values.reshape(-1, shape[-1])
+        if values.shape[0] > 1 and not (values.stride(1) == 1 and values.stride(0) >= shape[-1]):
+            values = values.contiguous()
+    ptr, stride = _rows("values", values)
+    _call(out.device.index, "h2o4gpu_microscale4_quantize", _TYPES[out.dtype], values.shape[0], out.cols, ptr, stride,
+          out._codes_ptr, out._scales_ptr)
     return out
 
 
 def _operands(x, weights, dtype):
-    for name, m in (("x", x), ("weights", weights)):
-        if not isinstance(m, Microscale4):
-            raise TypeError("%s must be a Microscale4 (quantize), got %s" % (name, type(m).__name__))
+    if type(x) is not Microscale4 or type(weights) is not Microscale4:
+        name, m = ("x", x) if type(x) is not Microscale4 else ("weights", weights)
+        raise TypeError("%s must be a Microscale4 (quantize), got %s" % (name, type(m).__name__))
     if x.n_experts:
         raise ValueError("x must be (tokens, cols), got a matrix per expert")
     if x.device != weights.device:
@@ -135,9 +166,9 @@ def product(x, weights, dtype=None):
     if weights.n_experts:
         raise ValueError("weights hold a matrix per expert: experts_product multiplies with those")
     out = weights.rows
-    y = torch.empty((x.rows, out), dtype=dtype, device=x.device)
-    _call(x.device.index, "h2o4gpu_microscale4_product", _TYPES[dtype], x.rows, out, x.cols, x.laid_codes.data_ptr(),
-          x.laid_scales.data_ptr(), weights.laid_codes.data_ptr(), weights.laid_scales.data_ptr(), y.data_ptr(), out)
+    y = x._buffer.new_empty((x.rows, out), dtype=dtype)
+    _call(x.device.index, "h2o4gpu_microscale4_product", _TYPES[dtype], x.rows, out, x.cols, x._codes_ptr, x._scales_ptr,
+          weights._codes_ptr, weights._scales_ptr, y.data_ptr(), out)
     return y
 
 
@@ -154,9 +185,8 @@ def experts_product(x, weights, order, in_order=False, dtype=None):
         raise ValueError("x must be (%d, %d), got (%d, %d)" % (slots if in_order else order.tokens, weights.cols,
                                                                x.rows, x.cols))
     out = weights.rows
-    y = torch.empty((slots, out), dtype=dtype, device=x.device)
+    y = x._buffer.new_empty((slots, out), dtype=dtype)
     _call(x.device.index, "h2o4gpu_microscale4_experts_product", _TYPES[dtype], order.tokens, order.top_k,
-          weights.n_experts, out, x.cols, x.laid_codes.data_ptr(), x.laid_scales.data_ptr(),
-          weights.laid_codes.data_ptr(), weights.laid_scales.data_ptr(), None if in_order else order._order_ptr,
-          order._offsets_ptr, y.data_ptr(), out)
+          weights.n_experts, out, x.cols, x._codes_ptr, x._scales_ptr, weights._codes_ptr, weights._scales_ptr,
+          None if in_order else order._order_ptr, order._offsets_ptr, y.data_ptr(), out)
     return y

@@ -137,16 +137,18 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
  * most rows. W_e: [out][cols], rows w_stride elements apart, at d_weights + e * expert_stride (0: one
  * matrix for all). Products and sums in float, one rounding at the end.
  * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
- * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none). */
+ * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none);
+ * d_workspace: product_dweights_workspace() bytes, 16-byte aligned (NULL where that is 0). */
 int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
                             size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                             const int *d_offsets, void *d_y, size_t y_stride, void *stream);
 int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
                                   size_t dy_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                                   const int *d_offsets, void *d_drows, size_t drows_stride, void *stream);
+size_t h2o4gpu_experts_product_dweights_workspace(size_t rows, int experts, size_t out, size_t cols);
 int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
                                      size_t dy_stride, const void *d_rows, size_t rows_stride, const int *d_offsets,
-                                     void *d_dweights, void *stream);
+                                     void *d_dweights, void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* Microscaled 4-bit matrices: every 32 columns of a row share a power of two, 2^(byte - 127), and an
  * element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 .. 7, the sign is 8) times it. A

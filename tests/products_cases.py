@@ -11,6 +11,9 @@ RAGGED = (
     (40, 3, 8, 64, 512), (3, 8, 300, 16, 64), (200, 2, 6, 48, 160), (33, 6, 64, 20, 2050), (300, 1, 2, 130, 129),
     (257, 2, 2, 255, 257), (500, 2, 7, 129, 65), (1000, 1, 3, 257, 200), (128, 1, 1, 128, 64), (2000, 1, 1, 300, 72),
     (900, 3, 4, 96, 384), (31, 2, 2, 520, 4104), (5000, 1, 5, 24, 40), (20, 1, 4100, 8, 33),
+    # more rows than a gradient's part, parts that end inside tiles, large tiles that end inside matrices and stages
+    (3001, 2, 3, 136, 264), (1500, 2, 2, 520, 1032), (700, 4, 5, 256, 512), (1100, 2, 7, 384, 136), (2500, 2, 1, 128, 128),
+    (9000, 1, 2300, 16, 24), (2600, 2, 4, 200, 128), (900, 1, 3, 1000, 72), (300, 1, 1, 264, 2056),
 )
 
 
@@ -22,7 +25,8 @@ def _products():
                             dropped=(0.0, 0.3)[i % 2], layout=LAYOUTS[(tokens + n) % 3], data="normal"))
     for data in ("nothing", "one_expert", "infinity", "nan_behind"):
         for dtype in TYPES:
-            for tokens, top_k, experts, n, cols in ((40, 2, 5, 24, 40), (300, 2, 4, 136, 200)):
+            for tokens, top_k, experts, n, cols in ((40, 2, 5, 24, 40), (300, 2, 4, 136, 200), (2100, 1, 3, 130, 40),
+                                                    (1300, 2, 3, 128, 192)):
                 out.append(dict(op="product", tokens=tokens, top_k=top_k, experts=experts, out=n, cols=cols, dtype=dtype,
                                 dropped=0.4 if data == "nan_behind" else 0.0, layout="plain", data=data))
     return out
@@ -38,7 +42,8 @@ def _fours():
     out = []
     for i, (rows, n, cols) in enumerate(((1, 1, 1), (1, 40, 33), (1, 300, 4096), (2, 17, 100), (5, 64, 256), (16, 128, 512), (17, 33, 513),
                                          (33, 200, 777), (64, 96, 1024), (65, 40, 2176), (130, 24, 520), (128, 128, 768),
-                                         (200, 130, 260), (300, 520, 96), (260, 257, 1300), (1, 8, 9000), (600, 700, 288))):
+                                         (200, 130, 260), (300, 520, 96), (260, 257, 1300), (1, 8, 9000), (600, 700, 288),
+                                         (513, 384, 1536), (1030, 129, 2560), (128, 4000, 128))):
         for dtype in TYPES:
             out.append(dict(op="four", rows=rows, out=n, cols=cols, dtype=dtype, made=("quantize", "codes")[i % 2]))
     return out
