@@ -369,15 +369,19 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   // Where a lane's pieces lie behind a stage's start. No piece is clamped: what lies behind the operand's last byte of
   // the stage is not read, and a piece of a row or column that does not exist is multiplied into what is not stored, or
   // masked. From one of a lane's pieces to its next, THREADS slots on, are so many rows or k, turned alike.
-  unsigned x_off, w_off;
+  // (float32 in columns: eight k on, every second is turned the other way.)
+  constexpr int ODD = SIZE == 4 ? 2 : 1;
+  unsigned x_off[ODD], w_off[ODD];
   const unsigned x_next = (unsigned)((XC ? THREADS / X::Tile::PER_K : THREADS / 8) * a.x_stride);
   const unsigned w_next = (unsigned)((WC ? THREADS / W::Tile::PER_K : THREADS / 8) * a.w_stride);
-  {
+#pragma unroll
+  for (int i = 0; i < ODD; ++i) {
     int r, k;
-    W::Tile::place(threadIdx.x, r, k);
-    w_off = WC ? (unsigned)(k * a.w_stride) + r * SIZE : (unsigned)(r * a.w_stride) + k * SIZE;
-    X::Tile::place(threadIdx.x, r, k);
-    x_off = GATHER ? k * SIZE : XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE;
+    W::Tile::place(i * THREADS + threadIdx.x, r, k);
+    w_off[i] = (WC ? (unsigned)(k * a.w_stride) + r * SIZE : (unsigned)(r * a.w_stride) + k * SIZE) - i * w_next;
+    X::Tile::place(i * THREADS + threadIdx.x, r, k);
+    x_off[i] = GATHER ? k * SIZE
+                      : (XC ? (unsigned)(k * a.x_stride) + r * SIZE : (unsigned)(r * a.x_stride) + k * SIZE) - i * x_next;
   }
   const size_t x_step = XC ? KS * a.x_stride : 128, w_step = WC ? KS * a.w_stride : 128;
   Tile in;  // the tile that is loaded
@@ -407,15 +411,16 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     }
   };
   unsigned x_size = 0, w_size = 0;
+  auto whole = [](int elements) { return (unsigned)(elements + EPP - 1) / EPP * 16; };  // bytes of their pieces
   auto size_up = [&]() {  // of the stage that is loaded now
     const int k_here = in_left < KS ? in_left : KS;
     x_size = k_here <= 0 ? 0
              : GATHER    ? (unsigned)(a.x_bytes - (size_t)in_stage * 128)
-             : XC        ? (unsigned)((k_here - 1) * a.x_stride) + in.m_here * SIZE
-                         : (unsigned)((in.m_here - 1) * a.x_stride) + k_here * SIZE;
+             : XC        ? (unsigned)((k_here - 1) * a.x_stride) + whole(in.m_here)
+                         : (unsigned)((in.m_here - 1) * a.x_stride) + whole(k_here);
     w_size = k_here <= 0 ? 0
-             : WC        ? (unsigned)((k_here - 1) * a.w_stride) + in.n_here * SIZE
-                         : (unsigned)((in.n_here - 1) * a.w_stride) + k_here * SIZE;
+             : WC        ? (unsigned)((k_here - 1) * a.w_stride) + whole(in.n_here)
+                         : (unsigned)((in.n_here - 1) * a.w_stride) + whole(k_here);
   };
   unsigned buffer = 0;  // of the stage that is loaded now: 0 or STAGE
   unsigned row_off[GATHER ? X::P : 1];
@@ -429,10 +434,10 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   };
   auto load_one = [&](int i) {
     if (i < X::P)
-      to_lds_16(buffer_of(in_x, x_size), x_off + (GATHER ? row_off[GATHER ? i : 0] : i * x_next),
+      to_lds_16(buffer_of(in_x, x_size), x_off[i % ODD] + (GATHER ? row_off[GATHER ? i : 0] : i * x_next),
                 to + buffer + i * THREADS * 16);
     else
-      to_lds_16(buffer_of(in_w, w_size), w_off + (i - X::P) * w_next, to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
+      to_lds_16(buffer_of(in_w, w_size), w_off[(i - X::P) % ODD] + (i - X::P) * w_next, to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
   };
   unsigned scales_in = 0;  // 0 or SCALES
   auto load_scales = [&]() {  // of this stage and the next, 512 columns, at every even stage of a tile

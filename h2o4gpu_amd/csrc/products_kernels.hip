@@ -174,14 +174,13 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const float *sums, cons
   store_four(c + (size_t)lo * size + at, total, valid);
 }
 
-// Whether every piece of 16 bytes of both operands lies at a multiple of 16 and within the reach of a buffer.
-template <typename T, Kind KIND>
-bool pieces_aligned(const ProductArgs &a) {
+// Whether every row of both operands begins at a multiple of 16 bytes, within the reach of a buffer. Then their pieces of
+// 16 bytes are read as they lie: what one holds behind a row's end is masked or not stored.
+template <typename T>
+bool rows_aligned(const ProductArgs &a) {
   constexpr size_t EPP = 16 / sizeof(T);
-  const size_t m = KIND == DWEIGHTS ? a.k : 0, k = KIND == DWEIGHTS ? 0 : a.k, n = KIND == FORWARD ? 0 : a.n;
   return aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % EPP == 0 && a.w_stride % EPP == 0 &&
-         a.w_expert % EPP == 0 && m % EPP == 0 && k % EPP == 0 && n % EPP == 0 &&
-         a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
+         a.w_expert % EPP == 0 && a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
 }
 
 // Rows of a part of a matrix's gradient: so many that all parts together are some four for each CU, and no fewer than
@@ -215,23 +214,19 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
       t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
       t.c_stride = a.c_stride, t.offsets = a.offsets;
       t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
-      return pieces_aligned<T, KIND>(a) ? launch_thin<T, T, true>(t, stream) : launch_thin<T, T, false>(t, stream);
+      return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
+                                                               : launch_thin<T, T, false>(t, stream);
     }
   }
-  if constexpr (sizeof(T) == 2) {
-    if (pieces_aligned<T, KIND>(a)) {
-      PipeArgs p = {};
-      p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
-      p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
-      p.c_stride = a.c_stride, p.c_expert = a.c_expert;
-      p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
-      const size_t rows = KIND == DWEIGHTS ? (size_t)a.k : a.rows / a.experts;
-      p.part = a.part, p.sums = a.sums;
-      if (rows >= 128 && a.n >= 128) {
-        KM_TRY((launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream)));
-        return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
-      }
-    }
+  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? a.k : a.rows / a.experts) >= 128 && a.n >= 128) {
+    PipeArgs p = {};
+    p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
+    p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
+    p.c_stride = a.c_stride, p.c_expert = a.c_expert;
+    p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
+    p.part = a.part, p.sums = a.sums;
+    KM_TRY((launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream)));
+    return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
   }
   constexpr int BM = 128, BN = 128;
   const size_t m_tiles = KIND == DWEIGHTS ? ragged_tiles(a.experts, a.rows, a.part) * ((a.k + BM - 1) / BM)
@@ -248,6 +243,17 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
 
 // Strides of rows of `cols` elements, each row apart from the next.
 bool fits(size_t rows, size_t cols, size_t stride) { return rows < 2 || stride >= cols; }
+
+// A thread a piece of 16 bytes: rows as they come, into rows that begin at multiples of 16 bytes, zeros behind their ends.
+template <typename T>
+__global__ __launch_bounds__(256) void align_kernel(const T *in, size_t stride, size_t matrix, size_t rows, size_t cols,
+                                                    size_t pieces, size_t total, u32x4 *out) {
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= total) return;
+  const size_t row = at / pieces, col = (at - row * pieces) * (16 / sizeof(T)), of = row / rows;
+  const size_t left = cols - col;
+  out[at] = load_piece(in + of * matrix + (row - of * rows) * stride + col, left < 16 ? (int)left : 16);
+}
 
 constexpr size_t MAX_SIDE = (size_t)1 << 30, MAX_MATRIX = (size_t)1 << 38;
 
@@ -315,5 +321,23 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
   a.part = rows_of_part(rows, out, cols), a.sums = static_cast<float *>(d_workspace);
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DWEIGHTS>(a, static_cast<hipStream_t>(stream));
+  });
+}
+
+KM_API int h2o4gpu_experts_align_rows(int dtype, size_t matrices, size_t rows, size_t cols, const void *d_in,
+                                      size_t matrix_stride, size_t stride, void *d_out, void *stream) {
+  if (!known_type(dtype) || cols < 1 || cols > MAX_SIDE || rows > (size_t)INT_MAX || matrices > (size_t)INT_MAX)
+    return H2O4GPU_KMEANS_EARG;
+  const size_t size = type_size(dtype), pieces = (cols * size + 15) / 16;
+  if (matrices * rows > ((size_t)1 << 40) / pieces) return H2O4GPU_KMEANS_EARG;
+  const size_t total = matrices * rows * pieces;
+  if (total == 0) return H2O4GPU_KMEANS_OK;
+  if (!d_in || !d_out || !aligned_to(d_out, 16)) return H2O4GPU_KMEANS_EARG;
+  return with_type(dtype, [&](auto tag) {
+    typedef typename decltype(tag)::type T;
+    hipLaunchKernelGGL((align_kernel<T>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const T *>(d_in), stride, matrix_stride, rows, cols,
+                       pieces, total, static_cast<u32x4 *>(d_out));
+    return launched();
   });
 }

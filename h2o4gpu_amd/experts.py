@@ -364,10 +364,51 @@ def _sums(rows, n_experts, out, cols):
     return experts_hip.lib().h2o4gpu_experts_product_dweights_workspace(rows, n_experts, out, cols)
 
 
+def _aligned(t):
+    """Whether all rows of a matrix, or of several, begin at multiples of 16 bytes."""
+    each = 16 // t.element_size()
+    return t.data_ptr() % 16 == 0 and all(s % each == 0 for s in t.stride()[:-1])
+
+
+def _align(worth, *tensors):
+    """The operands of a product, copied to rows that begin at multiples of 16 bytes where they do not and the
+    product is long enough. The kernels for such rows take a 16-bit product in a fifth of the time: about 3.5 us
+    less for 10^9 operations, while a copy takes 6 us and 1 us for every 2.2 MB (11044 x 5823, 6 experts: 230 us a
+    copy, 580 us less a product)."""
+    if worth < 2e9:
+        return tensors
+    odd = [t for t in tensors if not _aligned(t)]
+    if not odd or 3.5e-9 * worth < sum(6 + t.numel() * t.element_size() / 2.2e6 for t in odd):
+        return tensors
+    return tuple(t if _aligned(t) else _copy_aligned(t) for t in tensors)
+
+
+def _copy_aligned(t):
+    each = 16 // t.element_size()
+    cols = t.shape[-1]
+    wide = t.new_empty(t.shape[:-1] + (-(-cols // each) * each,))
+    matrices, rows = (t.shape[0], t.shape[1]) if t.dim() == 3 else (1, t.shape[0])
+    ptr, apart, stride = _matrices(t) if t.dim() == 3 else (t.data_ptr(), 0, _rows("rows", t)[1])
+    _call(t.device.index, "h2o4gpu_experts_align_rows", _TYPES[t.dtype], matrices, rows, cols, ptr, apart, stride,
+          wide.data_ptr())
+    return wide[..., :cols]
+
+
+def _worth(rows, weights):
+    """Operations of a product, where large tiles of 16-bit numbers may take it; 0 where they may not."""
+    n_experts, out, cols = weights.shape
+    if weights.dtype == torch.float32 or rows.shape[0] < 128 * n_experts or min(out, cols) < 128:
+        return 0
+    return 2.0 * rows.shape[0] * out * cols
+
+
 def _product(rows, weights, order):
-    ptr, stride = _rows("rows", rows)
     n_experts, out, cols = weights.shape
     y = rows.new_empty((rows.shape[0], out))
+    worth = _worth(rows, weights)
+    if worth:
+        rows, weights = _align(worth, rows, weights)
+    ptr, stride = _rows("rows", rows)
     _call(rows.device.index, "h2o4gpu_experts_product", _TYPES[rows.dtype], rows.shape[0], n_experts, out, cols, ptr,
           stride, *_matrices(weights), order._offsets_ptr, y.data_ptr(), out)
     return y
@@ -384,23 +425,31 @@ class _Product(torch.autograd.Function):
     def backward(ctx, dy):
         order = ctx.order
         rows, weights = ctx.saved_tensors
-        dy = _gradient(dy)
-        ptr, stride = _rows("dy", dy)
+        dy = given = _gradient(dy)
+        _rows("dy", dy)
         n_experts, out, cols = weights.shape
-        code, count = _TYPES[dy.dtype], dy.shape[0]
+        code, count, worth = _TYPES[dy.dtype], dy.shape[0], _worth(rows, weights)
         drows = dweights = None
         if ctx.needs_input_grad[0]:
+            w = weights
+            if worth:
+                dy, w = _align(worth * (2 if ctx.needs_input_grad[1] else 1), dy, w)
             drows = rows.new_empty(rows.shape)
-            _call(dy.device.index, "h2o4gpu_experts_product_drows", code, count, n_experts, out, cols, ptr, stride,
-                  *_matrices(weights), order._offsets_ptr, drows.data_ptr(), cols)
-            drows = _once(drows, weights, dy)
+            _call(dy.device.index, "h2o4gpu_experts_product_drows", code, count, n_experts, out, cols, *_rows("dy", dy),
+                  *_matrices(w), order._offsets_ptr, drows.data_ptr(), cols)
+            del w
+            drows = _once(drows, weights, given)
         if ctx.needs_input_grad[1]:
+            x = rows
+            if worth:
+                dy, x = _align(worth, dy, x)
             dweights = weights.new_empty(weights.shape)
             need = _sums(count, n_experts, out, cols)
             work = dy.new_empty(need // 4, dtype=torch.float32) if need else None
-            _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols, ptr, stride,
-                  *_rows("rows", rows), order._offsets_ptr, dweights.data_ptr(), work.data_ptr() if need else None, need)
-            dweights = _once(dweights, rows, dy)
+            _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols,
+                  *_rows("dy", dy), *_rows("rows", x), order._offsets_ptr, dweights.data_ptr(),
+                  work.data_ptr() if need else None, need)
+            dweights = _once(dweights, rows, given)
         return drows, dweights, None
 
 

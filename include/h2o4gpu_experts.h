@@ -150,6 +150,12 @@ int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t
                                      size_t dy_stride, const void *d_rows, size_t rows_stride, const int *d_offsets,
                                      void *d_dweights, void *d_workspace, size_t workspace_bytes, void *stream);
 
+/* Rows of `matrices` matrices [rows][cols], the matrices matrix_stride elements apart, to rows that begin at
+ * multiples of 16 bytes, as short as they can be, one matrix behind another; zeros behind column cols. The
+ * products above take long rows faster where strides and addresses of both operands are multiples of 16 bytes. */
+int h2o4gpu_experts_align_rows(int dtype, size_t matrices, size_t rows, size_t cols, const void *d_in,
+                               size_t matrix_stride, size_t stride, void *d_out, void *stream);
+
 /* Microscaled 4-bit matrices: every 32 columns of a row share a power of two, 2^(byte - 127), and an
  * element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 .. 7, the sign is 8) times it. A
  * scale byte of 255 is not a number, and neither is its block.
