@@ -276,7 +276,8 @@ __global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
 template <typename T>
 int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   const size_t pitch = codes_pitch(a.cols);
-  if (a.rows / (a.experts ? a.experts : 1) <= 64) {
+  const size_t tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.out + 127) / 128);
+  if (a.rows / (a.experts ? a.experts : 1) <= 64 || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);

@@ -1,6 +1,6 @@
 // Products of few rows: the matrices are read once, straight into the registers of the matrix instructions' operand, and
-// that is what bounds them. A workgroup has 16 NB rows of a matrix and MB blocks of 16 rows of x; its wavefronts share
-// the columns and add up their sums in LDS.
+// that is what bounds them. A wavefront has 16 NB rows of a matrix and MB blocks of 16 rows of x; `share` wavefronts of a
+// workgroup (a power of two) share the columns and add up their sums in LDS, the others have other rows of the matrix.
 #pragma once
 
 #include "product_pipe.h"
@@ -16,7 +16,7 @@ struct ThinArgs {
   const int *order, *offsets;                          // as in PipeArgs
   int top_k, experts, rows, n, k;                      // k in elements (Four: in groups of four columns)
   unsigned first_block;
-  int n_tiles;
+  int share, n_tiles;  // wavefronts that share columns; workgroups to a block of rows
 };
 
 // ALIGNED: every piece lies at a multiple of 16 bytes, and k is whole pieces.
@@ -29,13 +29,15 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4;
   const unsigned block = a.first_block + blockIdx.x;
-  const int n0 = (int)(block % (unsigned)a.n_tiles) * (16 * NB), number = (int)(block / (unsigned)a.n_tiles);
+  const int part = wave & (a.share - 1), row = wave / a.share;
+  const int n0 = ((int)(block % (unsigned)a.n_tiles) * (WAVES / a.share) + row) * (16 * NB), number = (int)(block / (unsigned)a.n_tiles);
   int expert = 0, first = number * (16 * MB), m_here = a.rows - first < 16 * MB ? a.rows - first : 16 * MB, k = a.k;
   if (a.experts) {
     if (!ragged_tile(a.offsets, a.experts, a.rows, 16 * MB, number, expert, first, m_here)) return;
     if (expert == a.experts) k = 0, expert = 0;  // rows without an expert: zeros
   }
-  const int n_here = a.n - n0 < 16 * NB ? a.n - n0 : 16 * NB;
+  const int n_here = a.n - n0 < 16 * NB ? a.n - n0 : 16 * NB;  // (not positive: nothing to do but to meet the others)
+  if (n_here <= 0) k = 0;
 
   f32x4 acc[MB][NB];
 #pragma unroll
@@ -54,13 +56,13 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
   }
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int r = n0 + (n * 16 + i < n_here ? n * 16 + i : n_here - 1);
+    const int r = n_here <= 0 ? 0 : n0 + (n * 16 + i < n_here ? n * 16 + i : n_here - 1);
     w[n] = a.w + (size_t)expert * a.w_expert + (size_t)r * a.w_stride + g * 16;
     if constexpr (FOUR) ws[n] = a.w_scales + ((size_t)expert * a.n + r) * a.scales_stride + 4 * g;
   }
   const int turns = (k + U * STEP - 1) / (U * STEP);
   // a wavefront's turns lie side by side
-  const int each = (turns + WAVES - 1) / WAVES, begin = wave * each, end = begin + each < turns ? begin + each : turns;
+  const int each = (turns + a.share - 1) / a.share, begin = part * each, end = begin + each < turns ? begin + each : turns;
   u32x4 fx[U][MB], fw[U][NB];
   unsigned sx[FOUR ? MB : 1], sw[FOUR ? NB : 1];
   auto load = [&](int t) {
@@ -109,18 +111,26 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
     step(Int<2>());
     step(Int<3>());
   }
+  auto store = [&](int b, f32x4 s) {
+    const int m = b / NB * 16 + i, n = b % NB * 16 + 4 * g;
+    if (m < m_here) store_four(static_cast<OUT *>(a.c) + (size_t)(first + m) * a.c_stride + n0 + n, s, n_here - n);
+  };
+  if (a.share == 1) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) store(m * NB + n, acc[m][n]);
+    return;
+  }
 #pragma unroll
   for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int n = 0; n < NB; ++n) sums[wave][m * NB + n][lane] = acc[m][n];
   __syncthreads();
-  for (int b = wave; b < MB * NB; b += WAVES) {
-    f32x4 s = sums[0][b][lane];
-#pragma unroll
-    for (int v = 1; v < WAVES; ++v) s += sums[v][b][lane];
-    const int m = b / NB * 16 + i, n = b % NB * 16 + 4 * g;
-    if (m < m_here)
-      store_four(static_cast<OUT *>(a.c) + (size_t)(first + m) * a.c_stride + n0 + n, s, n_here - n);
+  for (int b = part; b < MB * NB; b += a.share) {
+    f32x4 s = sums[wave - part][b][lane];
+    for (int v = 1; v < a.share; ++v) s += sums[wave - part + v][b][lane];
+    store(b, s);
   }
 }
 
@@ -131,7 +141,11 @@ int launch_thin(ThinArgs &a, hipStream_t stream) {
     constexpr int MB = decltype(mb)::value, NB = decltype(nb)::value, WAVES = 8;
     const size_t m_tiles =
         a.experts ? ragged_tiles(a.experts, a.rows, 16 * MB) : ((size_t)a.rows + 16 * MB - 1) / (16 * MB);
-    a.n_tiles = (a.n + 16 * NB - 1) / (16 * NB);
+    // a wavefront for each turn of a row, up to the workgroup's
+    constexpr int TURN = 4 * 4 * (16 / (int)sizeof(typename PipeElement<ELEMENT>::type));
+    const int turns = (a.k + TURN - 1) / TURN;
+    a.share = turns > 4 ? 8 : turns > 2 ? 4 : turns > 1 ? 2 : 1;
+    a.n_tiles = (a.n + 16 * NB * (WAVES / a.share) - 1) / (16 * NB * (WAVES / a.share));
     return in_launches(m_tiles * a.n_tiles, [&](unsigned first, unsigned blocks) {
       a.first_block = first;
       hipLaunchKernelGGL((thin_kernel<ELEMENT, OUT, MB, NB, WAVES, ALIGNED>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
@@ -142,6 +156,123 @@ int launch_thin(ThinArgs &a, hipStream_t stream) {
   if (each <= 32) return launch(Int<2>(), Int<2>());
   if (each <= 48) return launch(Int<3>(), Int<2>());
   return launch(Int<4>(), Int<2>());
+}
+
+// The same where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some k's of
+// its own; element b of all of them is its fragment of a block of 16 columns, EPP apart, so that a wavefront has
+// 16 EPP columns. What comes out for a lane and a j, block by block, is EPP columns side by side again.
+template <typename T, int MB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
+  constexpr int EPP = 16 / (int)sizeof(T), STEP = 4 * EPP, U = 64 / STEP;  // 64 k a turn
+  __shared__ f32x4 sums[WAVES][MB * EPP][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const unsigned block = a.first_block + blockIdx.x;
+  const int part = wave & (a.share - 1);
+  const int n0 = ((int)(block % (unsigned)a.n_tiles) * (WAVES / a.share) + wave / a.share) * (16 * EPP);
+  int expert, first, m_here, k = a.k;
+  if (!ragged_tile(a.offsets, a.experts, a.rows, 16 * MB, (int)(block / (unsigned)a.n_tiles), expert, first, m_here)) return;
+  if (expert == a.experts) k = 0, expert = 0;  // rows without an expert: zeros
+  const int left = a.n - n0 - EPP * i;         // of the lane's columns
+  if (a.n <= n0) k = 0;
+
+  f32x4 acc[MB][EPP];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int b = 0; b < EPP; ++b) acc[m][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T *x[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+    x[m] = reinterpret_cast<const T *>(a.x + (size_t)(first + (m * 16 + i < m_here ? m * 16 + i : m_here - 1)) * a.x_stride);
+  const char *w = a.w + (size_t)expert * a.w_expert + (size_t)(n0 + EPP * i) * sizeof(T);
+  const int turns = (k + 63) / 64, each = (turns + a.share - 1) / a.share;
+  const int begin = part * each, end = begin + each < turns ? begin + each : turns;
+  for (int t = begin; t < end; ++t) {
+    u32x4 fx[U][MB], v[U][EPP];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k0 = t * 64 + u * STEP + EPP * g;
+#pragma unroll
+      for (int r = 0; r < EPP; ++r)
+        v[u][r] = load_piece(reinterpret_cast<const T *>(w + (size_t)(k0 + r) * a.w_stride), k0 + r < k ? left : 0);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) fx[u][m] = load_piece(x[m] + k0, k - k0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int b = 0; b < EPP; ++b) {
+        u32x4 f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          if constexpr (sizeof(T) == 4)
+            f[d] = v[u][d][b];
+          else
+            f[d] = __builtin_amdgcn_perm(v[u][2 * d + 1][b / 2], v[u][2 * d][b / 2], b & 1 ? 0x07060302u : 0x05040100u);
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m) mfma_piece(acc[m][b], f, fx[u][m], Tag<T>());
+      }
+  }
+  typedef Beside<T, EPP> piece;
+  auto store = [&](int m, int j, const float (&s)[EPP]) {
+    const int n = n0 + EPP * (4 * g + j), valid = a.n - n;
+    if (m * 16 + i >= m_here || valid <= 0) return;
+    T *to = static_cast<T *>(a.c) + (size_t)(first + m * 16 + i) * a.c_stride + n;
+    piece p;
+#pragma unroll
+    for (int b = 0; b < EPP; ++b) p.v[b] = (T)s[b];
+    if (valid >= EPP) {
+      *reinterpret_cast<piece *>(to) = p;
+    } else {
+#pragma unroll
+      for (int b = 0; b < EPP - 1; ++b)
+        if (b < valid) to[b] = p.v[b];
+    }
+  };
+  if (a.share > 1) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int b = 0; b < EPP; ++b) sums[wave][m * EPP + b][lane] = acc[m][b];
+    __syncthreads();
+    for (int q = part; q < MB * 4; q += a.share) {
+      float s[EPP];
+#pragma unroll
+      for (int b = 0; b < EPP; ++b) s[b] = sums[wave - part][q / 4 * EPP + b][lane][q % 4];
+      for (int p = 1; p < a.share; ++p)
+#pragma unroll
+        for (int b = 0; b < EPP; ++b) s[b] += sums[wave - part + p][q / 4 * EPP + b][lane][q % 4];
+      store(q / 4, q % 4, s);
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float s[EPP];
+#pragma unroll
+        for (int b = 0; b < EPP; ++b) s[b] = acc[m][b][j];
+        store(m, j, s);
+      }
+  }
+}
+
+template <typename T>
+int launch_thin_columns(ThinArgs &a, hipStream_t stream) {
+  auto launch = [&](auto mb, auto waves) {
+    constexpr int MB = decltype(mb)::value, WAVES = decltype(waves)::value, COLS = 16 * (16 / (int)sizeof(T));
+    const int turns = (a.k + 63) / 64;
+    a.share = turns >= WAVES ? WAVES : turns > 2 ? 4 : turns > 1 ? 2 : 1;
+    a.n_tiles = (a.n + COLS * (WAVES / a.share) - 1) / (COLS * (WAVES / a.share));
+    return in_launches(ragged_tiles(a.experts, a.rows, 16 * MB) * a.n_tiles, [&](unsigned first, unsigned blocks) {
+      a.first_block = first;
+      hipLaunchKernelGGL((thin_columns_kernel<T, MB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+      return launched();
+    });
+  };
+  return a.rows / a.experts <= 16 ? launch(Int<1>(), Int<8>()) : launch(Int<2>(), Int<4>());
 }
 
 }  // namespace kmhip

@@ -207,18 +207,19 @@ int join_parts(const ProductArgs &a, hipStream_t stream) {
 
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
-  if constexpr (KIND == FORWARD) {
-    if (a.rows / a.experts <= 64) {
-      ThinArgs t = {};
-      t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
-      t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
-      t.c_stride = a.c_stride, t.offsets = a.offsets;
-      t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
-      return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
-                                                               : launch_thin<T, T, false>(t, stream);
-    }
+  const size_t each = a.rows / a.experts, tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.n + 127) / 128);
+  // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
+  if (KIND == FORWARD ? each <= 64 || (tiles <= 128 && (double)a.rows * a.n * a.k < 2e9) : KIND == DROWS && each <= 32) {
+    ThinArgs t = {};
+    t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
+    t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
+    t.c_stride = a.c_stride, t.offsets = a.offsets;
+    t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
+    if (KIND == DROWS) return launch_thin_columns<T>(t, stream);
+    return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
+                                                             : launch_thin<T, T, false>(t, stream);
   }
-  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? a.k : a.rows / a.experts) >= 128 && a.n >= 128) {
+  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? (size_t)a.k : each) >= 128 && a.n >= 128) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);

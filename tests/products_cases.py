@@ -13,7 +13,7 @@ RAGGED = (
     (900, 3, 4, 96, 384), (31, 2, 2, 520, 4104), (5000, 1, 5, 24, 40), (20, 1, 4100, 8, 33),
     # more rows than a gradient's part, parts that end inside tiles, large tiles that end inside matrices and stages
     (3001, 2, 3, 136, 264), (1500, 2, 2, 520, 1032), (700, 4, 5, 256, 512), (1100, 2, 7, 384, 136), (2500, 2, 1, 128, 128),
-    (9000, 1, 2300, 16, 24), (2600, 2, 4, 200, 128), (900, 1, 3, 1000, 72), (300, 1, 1, 264, 2056),
+    (9000, 1, 2300, 16, 24), (90, 1, 3, 1100, 300), (40, 2, 4, 513, 129), (7, 1, 2, 65, 1000), (100, 4, 20, 128, 40), (2600, 2, 4, 200, 128), (900, 1, 3, 1000, 72), (300, 1, 1, 264, 2056),
 )
 
 
