@@ -157,127 +157,15 @@ struct FourArgs {
   const int *order, *offsets;  // with experts only; order: x's row of y's row p is order[p] / top_k (none: p)
   int top_k, experts;          // experts 0: one matrix
   int rows, out, cols;
-  unsigned first_block;
-  int n_tiles;
 };
-
-__device__ __forceinline__ void to_lds(const void *from, char *lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)(lds), 16, 0, 0);
-#endif
-}
-
-// Stages of 256 columns go straight to LDS, two of them: the next is on its way while one is multiplied.
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64) void four_kernel(FourArgs a) {
-  typedef OperandTile<bfloat16_t, BM, false> TX;  // (bytes are bytes: a stage is 128 of each row)
-  typedef OperandTile<bfloat16_t, BN, false> TW;
-  constexpr int THREADS = WM * WN * 64;
-  constexpr int PX = TX::SLOTS / THREADS, PW = TW::SLOTS / THREADS;
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int STAGE = (BM + BN) * 128;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned block = a.first_block + blockIdx.x;
-  const int n0 = (int)(block % (unsigned)a.n_tiles) * BN, number = (int)(block / (unsigned)a.n_tiles);
-  int expert = 0, first = number * BM, m_here = a.rows - first < BM ? a.rows - first : BM;
-  int stages = (a.cols + 255) / 256;
-  if (a.experts) {
-    if (!ragged_tile(a.offsets, a.experts, a.rows, BM, number, expert, first, m_here)) return;
-    if (expert == a.experts) stages = 0, expert = 0;
-  }
-  const int n_here = a.out - n0 < BN ? a.out - n0 : BN;
-  const size_t pitch = codes_pitch(a.cols), spitch = scales_pitch(a.cols);
-  const size_t w_row = (size_t)expert * a.out + n0;
-  auto x_row = [&](int m) -> size_t {
-    m = first + (m < m_here ? m : m_here - 1);
-    return a.order ? (size_t)(a.order[m] / a.top_k) : (size_t)m;
-  };
-  const unsigned char *gx[PX], *gw[PW];
-  const int wm = wave / WN, wn = wave % WN;
-  const unsigned char *sx_at[FM], *sw_at[FN];
-  f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (stages) {
-#pragma unroll
-    for (int i = 0; i < PX; ++i) {
-      int r, k;
-      TX::place(i * THREADS + tid, r, k);
-      gx[i] = a.x + x_row(r) * pitch + k * 2;
-    }
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      int r, k;
-      TW::place(i * THREADS + tid, r, k);
-      gw[i] = a.w + (w_row + (r < n_here ? r : n_here - 1)) * pitch + k * 2;
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-      sx_at[i] = a.x_scales + x_row((wm * FM + i) * 16 + (lane & 15)) * spitch + 4 * (lane >> 4);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int r = (wn * FN + j) * 16 + (lane & 15);
-      sw_at[j] = a.w_scales + (w_row + (r < n_here ? r : n_here - 1)) * spitch + 4 * (lane >> 4);
-    }
-  }
-  auto load = [&](int t) {
-    char *at = lds + (t & 1) * STAGE + wave * 1024;
-#pragma unroll
-    for (int i = 0; i < PX; ++i) to_lds(gx[i] + (size_t)t * 128, at + i * THREADS * 16);
-#pragma unroll
-    for (int i = 0; i < PW; ++i) to_lds(gw[i] + (size_t)t * 128, at + BM * 128 + i * THREADS * 16);
-  };
-  if (stages) load(0);
-  for (int t = 0; t < stages; ++t) {
-    unsigned sx[FM], sw[FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-      sx[i] = *reinterpret_cast<const unsigned *>(sx_at[i] + (size_t)(t / 2) * 16) >> (16 * (t & 1));
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-      sw[j] = *reinterpret_cast<const unsigned *>(sw_at[j] + (size_t)(t / 2) * 16) >> (16 * (t & 1));
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the stage has arrived
-    __syncthreads();
-    if (t + 1 < stages) load(t + 1);
-    const char *at = lds + (t & 1) * STAGE;
-    auto step = [&](auto number) {
-      constexpr int STEP = decltype(number)::value;
-      u32x4 fx[FM], fw[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, wm * FM + i, STEP);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = TW::fragment(at + BM * 128, lane, wn * FN + j, STEP);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) mfma_four<STEP>(acc[i][j], fw[j], fx[i], sw[j], sx[i]);
-    };
-    step(Int<0>());
-    step(Int<1>());
-    __syncthreads();
-  }
-  T *y = static_cast<T *>(a.y) + (size_t)first * a.y_stride + n0;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = (wm * FM + i) * 16 + (lane & 15);
-    if (m >= m_here) continue;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = (wn * FN + j) * 16 + 4 * (lane >> 4);
-      store_four(y + (size_t)m * a.y_stride + n, acc[i][j], n_here - n);
-    }
-  }
-}
 
 template <typename T>
 int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
-  const size_t pitch = codes_pitch(a.cols);
+  const size_t pitch = codes_pitch(a.cols), each = a.rows / (a.experts ? a.experts : 1);
   const size_t tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.out + 127) / 128);
-  if (a.rows / (a.experts ? a.experts : 1) <= 64 || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
+  const bool reached = (!a.order || x_rows * pitch < BUFFER_BYTES) && pitch < BUFFER_BYTES / 512;
+  // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
+  if (each <= 64 || !reached || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);
@@ -285,26 +173,13 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
     t.experts = a.experts, t.rows = a.rows, t.n = a.out, t.k = (int)((a.cols + 127) / 128 * 32);
     return launch_thin<Four, T, true>(t, stream);
   }
-  if (x_rows * pitch < BUFFER_BYTES && pitch < BUFFER_BYTES / 512 && a.out >= 128 &&
-      a.rows / (a.experts ? a.experts : 1) >= 128) {
-    PipeArgs p = {};
-    p.x = (const char *)a.x, p.w = (const char *)a.w, p.x_scales = a.x_scales, p.w_scales = a.w_scales, p.c = a.y;
-    p.x_stride = p.w_stride = pitch, p.w_expert = pitch * a.out, p.scales_stride = scales_pitch(a.cols);
-    p.c_stride = a.y_stride, p.x_bytes = x_rows * pitch;
-    p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
-    p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
-    return a.order ? launch_pipe<Four, T, FORWARD, true, 256, 256, 2, 4>(p, stream)
-                   : launch_pipe<Four, T, FORWARD, false, 256, 256, 2, 4>(p, stream);
-  }
-  constexpr int BM = 128, BN = 128;
-  const size_t m_tiles = a.experts ? ragged_tiles(a.experts, a.rows, BM) : ((size_t)a.rows + BM - 1) / BM;
-  FourArgs f = a;
-  f.n_tiles = (a.out + BN - 1) / BN;
-  return in_launches(m_tiles * f.n_tiles, [&](unsigned first, unsigned blocks) {
-    f.first_block = first;
-    hipLaunchKernelGGL((four_kernel<T, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, f);
-    return launched();
-  });
+  PipeArgs p = {};
+  p.x = (const char *)a.x, p.w = (const char *)a.w, p.x_scales = a.x_scales, p.w_scales = a.w_scales, p.c = a.y;
+  p.x_stride = p.w_stride = pitch, p.w_expert = pitch * a.out, p.scales_stride = scales_pitch(a.cols);
+  p.c_stride = a.y_stride, p.x_bytes = x_rows * pitch;
+  p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
+  p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
+  return a.order ? launch_large<Four, T, FORWARD, true>(p, stream) : launch_large<Four, T, FORWARD, false>(p, stream);
 }
 
 bool sized(size_t rows, size_t cols) { return cols >= 1 && cols <= MAX_SIDE && rows <= ((size_t)1 << 40) / codes_pitch(cols); }

@@ -147,7 +147,7 @@ struct PipeOperand {
   }
 };
 
-constexpr int PIPE_TABLE = 2046;  // experts + 2 numbers of 4 bytes fit 8 KB of LDS
+constexpr int PIPE_TABLE = 1022;  // experts + 2 numbers of 4 bytes fit 4 KB of LDS
 
 // table[e]: the sum of count(rows of an expert) over the experts before e; [experts + 1]: over all, and over the rows
 // without an expert.
@@ -609,7 +609,6 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads that read nothing end before the LDS is another's)
 }
 
-constexpr size_t PIPE_WORKGROUPS = 256;    // one to a CU, as many as the LDS allows
 constexpr size_t BUFFER_BYTES = (size_t)1 << 32;  // what a buffer's offsets reach
 
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
@@ -626,9 +625,28 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
       (BM + BN) * (256 + (__is_same(ELEMENT, Four) ? 32 : 0)) + (GATHER ? BM * 8 : 0) + (PIPE_TABLE + 2 + WM * WN) * 4;
   const auto kernel = pipe_kernel<ELEMENT, OUT, KIND, GATHER, BM, BN, WM, WN>;
   KM_TRY(ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds));
-  const size_t blocks = tiles < PIPE_WORKGROUPS ? (tiles + 7) / 8 * 8 : PIPE_WORKGROUPS;
+  constexpr size_t WORKGROUPS = BM + BN == 512 ? 256 : 512;  // as many as the CUs' LDS allows
+  const size_t blocks = tiles < WORKGROUPS ? (tiles + 7) / 8 * 8 : WORKGROUPS;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WM * WN * 64), lds, stream, a);
   return launched();
+}
+
+// Tiles of 256 x 256, or of 128 x 128, of which a CU holds two: by how often the card is filled with either (an expert's
+// last tile is taken to be half full), and how long a stage then takes, 1.7 and 1.3 us. 64 experts' 65536 rows of 2048 with
+// 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones, 4 experts' 8000 rows of 1024 with 512 x 1024
+// 27 and 16 us, 10 experts' 16941 rows of 4544 with 384 89 and 64, 160 experts' 49552 rows of 256 with 3392 188 and 191.
+template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER>
+int launch_large(PipeArgs &a, hipStream_t stream) {
+  auto turns = [&](int tile, int at_once) {
+    const double n = (a.n + tile - 1) / tile;
+    const double m = KIND == DWEIGHTS ? (double)((a.k + tile - 1) / tile) *
+                                            (a.part < a.rows ? a.rows / a.part + a.experts / 2 : a.experts)
+                                      : (double)a.rows / tile + a.experts / 2.0;
+    return ceil(m * n / at_once);
+  };
+  if (1.7 * turns(256, 256) <= 1.3 * turns(128, 512))
+    return launch_pipe<ELEMENT, OUT, KIND, GATHER, 256, 256, 2, 4>(a, stream);
+  return launch_pipe<ELEMENT, OUT, KIND, GATHER, 128, 128, 2, 2>(a, stream);
 }
 
 }  // namespace kmhip

@@ -219,14 +219,14 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? (size_t)a.k : each) >= 128 && a.n >= 128) {
+  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : each >= 128) && a.n >= 128) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
     p.c_stride = a.c_stride, p.c_expert = a.c_expert;
     p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
     p.part = a.part, p.sums = a.sums;
-    KM_TRY((launch_pipe<T, T, KIND, false, 256, 256, 2, 4>(p, stream)));
+    KM_TRY((launch_large<T, T, KIND, false>(p, stream)));
     return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
   }
   constexpr int BM = 128, BN = 128;

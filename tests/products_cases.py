@@ -10,7 +10,7 @@ RAGGED = (
     (1, 1, 1, 1, 1), (1, 2, 16, 100, 256), (3, 2, 5, 7, 5), (17, 1, 3, 33, 31), (1, 4, 4, 17, 1000), (64, 4, 3, 33, 96),
     (40, 3, 8, 64, 512), (3, 8, 300, 16, 64), (200, 2, 6, 48, 160), (33, 6, 64, 20, 2050), (300, 1, 2, 130, 129),
     (257, 2, 2, 255, 257), (500, 2, 7, 129, 65), (1000, 1, 3, 257, 200), (128, 1, 1, 128, 64), (2000, 1, 1, 300, 72),
-    (900, 3, 4, 96, 384), (31, 2, 2, 520, 4104), (5000, 1, 5, 24, 40), (20, 1, 4100, 8, 33),
+    (900, 3, 4, 96, 384), (31, 2, 2, 520, 4104), (5000, 1, 5, 24, 40), (20, 1, 4100, 8, 33), (140000, 1, 1030, 136, 72),
     # more rows than a gradient's part, parts that end inside tiles, large tiles that end inside matrices and stages
     (3001, 2, 3, 136, 264), (1500, 2, 2, 520, 1032), (700, 4, 5, 256, 512), (1100, 2, 7, 384, 136), (2500, 2, 1, 128, 128),
     (9000, 1, 2300, 16, 24), (90, 1, 3, 1100, 300), (40, 2, 4, 513, 129), (7, 1, 2, 65, 1000), (100, 4, 20, 128, 40), (2600, 2, 4, 200, 128), (900, 1, 3, 1000, 72), (300, 1, 1, 264, 2056),
