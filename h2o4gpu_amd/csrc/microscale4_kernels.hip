@@ -110,13 +110,18 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const unsigned *codes, 
   const float power = power_of(scales[row * scales_row + scale_place(word / 4)]);
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = element(code >> (4 * i)) * power;
+  for (int i = 0; i < 8; ++i) {
+    v[i] = element(code >> (4 * i)) * power;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(v[i]));  // (as one instruction with a conversion to float16, -0 would become 0)
+#endif
+  }
   T *o = out + row * out_stride + word * 8;
   const int left = (int)cols - (int)word * 8;
   if (left >= 8) {
-    typedef Beside<T, 8> eight;
-    reinterpret_cast<eight *>(o)->v =
-        typename eight::vector{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
+    typedef typename Beside<T, 8>::vector eight;
+    const eight all = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
+    store_beside<T, 8>(o, all);
   } else {
     store_four(o, f32x4{v[0], v[1], v[2], v[3]}, left);
     store_four(o + 4, f32x4{v[4], v[5], v[6], v[7]}, left - 4);

@@ -246,7 +246,7 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
         const int n = n0 + j * 16 + 8 * q;
         if (m < m_here && n < n_here) {
           if (n + EPP <= n_here) {
-            reinterpret_cast<Beside<OUT, EPP> *>(row + n)->v = __builtin_bit_cast(typename Beside<OUT, EPP>::vector, piece);
+            store_beside<OUT, EPP>(row + n, __builtin_bit_cast(typename Beside<OUT, EPP>::vector, piece));
           } else {
 #pragma unroll
             for (int e = 0; e < EPP; ++e)
@@ -532,12 +532,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   auto mask = [&](auto step, int left) {
     constexpr int S = decltype(step)::value;
     left -= S * (KS / 2) + EPP * ((threadIdx.x & 63) >> 4);
-    u32x4 keep;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int bytes = left * SIZE - 4 * i;
-      keep[i] = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : 0xffffu;
-    }
+    const u32x4 keep = first_of<T>(left);
 #pragma unroll
     for (int i = 0; i < FM; ++i) f[S].x[i] &= keep;
 #pragma unroll

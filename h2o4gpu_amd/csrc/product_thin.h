@@ -7,6 +7,8 @@
 
 namespace kmhip {
 
+constexpr size_t THIN_ROWS = 64;  // of an expert, on average
+
 struct ThinArgs {
   const char *x, *w;
   const unsigned char *x_scales, *w_scales;            // Four only, rows of `scales_stride` bytes
@@ -16,6 +18,7 @@ struct ThinArgs {
   const int *order, *offsets;                          // as in PipeArgs
   int top_k, experts, rows, n, k;                      // k in elements (Four: in groups of four columns)
   unsigned first_block;
+  int halves;          // some row of x or of a matrix begins between words
   int share, n_tiles;  // wavefronts that share columns; workgroups to a block of rows
 };
 
@@ -66,23 +69,42 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
   u32x4 fx[U][MB], fw[U][NB];
   unsigned sx[FOUR ? MB : 1], sw[FOUR ? NB : 1];
   auto load = [&](int t) {
+    auto all = [&](bool halves) __attribute__((always_inline)) {  // (no branches: all loads are on their way at once)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const size_t at = ((size_t)t * U + u) * 64;
-      const int left = k - ((t * U + u) * STEP + g * EPP);
+      for (int u = 0; u < U; ++u) {
+        const size_t at = ((size_t)t * U + u) * 64;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        if constexpr (ALIGNED)
-          fw[u][n] = left > 0 ? *reinterpret_cast<const u32x4 *>(w[n] + at) : u32x4{0, 0, 0, 0};
-        else
-          fw[u][n] = load_piece(reinterpret_cast<const T *>(w[n] + at), left);
+        for (int n = 0; n < NB; ++n)
+          fw[u][n] = ALIGNED ? *reinterpret_cast<const u32x4 *>(w[n] + at) : load_whole(reinterpret_cast<const T *>(w[n] + at), halves);
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+          fx[u][m] = ALIGNED ? *reinterpret_cast<const u32x4 *>(x[m] + at) : load_whole(reinterpret_cast<const T *>(x[m] + at), halves);
       }
+    };
+    if ((t + 1) * (U * STEP) <= k) {
+      if (!ALIGNED && a.halves)
+        all(true);
+      else
+        all(false);
+    } else {
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        if constexpr (ALIGNED)
-          fx[u][m] = left > 0 ? *reinterpret_cast<const u32x4 *>(x[m] + at) : u32x4{0, 0, 0, 0};
-        else
-          fx[u][m] = load_piece(reinterpret_cast<const T *>(x[m] + at), left);
+      for (int u = 0; u < U; ++u) {
+        const size_t at = ((size_t)t * U + u) * 64;
+        const int left = k - ((t * U + u) * STEP + g * EPP);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if constexpr (ALIGNED)
+            fw[u][n] = left > 0 ? *reinterpret_cast<const u32x4 *>(w[n] + at) : u32x4{0, 0, 0, 0};
+          else
+            fw[u][n] = load_piece(reinterpret_cast<const T *>(w[n] + at), left);
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          if constexpr (ALIGNED)
+            fx[u][m] = left > 0 ? *reinterpret_cast<const u32x4 *>(x[m] + at) : u32x4{0, 0, 0, 0};
+          else
+            fx[u][m] = load_piece(reinterpret_cast<const T *>(x[m] + at), left);
+        }
       }
     }
     if constexpr (FOUR) {
@@ -190,8 +212,25 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
   const int begin = part * each, end = begin + each < turns ? begin + each : turns;
   for (int t = begin; t < end; ++t) {
     u32x4 fx[U][MB], v[U][EPP];
+    const bool whole = (t + 1) * 64 <= k && n0 + 16 * EPP <= a.n;  // (no branches: all loads are on their way at once)
+    auto all = [&](bool halves) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < U; ++u) {
+        const int k0 = t * 64 + u * STEP + EPP * g;
+#pragma unroll
+        for (int r = 0; r < EPP; ++r) v[u][r] = load_whole(reinterpret_cast<const T *>(w + (size_t)(k0 + r) * a.w_stride), halves);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) fx[u][m] = load_whole(x[m] + k0, halves);
+      }
+    };
+    if (whole) {
+      if (a.halves)
+        all(true);
+      else
+        all(false);
+    }
+#pragma unroll
+    for (int u = 0; u < U && !whole; ++u) {
       const int k0 = t * 64 + u * STEP + EPP * g;
 #pragma unroll
       for (int r = 0; r < EPP; ++r)
@@ -215,20 +254,19 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
         for (int m = 0; m < MB; ++m) mfma_piece(acc[m][b], f, fx[u][m], Tag<T>());
       }
   }
-  typedef Beside<T, EPP> piece;
   auto store = [&](int m, int j, const float (&s)[EPP]) {
     const int n = n0 + EPP * (4 * g + j), valid = a.n - n;
     if (m * 16 + i >= m_here || valid <= 0) return;
     T *to = static_cast<T *>(a.c) + (size_t)(first + m * 16 + i) * a.c_stride + n;
-    piece p;
+    typename Beside<T, EPP>::vector p;
 #pragma unroll
-    for (int b = 0; b < EPP; ++b) p.v[b] = (T)s[b];
+    for (int b = 0; b < EPP; ++b) p[b] = (T)s[b];
     if (valid >= EPP) {
-      *reinterpret_cast<piece *>(to) = p;
+      store_beside<T, EPP>(to, p);
     } else {
 #pragma unroll
       for (int b = 0; b < EPP - 1; ++b)
-        if (b < valid) to[b] = p.v[b];
+        if (b < valid) to[b] = p[b];
     }
   };
   if (a.share > 1) {

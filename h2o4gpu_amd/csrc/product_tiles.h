@@ -98,15 +98,70 @@ struct OperandTile {
   }
 };
 
+// Words from a buffer, zeros behind its end; all addresses are multiples of 4.
+__device__ __forceinline__ u32x4 buffer_words(const char *from, unsigned size, unsigned at) {
+  u32x4 v = {0, 0, 0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+  v = __builtin_amdgcn_raw_buffer_load_b128(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from), 0, (int)size, 0x00020000), (int)at, 0, 0);
+#endif
+  return v;
+}
+__device__ __forceinline__ unsigned buffer_word(const char *from, unsigned size, unsigned at) {
+  unsigned v = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  v = __builtin_amdgcn_raw_buffer_load_b32(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from), 0, (int)size, 0x00020000), (int)at, 0, 0);
+#endif
+  return v;
+}
+// A piece out of five words, the last beside: it begins `by` bytes, 0 or 2, behind the first.
+__device__ __forceinline__ u32x4 shifted(u32x4 v, unsigned last, unsigned by) {
+  by *= 8;
+  return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], by), __builtin_amdgcn_alignbit(v[2], v[1], by),
+               __builtin_amdgcn_alignbit(v[3], v[2], by), __builtin_amdgcn_alignbit(last, v[3], by)};
+}
+// All bits of a piece's first `elements`.
+template <typename T>
+__device__ __forceinline__ u32x4 first_of(int elements) {
+  u32x4 keep;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int bytes = elements * (int)sizeof(T) - 4 * i;
+    keep[i] = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : 0xffffu;
+  }
+  return keep;
+}
+
+// A whole piece, from any address that a T may have. The memory unit takes words at multiples of 4 as fast as at multiples
+// of 16, and others three times slower: of 2-byte elements that lie between words (`halves`: some of the caller's do), the
+// words that hold them are loaded and shifted. No word is touched that holds none of the piece.
+template <typename T>
+__device__ __forceinline__ u32x4 load_whole(const T *p, bool halves) {
+  struct __attribute__((packed, aligned(4))) Words {
+    u32x4 v;
+  };
+  if constexpr (sizeof(T) == 4) {
+    return reinterpret_cast<const Words *>(p)->v;
+  } else {
+    if (!halves) return reinterpret_cast<const Words *>(p)->v;
+    const size_t at = (size_t)p;
+    return shifted(reinterpret_cast<const Words *>(at & ~(size_t)3)->v,
+                   *reinterpret_cast<const unsigned *>((at + 14) & ~(size_t)3), (unsigned)(at & 2));
+  }
+}
+// Whether some row of a matrix begins between words.
+template <typename T>
+inline bool between_words(const void *p, size_t stride) {
+  return sizeof(T) == 2 && (((uintptr_t)p & 3) || (stride & 1));
+}
+
 // A piece of which the first `valid` elements exist, zeros behind (and all zeros for valid <= 0), from any address
 // that a T may have.
 template <typename T>
 __device__ __forceinline__ u32x4 load_piece(const T *p, int valid) {
   constexpr int EPP = 16 / (int)sizeof(T);
-  struct __attribute__((packed, aligned(sizeof(T)))) Any {
-    u32x4 v;
-  };
-  if (valid >= EPP) return reinterpret_cast<const Any *>(p)->v;
+  if (valid >= EPP) return load_whole(p, true);
   u32x4 out = {0, 0, 0, 0};
   if (valid > 0) {
 #pragma unroll
@@ -184,16 +239,35 @@ inline int in_launches(size_t blocks, F launch) {
   return H2O4GPU_KMEANS_OK;
 }
 
-// N values side by side, at any address that a T may have; the first `valid` of them.
+// N values (of 4 or 8) side by side, at any address that a T may have: 2-byte ones that begin between words as one, the
+// words behind it, and the last.
 template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Beside {
+struct Beside {
   typedef T vector __attribute__((ext_vector_type(N)));
-  vector v;
 };
+template <typename T, int N>
+__device__ __forceinline__ void store_beside(T *to, typename Beside<T, N>::vector v) {
+  constexpr int WORDS = N * (int)sizeof(T) / 4;
+  typedef unsigned words __attribute__((ext_vector_type(WORDS)));
+  struct __attribute__((packed, aligned(4))) Words {
+    words v;
+  };
+  const words w = __builtin_bit_cast(words, v);
+  if (sizeof(T) == 4 || !((size_t)to & 2)) {
+    reinterpret_cast<Words *>(to)->v = w;
+    return;
+  }
+  unsigned short *ends = reinterpret_cast<unsigned short *>(to);
+  ends[0] = (unsigned short)w[0];
+  unsigned *between = reinterpret_cast<unsigned *>(to + 1);
+#pragma unroll
+  for (int i = 0; i < WORDS - 1; ++i) between[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], 16);
+  ends[N - 1] = (unsigned short)(w[WORDS - 1] >> 16);
+}
 template <typename T>
 __device__ __forceinline__ void store_four(T *c, f32x4 v, int valid) {
   if (valid >= 4) {
-    reinterpret_cast<Beside<T, 4> *>(c)->v = typename Beside<T, 4>::vector{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    store_beside<T, 4>(c, typename Beside<T, 4>::vector{(T)v[0], (T)v[1], (T)v[2], (T)v[3]});
   } else {
 #pragma unroll
     for (int j = 0; j < 3; ++j)

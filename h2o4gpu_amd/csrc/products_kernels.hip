@@ -23,13 +23,14 @@ struct ProductArgs {
   int n_tiles;
 };
 
-// Any strides and alignment: pieces come through registers, masked at the edges. Two stages in LDS.
-template <typename T, Kind KIND, int BM, int BN, int WM, int WN>
+// Any alignment: pieces come through registers, masked at the edges. Two stages in LDS. HALVES: some row of an operand of
+// 2-byte elements begins between two words.
+template <typename T, Kind KIND, bool HALVES, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   constexpr bool XC = KIND == DWEIGHTS, WC = KIND != FORWARD;
   typedef OperandTile<T, BM, XC> TX;
   typedef OperandTile<T, BN, WC> TW;
-  constexpr int THREADS = WM * WN * 64, KS = TX::KS;
+  constexpr int THREADS = WM * WN * 64, KS = TX::KS, EPP = TX::EPP;
   constexpr int PX = TX::SLOTS / THREADS, PW = TW::SLOTS / THREADS;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int STAGE = (BM + BN) * 128;
@@ -64,27 +65,81 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   const int n_here = a.n - n0 < BN ? a.n - n0 : BN;
   w += WC ? (size_t)n0 : (size_t)n0 * a.w_stride;
 
+  // A stage of an operand: its first word, its size up to the last word that holds any of it, and what its first element
+  // lies behind the first word. What is behind the end is not read. Behind the last k may lie anything (the next row, or
+  // the half of the last word that is not the operand's): settle() takes it out; of rows and columns that do not exist
+  // nothing is stored.
+  struct Stage {
+    const char *from;
+    unsigned size, behind;
+  };
+  auto stage_of = [&](const T *first_element, size_t lines, size_t stride, size_t side) {
+    const size_t at = (size_t)first_element;
+    const unsigned behind = (unsigned)(at & 3);
+    const unsigned size = lines > 0 && side > 0 ? (unsigned)(((lines - 1) * stride + side) * sizeof(T)) + behind : 0;
+    return Stage{(const char *)(at - behind), (size + 3) & ~3u, behind};
+  };
+  const auto stage_x = [&](int k0) {
+    const int left = k_end - k0;
+    return XC ? stage_of(x + (size_t)k0 * a.x_stride, left < KS ? left : KS, a.x_stride, m_here)
+              : stage_of(x + k0, m_here, a.x_stride, left);
+  };
+  const auto stage_w = [&](int k0) {
+    const int left = k_end - k0;
+    return WC ? stage_of(w + (size_t)k0 * a.w_stride, left < KS ? left : KS, a.w_stride, n_here)
+              : stage_of(w + k0, n_here, a.w_stride, left);
+  };
   u32x4 px[PX], pw[PW];
-  auto load = [&](int k0) {
+  unsigned last_x[HALVES ? PX : 1], last_w[HALVES ? PW : 1];
+  auto load = [&](int k0) __attribute__((always_inline)) {
+    const Stage sx = stage_x(k0), sw = stage_w(k0);
 #pragma unroll
     for (int i = 0; i < PX; ++i) {
       int r, k;
       TX::place(i * THREADS + tid, r, k);
-      k += k0;
-      if (XC)
-        px[i] = load_piece(x + (size_t)k * a.x_stride + r, k < k_end ? m_here - r : 0);
-      else
-        px[i] = load_piece(x + (size_t)r * a.x_stride + k, r < m_here ? k_end - k : 0);
+      const unsigned at = (unsigned)((XC ? k * a.x_stride + r : r * a.x_stride + k) * sizeof(T)) + sx.behind;
+      px[i] = buffer_words(sx.from, sx.size, HALVES ? at & ~3u : at);
+      if (HALVES) last_x[i] = buffer_word(sx.from, sx.size, (at + 14) & ~3u);
     }
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       int r, k;
       TW::place(i * THREADS + tid, r, k);
-      k += k0;
-      if (WC)
-        pw[i] = load_piece(w + (size_t)k * a.w_stride + r, k < k_end ? n_here - r : 0);
-      else
-        pw[i] = load_piece(w + (size_t)r * a.w_stride + k, r < n_here ? k_end - k : 0);
+      const unsigned at = (unsigned)((WC ? k * a.w_stride + r : r * a.w_stride + k) * sizeof(T)) + sw.behind;
+      pw[i] = buffer_words(sw.from, sw.size, HALVES ? at & ~3u : at);
+      if (HALVES) last_w[i] = buffer_word(sw.from, sw.size, (at + 14) & ~3u);
+    }
+  };
+  // 2-byte elements that lie between words are shifted, and behind the last k are zeros
+  auto settle = [&](int k0) __attribute__((always_inline)) {
+    if constexpr (HALVES) {
+      const unsigned bx = stage_x(k0).behind, bw = stage_w(k0).behind;
+#pragma unroll
+      for (int i = 0; i < PX; ++i) {
+        int r, k;
+        TX::place(i * THREADS + tid, r, k);
+        px[i] = shifted(px[i], last_x[i], (bx + (unsigned)((XC ? k * a.x_stride + r : r * a.x_stride + k) * 2)) & 2);
+      }
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        int r, k;
+        TW::place(i * THREADS + tid, r, k);
+        pw[i] = shifted(pw[i], last_w[i], (bw + (unsigned)((WC ? k * a.w_stride + r : r * a.w_stride + k) * 2)) & 2);
+      }
+    }
+    if (k0 + KS > k_end) {
+#pragma unroll
+      for (int i = 0; i < PX; ++i) {
+        int r, k;
+        TX::place(i * THREADS + tid, r, k);
+        px[i] &= first_of<T>(XC ? (k < k_end - k0 ? EPP : 0) : k_end - k0 - k);
+      }
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        int r, k;
+        TW::place(i * THREADS + tid, r, k);
+        pw[i] &= first_of<T>(WC ? (k < k_end - k0 ? EPP : 0) : k_end - k0 - k);
+      }
     }
   };
   auto put = [&](char *at) {
@@ -105,6 +160,7 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   const int stages = (k_end + KS - 1) / KS;
   if (stages > 0) {
     load(0);
+    settle(0);
     put(lds);
   }
   __syncthreads();
@@ -126,7 +182,10 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
             if (j < n_blocks) mfma_piece(acc[i][j], fw[j], fx[i], Tag<T>());
         }
     }
-    if (t + 1 < stages) put(lds + ((t + 1) & 1) * STAGE);
+    if (t + 1 < stages) {
+      settle((t + 1) * KS);
+      put(lds + ((t + 1) & 1) * STAGE);
+    }
     __syncthreads();
   }
 
@@ -207,14 +266,17 @@ int join_parts(const ProductArgs &a, hipStream_t stream) {
 
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
+  const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
   const size_t each = a.rows / a.experts, tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.n + 127) / 128);
   // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
-  if (KIND == FORWARD ? each <= 64 || (tiles <= 128 && (double)a.rows * a.n * a.k < 2e9) : KIND == DROWS && each <= 32) {
+  const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
+  if (far || (KIND == FORWARD ? each <= THIN_ROWS || (tiles <= 128 && (double)a.rows * a.n * a.k < 2e9) : KIND == DROWS && each <= 32)) {
     ThinArgs t = {};
     t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
     t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
     t.c_stride = a.c_stride, t.offsets = a.offsets;
     t.experts = a.experts, t.rows = a.rows, t.n = a.n, t.k = a.k;
+    t.halves = halves;
     if (KIND == DROWS) return launch_thin_columns<T>(t, stream);
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
@@ -236,7 +298,10 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
   p.n_tiles = (a.n + BN - 1) / BN;
   KM_TRY(in_launches(m_tiles * p.n_tiles, [&](unsigned first, unsigned blocks) {
     p.first_block = first;
-    hipLaunchKernelGGL((product_kernel<T, KIND, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, p);
+    if (sizeof(T) == 2 && halves)
+      hipLaunchKernelGGL((product_kernel<T, KIND, sizeof(T) == 2, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((product_kernel<T, KIND, false, BM, BN, 2, 2>), dim3(blocks), dim3(256), 0, stream, p);
     return launched();
   }));
   return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
@@ -256,7 +321,7 @@ __global__ __launch_bounds__(256) void align_kernel(const T *in, size_t stride, 
   out[at] = load_piece(in + of * matrix + (row - of * rows) * stride + col, left < 16 ? (int)left : 16);
 }
 
-constexpr size_t MAX_SIDE = (size_t)1 << 30, MAX_MATRIX = (size_t)1 << 38;
+constexpr size_t MAX_SIDE = (size_t)1 << 30;
 
 // What all three have in common. > 0: go on, else the status to return.
 int check(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *offsets) {
@@ -304,7 +369,7 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
 }
 
 KM_API size_t h2o4gpu_experts_product_dweights_workspace(size_t rows, int experts, size_t out, size_t cols) {
-  return check(0, rows, experts, out, cols, "") <= 0 || out * cols > MAX_MATRIX ? 0 : sums_bytes(rows, out, cols);
+  return check(0, rows, experts, out, cols, "") <= 0 ? 0 : sums_bytes(rows, out, cols);
 }
 
 KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols,
@@ -312,9 +377,11 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
                                             const int *d_offsets, void *d_dweights, void *d_workspace,
                                             size_t workspace_bytes, void *stream) {
   if (int rc = check(dtype, rows, experts, out, cols, d_offsets); rc <= 0) return rc;
-  if (out * cols > MAX_MATRIX) return H2O4GPU_KMEANS_EARG;
   const size_t need = sums_bytes(rows, out, cols);
   if (need > workspace_bytes || (need && (!d_workspace || !aligned_to(d_workspace, 16)))) return H2O4GPU_KMEANS_EARG;
+  if (out > H2O4GPU_EXPERTS_MAX_SIDE || cols > H2O4GPU_EXPERTS_MAX_SIDE ||
+      (rows > 1 && (dy_stride > H2O4GPU_EXPERTS_MAX_SIDE || rows_stride > H2O4GPU_EXPERTS_MAX_SIDE)))
+    return H2O4GPU_KMEANS_EARG;
   if (!d_dweights || (rows && (!d_dy || !d_rows)) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,

@@ -383,6 +383,11 @@ def _align(worth, *tensors):
     return tuple(t if _aligned(t) else _copy_aligned(t) for t in tensors)
 
 
+def _near(t):
+    """The matrix with its rows as near to each other as their gradient's kernel takes them."""
+    return t.contiguous() if t.stride(0) > experts_hip.MAX_SIDE and t.shape[0] > 1 else t
+
+
 def _copy_aligned(t):
     each = 16 // t.element_size()
     cols = t.shape[-1]
@@ -443,6 +448,7 @@ class _Product(torch.autograd.Function):
             x = rows
             if worth:
                 dy, x = _align(worth, dy, x)
+            dy, x = _near(dy), _near(x)
             dweights = weights.new_empty(weights.shape)
             need = _sums(count, n_experts, out, cols)
             work = dy.new_empty(need // 4, dtype=torch.float32) if need else None
@@ -471,5 +477,8 @@ def product(rows, weights, order):
                                                             tuple(rows.shape)))
     _no_tangents(rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        if weights.requires_grad and max(weights.shape[1:]) > experts_hip.MAX_SIDE:
+            raise ValueError("matrices of more than %d rows or columns have no gradient, got %s" % (
+                experts_hip.MAX_SIDE, tuple(weights.shape)))
         return _Product.apply(rows, weights, order)
     return _product(rows, weights, order)

@@ -36,6 +36,7 @@ extern "C" {
 #define H2O4GPU_EXPERTS_MAX_EXPERTS 16384
 #define H2O4GPU_EXPERTS_MAX_TOP_K 64
 #define H2O4GPU_CODEBOOK4_MAX_GROUP (1 << 30)
+#define H2O4GPU_EXPERTS_MAX_SIDE (1 << 20)
 
 /* The top_k best experts of every row and their weights.
  * d_scores: rows x experts of `dtype`; element (t, e) lies at t * row_stride + e * expert_stride,
@@ -137,7 +138,8 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
  * most rows. W_e: [out][cols], rows w_stride elements apart, at d_weights + e * expert_stride (0: one
  * matrix for all). Products and sums in float, one rounding at the end.
  * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
- * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none);
+ * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none), out, cols
+ * and both strides at most MAX_SIDE;
  * d_workspace: product_dweights_workspace() bytes, 16-byte aligned (NULL where that is 0). */
 int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
                             size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
