@@ -183,9 +183,9 @@ int launch_thin(ThinArgs &a, hipStream_t stream) {
 // The same where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some k's of
 // its own; element b of all of them is its fragment of a block of 16 columns, EPP apart, so that a wavefront has
 // 16 EPP columns. What comes out for a lane and a j, block by block, is EPP columns side by side again.
-template <typename T, int MB, int WAVES>
+template <typename T, bool HALVES, int MB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
-  constexpr int EPP = 16 / (int)sizeof(T), STEP = 4 * EPP, U = 64 / STEP;  // 64 k a turn
+  constexpr int EPP = 16 / (int)sizeof(T), STEP = 4 * EPP, TURN = 32, U = TURN / STEP;  // k of a turn
   __shared__ f32x4 sums[WAVES][MB * EPP][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4;
@@ -195,7 +195,6 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
   int expert, first, m_here, k = a.k;
   if (!ragged_tile(a.offsets, a.experts, a.rows, 16 * MB, (int)(block / (unsigned)a.n_tiles), expert, first, m_here)) return;
   if (expert == a.experts) k = 0, expert = 0;  // rows without an expert: zeros
-  const int left = a.n - n0 - EPP * i;         // of the lane's columns
   if (a.n <= n0) k = 0;
 
   f32x4 acc[MB][EPP];
@@ -207,52 +206,77 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
 #pragma unroll
   for (int m = 0; m < MB; ++m)
     x[m] = reinterpret_cast<const T *>(a.x + (size_t)(first + (m * 16 + i < m_here ? m * 16 + i : m_here - 1)) * a.x_stride);
-  const char *w = a.w + (size_t)expert * a.w_expert + (size_t)(n0 + EPP * i) * sizeof(T);
-  const int turns = (k + 63) / 64, each = (turns + a.share - 1) / a.share;
+  const size_t w = (size_t)(a.w + (size_t)expert * a.w_expert + (size_t)n0 * sizeof(T));
+  const unsigned behind = (unsigned)(w & 3);  // of the first word
+  const int turns = (k + TURN - 1) / TURN, each = (turns + a.share - 1) / a.share;
   const int begin = part * each, end = begin + each < turns ? begin + each : turns;
-  for (int t = begin; t < end; ++t) {
-    u32x4 fx[U][MB], v[U][EPP];
-    const bool whole = (t + 1) * 64 <= k && n0 + 16 * EPP <= a.n;  // (no branches: all loads are on their way at once)
-    auto all = [&](bool halves) __attribute__((always_inline)) {
+  struct Turn {
+    u32x4 x[U][MB], w[U][EPP];
+    unsigned last[HALVES ? U : 1][EPP];
+  } turn[2];
+  auto load = [&](Turn &f, int t) __attribute__((always_inline)) {
+    const char *from = same_in_all((const char *)(w - behind + (size_t)t * TURN * a.w_stride));
+    const int here = k - t * TURN < TURN ? k - t * TURN : TURN;
+    const unsigned size = ((unsigned)((here - 1) * a.w_stride + (size_t)(a.n - n0) * sizeof(T)) + behind + 3) & ~3u;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k0 = t * 64 + u * STEP + EPP * g;
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int r = 0; r < EPP; ++r) v[u][r] = load_whole(reinterpret_cast<const T *>(w + (size_t)(k0 + r) * a.w_stride), halves);
-#pragma unroll
-        for (int m = 0; m < MB; ++m) fx[u][m] = load_whole(x[m] + k0, halves);
+      for (int r = 0; r < EPP; ++r) {
+        const unsigned at = (unsigned)((u * STEP + EPP * g + r) * a.w_stride) + EPP * i * (unsigned)sizeof(T) + behind;
+        f.w[u][r] = buffer_words(from, size, HALVES ? at & ~3u : at);
+        if (HALVES) f.last[u][r] = buffer_word(from, size, (at + 14) & ~3u);
       }
-    };
-    if (whole) {
-      if (a.halves)
-        all(true);
-      else
-        all(false);
     }
+    // (the last k's of a row of x one by one: behind it may be nothing)
+    if ((t + 1) * TURN <= k) {
 #pragma unroll
-    for (int u = 0; u < U && !whole; ++u) {
-      const int k0 = t * 64 + u * STEP + EPP * g;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int r = 0; r < EPP; ++r)
-        v[u][r] = load_piece(reinterpret_cast<const T *>(w + (size_t)(k0 + r) * a.w_stride), k0 + r < k ? left : 0);
+        for (int m = 0; m < MB; ++m) f.x[u][m] = load_whole(x[m] + t * TURN + u * STEP + EPP * g, HALVES);
+    } else {
 #pragma unroll
-      for (int m = 0; m < MB; ++m) fx[u][m] = load_piece(x[m] + k0, k - k0);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+          f.x[u][m] = load_piece(x[m] + t * TURN + u * STEP + EPP * g, k - (t * TURN + u * STEP + EPP * g));
     }
+  };
+  auto multiply = [&](Turn &f, int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const int k0 = t * TURN + u * STEP + EPP * g;
+#pragma unroll
+      for (int r = 0; r < EPP; ++r) {
+        if (HALVES)
+          f.w[u][r] = shifted(f.w[u][r], f.last[u][r],
+                              (unsigned)((u * STEP + EPP * g + r) * a.w_stride + EPP * i * sizeof(T) + behind) & 2);
+        if (k0 + r >= k) f.w[u][r] = u32x4{0, 0, 0, 0};  // (whatever lies there)
+      }
 #pragma unroll
       for (int b = 0; b < EPP; ++b) {
-        u32x4 f;
+        u32x4 v;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           if constexpr (sizeof(T) == 4)
-            f[d] = v[u][d][b];
+            v[d] = f.w[u][d][b];
           else
-            f[d] = __builtin_amdgcn_perm(v[u][2 * d + 1][b / 2], v[u][2 * d][b / 2], b & 1 ? 0x07060302u : 0x05040100u);
+            v[d] = __builtin_amdgcn_perm(f.w[u][2 * d + 1][b / 2], f.w[u][2 * d][b / 2], b & 1 ? 0x07060302u : 0x05040100u);
         }
 #pragma unroll
-        for (int m = 0; m < MB; ++m) mfma_piece(acc[m][b], f, fx[u][m], Tag<T>());
+        for (int m = 0; m < MB; ++m) mfma_piece(acc[m][b], v, f.x[u][m], Tag<T>());
       }
+    }
+  };
+  if (begin < end) {
+    load(turn[0], begin);
+    for (int t = begin;; t += 2) {  // a turn is on its way while one is multiplied
+      if (t + 1 < end) load(turn[1], t + 1);
+      multiply(turn[0], t);
+      if (t + 1 >= end) break;
+      if (t + 2 < end) load(turn[0], t + 2);
+      multiply(turn[1], t + 1);
+      if (t + 2 >= end) break;
+    }
   }
   auto store = [&](int m, int j, const float (&s)[EPP]) {
     const int n = n0 + EPP * (4 * g + j), valid = a.n - n;
@@ -301,12 +325,15 @@ template <typename T>
 int launch_thin_columns(ThinArgs &a, hipStream_t stream) {
   auto launch = [&](auto mb, auto waves) {
     constexpr int MB = decltype(mb)::value, WAVES = decltype(waves)::value, COLS = 16 * (16 / (int)sizeof(T));
-    const int turns = (a.k + 63) / 64;
+    const int turns = (a.k + 31) / 32;
     a.share = turns >= WAVES ? WAVES : turns > 2 ? 4 : turns > 1 ? 2 : 1;
     a.n_tiles = (a.n + COLS * (WAVES / a.share) - 1) / (COLS * (WAVES / a.share));
     return in_launches(ragged_tiles(a.experts, a.rows, 16 * MB) * a.n_tiles, [&](unsigned first, unsigned blocks) {
       a.first_block = first;
-      hipLaunchKernelGGL((thin_columns_kernel<T, MB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+      if (sizeof(T) == 2 && a.halves)
+        hipLaunchKernelGGL((thin_columns_kernel<T, sizeof(T) == 2, MB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+      else
+        hipLaunchKernelGGL((thin_columns_kernel<T, false, MB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
       return launched();
     });
   };

@@ -324,9 +324,10 @@ __global__ __launch_bounds__(256) void align_kernel(const T *in, size_t stride, 
 constexpr size_t MAX_SIDE = (size_t)1 << 30;
 
 // What all three have in common. > 0: go on, else the status to return.
-int check(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *offsets) {
+int check(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *offsets, size_t w_stride = 0) {
   if (!known_type(dtype) || experts < 1 || experts > H2O4GPU_EXPERTS_MAX_EXPERTS) return H2O4GPU_KMEANS_EARG;
-  if (out < 1 || cols < 1 || out > MAX_SIDE || cols > MAX_SIDE || rows > (size_t)INT_MAX - 65536 || !offsets)
+  if (out < 1 || cols < 1 || out > MAX_SIDE || cols > MAX_SIDE || rows > (size_t)INT_MAX - 65536 || !offsets ||
+      (out > 1 && w_stride > ((size_t)1 << 23)))  // (64 rows of a matrix are within a buffer's reach)
     return H2O4GPU_KMEANS_EARG;
   return 1;
 }
@@ -339,7 +340,7 @@ using namespace kmhip;
 KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
                                    size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                                    const int *d_offsets, void *d_y, size_t y_stride, void *stream) {
-  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "");
+  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "", w_stride);
       rc <= 0)
     return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
@@ -356,7 +357,8 @@ KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t o
 KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
                                          size_t dy_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                                          const int *d_offsets, void *d_drows, size_t drows_stride, void *stream) {
-  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : ""); rc <= 0) return rc;
+  if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "", w_stride); rc <= 0)
+    return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
   if (!d_dy || !d_weights || !d_drows || !fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
       !fits(rows, cols, drows_stride))

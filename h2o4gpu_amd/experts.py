@@ -356,6 +356,8 @@ def _matrices(weights):
         stride = cols
     elif stride < cols:
         raise ValueError("the rows of weights overlap (strides %s)" % (weights.stride(),))
+    elif stride > 1 << 23:
+        raise ValueError("the rows of weights are more than 2^23 elements apart (strides %s)" % (weights.stride(),))
     return weights.data_ptr(), expert_stride, stride
 
 

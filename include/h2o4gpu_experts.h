@@ -135,7 +135,7 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
 /* The experts' own products, rows in expert order: d_y[p] = W_e d_rows[p] for the rows p in
  * [d_offsets[e], d_offsets[e + 1]) of each expert e, zeros for those behind d_offsets[experts] (what
  * lies there is not read). d_offsets [experts + 1] as experts_sort writes it: from 0, ascending, at
- * most rows. W_e: [out][cols], rows w_stride elements apart, at d_weights + e * expert_stride (0: one
+ * most rows. W_e: [out][cols], rows w_stride (at most 2^23) elements apart, at d_weights + e * expert_stride (0: one
  * matrix for all). Products and sums in float, one rounding at the end.
  * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
  * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none), out, cols
