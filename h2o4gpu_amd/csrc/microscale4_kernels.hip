@@ -170,12 +170,13 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   const size_t tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.out + 127) / 128);
   const bool reached = (!a.order || x_rows * pitch < BUFFER_BYTES) && pitch < BUFFER_BYTES / 512;
   // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
-  if (each <= 64 || !reached || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
+  if (each <= THIN_ROWS<bfloat16_t> || !reached || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);
     t.c_stride = a.y_stride, t.order = a.order, t.offsets = a.offsets, t.top_k = a.top_k;
     t.experts = a.experts, t.rows = a.rows, t.n = a.out, t.k = (int)((a.cols + 127) / 128 * 32);
+    if (!a.experts && a.rows > 16 && a.rows <= 64 && a.cols <= 8192 && a.out >= 4096) return launch_kept<T>(t, stream);
     return launch_thin<Four, T, true>(t, stream);
   }
   PipeArgs p = {};

@@ -7,7 +7,10 @@
 
 namespace kmhip {
 
-constexpr size_t THIN_ROWS = 64;  // of an expert, on average
+// Of an expert, on average: beyond, tiles of 128 x 128 are faster (27 experts of 5184 x 2504, 24 rows each: bfloat16 185 us
+// against 199, 4 bits 63 against 68, float32 709 against 423; 40 rows 193, 63 and 709 against 263, 99 and 566).
+template <typename T>
+constexpr size_t THIN_ROWS = sizeof(T) == 4 ? 48 : 16;
 
 struct ThinArgs {
   const char *x, *w;
@@ -154,6 +157,106 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
     for (int v = 1; v < a.share; ++v) s += sums[wave - part + v][b][lane];
     store(b, s);
   }
+}
+
+// One matrix in 4 bits, x of 17 to 64 rows and at most 8192 columns: a workgroup keeps its part of x, which it would read
+// from L2 for every 32 rows of the matrix (33 rows of 8190 times 11003: 29 us that way and 23 this, of which the
+// matrix takes 10), and takes 16 rows after others, the next of which are on their way while these are multiplied.
+template <typename OUT, int MB>
+__global__ __launch_bounds__(512) void kept_kernel(ThinArgs a) {
+  constexpr int WAVES = 8, U = 4, TURNS = 2;
+  __shared__ f32x4 sums[2][WAVES][MB][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const int steps = (a.k + 31) / 32;  // of 64 bytes a row
+  const int first = wave * TURNS * U;  // of this wavefront's
+  u32x4 fx[TURNS][U][MB], fw[2][TURNS][U];
+  unsigned sx[TURNS][MB], sw[2][TURNS];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const size_t row = m * 16 + i < a.rows ? m * 16 + i : a.rows - 1;
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = first + t * U + u;
+        fx[t][u][m] = s < steps ? *reinterpret_cast<const u32x4 *>(a.x + row * a.x_stride + (size_t)s * 64 + g * 16)
+                                : u32x4{0, 0, 0, 0};
+      }
+      sx[t][m] = first + t * U < steps ? *reinterpret_cast<const unsigned *>(a.x_scales + row * a.scales_stride +
+                                                                            (size_t)(wave * TURNS + t) * 16 + 4 * g)
+                                       : 0;
+    }
+  }
+  auto load = [&](auto b, int tile) {
+    constexpr int B = decltype(b)::value;
+    const int n = tile * 16 + i;
+    const size_t row = n < a.n ? n : a.n - 1;
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = first + t * U + u;
+        if (s < steps) fw[B][t][u] = *reinterpret_cast<const u32x4 *>(a.w + row * a.w_stride + (size_t)s * 64 + g * 16);
+      }
+      if (first + t * U < steps)
+        sw[B][t] = *reinterpret_cast<const unsigned *>(a.w_scales + row * a.scales_stride + (size_t)(wave * TURNS + t) * 16 +
+                                                       4 * g);
+    }
+  };
+  auto multiply = [&](auto b, int tile) {
+    constexpr int B = decltype(b)::value;
+    f32x4 acc[MB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+      auto step = [&](auto number) {
+        constexpr int S = decltype(number)::value;
+        if (first + t * U + S < steps) {
+#pragma unroll
+          for (int m = 0; m < MB; ++m) mfma_four<S>(acc[m], fw[B][t][S], fx[t][S][m], sw[B][t], sx[t][m]);
+        }
+      };
+      step(Int<0>());
+      step(Int<1>());
+      step(Int<2>());
+      step(Int<3>());
+    }
+#pragma unroll
+    for (int m = 0; m < MB; ++m) sums[B][wave][m][lane] = acc[m];
+    __syncthreads();
+    if (wave < MB) {
+      f32x4 s = sums[B][0][wave][lane];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) s += sums[B][v][wave][lane];
+      const int m = wave * 16 + i, n = tile * 16 + 4 * g;
+      if (m < a.rows) store_four(static_cast<OUT *>(a.c) + (size_t)m * a.c_stride + n, s, a.n - n);
+    }
+  };
+  int tile = blockIdx.x;
+  load(Int<0>(), tile);
+  for (;;) {
+    const int next = tile + (int)gridDim.x, after = next + (int)gridDim.x;
+    if (next < a.n_tiles) load(Int<1>(), next);
+    multiply(Int<0>(), tile);
+    if (next >= a.n_tiles) break;
+    if (after < a.n_tiles) load(Int<0>(), after);
+    multiply(Int<1>(), next);
+    if (after >= a.n_tiles) break;
+    tile = after;
+  }
+}
+
+template <typename OUT>
+int launch_kept(ThinArgs &a, hipStream_t stream) {
+  a.n_tiles = (a.n + 15) / 16;
+  const unsigned blocks = a.n_tiles < 256 ? a.n_tiles : 256;
+  auto launch = [&](auto mb) {
+    hipLaunchKernelGGL((kept_kernel<OUT, decltype(mb)::value>), dim3(blocks), dim3(512), 0, stream, a);
+    return launched();
+  };
+  return a.rows <= 32 ? launch(Int<2>()) : a.rows <= 48 ? launch(Int<3>()) : launch(Int<4>());
 }
 
 template <typename ELEMENT, typename OUT, bool ALIGNED>

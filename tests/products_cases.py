@@ -43,7 +43,9 @@ def _fours():
     for i, (rows, n, cols) in enumerate(((1, 1, 1), (1, 40, 33), (1, 300, 4096), (2, 17, 100), (5, 64, 256), (16, 128, 512), (17, 33, 513),
                                          (33, 200, 777), (64, 96, 1024), (65, 40, 2176), (130, 24, 520), (128, 128, 768),
                                          (200, 130, 260), (300, 520, 96), (260, 257, 1300), (1, 8, 9000), (600, 700, 288),
-                                         (513, 384, 1536), (1030, 129, 2560), (128, 4000, 128))):
+                                         (513, 384, 1536), (1030, 129, 2560), (128, 4000, 128),
+                                         (33, 4100, 777), (64, 4096, 8192), (20, 5000, 500), (47, 4099, 2100), (17, 4097, 7700),
+                                         (60, 9000, 33))):
         for dtype in TYPES:
             out.append(dict(op="four", rows=rows, out=n, cols=cols, dtype=dtype, made=("quantize", "codes")[i % 2]))
     return out
