@@ -411,7 +411,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
     }
   };
   unsigned x_size = 0, w_size = 0;
-  auto whole = [](int elements) { return (unsigned)(elements + EPP - 1) / EPP * 16; };  // bytes of their pieces
+  auto whole = [](int elements) { return (unsigned)(elements * SIZE + 3) & ~3u; };  // bytes of their words
   auto size_up = [&]() {  // of the stage that is loaded now
     const int k_here = in_left < KS ? in_left : KS;
     x_size = k_here <= 0 ? 0

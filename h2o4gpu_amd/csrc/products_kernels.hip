@@ -281,7 +281,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (rows_aligned<T>(a) && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : each > THIN_ROWS<T>) && a.n >= 128) {
+  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : each > THIN_ROWS<T>) && a.n >= 128) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);

@@ -368,8 +368,8 @@ def _sums(rows, n_experts, out, cols):
 
 def _aligned(t):
     """Whether all rows of a matrix, or of several, begin at multiples of 16 bytes."""
-    each = 16 // t.element_size()
-    return t.data_ptr() % 16 == 0 and all(s % each == 0 for s in t.stride()[:-1])
+    each = 4 // t.element_size()
+    return t.data_ptr() % 4 == 0 and all(s % each == 0 for s in t.stride()[:-1])
 
 
 def _align(worth, *tensors):
