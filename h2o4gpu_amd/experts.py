@@ -366,23 +366,22 @@ def _sums(rows, n_experts, out, cols):
     return experts_hip.lib().h2o4gpu_experts_product_dweights_workspace(rows, n_experts, out, cols)
 
 
-def _aligned(t):
-    """Whether all rows of a matrix, or of several, begin at multiples of 16 bytes."""
+def _at_words(t):
+    """Whether all rows of a matrix, or of several, begin at multiples of 4 bytes."""
     each = 4 // t.element_size()
     return t.data_ptr() % 4 == 0 and all(s % each == 0 for s in t.stride()[:-1])
 
 
 def _align(worth, *tensors):
-    """The operands of a product, copied to rows that begin at multiples of 16 bytes where they do not and the
-    product is long enough. The kernels for such rows take a 16-bit product in a fifth of the time: about 3.5 us
-    less for 10^9 operations, while a copy takes 6 us and 1 us for every 2.2 MB (11044 x 5823, 6 experts: 230 us a
-    copy, 580 us less a product)."""
-    if worth < 2e9:
+    """The operands of a product, copied to rows that begin at multiples of 16 bytes where some begin between words
+    and the product is long enough. The kernel for rows at words is faster by 1.5 us and more for 10^9 operations, a
+    copy takes 6 us and 1 us for every 1.8 MB. 32 experts' matrices of 2049 x 2047, bfloat16, with copies and without:
+    1024 rows each 458 and 651 us, 256 rows each 258 and 213; the matrices' gradient, where only rows are copied, of
+    256 rows each 179 and 285, of 128 144 and 230."""
+    odd = [t for t in tensors if not _at_words(t)]
+    if not odd or 1.5e-9 * worth < sum(6 + t.numel() * t.element_size() / 1.8e6 for t in odd):
         return tensors
-    odd = [t for t in tensors if not _aligned(t)]
-    if not odd or 3.5e-9 * worth < sum(6 + t.numel() * t.element_size() / 2.2e6 for t in odd):
-        return tensors
-    return tuple(t if _aligned(t) else _copy_aligned(t) for t in tensors)
+    return tuple(t if _at_words(t) else _copy_aligned(t) for t in tensors)
 
 
 def _near(t):
@@ -404,7 +403,7 @@ def _copy_aligned(t):
 def _worth(rows, weights):
     """Operations of a product, where large tiles of 16-bit numbers may take it; 0 where they may not."""
     n_experts, out, cols = weights.shape
-    if weights.dtype == torch.float32 or rows.shape[0] < 128 * n_experts or min(out, cols) < 128:
+    if weights.dtype == torch.float32 or rows.shape[0] < 64 * n_experts or min(out, cols) < 128:
         return 0
     return 2.0 * rows.shape[0] * out * cols
 
@@ -437,19 +436,8 @@ class _Product(torch.autograd.Function):
         n_experts, out, cols = weights.shape
         code, count, worth = _TYPES[dy.dtype], dy.shape[0], _worth(rows, weights)
         drows = dweights = None
-        if ctx.needs_input_grad[0]:
-            w = weights
-            if worth:
-                dy, w = _align(worth * (2 if ctx.needs_input_grad[1] else 1), dy, w)
-            drows = rows.new_empty(rows.shape)
-            _call(dy.device.index, "h2o4gpu_experts_product_drows", code, count, n_experts, out, cols, *_rows("dy", dy),
-                  *_matrices(w), order._offsets_ptr, drows.data_ptr(), cols)
-            del w
-            drows = _once(drows, weights, given)
         if ctx.needs_input_grad[1]:
-            x = rows
-            if worth:
-                dy, x = _align(worth, dy, x)
+            dy, x = _align(worth, dy, rows) if worth else (dy, rows)
             dy, x = _near(dy), _near(x)
             dweights = weights.new_empty(weights.shape)
             need = _sums(count, n_experts, out, cols)
@@ -457,7 +445,14 @@ class _Product(torch.autograd.Function):
             _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols,
                   *_rows("dy", dy), *_rows("rows", x), order._offsets_ptr, dweights.data_ptr(),
                   work.data_ptr() if need else None, need)
+            del x, work
             dweights = _once(dweights, rows, given)
+        if ctx.needs_input_grad[0]:
+            dy, w = _align(worth, dy, weights) if worth else (dy, weights)
+            drows = rows.new_empty(rows.shape)
+            _call(dy.device.index, "h2o4gpu_experts_product_drows", code, count, n_experts, out, cols, *_rows("dy", dy),
+                  *_matrices(w), order._offsets_ptr, drows.data_ptr(), cols)
+            drows = _once(drows, weights, given)
         return drows, dweights, None
 
 
