@@ -166,11 +166,9 @@ struct FourArgs {
 
 template <typename T>
 int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
-  const size_t pitch = codes_pitch(a.cols), each = a.rows / (a.experts ? a.experts : 1);
-  const size_t tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.out + 127) / 128);
+  const size_t pitch = codes_pitch(a.cols);
   const bool reached = (!a.order || x_rows * pitch < BUFFER_BYTES) && pitch < BUFFER_BYTES / 512;
-  // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
-  if (each <= THIN_ROWS<bfloat16_t> || !reached || (tiles <= 128 && (double)a.rows * a.out * a.cols < 8e9)) {
+  if (!reached || few_rows<Four>(a.rows, a.experts, a.out)) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);

@@ -7,10 +7,19 @@
 
 namespace kmhip {
 
-// Of an expert, on average: beyond, tiles of 128 x 128 are faster (27 experts of 5184 x 2504, 24 rows each: bfloat16 185 us
-// against 199, 4 bits 63 against 68, float32 709 against 423; 40 rows 193, 63 and 709 against 263, 99 and 566).
-template <typename T>
-constexpr size_t THIN_ROWS = sizeof(T) == 4 ? 48 : 16;
+// Whether a product is one of few rows: of an expert at most 16 (float32: 48) on average, beyond which tiles of 128 x 128
+// are faster (27 experts of 5184 x 2504, 24 rows each: bfloat16 185 us against 199, 4 bits 63 against 68, float32 709
+// against 423; 40 rows 193, 63 and 709 against 263, 99 and 566), or so few that the workgroups of 64 rows times 32 of the
+// matrix are about as many as the CUs. Such tiles would be too few, and each has all of the columns: in one matrix of
+// 2048 x 8192, 200 rows take 45 us here and 77 there, float16; 400 (432 workgroups) 89 and 77. In 4 bits and in float32 a
+// tile's turn takes as long as three of these (4 bits, 400 rows 32 and 56 us, 800 60 and 55; float32 of 2048 x 4096, 400
+// rows 114 and 244, 800 219 and 245).
+template <typename ELEMENT>
+bool few_rows(int rows, int experts, int n) {
+  constexpr bool HALF = sizeof(ELEMENT) == 2, FLOAT = sizeof(ELEMENT) == 4;
+  const int matrices = experts ? experts : 1;
+  return rows / matrices <= (FLOAT ? 48 : 16) || (rows / 64.0 + matrices / 2.0) * ((n + 31) / 32) <= (HALF ? 320 : 768);
+}
 
 struct ThinArgs {
   const char *x, *w;
@@ -311,6 +320,7 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
     x[m] = reinterpret_cast<const T *>(a.x + (size_t)(first + (m * 16 + i < m_here ? m * 16 + i : m_here - 1)) * a.x_stride);
   const size_t w = (size_t)(a.w + (size_t)expert * a.w_expert + (size_t)n0 * sizeof(T));
   const unsigned behind = (unsigned)(w & 3);  // of the first word
+  const int n_here = a.n - n0 < 16 * EPP ? a.n - n0 : 16 * EPP;
   const int turns = (k + TURN - 1) / TURN, each = (turns + a.share - 1) / a.share;
   const int begin = part * each, end = begin + each < turns ? begin + each : turns;
   struct Turn {
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
   auto load = [&](Turn &f, int t) __attribute__((always_inline)) {
     const char *from = same_in_all((const char *)(w - behind + (size_t)t * TURN * a.w_stride));
     const int here = k - t * TURN < TURN ? k - t * TURN : TURN;
-    const unsigned size = ((unsigned)((here - 1) * a.w_stride + (size_t)(a.n - n0) * sizeof(T)) + behind + 3) & ~3u;
+    const unsigned size = ((unsigned)((here - 1) * a.w_stride + (size_t)n_here * sizeof(T)) + behind + 3) & ~3u;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll

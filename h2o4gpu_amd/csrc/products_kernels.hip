@@ -267,10 +267,9 @@ int join_parts(const ProductArgs &a, hipStream_t stream) {
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
   const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
-  const size_t each = a.rows / a.experts, tiles = ragged_tiles(a.experts, a.rows, 128) * (((size_t)a.n + 127) / 128);
-  // few rows of an expert, or few tiles, of which none would have as many wavefronts on its columns
+  const int each = a.rows / a.experts;
   const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
-  if (far || (KIND == FORWARD ? each <= THIN_ROWS<T> || (tiles <= 128 && (double)a.rows * a.n * a.k < 2e9) : KIND == DROWS && each <= 32)) {
+  if (KIND != DWEIGHTS && (far || (KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= 32))) {
     ThinArgs t = {};
     t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
     t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
@@ -281,7 +280,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : each > THIN_ROWS<T>) && a.n >= 128) {
+  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : true) && a.n >= 128) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
