@@ -23,18 +23,22 @@ struct ProductArgs {
   int n_tiles;
 };
 
-// Any alignment: pieces come through registers, masked at the edges. Two stages in LDS. HALVES: some row of an operand of
-// 2-byte elements begins between two words.
+// Any alignment and any sizes: pieces come through registers, masked at the edges, the next stage's while this one is
+// multiplied. A wavefront's shifts and masks take about as long as its products, so a CU has three workgroups of 2-byte
+// elements, with one buffer of LDS each: 28800 rows of 300 experts of 777 x 1001 take 195 us, with two buffers, two
+// workgroups, 205 (their matrices' gradient 304 and 339); 4096 rows of 8 experts of 2049 x 4047 214 and 242. Of float32,
+// which the matrix instructions bound, it is two: 64000 rows of 16 experts of 96 x 1024 118 us, with one buffer 127 (145 and
+// 180). HALVES: some row of an operand of 2-byte elements begins between two words.
 template <typename T, Kind KIND, bool HALVES, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 4 ? 2 : 3) void product_kernel(ProductArgs a) {
   constexpr bool XC = KIND == DWEIGHTS, WC = KIND != FORWARD;
   typedef OperandTile<T, BM, XC> TX;
   typedef OperandTile<T, BN, WC> TW;
   constexpr int THREADS = WM * WN * 64, KS = TX::KS, EPP = TX::EPP;
   constexpr int PX = TX::SLOTS / THREADS, PW = TW::SLOTS / THREADS;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int STAGE = (BM + BN) * 128;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  constexpr int STAGE = (BM + BN) * 128, BUFFERS = sizeof(T) == 4 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) char lds[BUFFERS * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned block = a.first_block + blockIdx.x, number = block / (unsigned)a.n_tiles;
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
   }
   __syncthreads();
   for (int t = 0; t < stages; ++t) {
-    const char *at = lds + (t & 1) * STAGE;
+    const char *at = lds + (BUFFERS == 2 ? (t & 1) * STAGE : 0);
     if (t + 1 < stages) load((t + 1) * KS);
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -182,9 +186,10 @@ __global__ __launch_bounds__(WM *WN * 64) void product_kernel(ProductArgs a) {
             if (j < n_blocks) mfma_piece(acc[i][j], fw[j], fx[i], Tag<T>());
         }
     }
+    if (BUFFERS == 1) __syncthreads();
     if (t + 1 < stages) {
       settle((t + 1) * KS);
-      put(lds + ((t + 1) & 1) * STAGE);
+      put(lds + (BUFFERS == 2 ? ((t + 1) & 1) * STAGE : 0));
     }
     __syncthreads();
   }
@@ -210,27 +215,25 @@ template <typename T>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float *sums, const int *offsets, int experts, int part,
                                                          size_t size, T *c) {
   const int window = blockIdx.y;
-  int lo = 0, n = experts;  // the last expert that begins within or before these rows
-  while (n > 1) {
-    const int half = n / 2;
-    if ((long long)offsets[lo + half] < (long long)(window + 1) * part)
-      lo += half, n -= half;
-    else
-      n = half;
-  }
+  const long long end = (long long)(window + 1) * part;  // the last expert that begins within or before these rows
+  const int lo = last_below(offsets, experts, end < INT_MAX ? (int)end - 1 : INT_MAX);
   const int begin = offsets[lo], rows = offsets[lo + 1] - begin;
   if (begin / part != window || rows <= part) return;
-  const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= size) return;
-  const int valid = size - at < 4 ? (int)(size - at) : 4;
-  f32x4 total = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; (long long)j * part < rows; ++j) {
-    const float *from = sums + (size_t)(2 * (window + j) + (j == 0)) * size + at;
+  const int parts = (rows + part - 1) / part;
+  const float *from = sums + (size_t)(2 * window + 1) * size + at;  // of the first part; then every second
+  float total = *from;
+  from += size;
+  for (int j = 1; j < parts; j += 8) {  // (eight loads on their way at once)
+    float next[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < valid) total[i] += from[i];
+    for (int i = 0; i < 8; ++i) next[i] = j + i < parts ? from[(size_t)2 * (j + i - 1) * size] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < parts) total += next[i];
   }
-  store_four(c + (size_t)lo * size + at, total, valid);
+  c[(size_t)lo * size + at] = (T)total;
 }
 
 // Whether every row of both operands begins at a multiple of 16 bytes, within the reach of a buffer. Then their pieces of
@@ -258,7 +261,7 @@ size_t sums_bytes(size_t rows, size_t out, size_t cols) {
 template <typename T>
 int join_parts(const ProductArgs &a, hipStream_t stream) {
   if (a.rows <= a.part) return H2O4GPU_KMEANS_OK;
-  const size_t blocks = (a.c_expert + 1023) / 1024;
+  const size_t blocks = (a.c_expert + 255) / 256;
   hipLaunchKernelGGL((join_parts_kernel<T>), dim3((unsigned)blocks, (unsigned)(a.rows / a.part + 1)), dim3(256), 0, stream,
                      a.sums, a.offsets, a.experts, a.part, a.c_expert, static_cast<T *>(a.c));
   return launched();
@@ -280,7 +283,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : true) && a.n >= 128) {
+  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : true) && a.n >= (sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16)) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
