@@ -15,10 +15,12 @@ namespace kmhip {
 // tile's turn takes as long as three of these (4 bits, 400 rows 32 and 56 us, 800 60 and 55; float32 of 2048 x 4096, 400
 // rows 114 and 244, 800 219 and 245).
 template <typename ELEMENT>
+constexpr int FEW = sizeof(ELEMENT) == 4 ? 48 : 16;
+template <typename ELEMENT>
 bool few_rows(int rows, int experts, int n) {
-  constexpr bool HALF = sizeof(ELEMENT) == 2, FLOAT = sizeof(ELEMENT) == 4;
+  constexpr int MOST = sizeof(ELEMENT) == 2 ? 320 : 768;
   const int matrices = experts ? experts : 1;
-  return rows / matrices <= (FLOAT ? 48 : 16) || (rows / 64.0 + matrices / 2.0) * ((n + 31) / 32) <= (HALF ? 320 : 768);
+  return rows / matrices <= FEW<ELEMENT> || (rows / 64.0 + matrices / 2.0) * ((n + 31) / 32) <= MOST;
 }
 
 struct ThinArgs {

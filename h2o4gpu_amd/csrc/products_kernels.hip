@@ -245,16 +245,26 @@ bool rows_aligned(const ProductArgs &a) {
          a.w_expert % EPP == 0 && a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
 }
 
-// Rows of a part of a matrix's gradient: so many that all parts together are some four for each CU, and no fewer than
-// 1024, beside which writing and reading a sum is little. An expert's matrix of many tiles needs no parts.
-int rows_of_part(size_t rows, size_t out, size_t cols) {
+// Rows of a part of a matrix's gradient. The tiles of all parts are to be two for each CU at most, an expert's last part taken to be
+// half full; but no part has fewer than 512 rows, which take a tile some 10 us (float32 30), beside which a sum's way to
+// memory and back is little. 2 experts' 100000 rows of 102 with 102, bfloat16, take 26 us in parts of 512 rows, 30 of 1024
+// and 45 of 2048 (float32 56, 88, 163); 16 experts' 96000 of 256 with 256 59, 44 and 44. (For two tiles to a CU numbers
+// are aimed at that the parts' unevenness leaves below 512: aimed at 512 themselves, that last case took 54 us.)
+// Where the experts have as many tiles by themselves, parts are for one that has most of the rows, and have 4096 (float32
+// 2048): 32 experts' 3200 rows of 1024 with 1024 take 37 us in parts of 1024 and 23 in none. Where a matrix has 128
+// tiles there are enough whoever has the rows.
+int rows_of_part(int size, size_t rows, int experts, size_t out, size_t cols) {
   const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
   if (tiles >= 128) return INT_MAX;
-  const size_t part = rows * tiles / 1024;
-  return (int)((part > 1024 ? part : 1024) + 63) / 64 * 64;
+  if (experts * tiles >= 512) {
+    const size_t part = rows * tiles / 512, least = size == 4 ? 2048 : 4096;
+    return (int)((part > least ? part : least) + 63) / 64 * 64;
+  }
+  const size_t part = 2 * rows * tiles / (768 - experts * tiles);
+  return (int)((part > 512 ? part : 512) + 63) / 64 * 64;
 }
-size_t sums_bytes(size_t rows, size_t out, size_t cols) {
-  const int part = rows_of_part(rows, out, cols);
+size_t sums_bytes(int size, size_t rows, int experts, size_t out, size_t cols) {
+  const int part = rows_of_part(size, rows, experts, out, cols);
   return rows <= (size_t)part ? 0 : part_sums((int)rows, part) * out * cols * sizeof(float);
 }
 
@@ -271,8 +281,10 @@ template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
   const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
   const int each = a.rows / a.experts;
+  // (of gradients 8 experts' of 4096 x 4096, 24 rows each, bfloat16, 46 us there and 54 in tiles, but 300 experts' of 512 x
+  // 512, 20 rows each, 50 and 32; float32 of 48 rows each 173 and 262, of 100 360 and 262)
   const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
-  if (KIND != DWEIGHTS && (far || (KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= 32))) {
+  if (KIND != DWEIGHTS && (far || (KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= (sizeof(T) == 4 ? 64 : 16)))) {
     ThinArgs t = {};
     t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
     t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
@@ -283,7 +295,7 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 64 : true) && a.n >= (sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16)) {
+  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 32 : true) && a.n >= (sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16)) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
@@ -372,8 +384,8 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
   });
 }
 
-KM_API size_t h2o4gpu_experts_product_dweights_workspace(size_t rows, int experts, size_t out, size_t cols) {
-  return check(0, rows, experts, out, cols, "") <= 0 ? 0 : sums_bytes(rows, out, cols);
+KM_API size_t h2o4gpu_experts_product_dweights_workspace(int dtype, size_t rows, int experts, size_t out, size_t cols) {
+  return check(dtype, rows, experts, out, cols, "") <= 0 ? 0 : sums_bytes(type_size(dtype), rows, experts, out, cols);
 }
 
 KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols,
@@ -381,7 +393,7 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
                                             const int *d_offsets, void *d_dweights, void *d_workspace,
                                             size_t workspace_bytes, void *stream) {
   if (int rc = check(dtype, rows, experts, out, cols, d_offsets); rc <= 0) return rc;
-  const size_t need = sums_bytes(rows, out, cols);
+  const size_t need = sums_bytes(type_size(dtype), rows, experts, out, cols);
   if (need > workspace_bytes || (need && (!d_workspace || !aligned_to(d_workspace, 16)))) return H2O4GPU_KMEANS_EARG;
   if (out > H2O4GPU_EXPERTS_MAX_SIDE || cols > H2O4GPU_EXPERTS_MAX_SIDE ||
       (rows > 1 && (dy_stride > H2O4GPU_EXPERTS_MAX_SIDE || rows_stride > H2O4GPU_EXPERTS_MAX_SIDE)))
@@ -390,7 +402,7 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
                    (int)cols, (int)out, 0, nullptr, 0, 0};
-  a.part = rows_of_part(rows, out, cols), a.sums = static_cast<float *>(d_workspace);
+  a.part = rows_of_part(type_size(dtype), rows, experts, out, cols), a.sums = static_cast<float *>(d_workspace);
   return with_type(dtype, [&](auto tag) {
     return launch_product<typename decltype(tag)::type, DWEIGHTS>(a, static_cast<hipStream_t>(stream));
   });

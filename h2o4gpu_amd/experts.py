@@ -362,8 +362,8 @@ def _matrices(weights):
 
 
 @functools.lru_cache(maxsize=256)
-def _sums(rows, n_experts, out, cols):
-    return experts_hip.lib().h2o4gpu_experts_product_dweights_workspace(rows, n_experts, out, cols)
+def _sums(code, rows, n_experts, out, cols):
+    return experts_hip.lib().h2o4gpu_experts_product_dweights_workspace(code, rows, n_experts, out, cols)
 
 
 def _at_words(t):
@@ -440,7 +440,7 @@ class _Product(torch.autograd.Function):
             dy, x = _align(worth, dy, rows) if worth else (dy, rows)
             dy, x = _near(dy), _near(x)
             dweights = weights.new_empty(weights.shape)
-            need = _sums(count, n_experts, out, cols)
+            need = _sums(code, count, n_experts, out, cols)
             work = dy.new_empty(need // 4, dtype=torch.float32) if need else None
             _call(dy.device.index, "h2o4gpu_experts_product_dweights", code, count, n_experts, out, cols,
                   *_rows("dy", dy), *_rows("rows", x), order._offsets_ptr, dweights.data_ptr(),

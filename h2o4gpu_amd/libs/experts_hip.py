@@ -58,7 +58,7 @@ PROTOTYPES = {
                                                  c_void_p]),
     "h2o4gpu_experts_align_rows": (c_int, [c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, c_size_t, c_void_p,
                                            c_void_p]),
-    "h2o4gpu_experts_product_dweights_workspace": (c_size_t, [c_size_t, c_int, c_size_t, c_size_t]),
+    "h2o4gpu_experts_product_dweights_workspace": (c_size_t, [c_int, c_size_t, c_int, c_size_t, c_size_t]),
     "h2o4gpu_microscale4_codes_pitch": (c_size_t, [c_size_t]),
     "h2o4gpu_microscale4_scales_pitch": (c_size_t, [c_size_t]),
     "h2o4gpu_microscale4_quantize": (c_int, [c_int, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p,

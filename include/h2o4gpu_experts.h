@@ -147,7 +147,7 @@ int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, siz
 int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
                                   size_t dy_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                                   const int *d_offsets, void *d_drows, size_t drows_stride, void *stream);
-size_t h2o4gpu_experts_product_dweights_workspace(size_t rows, int experts, size_t out, size_t cols);
+size_t h2o4gpu_experts_product_dweights_workspace(int dtype, size_t rows, int experts, size_t out, size_t cols);
 int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_dy,
                                      size_t dy_stride, const void *d_rows, size_t rows_stride, const int *d_offsets,
                                      void *d_dweights, void *d_workspace, size_t workspace_bytes, void *stream);
