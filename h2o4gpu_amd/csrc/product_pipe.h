@@ -1,4 +1,4 @@
-// The large tile of a matrix product on gfx950, for operands whose pieces of 16 bytes lie at multiples of 16.
+// The large tiles of a matrix product on gfx950, for operands whose rows begin at multiples of 4 bytes.
 //
 // C[m][n] = sum over k of X[m][k] W[n][k], 2-byte and 4-byte elements, or microscaled 4-bit ones (which are handled
 // as 2-byte elements that hold four columns each, with their scales beside). A stage of 128 bytes of k for each row
@@ -212,7 +212,8 @@ __device__ __forceinline__ void listed_tile(const int *table, const int *offsets
 // A wavefront's part of a tile to memory, 16 bytes a lane and 64 of a row side by side. A lane has four numbers of a row;
 // of 2-byte ones, the quarters of the wavefront (16 lanes) that hold neighbours exchange halves of two blocks: what bit 0
 // of the block's number and the two of the quarter's say (b; q1 q0) lies after the first exchange at (q1; b q0), after
-// the second at (q0; b q1). (Stored as they are, eight bytes a lane, 8192^3 took 100 us longer.)
+// the second at (q0; b q1). (Stored as they are, eight bytes a lane, 8192^3 in 4 bits takes 265 us instead of 245, and
+// 64 experts' 64000 rows of 512 with 512 x 512, bfloat16, 45 instead of 37.)
 template <typename OUT, int FM, int FN>
 __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN], OUT *c, size_t stride, int m0, int n0,
                                            int m_here, int n_here) {
@@ -260,6 +261,13 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
 
 // One stage after another, of one tile after another: what is loaded is two stages ahead of what is multiplied, and may
 // be the next tile's, so that a tile's first stages arrive while the one before ends and goes out.
+//
+// Bound by the matrix instructions, and for random numbers by the clock that the card's power leaves: 8192^3 in bfloat16
+// takes 790 to 910 us (1200 to 1390 TFLOP/s; zeros 740), in 4 bits 245 (4500; zeros 201), 8192 x 4096 x 4096 in float32
+// 1850 (149). 64 experts' 65536 rows of 2048 with 2048 x 2048 take 493 us, the rows' gradient 491, the matrices' 531 (1115,
+// 1120 and 1035 TFLOP/s). A tile of 256 x 256 reads each of its operands' elements from LDS as often as there are
+// wavefronts beside it, twice and four times: what eight wavefronts read in a step takes three quarters of the time of
+// their matrix instructions, where four wavefronts of 128 x 64, one to a SIMD, would leave nothing to fill the waits with.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   typedef typename PipeElement<ELEMENT>::type T;
@@ -588,11 +596,11 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       if (KIND == DWEIGHTS && now.sum >= 0)
         store_tile<float, FM, FN>(tid & 63, acc, a.sums + (size_t)now.sum * a.c_expert + (size_t)now.first * a.c_stride + now.n0,
                                   a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here);
-      else {
-      OUT *c = static_cast<OUT *>(a.c) + (KIND == DWEIGHTS ? (size_t)now.expert * a.c_expert : 0) +
-               (size_t)now.first * a.c_stride + now.n0;
-      store_tile<OUT, FM, FN>(tid & 63, acc, c, a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here);
-      }
+      else
+        store_tile<OUT, FM, FN>(tid & 63, acc,
+                                static_cast<OUT *>(a.c) + (KIND == DWEIGHTS ? (size_t)now.expert * a.c_expert : 0) +
+                                    (size_t)now.first * a.c_stride + now.n0,
+                                a.c_stride, wm * FM * 16, wn * FN * 16, now.m_here, now.n_here);
       put_order(slot);
       now = next;
       if (now.m_here == 0) break;
@@ -613,6 +621,8 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
                          : a.experts      ? ragged_tiles(a.experts, a.rows, BM)
                                           : ((size_t)a.rows + BM - 1) / BM;
   a.m_tiles = (int)m_tiles, a.n_tiles = (a.n + BN - 1) / BN;
+  // (as many tiles of m beside each other as make the operands that a chiplet's workgroups read at once few: 8192^3 in
+  // bfloat16 912 us, with bands of one tile 985, of 64 1150)
   a.band = a.n_tiles >= 8 ? 4 : a.n_tiles >= 4 ? 8 : 16;
   const size_t tiles = m_tiles * a.n_tiles;
   if (m_tiles > (size_t)INT_MAX || tiles > (size_t)INT_MAX) return H2O4GPU_KMEANS_EARG;
@@ -628,7 +638,7 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
 
 // Tiles of 256 x 256, or of 128 x 128, of which a CU holds two: by how often the card is filled with either (an expert's
 // last tile is taken to be half full), and how long a stage then takes, 1.7 and 1.3 us. 64 experts' 65536 rows of 2048 with
-// 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones, 4 experts' 8000 rows of 1024 with 512 x 1024
+// 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones (both before the tiles were stored as above), 4 experts' 8000 rows of 1024 with 512 x 1024
 // 27 and 16 us, 10 experts' 16941 rows of 4544 with 384 89 and 64, 160 experts' 49552 rows of 256 with 3392 188 and 191.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER>
 int launch_large(PipeArgs &a, hipStream_t stream) {

@@ -1,6 +1,8 @@
 // Products of few rows: the matrices are read once, straight into the registers of the matrix instructions' operand, and
 // that is what bounds them. A wavefront has 16 NB rows of a matrix and MB blocks of 16 rows of x; `share` wavefronts of a
 // workgroup (a power of two) share the columns and add up their sums in LDS, the others have other rows of the matrix.
+// 8 experts' 16 rows with 7168 x 4096, bfloat16 (470 MB of matrices), take 78 us, 6.0 TB/s, the rows' gradient 85; 64
+// experts' 256 rows with 2048 x 2048 104 and 100 us; 16 rows times 8192 x 8192 in 4 bits (36 MB) 12, one row 8.
 #pragma once
 
 #include "product_pipe.h"
@@ -171,8 +173,8 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
 }
 
 // One matrix in 4 bits, x of 17 to 64 rows and at most 8192 columns: a workgroup keeps its part of x, which it would read
-// from L2 for every 32 rows of the matrix (33 rows of 8190 times 11003: 29 us that way and 23 this, of which the
-// matrix takes 10), and takes 16 rows after others, the next of which are on their way while these are multiplied.
+// from L2 for every 32 rows of the matrix (33 rows of 8190 times 11003, with what makes 4 bits of x: 29 us that way and 21
+// this, of which the matrix takes 10), and takes 16 rows after others, the next of which are on their way while these are multiplied.
 template <typename OUT, int MB>
 __global__ __launch_bounds__(512) void kept_kernel(ThinArgs a) {
   constexpr int WAVES = 8, U = 4, TURNS = 2;
@@ -294,7 +296,7 @@ int launch_thin(ThinArgs &a, hipStream_t stream) {
   return launch(Int<4>(), Int<2>());
 }
 
-// The same where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some k's of
+// thin_kernel's product where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some k's of
 // its own; element b of all of them is its fragment of a block of 16 columns, EPP apart, so that a wavefront has
 // 16 EPP columns. What comes out for a lane and a j, block by block, is EPP columns side by side again.
 template <typename T, bool HALVES, int MB, int WAVES>

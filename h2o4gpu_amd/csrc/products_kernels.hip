@@ -4,7 +4,8 @@
 //   product_drows:    dx[p] = W[e]^T dy[p]
 //   product_dweights: dW[e] = sum over p of dy[p] x[p]^T
 //
-// Sums are float32, in an order that depends on the sizes alone; one rounding at the end.
+// Sums are float32, in an order that depends on the sizes and the offsets alone; one rounding at the end. Long products
+// of rows that begin at words go to pipe_kernel, those of few rows to thin_kernel, and what is left is here.
 #include "product_thin.h"
 
 namespace kmhip {
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 4 ? 2 : 3) void product_k
 }
 
 // The parts' sums of the experts that have several, added up in order: a workgroup has a stretch of the matrix of the
-// expert whose first part begins in its `part` rows.
+// expert whose first part begins in its `part` rows, a thread an element. What the parts' sums take to be read bounds it (98
+// parts of 2 experts of 101 x 101: 6 us).
 template <typename T>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float *sums, const int *offsets, int experts, int part,
                                                          size_t size, T *c) {
@@ -236,13 +238,12 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const float *sums, cons
   c[(size_t)lo * size + at] = (T)total;
 }
 
-// Whether every row of both operands begins at a multiple of 16 bytes, within the reach of a buffer. Then their pieces of
-// 16 bytes are read as they lie: what one holds behind a row's end is masked or not stored.
+// Whether every row of both operands begins at a multiple of 16 bytes.
 template <typename T>
 bool rows_aligned(const ProductArgs &a) {
   constexpr size_t EPP = 16 / sizeof(T);
   return aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % EPP == 0 && a.w_stride % EPP == 0 &&
-         a.w_expert % EPP == 0 && a.x_stride * sizeof(T) < BUFFER_BYTES / 512 && a.w_stride * sizeof(T) < BUFFER_BYTES / 512;
+         a.w_expert % EPP == 0;
 }
 
 // Rows of a part of a matrix's gradient. The tiles of all parts are to be two for each CU at most, an expert's last part taken to be
@@ -281,8 +282,9 @@ template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
   const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
   const int each = a.rows / a.experts;
-  // (of gradients 8 experts' of 4096 x 4096, 24 rows each, bfloat16, 46 us there and 54 in tiles, but 300 experts' of 512 x
-  // 512, 20 rows each, 50 and 32; float32 of 48 rows each 173 and 262, of 100 360 and 262)
+  // few rows of an expert, see few_rows (the rows' gradient: 8 experts of 4096 x 4096, 24 rows each, bfloat16, 46 us there and
+  // 54 in tiles, but 300 experts of 512 x 512, 20 rows each, 50 and 32; float32 of the first with 48 rows each 173 and 262,
+  // of 300 experts with 50 rows each 144 and 357); far: an offset of a tile's last row would not fit a buffer
   const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
   if (KIND != DWEIGHTS && (far || (KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= (sizeof(T) == 4 ? 64 : 16)))) {
     ThinArgs t = {};
@@ -295,7 +297,13 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  if (!halves && (KIND == DWEIGHTS ? a.k >= 128 && each >= 32 : true) && a.n >= (sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16)) {
+  // Tiles that a matrix does not fill cost float32 and the matrices' gradient their products, which the kernel here leaves
+  // out (16 experts' 64000 rows of 2048 with 64 x 2048, float32, 181 us here and 246 there, the gradient 222 and 347); other
+  // products wait for memory (64 experts' 64000 rows of 640 with 16 x 640, bfloat16, 31 and 18). float32 gradients of few
+  // rows are faster here (8 experts' of 4096 x 4096, 24 rows each, 163 and 195, 48 rows each 225 and 196; bfloat16 86 and
+  // 68, 88 and 67).
+  constexpr int LEAST = sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16;
+  if (!halves && a.n >= LEAST && (KIND != DWEIGHTS || (a.k >= LEAST && (sizeof(T) == 2 || each >= 32)))) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
@@ -321,14 +329,18 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
   return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
 }
 
+// Where elements of a type may lie.
+bool elements(int dtype, const void *p) { return p && aligned_to(p, type_size(dtype)); }
+
 // Strides of rows of `cols` elements, each row apart from the next.
 bool fits(size_t rows, size_t cols, size_t stride) { return rows < 2 || stride >= cols; }
 
 // A thread a piece of 16 bytes: rows as they come, into rows that begin at multiples of 16 bytes, zeros behind their ends.
+// Bound by memory: 456750 rows of 781 (bfloat16, 714 MB in, 716 out) take 355 us, 4.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void align_kernel(const T *in, size_t stride, size_t matrix, size_t rows, size_t cols,
-                                                    size_t pieces, size_t total, u32x4 *out) {
-  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+                                                    size_t pieces, size_t total, u32x4 *out, unsigned first_block) {
+  const size_t at = (size_t)(first_block + blockIdx.x) * 256 + threadIdx.x;
   if (at >= total) return;
   const size_t row = at / pieces, col = (at - row * pieces) * (16 / sizeof(T)), of = row / rows;
   const size_t left = cols - col;
@@ -358,7 +370,7 @@ KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t o
       rc <= 0)
     return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!d_rows || !d_weights || !d_y || !fits(rows, cols, rows_stride) || !fits(out, cols, w_stride) ||
+  if (!elements(dtype, d_rows) || !elements(dtype, d_weights) || !elements(dtype, d_y) || !fits(rows, cols, rows_stride) || !fits(out, cols, w_stride) ||
       !fits(rows, out, y_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_rows, d_weights, d_y, rows_stride, w_stride, expert_stride, y_stride, 0, d_offsets, experts, (int)rows,
@@ -374,7 +386,7 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
   if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "", w_stride); rc <= 0)
     return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!d_dy || !d_weights || !d_drows || !fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
+  if (!elements(dtype, d_dy) || !elements(dtype, d_weights) || !elements(dtype, d_drows) || !fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
       !fits(rows, cols, drows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_weights, d_drows, dy_stride, w_stride, expert_stride, drows_stride, 0, d_offsets, experts,
@@ -398,7 +410,7 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
   if (out > H2O4GPU_EXPERTS_MAX_SIDE || cols > H2O4GPU_EXPERTS_MAX_SIDE ||
       (rows > 1 && (dy_stride > H2O4GPU_EXPERTS_MAX_SIDE || rows_stride > H2O4GPU_EXPERTS_MAX_SIDE)))
     return H2O4GPU_KMEANS_EARG;
-  if (!d_dweights || (rows && (!d_dy || !d_rows)) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
+  if (!elements(dtype, d_dweights) || (rows && (!elements(dtype, d_dy) || !elements(dtype, d_rows))) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
                    (int)cols, (int)out, 0, nullptr, 0, 0};
@@ -416,12 +428,14 @@ KM_API int h2o4gpu_experts_align_rows(int dtype, size_t matrices, size_t rows, s
   if (matrices * rows > ((size_t)1 << 40) / pieces) return H2O4GPU_KMEANS_EARG;
   const size_t total = matrices * rows * pieces;
   if (total == 0) return H2O4GPU_KMEANS_OK;
-  if (!d_in || !d_out || !aligned_to(d_out, 16)) return H2O4GPU_KMEANS_EARG;
+  if (!elements(dtype, d_in) || !d_out || !aligned_to(d_out, 16)) return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
     typedef typename decltype(tag)::type T;
-    hipLaunchKernelGGL((align_kernel<T>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T *>(d_in), stride, matrix_stride, rows, cols,
-                       pieces, total, static_cast<u32x4 *>(d_out));
-    return launched();
+    return in_launches((total + 255) / 256, [&](unsigned first, unsigned here) {
+      hipLaunchKernelGGL((align_kernel<T>), dim3(here), dim3(256), 0, static_cast<hipStream_t>(stream),
+                         static_cast<const T *>(d_in), stride, matrix_stride, rows, cols, pieces, total,
+                         static_cast<u32x4 *>(d_out), first);
+      return launched();
+    });
   });
 }

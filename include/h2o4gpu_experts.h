@@ -11,8 +11,8 @@
  * allocates, copies to the host or keeps data or a workspace between calls, so all of them can be
  * recorded into a graph. What stays is a kernel's limit of shared memory on a device: a call that
  * needs more than 64 KB and more than any before it raises it, and is to be outside a capture, so
- * make one of the same type and sizes before recording. That may be route (distances), sort and
- * both products. Strides count elements. A call that returns an error has queued nothing, but for
+ * make one of the same type and sizes before recording. That may be route (distances), sort, both
+ * products with codebooks, the experts' own products, their gradients and the microscaled products. Strides count elements. A call that returns an error has queued nothing, but for
  * H2O4GPU_KMEANS_EDEVICE. Sizes of 0 rows are a success that queues nothing (but for the offsets
  * of experts_sort). Same inputs give the same bits in every call.
  * Status codes are those of h2o4gpu_kmeans.h.
@@ -136,7 +136,7 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
  * [d_offsets[e], d_offsets[e + 1]) of each expert e, zeros for those behind d_offsets[experts] (what
  * lies there is not read). d_offsets [experts + 1] as experts_sort writes it: from 0, ascending, at
  * most rows. W_e: [out][cols], rows w_stride (at most 2^23) elements apart, at d_weights + e * expert_stride (0: one
- * matrix for all). Products and sums in float, one rounding at the end.
+ * matrix for all). Sums in float, one rounding at the end.
  * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
  * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none), out, cols
  * and both strides at most MAX_SIDE;
@@ -154,7 +154,8 @@ int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts, size_t
 
 /* Rows of `matrices` matrices [rows][cols], the matrices matrix_stride elements apart, to rows that begin at
  * multiples of 16 bytes, as short as they can be, one matrix behind another; zeros behind column cols. The
- * products above take long rows faster where strides and addresses of both operands are multiples of 16 bytes. */
+ * products above are faster where strides and addresses of both operands are multiples of 4 bytes, most so
+ * those of 16-bit elements and many rows: 1.5 us and more for 10^9 operations, beside 1 us for 1.8 MB copied. */
 int h2o4gpu_experts_align_rows(int dtype, size_t matrices, size_t rows, size_t cols, const void *d_in,
                                size_t matrix_stride, size_t stride, void *d_out, void *stream);
 
