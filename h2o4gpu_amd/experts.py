@@ -13,9 +13,11 @@ centroids or scores, and the results come back and are joined by weight.
 rows, the matrices and the weights); forward-mode derivatives are refused. All work is queued on the current stream of
 the tensors' device, nothing waits for it and nothing is copied to the host, so the calls can be
 recorded into a graph (after a call of the same type and sizes outside of one, which may raise a
-kernel's limit of shared memory). Tensors are read on that stream: one that another stream writes has
-to be waited for, as with any torch operation, and an ExpertOrder used on another stream than it was
-made on likewise. Same inputs give the same bits. The kernels are the library's
+kernel's limit of shared memory). A backward pass is recorded when no graph of eager calls with the same
+leaves is alive any more (delete their results and losses first): autograd would accumulate on the stream of
+those calls, which the recording does not cover, and the process would end. Tensors are read on the current
+stream: one that another stream writes has to be waited for, as with any torch operation, and an ExpertOrder
+used on another stream than it was made on likewise. Same inputs give the same bits. The kernels are the library's
 (include/h2o4gpu_experts.h); there is no CPU path.
 """
 import functools
@@ -379,9 +381,14 @@ def _align(worth, *tensors):
     1024 rows each 458 and 651 us, 256 rows each 258 and 213; the matrices' gradient, where only rows are copied, of
     256 rows each 179 and 285, of 128 144 and 230."""
     odd = [t for t in tensors if not _at_words(t)]
-    if not odd or 1.5e-9 * worth < sum(6 + t.numel() * t.element_size() / 1.8e6 for t in odd):
+    if not odd or 1.5e-9 * worth < sum(6 + _one(t).numel() * t.element_size() / 1.8e6 for t in odd):
         return tensors
     return tuple(t if _at_words(t) else _copy_aligned(t) for t in tensors)
+
+
+def _one(t):
+    """One matrix for all experts, where they share it."""
+    return t[:1] if t.dim() == 3 and t.stride(0) == 0 else t
 
 
 def _near(t):
@@ -390,6 +397,8 @@ def _near(t):
 
 
 def _copy_aligned(t):
+    if _one(t).shape != t.shape:
+        return _copy_aligned(t[:1]).expand(t.shape)
     each = 16 // t.element_size()
     cols = t.shape[-1]
     wide = t.new_empty(t.shape[:-1] + (-(-cols // each) * each,))
@@ -459,9 +468,14 @@ class _Product(torch.autograd.Function):
 def product(rows, weights, order):
     """(tokens * top_k, out): every row times the transpose of its expert's matrix, zeros in the places
     behind order.offsets[-1] (what lies there in `rows` is not read). rows: (tokens * top_k, cols) in
-    expert order, as `dispatch` gives them; weights: (experts, out, cols) of the same type, rows of both
-    contiguous. Sums are float32, rounded once. Gradients for rows and weights; an expert without
-    rows has a gradient of zeros."""
+    expert order, as `dispatch` gives them; weights: (experts, out, cols) of the same type (or one matrix, expanded),
+    rows of both contiguous. Sums are float32, rounded once. Gradients for rows and weights; an expert without
+    rows has a gradient of zeros.
+
+    Sizes, types, strides and addresses choose between kernels that add up in another order: the same numbers laid out
+    otherwise may differ in the last bit. Fastest are rows that begin at multiples of 4 bytes (of 16-bit types, an even
+    number of columns); of others a long product makes copies that do. The gradient of matrices of less than 128
+    x 128 x 128 elements takes memory for up to 800 partial sums of one, float32, while it runs."""
     if not (isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _TYPES):
         _tensor("rows", rows, 2)
         _type_of("rows", rows)

@@ -140,7 +140,9 @@ int h2o4gpu_codebook4_experts_product(int dtype, size_t tokens, int top_k, int e
  * product_drows: d_drows[p] = W_e^T d_dy[p], zeros likewise. product_dweights: d_dweights
  * [experts][out][cols], W_e's is the sum over its rows of d_dy[p] d_rows[p]^T (zeros for none), out, cols
  * and both strides at most MAX_SIDE;
- * d_workspace: product_dweights_workspace() bytes, 16-byte aligned (NULL where that is 0). */
+ * d_workspace: product_dweights_workspace() bytes, 16-byte aligned (NULL where that is 0): sums of parts of the
+ * rows, where few matrices of few tiles of 128 x 128 have many rows. Which kernel adds up depends on sizes, strides
+ * and addresses, and with it the last bit of a result. */
 int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t out, size_t cols, const void *d_rows,
                             size_t rows_stride, const void *d_weights, size_t expert_stride, size_t w_stride,
                             const int *d_offsets, void *d_y, size_t y_stride, void *stream);

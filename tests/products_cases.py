@@ -16,6 +16,18 @@ RAGGED = (
     (9000, 1, 2300, 16, 24), (90, 1, 3, 1100, 300), (40, 2, 4, 513, 129), (7, 1, 2, 65, 1000), (100, 4, 20, 128, 40), (2600, 2, 4, 200, 128), (900, 1, 3, 1000, 72), (300, 1, 1, 264, 2056),
 )
 
+# rows that begin at words and no more (cols % 8 = 2), narrow matrices, an expert of many parts, more experts than a table
+# in LDS holds, few rows with large matrices
+WORDS = ((701, 1, 3, 2002, 330), (702, 1, 3, 2002, 330), (21000, 1, 2, 18, 34), (30000, 1, 2, 30, 22), (170, 1, 3, 40, 50),
+         (21, 1, 4, 264, 130), (3000, 1, 1030, 136, 130))
+
+
+def _words():
+    out = [dict(op="product", tokens=tokens, top_k=top_k, experts=experts, out=n, cols=cols, dtype=dtype, dropped=0.1,
+                layout=LAYOUTS[(tokens + n) % 3], data="normal") for tokens, top_k, experts, n, cols in WORDS for dtype in TYPES]
+    return out + [dict(op="product", tokens=9000, top_k=1, experts=520, out=20, cols=30, dtype=dtype, dropped=0.0,
+                       layout="plain", data="one_expert") for dtype in TYPES]
+
 
 def _products():
     out = []
@@ -68,7 +80,7 @@ CHECKS = ("differences", "broadcast", "graph", "graph_of_training", "other_strea
 
 def all_cases():
     cases = _products() + _quantize() + _fours() + _fours_of_experts()
-    cases += [dict(op=name) for name in CHECKS]
+    cases += [dict(op=name) for name in CHECKS] + _words() + [dict(op="broadcast_between_words")]
     for i, c in enumerate(cases):
         c["name"] = "%03d_%s" % (i, "_".join(str(v) for v in c.values()))
     return cases

@@ -305,6 +305,20 @@ def check_broadcast(_):
         near(gW, (ones.t() @ a)[None], (roundings(2 * T, dt) * U32 + 6 * ROUND[dt]) * size, "gradient of the matrix")
 
 
+def check_broadcast_between_words(_):
+    """One matrix for all experts whose rows begin between words, in a product that copies such: as three matrices."""
+    E, N, K = 3, 3001, 901
+    order = experts.sort_by_expert((torch.arange(6000) % E).int().view(-1, 1).cuda(), E)
+    x = torch.randn(6000, K, generator=gen(1)).bfloat16().cuda().requires_grad_()
+    one = torch.randn(1, N, K, generator=gen(2)).bfloat16().cuda()
+    g = torch.randn(6000, N, generator=gen(3)).bfloat16().cuda()
+    y, z = experts.product(x, one.expand(E, N, K), order), experts.product(x, one.repeat(E, 1, 1), order)
+    same(y, z, "y")
+    same(torch.autograd.grad(y, x, g)[0], torch.autograd.grad(z, x, g)[0], "gradient of the rows")
+    a, b = x[:50].detach().double().cpu(), one[0].double().cpu()
+    near(y[:50], a @ b.t(), roundings(K, x.dtype) * U32 * (a.abs() @ b.abs().t()), "y")
+
+
 def layer(x, scores, W, packed, top_k):
     chosen, weights = experts.route(scores, top_k)
     order = experts.sort_by_expert(chosen, W.shape[0])
