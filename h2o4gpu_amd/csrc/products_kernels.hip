@@ -251,14 +251,16 @@ bool rows_aligned(const ProductArgs &a) {
 // memory and back is little. 2 experts' 100000 rows of 102 with 102, bfloat16, take 26 us in parts of 512 rows, 30 of 1024
 // and 45 of 2048 (float32 56, 88, 163); 16 experts' 96000 of 256 with 256 59, 44 and 44. (For two tiles to a CU numbers
 // are aimed at that the parts' unevenness leaves below 512: aimed at 512 themselves, that last case took 54 us.)
-// Where the experts have as many tiles by themselves, parts are for one that has most of the rows, and have 4096 (float32
-// 2048): 32 experts' 3200 rows of 1024 with 1024 take 37 us in parts of 1024 and 23 in none. Where a matrix has 128
+// Where the experts have as many tiles by themselves, parts are for one that has most of the rows. pipe_kernel shares its
+// tiles out by their rows where there are none, so its parts have 4096 (float32 2048): 32 experts' 3200 rows of 1024 with
+// 1024 take 37 us in parts of 1024 and 23 in none. Narrow matrices are product_kernel's, which does not, and have 512:
+// 1000 experts of 77 x 101 float32, 300 rows on average and one with 3794, take 137 us, in parts of 1024 156, of 2048 199. Where a matrix has 128
 // tiles there are enough whoever has the rows.
 int rows_of_part(int size, size_t rows, int experts, size_t out, size_t cols) {
   const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
   if (tiles >= 128) return INT_MAX;
   if (experts * tiles >= 512) {
-    const size_t part = rows * tiles / 512, least = size == 4 ? 2048 : 4096;
+    const size_t part = rows * tiles / 512, least = out < 128 || cols < 128 ? 512 : size == 4 ? 2048 : 4096;
     return (int)((part > least ? part : least) + 63) / 64 * 64;
   }
   const size_t part = 2 * rows * tiles / (768 - experts * tiles);
