@@ -265,7 +265,8 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
 // Bound by the matrix instructions, and for random numbers by the clock that the card's power leaves: 8192^3 in bfloat16
 // takes 790 to 910 us (1200 to 1390 TFLOP/s; zeros 740), in 4 bits 245 (4500; zeros 201), 8192 x 4096 x 4096 in float32
 // 1850 (149). 64 experts' 65536 rows of 2048 with 2048 x 2048 take 493 us, the rows' gradient 491, the matrices' 531 (1115,
-// 1120 and 1035 TFLOP/s). A tile of 256 x 256 reads each of its operands' elements from LDS as often as there are
+// 1120 and 1035 TFLOP/s). With few columns a tile's way out counts: 64 experts' 65536 rows of 2048 with 4096 x 2048 in 4 bits
+// take 402 us, of which 105 are for y's 537 MB. A tile of 256 x 256 reads each of its operands' elements from LDS as often as there are
 // wavefronts beside it, twice and four times: what eight wavefronts read in a step takes three quarters of the time of
 // their matrix instructions, where four wavefronts of 128 x 64, one to a SIMD, would leave nothing to fill the waits with.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
