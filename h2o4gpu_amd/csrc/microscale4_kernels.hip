@@ -28,12 +28,12 @@ __device__ __forceinline__ float power_of(unsigned byte) {
   return byte == 255 ? __builtin_nanf("") : __uint_as_float(byte ? byte << 23 : 0x400000u);
 }
 
-// One thread: eight columns, a word of codes; four threads a block, which share its largest magnitude. A block's
-// power of two is that of the largest magnitude over 4, so that it lands in [4, 8), where 6 is the largest element
-// and what is beyond stays 6. Magnitudes are compared as their bits, in which NaN and infinities are the largest:
-// their block's scale is 255, not a number. Bound by memory, 1024 bytes of 16-bit elements in and 272 out a wavefront: two
-// words a thread, both loads on their way at once, and no other pass. 11003 x 8190 float16 (228 MB in all) take 42 us, 5.5
-// TB/s out of a warm cache; with one word a thread 47, with four 43 (8192 x 8192 28, 30 and 32). 64 x 4096 take a launch, 4 us.
+// One thread: eight columns, a word of codes; four threads a block, which share its largest magnitude. A block's power of
+// two is that of the largest magnitude over 4, so that it lands in [4, 8), where 6 is the largest element and what is
+// beyond stays 6. Magnitudes are compared as their bits, in which NaN and infinities are the largest: their block's scale
+// is 255, not a number. Bound by memory, 1024 bytes of 16-bit elements in and 272 out a wavefront: two words a thread,
+// both loads on their way at once, and no other pass. 11003 x 8190 float16 (228 MB in all) take 42 us, 5.5 TB/s out of a
+// warm cache; with one word a thread 47, with four 43 (8192 x 8192 28, 30 and 32). 64 x 4096 take a launch, 4 us.
 template <typename T, int UNROLL>
 __global__ __launch_bounds__(256) void quantize_kernel(const T *x, size_t x_stride, unsigned cols, size_t words,
                                                        unsigned row_words, unsigned *codes, unsigned char *scales,
@@ -208,7 +208,8 @@ KM_API int h2o4gpu_microscale4_quantize(int dtype, size_t rows, size_t cols, con
                                         void *d_codes, void *d_scales, void *stream) {
   if (!known_type(dtype) || !sized(rows, cols)) return H2O4GPU_KMEANS_EARG;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!d_x || !d_codes || !d_scales || (rows > 1 && x_stride < cols) || !aligned_to(d_x, type_size(dtype)) || !aligned_to(d_codes, 16) ||
+  if (!d_x || !d_codes || !d_scales || (rows > 1 && x_stride < cols) ||
+      !aligned_to(d_x, type_size(dtype)) || !aligned_to(d_codes, 16) ||
       !aligned_to(d_scales, 16))
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {
@@ -230,7 +231,8 @@ KM_API int h2o4gpu_microscale4_dequantize(int dtype, size_t rows, size_t cols, c
                                           void *d_out, size_t out_stride, void *stream) {
   if (!known_type(dtype) || !sized(rows, cols)) return H2O4GPU_KMEANS_EARG;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!d_out || !d_codes || !d_scales || (rows > 1 && out_stride < cols) || !aligned_to(d_out, type_size(dtype)) || !aligned_to(d_codes, 16) ||
+  if (!d_out || !d_codes || !d_scales || (rows > 1 && out_stride < cols) ||
+      !aligned_to(d_out, type_size(dtype)) || !aligned_to(d_codes, 16) ||
       !aligned_to(d_scales, 16))
     return H2O4GPU_KMEANS_EARG;
   return with_type(dtype, [&](auto tag) {

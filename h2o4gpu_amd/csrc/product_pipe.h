@@ -259,16 +259,17 @@ __device__ __forceinline__ void store_tile(int lane, const f32x4 (&acc)[FM][FN],
   }
 }
 
-// One stage after another, of one tile after another: what is loaded is two stages ahead of what is multiplied, and may
-// be the next tile's, so that a tile's first stages arrive while the one before ends and goes out.
+// One stage after another, of one tile after another: what is loaded is two stages ahead of what is multiplied, and may be
+// the next tile's, so that a tile's first stages arrive while the one before ends and goes out.
 //
 // Bound by the matrix instructions, and for random numbers by the clock that the card's power leaves: 8192^3 in bfloat16
 // takes 790 to 910 us (1200 to 1390 TFLOP/s; zeros 740), in 4 bits 245 (4500; zeros 201), 8192 x 4096 x 4096 in float32
-// 1850 (149). 64 experts' 65536 rows of 2048 with 2048 x 2048 take 493 us, the rows' gradient 491, the matrices' 531 (1115,
-// 1120 and 1035 TFLOP/s). With few columns a tile's way out counts: 64 experts' 65536 rows of 2048 with 4096 x 2048 in 4 bits
-// take 402 us, of which 105 are for y's 537 MB. A tile of 256 x 256 reads each of its operands' elements from LDS as often as there are
-// wavefronts beside it, twice and four times: what eight wavefronts read in a step takes three quarters of the time of
-// their matrix instructions, where four wavefronts of 128 x 64, one to a SIMD, would leave nothing to fill the waits with.
+// 1850 (149). 64 experts' 65536 rows of 2048 with 2048 x 2048 take 493 us, the rows' gradient 491, the matrices' 531
+// (1115, 1120 and 1035 TFLOP/s). With few columns a tile's way out counts: 64 experts' 65536 rows of 2048 with 4096 x 2048
+// in 4 bits take 402 us, of which 105 are for y's 537 MB. A tile of 256 x 256 reads each of its operands' elements from
+// LDS as often as there are wavefronts beside it, twice and four times: what eight wavefronts read in a step takes three
+// quarters of the time of their matrix instructions. Four of 128 x 128 would read two thirds of that, but the sums leave
+// them too few registers.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   typedef typename PipeElement<ELEMENT>::type T;
@@ -446,7 +447,8 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       to_lds_16(buffer_of(in_x, x_size), x_off[i % ODD] + (GATHER ? row_off[GATHER ? i : 0] : i * x_next),
                 to + buffer + i * THREADS * 16);
     else
-      to_lds_16(buffer_of(in_w, w_size), w_off[(i - X::P) % ODD] + (i - X::P) * w_next, to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
+      to_lds_16(buffer_of(in_w, w_size), w_off[(i - X::P) % ODD] + (i - X::P) * w_next,
+                to + buffer + BM * 128 + (i - X::P) * THREADS * 16);
   };
   unsigned scales_in = 0;  // 0 or SCALES
   auto load_scales = [&]() {  // of this stage and the next, 512 columns, at every even stage of a tile
@@ -638,9 +640,10 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
 }
 
 // Tiles of 256 x 256, or of 128 x 128, of which a CU holds two: by how often the card is filled with either (an expert's
-// last tile is taken to be half full), and how long a stage then takes, 1.7 and 1.3 us. 64 experts' 65536 rows of 2048 with
-// 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones (both before the tiles were stored as above), 4 experts' 8000 rows of 1024 with 512 x 1024
-// 27 and 16 us, 10 experts' 16941 rows of 4544 with 384 89 and 64, 160 experts' 49552 rows of 256 with 3392 188 and 191.
+// last tile is taken to be half full), and how long a stage then takes, 1.7 and 1.3 us. 64 experts' 65536 rows of 2048
+// with 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones (both before the tiles were stored as above),
+// 4 experts' 8000 rows of 1024 with 512 x 1024 27 and 16 us, 10 experts' 16941 rows of 4544 with 384 89 and 64, 160
+// experts' 49552 rows of 256 with 3392 188 and 191.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER>
 int launch_large(PipeArgs &a, hipStream_t stream) {
   auto turns = [&](int tile, int at_once) {

@@ -49,7 +49,8 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
   const int i = lane & 15, g = lane >> 4;
   const unsigned block = a.first_block + blockIdx.x;
   const int part = wave & (a.share - 1), row = wave / a.share;
-  const int n0 = ((int)(block % (unsigned)a.n_tiles) * (WAVES / a.share) + row) * (16 * NB), number = (int)(block / (unsigned)a.n_tiles);
+  const int n0 = ((int)(block % (unsigned)a.n_tiles) * (WAVES / a.share) + row) * (16 * NB);
+  const int number = (int)(block / (unsigned)a.n_tiles);
   int expert = 0, first = number * (16 * MB), m_here = a.rows - first < 16 * MB ? a.rows - first : 16 * MB, k = a.k;
   if (a.experts) {
     if (!ragged_tile(a.offsets, a.experts, a.rows, 16 * MB, number, expert, first, m_here)) return;
@@ -91,10 +92,12 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
         const size_t at = ((size_t)t * U + u) * 64;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
-          fw[u][n] = ALIGNED ? *reinterpret_cast<const u32x4 *>(w[n] + at) : load_whole(reinterpret_cast<const T *>(w[n] + at), halves);
+          fw[u][n] = ALIGNED ? *reinterpret_cast<const u32x4 *>(w[n] + at)
+                             : load_whole(reinterpret_cast<const T *>(w[n] + at), halves);
 #pragma unroll
         for (int m = 0; m < MB; ++m)
-          fx[u][m] = ALIGNED ? *reinterpret_cast<const u32x4 *>(x[m] + at) : load_whole(reinterpret_cast<const T *>(x[m] + at), halves);
+          fx[u][m] = ALIGNED ? *reinterpret_cast<const u32x4 *>(x[m] + at)
+                             : load_whole(reinterpret_cast<const T *>(x[m] + at), halves);
       }
     };
     if ((t + 1) * (U * STEP) <= k) {
@@ -174,7 +177,8 @@ __global__ __launch_bounds__(WAVES * 64) void thin_kernel(ThinArgs a) {
 
 // One matrix in 4 bits, x of 17 to 64 rows and at most 8192 columns: a workgroup keeps its part of x, which it would read
 // from L2 for every 32 rows of the matrix (33 rows of 8190 times 11003, with what makes 4 bits of x: 29 us that way and 21
-// this, of which the matrix takes 10), and takes 16 rows after others, the next of which are on their way while these are multiplied.
+// this, of which the matrix takes 10), and takes 16 rows after others, the next of which are on their way while these are
+// multiplied.
 template <typename OUT, int MB>
 __global__ __launch_bounds__(512) void kept_kernel(ThinArgs a) {
   constexpr int WAVES = 8, U = 4, TURNS = 2;
@@ -296,9 +300,9 @@ int launch_thin(ThinArgs &a, hipStream_t stream) {
   return launch(Int<4>(), Int<2>());
 }
 
-// thin_kernel's product where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some k's of
-// its own; element b of all of them is its fragment of a block of 16 columns, EPP apart, so that a wavefront has
-// 16 EPP columns. What comes out for a lane and a j, block by block, is EPP columns side by side again.
+// thin_kernel's product where the matrix lies with n side by side (W^T dy): a lane loads 16 bytes, EPP columns, of some
+// k's of its own; element b of all of them is its fragment of a block of 16 columns, EPP apart, so that a wavefront has 16
+// EPP columns. What comes out for a lane and a j, block by block, is EPP columns side by side again.
 template <typename T, bool HALVES, int MB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void thin_columns_kernel(ThinArgs a) {
   constexpr int EPP = 16 / (int)sizeof(T), STEP = 4 * EPP, TURN = 32, U = TURN / STEP;  // k of a turn

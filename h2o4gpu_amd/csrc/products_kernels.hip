@@ -174,6 +174,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 4 ? 2 : 3) void product_k
     if (t + 1 < stages) load((t + 1) * KS);
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
+      if (step == 1 && k_end - t * KS <= KS / 2) break;  // (zeros)
       u32x4 fx[FM], fw[FN];
 #pragma unroll
       for (int i = 0; i < FM; ++i) fx[i] = TX::fragment(at, lane, i * WM + wm, step);
@@ -246,25 +247,29 @@ bool rows_aligned(const ProductArgs &a) {
          a.w_expert % EPP == 0;
 }
 
-// Rows of a part of a matrix's gradient. The tiles of all parts are to be two for each CU at most, an expert's last part taken to be
-// half full; but no part has fewer than 512 rows, which take a tile some 10 us (float32 30), beside which a sum's way to
-// memory and back is little. 2 experts' 100000 rows of 102 with 102, bfloat16, take 26 us in parts of 512 rows, 30 of 1024
-// and 45 of 2048 (float32 56, 88, 163); 16 experts' 96000 of 256 with 256 59, 44 and 44. (For two tiles to a CU numbers
-// are aimed at that the parts' unevenness leaves below 512: aimed at 512 themselves, that last case took 54 us.)
-// Where the experts have as many tiles by themselves, parts are for one that has most of the rows. pipe_kernel shares its
-// tiles out by their rows where there are none, so its parts have 4096 (float32 2048): 32 experts' 3200 rows of 1024 with
-// 1024 take 37 us in parts of 1024 and 23 in none. Narrow matrices are product_kernel's, which does not, and have 512:
-// 1000 experts of 77 x 101 float32, 300 rows on average and one with 3794, take 137 us, in parts of 1024 156, of 2048 199. Where a matrix has 128
-// tiles there are enough whoever has the rows.
+// Rows of a part of a matrix's gradient. The tiles of all parts are to be two for each CU at most, an expert's last part
+// taken to be half full; but no part has fewer than 512 rows, which take a tile some 10 us (float32 30), beside which a
+// sum's way to memory and back is little. 2 experts' 100000 rows of 102 with 102, bfloat16, take 26 us in parts of 512
+// rows, 30 of 1024 and 45 of 2048 (float32 56, 88, 163); 16 experts' 96000 of 256 with 256 59, 44 and 44. (For two tiles
+// to a CU numbers are aimed at that the parts' unevenness leaves below 512: aimed at 512 themselves, that last case took
+// 54 us.) Where the experts have as many tiles by themselves, parts are for one that has most of the rows. pipe_kernel
+// shares its tiles out by their rows where there are none, so its parts have 4096 (float32 2048): 32 experts' 3200 rows of
+// 1024 with 1024 take 37 us in parts of 1024 and 23 in none. Narrow matrices are product_kernel's, which does not:
+// four tiles for each CU, and no fewer than 512 rows (1000 experts of 77 x 101 float32, 300 rows on average and one with
+// 3794, take 130 us, in parts of 1024 156, of 2048 199; 16 experts' 64000 rows of 64 with 2048, in parts of 1024, 217, in
+// one part an expert 325). Where a matrix has 128 tiles there are enough whoever has the rows. All parts' sums are at most
+// 2 (1024 + 128) tiles of 64 KB.
 int rows_of_part(int size, size_t rows, int experts, size_t out, size_t cols) {
   const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
   if (tiles >= 128) return INT_MAX;
-  if (experts * tiles >= 512) {
-    const size_t part = rows * tiles / 512, least = out < 128 || cols < 128 ? 512 : size == 4 ? 2048 : 4096;
-    return (int)((part > least ? part : least) + 63) / 64 * 64;
-  }
-  const size_t part = 2 * rows * tiles / (768 - experts * tiles);
-  return (int)((part > 512 ? part : 512) + 63) / 64 * 64;
+  size_t part, least = 512;
+  if (out < 128 || cols < 128)
+    part = rows * tiles / 1024;
+  else if (experts * tiles >= 512)
+    part = rows * tiles / 512, least = size == 4 ? 2048 : 4096;
+  else
+    part = 2 * rows * tiles / (768 - experts * tiles);
+  return (int)((part > least ? part : least) + 63) / 64 * 64;
 }
 size_t sums_bytes(int size, size_t rows, int experts, size_t out, size_t cols) {
   const int part = rows_of_part(size, rows, experts, out, cols);
@@ -284,11 +289,12 @@ template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
   const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
   const int each = a.rows / a.experts;
-  // few rows of an expert, see few_rows (the rows' gradient: 8 experts of 4096 x 4096, 24 rows each, bfloat16, 46 us there and
-  // 54 in tiles, but 300 experts of 512 x 512, 20 rows each, 50 and 32; float32 of the first with 48 rows each 173 and 262,
-  // of 300 experts with 50 rows each 144 and 357); far: an offset of a tile's last row would not fit a buffer
+  // few rows of an expert, see few_rows (the rows' gradient: 8 experts of 4096 x 4096, 24 rows each, bfloat16, 46 us there
+  // and 54 in tiles, but 300 experts of 512 x 512, 20 rows each, 50 and 32; float32 of the first with 48 rows each 173 and
+  // 262, of 300 experts with 50 rows each 144 and 357); far: an offset of a tile's last row would not fit a buffer
   const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
-  if (KIND != DWEIGHTS && (far || (KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= (sizeof(T) == 4 ? 64 : 16)))) {
+  const bool few = KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= (sizeof(T) == 4 ? 64 : 16);
+  if (KIND != DWEIGHTS && (far || few)) {
     ThinArgs t = {};
     t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
     t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
@@ -372,7 +378,9 @@ KM_API int h2o4gpu_experts_product(int dtype, size_t rows, int experts, size_t o
       rc <= 0)
     return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!elements(dtype, d_rows) || !elements(dtype, d_weights) || !elements(dtype, d_y) || !fits(rows, cols, rows_stride) || !fits(out, cols, w_stride) ||
+  if (!elements(dtype, d_rows) || !elements(dtype, d_weights) || !elements(dtype, d_y))
+    return H2O4GPU_KMEANS_EARG;
+  if (!fits(rows, cols, rows_stride) || !fits(out, cols, w_stride) ||
       !fits(rows, out, y_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_rows, d_weights, d_y, rows_stride, w_stride, expert_stride, y_stride, 0, d_offsets, experts, (int)rows,
@@ -388,7 +396,9 @@ KM_API int h2o4gpu_experts_product_drows(int dtype, size_t rows, int experts, si
   if (int rc = check(dtype, rows, experts, out, cols, rows ? (const void *)d_offsets : "", w_stride); rc <= 0)
     return rc;
   if (rows == 0) return H2O4GPU_KMEANS_OK;
-  if (!elements(dtype, d_dy) || !elements(dtype, d_weights) || !elements(dtype, d_drows) || !fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
+  if (!elements(dtype, d_dy) || !elements(dtype, d_weights) || !elements(dtype, d_drows))
+    return H2O4GPU_KMEANS_EARG;
+  if (!fits(rows, out, dy_stride) || !fits(out, cols, w_stride) ||
       !fits(rows, cols, drows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_weights, d_drows, dy_stride, w_stride, expert_stride, drows_stride, 0, d_offsets, experts,
@@ -412,7 +422,9 @@ KM_API int h2o4gpu_experts_product_dweights(int dtype, size_t rows, int experts,
   if (out > H2O4GPU_EXPERTS_MAX_SIDE || cols > H2O4GPU_EXPERTS_MAX_SIDE ||
       (rows > 1 && (dy_stride > H2O4GPU_EXPERTS_MAX_SIDE || rows_stride > H2O4GPU_EXPERTS_MAX_SIDE)))
     return H2O4GPU_KMEANS_EARG;
-  if (!elements(dtype, d_dweights) || (rows && (!elements(dtype, d_dy) || !elements(dtype, d_rows))) || !fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
+  if (!elements(dtype, d_dweights) || (rows && (!elements(dtype, d_dy) || !elements(dtype, d_rows))))
+    return H2O4GPU_KMEANS_EARG;
+  if (!fits(rows, out, dy_stride) || !fits(rows, cols, rows_stride))
     return H2O4GPU_KMEANS_EARG;
   ProductArgs a = {d_dy, d_rows, d_dweights, dy_stride, rows_stride, 0, cols, out * cols, d_offsets, experts, (int)rows,
                    (int)cols, (int)out, 0, nullptr, 0, 0};
