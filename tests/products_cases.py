@@ -80,7 +80,7 @@ CHECKS = ("differences", "broadcast", "graph", "graph_of_training", "other_strea
 
 def all_cases():
     cases = _products() + _quantize() + _fours() + _fours_of_experts()
-    cases += [dict(op=name) for name in CHECKS] + _words() + [dict(op="broadcast_between_words")]
+    cases += [dict(op=name) for name in CHECKS] + _words() + [dict(op="broadcast_between_words"), dict(op="two_at_once")]
     for i, c in enumerate(cases):
         c["name"] = "%03d_%s" % (i, "_".join(str(v) for v in c.values()))
     return cases

@@ -10,6 +10,7 @@ import json
 import math
 import os
 import sys
+import threading
 import traceback
 
 import numpy as np
@@ -387,6 +388,59 @@ def check_graph_of_training(_):
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(a, b), "replay %d differs" % k
+
+
+def check_two_at_once(_):
+    """Two captured steps with partial sums and aligned copies of their own, and two threads, all at the same time."""
+    for E, N, K, T, dt in ((3, 61, 75, 20000, torch.float32), (2, 131, 70, 9000, torch.bfloat16),
+                           (3, 1025, 1023, 12000, torch.bfloat16)):
+        order = routed(T, 1, E)
+        sets = []
+        for k in range(2):
+            x = torch.randn(T, K, generator=gen(60 + k)).to(dt).cuda().requires_grad_()
+            W = torch.randn(E, N, K, generator=gen(70 + k)).to(dt).cuda().requires_grad_()
+            sets.append((x, W, torch.randn(T, N, generator=gen(80 + k)).to(dt).cuda()))
+
+        def step(x, W, g):
+            y = experts.product(x, W, order)
+            return (y.detach(),) + torch.autograd.grad(y, (x, W), g)
+
+        want = [[t.clone() for t in step(*s)] for s in sets]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        graphs, outs = [], []
+        torch.cuda.synchronize()
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                step(*s)
+            stream.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(step(*s))
+        for k in range(3):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            eager = step(*sets[k % 2])
+            torch.cuda.synchronize()
+            for got, right in zip(outs + [eager], want + [want[k % 2]]):
+                for a, b in zip(got, right):
+                    assert torch.equal(a, b), "replay %d of %d x %d differs" % (k, N, K)
+        found = [None, None]
+
+        def work(k):
+            with torch.cuda.stream(streams[k]):
+                for _ in range(4):
+                    found[k] = step(*sets[k])
+            streams[k].synchronize()
+
+        threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for got, right in zip(found, want):
+            for a, b in zip(got, right):
+                assert torch.equal(a, b), "a thread's %d x %d differs" % (N, K)
 
 
 def check_other_stream(_):
