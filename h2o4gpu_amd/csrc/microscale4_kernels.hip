@@ -172,15 +172,14 @@ struct FourArgs {
 template <typename T>
 int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   const size_t pitch = codes_pitch(a.cols);
-  // what a buffer's offsets reach: the gathered x in all, 256 rows of a matrix
-  const bool reached = (!a.order || x_rows * pitch < BUFFER_BYTES) && pitch < BUFFER_BYTES / 512;
-  if (!reached || few_rows<Four>(a.rows, a.experts, a.out)) {
+  const Way way = way_of_four(a.rows, a.experts, a.out, a.cols, pitch, a.order != nullptr, x_rows);
+  if (way == FEW_ROWS || way == KEPT) {
     ThinArgs t = {};
     t.x = (const char *)a.x, t.w = (const char *)a.w, t.x_scales = a.x_scales, t.w_scales = a.w_scales, t.c = a.y;
     t.x_stride = t.w_stride = pitch, t.w_expert = pitch * a.out, t.scales_stride = scales_pitch(a.cols);
     t.c_stride = a.y_stride, t.order = a.order, t.offsets = a.offsets, t.top_k = a.top_k;
     t.experts = a.experts, t.rows = a.rows, t.n = a.out, t.k = (int)((a.cols + 127) / 128 * 32);
-    if (!a.experts && a.rows > 16 && a.rows <= 64 && a.cols <= 8192 && a.out >= 4096) return launch_kept<T>(t, stream);
+    if (way == KEPT) return launch_kept<T>(t, stream);
     return launch_thin<Four, T, true>(t, stream);
   }
   PipeArgs p = {};
@@ -189,7 +188,8 @@ int launch_four(const FourArgs &a, size_t x_rows, hipStream_t stream) {
   p.c_stride = a.y_stride, p.x_bytes = x_rows * pitch;
   p.order = a.order, p.offsets = a.offsets, p.top_k = a.top_k, p.experts = a.experts;
   p.rows = a.rows, p.n = a.out, p.k = (int)(pitch / 2);
-  return a.order ? launch_large<Four, T, FORWARD, true>(p, stream) : launch_large<Four, T, FORWARD, false>(p, stream);
+  return a.order ? launch_large<Four, T, FORWARD, true>(p, way, stream)
+                 : launch_large<Four, T, FORWARD, false>(p, way, stream);
 }
 
 bool sized(size_t rows, size_t cols) { return cols >= 1 && cols <= MAX_SIDE && rows <= ((size_t)1 << 40) / codes_pitch(cols); }

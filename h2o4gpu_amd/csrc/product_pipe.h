@@ -14,8 +14,6 @@ namespace kmhip {
 
 struct Four {};  // as an element type: microscaled 4-bit numbers
 
-enum Kind { FORWARD, DROWS, DWEIGHTS };
-
 struct PipeArgs {
   const char *x, *w;                        // x: m's operand, w: n's
   const unsigned char *x_scales, *w_scales; // Four only, rows of `scales_stride` bytes
@@ -615,8 +613,6 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads that read nothing end before the LDS is another's)
 }
 
-constexpr size_t BUFFER_BYTES = (size_t)1 << 32;  // what a buffer's offsets reach
-
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER, int BM, int BN, int WM, int WN>
 int launch_pipe(PipeArgs &a, hipStream_t stream) {
   const size_t m_tiles = KIND == DWEIGHTS ? (a.part < a.rows ? ragged_tiles(a.experts, a.rows, a.part) : (size_t)a.experts) *
@@ -639,22 +635,10 @@ int launch_pipe(PipeArgs &a, hipStream_t stream) {
   return launched();
 }
 
-// Tiles of 256 x 256, or of 128 x 128, of which a CU holds two: by how often the card is filled with either (an expert's
-// last tile is taken to be half full), and how long a stage then takes, 1.7 and 1.3 us. 64 experts' 65536 rows of 2048
-// with 2048 x 2048 bfloat16 take 543 us in large tiles and 674 in small ones (both before the tiles were stored as above),
-// 4 experts' 8000 rows of 1024 with 512 x 1024 27 and 16 us, 10 experts' 16941 rows of 4544 with 384 89 and 64, 160
-// experts' 49552 rows of 256 with 3392 188 and 191.
+// In tiles of 256 x 256, or of 128 x 128, of which a CU holds two.
 template <typename ELEMENT, typename OUT, Kind KIND, bool GATHER>
-int launch_large(PipeArgs &a, hipStream_t stream) {
-  auto turns = [&](int tile, int at_once) {
-    const double n = (a.n + tile - 1) / tile;
-    const double m = KIND == DWEIGHTS ? (double)((a.k + tile - 1) / tile) *
-                                            (a.part < a.rows ? a.rows / a.part + a.experts / 2 : a.experts)
-                                      : (double)a.rows / tile + a.experts / 2.0;
-    return ceil(m * n / at_once);
-  };
-  if (1.7 * turns(256, 256) <= 1.3 * turns(128, 512))
-    return launch_pipe<ELEMENT, OUT, KIND, GATHER, 256, 256, 2, 4>(a, stream);
+int launch_large(PipeArgs &a, Way way, hipStream_t stream) {
+  if (way == TILES_256) return launch_pipe<ELEMENT, OUT, KIND, GATHER, 256, 256, 2, 4>(a, stream);
   return launch_pipe<ELEMENT, OUT, KIND, GATHER, 128, 128, 2, 2>(a, stream);
 }
 

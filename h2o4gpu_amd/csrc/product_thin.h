@@ -9,22 +9,6 @@
 
 namespace kmhip {
 
-// Whether a product is one of few rows: of an expert at most 16 (float32: 48) on average, beyond which tiles of 128 x 128
-// are faster (27 experts of 5184 x 2504, 24 rows each: bfloat16 185 us against 199, 4 bits 63 against 68, float32 709
-// against 423; 40 rows 193, 63 and 709 against 263, 99 and 566), or so few that the workgroups of 64 rows times 32 of the
-// matrix are about as many as the CUs. Such tiles would be too few, and each has all of the columns: in one matrix of
-// 2048 x 8192, 200 rows take 45 us here and 77 there, float16; 400 (432 workgroups) 89 and 77. In 4 bits and in float32 a
-// tile's turn takes as long as three of these (4 bits, 400 rows 32 and 56 us, 800 60 and 55; float32 of 2048 x 4096, 400
-// rows 114 and 244, 800 219 and 245).
-template <typename ELEMENT>
-constexpr int FEW = sizeof(ELEMENT) == 4 ? 48 : 16;
-template <typename ELEMENT>
-bool few_rows(int rows, int experts, int n) {
-  constexpr int MOST = sizeof(ELEMENT) == 2 ? 320 : 768;
-  const int matrices = experts ? experts : 1;
-  return rows / matrices <= FEW<ELEMENT> || (rows / 64.0 + matrices / 2.0) * ((n + 31) / 32) <= MOST;
-}
-
 struct ThinArgs {
   const char *x, *w;
   const unsigned char *x_scales, *w_scales;            // Four only, rows of `scales_stride` bytes

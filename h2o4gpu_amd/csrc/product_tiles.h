@@ -9,6 +9,7 @@
 #include <limits.h>
 
 #include "experts_common.h"
+#include "product_rules.h"
 
 namespace kmhip {
 
@@ -150,12 +151,6 @@ __device__ __forceinline__ u32x4 load_whole(const T *p, bool halves) {
                    *reinterpret_cast<const unsigned *>((at + 14) & ~(size_t)3), (unsigned)(at & 2));
   }
 }
-// Whether some row of a matrix begins between words.
-template <typename T>
-inline bool between_words(const void *p, size_t stride) {
-  return sizeof(T) == 2 && (((uintptr_t)p & 3) || (stride & 1));
-}
-
 // A piece of which the first `valid` elements exist, zeros behind (and all zeros for valid <= 0), from any address
 // that a T may have.
 template <typename T>
@@ -228,7 +223,6 @@ __device__ __forceinline__ bool part_of_rows(const int *offsets, int experts, in
   p.sum = end - begin > part ? 2 * (p.first / part) + (p.first == begin) : -1;
   return true;
 }
-inline size_t part_sums(int rows, int part) { return 2 * ((size_t)rows / part + 1); }
 
 // launch(first block, blocks) until all of them are; a launch has at most 2^32 threads.
 template <typename F>

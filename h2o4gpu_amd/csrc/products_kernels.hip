@@ -247,35 +247,6 @@ bool rows_aligned(const ProductArgs &a) {
          a.w_expert % EPP == 0;
 }
 
-// Rows of a part of a matrix's gradient. The tiles of all parts are to be two for each CU at most, an expert's last part
-// taken to be half full; but no part has fewer than 512 rows, which take a tile some 10 us (float32 30), beside which a
-// sum's way to memory and back is little. 2 experts' 100000 rows of 102 with 102, bfloat16, take 26 us in parts of 512
-// rows, 30 of 1024 and 45 of 2048 (float32 56, 88, 163); 16 experts' 96000 of 256 with 256 59, 44 and 44. (For two tiles
-// to a CU numbers are aimed at that the parts' unevenness leaves below 512: aimed at 512 themselves, that last case took
-// 54 us.) Where the experts have as many tiles by themselves, parts are for one that has most of the rows. pipe_kernel
-// shares its tiles out by their rows where there are none, so its parts have 4096 (float32 2048): 32 experts' 3200 rows of
-// 1024 with 1024 take 37 us in parts of 1024 and 23 in none. Narrow matrices are product_kernel's, which does not:
-// four tiles for each CU, and no fewer than 512 rows (1000 experts of 77 x 101 float32, 300 rows on average and one with
-// 3794, take 130 us, in parts of 1024 156, of 2048 199; 16 experts' 64000 rows of 64 with 2048, in parts of 1024, 217, in
-// one part an expert 325). Where a matrix has 128 tiles there are enough whoever has the rows. All parts' sums are at most
-// 2 (1024 + 128) tiles of 64 KB.
-int rows_of_part(int size, size_t rows, int experts, size_t out, size_t cols) {
-  const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
-  if (tiles >= 128) return INT_MAX;
-  size_t part, least = 512;
-  if (out < 128 || cols < 128)
-    part = rows * tiles / 1024;
-  else if (experts * tiles >= 512)
-    part = rows * tiles / 512, least = size == 4 ? 2048 : 4096;
-  else
-    part = 2 * rows * tiles / (768 - experts * tiles);
-  return (int)((part > least ? part : least) + 63) / 64 * 64;
-}
-size_t sums_bytes(int size, size_t rows, int experts, size_t out, size_t cols) {
-  const int part = rows_of_part(size, rows, experts, out, cols);
-  return rows <= (size_t)part ? 0 : part_sums((int)rows, part) * out * cols * sizeof(float);
-}
-
 template <typename T>
 int join_parts(const ProductArgs &a, hipStream_t stream) {
   if (a.rows <= a.part) return H2O4GPU_KMEANS_OK;
@@ -287,14 +258,11 @@ int join_parts(const ProductArgs &a, hipStream_t stream) {
 
 template <typename T, Kind KIND>
 int launch_product(const ProductArgs &a, hipStream_t stream) {
-  const bool halves = between_words<T>(a.x, a.x_stride) || between_words<T>(a.w, a.w_stride) || (a.w_expert & 1);
-  const int each = a.rows / a.experts;
-  // few rows of an expert, see few_rows (the rows' gradient: 8 experts of 4096 x 4096, 24 rows each, bfloat16, 46 us there
-  // and 54 in tiles, but 300 experts of 512 x 512, 20 rows each, 50 and 32; float32 of the first with 48 rows each 173 and
-  // 262, of 300 experts with 50 rows each 144 and 357); far: an offset of a tile's last row would not fit a buffer
-  const bool far = a.x_stride * sizeof(T) >= BUFFER_BYTES / 512 || a.w_stride * sizeof(T) >= BUFFER_BYTES / 512;
-  const bool few = KIND == FORWARD ? few_rows<T>(a.rows, a.experts, a.n) : each <= (sizeof(T) == 4 ? 64 : 16);
-  if (KIND != DWEIGHTS && (far || few)) {
+  const ProductSizes sizes = {KIND,       (int)sizeof(T), a.x, a.w, a.x_stride, a.w_stride, a.w_expert, a.experts,
+                              a.rows, a.n,            a.k, a.part};
+  const bool halves = between_words(sizes);
+  const Way way = way_of(sizes);
+  if (KIND != DWEIGHTS && way == FEW_ROWS) {
     ThinArgs t = {};
     t.x = static_cast<const char *>(a.x), t.w = static_cast<const char *>(a.w), t.c = a.c;
     t.x_stride = a.x_stride * sizeof(T), t.w_stride = a.w_stride * sizeof(T), t.w_expert = a.w_expert * sizeof(T);
@@ -305,20 +273,14 @@ int launch_product(const ProductArgs &a, hipStream_t stream) {
     return rows_aligned<T>(a) && a.k % (16 / sizeof(T)) == 0 ? launch_thin<T, T, true>(t, stream)
                                                              : launch_thin<T, T, false>(t, stream);
   }
-  // Tiles that a matrix does not fill cost float32 and the matrices' gradient their products, which the kernel here leaves
-  // out (16 experts' 64000 rows of 2048 with 64 x 2048, float32, 181 us here and 246 there, the gradient 222 and 347); other
-  // products wait for memory (64 experts' 64000 rows of 640 with 16 x 640, bfloat16, 31 and 18). float32 gradients of few
-  // rows are faster here (8 experts' of 4096 x 4096, 24 rows each, 163 and 195, 48 rows each 225 and 196; bfloat16 86 and
-  // 68, 88 and 67).
-  constexpr int LEAST = sizeof(T) == 4 || KIND == DWEIGHTS ? 128 : 16;
-  if (!halves && a.n >= LEAST && (KIND != DWEIGHTS || (a.k >= LEAST && (sizeof(T) == 2 || each >= 32)))) {
+  if (way == TILES_128 || way == TILES_256) {
     PipeArgs p = {};
     p.x = static_cast<const char *>(a.x), p.w = static_cast<const char *>(a.w), p.c = a.c;
     p.x_stride = a.x_stride * sizeof(T), p.w_stride = a.w_stride * sizeof(T), p.w_expert = a.w_expert * sizeof(T);
     p.c_stride = a.c_stride, p.c_expert = a.c_expert;
     p.offsets = a.offsets, p.experts = a.experts, p.rows = a.rows, p.n = a.n, p.k = a.k;
     p.part = a.part, p.sums = a.sums;
-    KM_TRY((launch_large<T, T, KIND, false>(p, stream)));
+    KM_TRY((launch_large<T, T, KIND, false>(p, way, stream)));
     return KIND == DWEIGHTS ? join_parts<T>(a, stream) : H2O4GPU_KMEANS_OK;
   }
   constexpr int BM = 128, BN = 128;

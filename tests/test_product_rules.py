@@ -1,0 +1,40 @@
+"""Which kernel takes a product (csrc/product_rules.h), on the CPU: the sizes named beside the rules go where these say
+that they are fast."""
+import pytest
+
+from product_rules import Rules
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    return Rules(str(tmp_path_factory.mktemp("product_rules")))
+
+
+@pytest.mark.parametrize("kind,dtype,rows,experts,out,cols,way", [
+    ("forward", "bfloat16", 16, 8, 7168, 4096, "few rows"), ("forward", "bfloat16", 27 * 24, 27, 5184, 2504, "128"),
+    ("forward", "float32", 27 * 40, 27, 5184, 2504, "few rows"), ("forward", "float16", 200, 1, 2048, 8192, "few rows"),
+    ("forward", "float16", 400, 1, 2048, 8192, "128"), ("forward", "bfloat16", 65536, 64, 2048, 2048, "256"),
+    ("forward", "bfloat16", 8000, 4, 512, 1024, "128"), ("forward", "float32", 64000, 16, 64, 2048, "any rows"),
+    ("forward", "bfloat16", 64000, 64, 16, 640, "128"), ("forward", "bfloat16", 28800, 300, 777, 1001, "any rows"),
+    ("drows", "bfloat16", 8 * 24, 8, 4096, 4096, "128"), ("drows", "float32", 8 * 48, 8, 4096, 4096, "few rows"),
+    ("drows", "bfloat16", 65536, 64, 2048, 2048, "256"), ("dweights", "bfloat16", 65536, 64, 2048, 2048, "256"),
+    ("dweights", "float32", 8 * 24, 8, 4096, 4096, "any rows"), ("dweights", "float32", 8 * 48, 8, 4096, 4096, "256"),
+    ("dweights", "float32", 300000, 1000, 77, 101, "any rows"), ("dweights", "bfloat16", 16, 8, 4096, 4096, "256"),
+])
+def test_way(rules, kind, dtype, rows, experts, out, cols, way):
+    assert rules.way(kind, dtype, rows, experts, out, cols) == way
+
+
+@pytest.mark.parametrize("rows,out,cols,experts,gathered,way", [
+    (1, 4096, 4096, 0, 0, "few rows"), (33, 11003, 8190, 0, 0, "kept"), (64, 2048, 4096, 0, 0, "few rows"),
+    (800, 2048, 8192, 0, 0, "128"), (8192, 8192, 8192, 0, 0, "256"), (256, 2048, 4096, 64, 64, "few rows"),
+    (65536, 4096, 2048, 64, 16384, "256"), (1 << 23, 4096, 2048, 64, 1 << 23, "few rows"),
+])
+def test_way_of_four(rules, rows, out, cols, experts, gathered, way):
+    assert rules.way_four(rows, out, cols, experts, gathered) == way
+
+
+def test_parts(rules):
+    assert rules.part("bfloat16", 100000, 2, 102, 102) == 512 and rules.part("bfloat16", 96000, 16, 256, 256) == 1152
+    assert rules.part("bfloat16", 3200, 32, 1024, 1024) == 4096 and rules.part("float32", 3200, 32, 1024, 1024) == 2048
+    assert rules.part("float32", 64000, 16, 2048, 64) == 1024 and rules.part("bfloat16", 1 << 20, 1, 2048, 1024) == 2 ** 31 - 1
