@@ -38,3 +38,14 @@ def test_parts(rules):
     assert rules.part("bfloat16", 100000, 2, 102, 102) == 512 and rules.part("bfloat16", 96000, 16, 256, 256) == 1152
     assert rules.part("bfloat16", 3200, 32, 1024, 1024) == 4096 and rules.part("float32", 3200, 32, 1024, 1024) == 2048
     assert rules.part("float32", 64000, 16, 2048, 64) == 1024 and rules.part("bfloat16", 1 << 20, 1, 2048, 1024) == 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("kind,rows,experts,out,cols,way", [
+    ("forward", 4096, 4, 2048, 2048, "128"), ("drows", 4096, 4, 2048, 2048, "128"), ("forward", 8192, 16, 1024, 1024, "128"),
+    ("forward", 6000, 8, 1536, 768, "128"), ("forward", 20000, 4, 640, 640, "256"), ("drows", 20000, 4, 640, 640, "256"),
+    ("forward", 20000, 32, 768, 1536, "128"), ("dweights", 16384, 8, 512, 2048, "128"), ("dweights", 8192, 16, 1024, 1024, "128"),
+    ("dweights", 4096, 1, 4096, 4096, "256"), ("dweights", 65536, 64, 1024, 1024, "128"),
+])
+def test_tiles_of_float32(rules, kind, rows, experts, out, cols, way):
+    """A tile of float32 takes its operations' time, whether a CU has another or not."""
+    assert rules.way(kind, "float32", rows, experts, out, cols) == way
