@@ -244,7 +244,7 @@ template <typename T>
 bool rows_aligned(const ProductArgs &a) {
   constexpr size_t EPP = 16 / sizeof(T);
   return aligned_to(a.x, 16) && aligned_to(a.w, 16) && a.x_stride % EPP == 0 && a.w_stride % EPP == 0 &&
-         a.w_expert % EPP == 0;
+         (a.experts == 1 || a.w_expert % EPP == 0);
 }
 
 template <typename T>

@@ -371,7 +371,7 @@ def _sums(code, rows, n_experts, out, cols):
 def _at_words(t):
     """Whether all rows of a matrix, or of several, begin at multiples of 4 bytes."""
     each = 4 // t.element_size()
-    return t.data_ptr() % 4 == 0 and all(s % each == 0 for s in t.stride()[:-1])
+    return t.data_ptr() % 4 == 0 and all(s % each == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
 
 
 def _align(worth, *tensors):

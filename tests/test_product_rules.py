@@ -49,3 +49,28 @@ def test_parts(rules):
 def test_tiles_of_float32(rules, kind, rows, experts, out, cols, way):
     """A tile of float32 takes its operations' time, whether a CU has another or not."""
     assert rules.way(kind, "float32", rows, experts, out, cols) == way
+
+
+@pytest.mark.parametrize("kind", ["forward", "drows", "dweights"])
+def test_float32_always_begins_at_words(rules, kind):
+    """Matrices of an odd number of elements go where even ones do: 4 bytes are a word."""
+    for experts, rows in ((4, 4 * 64), (4, 4000), (300, 300 * 100)):
+        assert rules.way(kind, "float32", rows, experts, 2049, 2047) == rules.way(kind, "float32", rows, experts, 2049, 2048)
+        assert rules.way(kind, "bfloat16", rows, experts, 2049, 2047) == "any rows"
+
+
+@pytest.mark.parametrize("kind", ["forward", "drows"])
+def test_distance_of_one_matrix_is_nothing(rules, kind):
+    """How far the next matrix would be is asked where there is one."""
+    far = 2050 * 2048 + 1
+    assert rules.way(kind, "bfloat16", 4000, 1, 2050, 2048, apart=far) == rules.way(kind, "bfloat16", 4000, 1, 2050, 2048)
+    assert rules.way(kind, "bfloat16", 4000, 2, 2050, 2048, apart=far) == "any rows"
+
+
+def test_one_matrix_is_not_copied_for_its_distance():
+    import torch
+    from h2o4gpu_amd import experts
+    one = torch.zeros(200 * 128 + 1, dtype=torch.bfloat16).as_strided((1, 200, 128), (200 * 128 + 1, 128, 1))
+    two = torch.zeros(2 * 200 * 128 + 1, dtype=torch.bfloat16).as_strided((2, 200, 128), (200 * 128 + 1, 128, 1))
+    assert experts._at_words(one) and not experts._at_words(two)
+    assert experts._at_words(torch.zeros(2, 3, 5)) and not experts._at_words(torch.zeros(2, 3, 5, dtype=torch.float16))
