@@ -89,7 +89,9 @@ inline size_t sums_bytes(int size, size_t rows, int experts, size_t out, size_t 
 // takes 1.95 us for each that its CU has, a large one's 7.3, and what counts is how many a CU gets. In large and in small
 // tiles take: 4 experts' 4096 rows of 2048 with 2048 x 2048 467 and 239 us (the rows' gradient 482 and 249), 8 experts'
 // 6000 of 768 with 1536 186 and 145, 4 experts' 20000 of 640 with 640 158 and 166, 64 experts' 65536 of 1024 with 1024 951
-// and 955; matrices' gradients 8 experts' 16384 of 512 with 2048 962 and 397, one expert's 4096 of 4096 with 4096 950 and 973.
+// and 955; matrices' gradients 8 experts' 16384 of 512 with 2048 962 and 397, one expert's 4096 of 4096 with 4096 950 and 973. Of parts
+// some numbers have no rows, and a CU may get two large tiles where another gets none, for the 6 % that they gain at best (8
+// experts' 16384 rows of 1023 with 1025 968 and 627).
 inline Way tiles_of(const ProductSizes &a) {
   auto turns = [&](int tile, int at_once) {
     const double n = (a.n + tile - 1) / tile;
@@ -98,6 +100,7 @@ inline Way tiles_of(const ProductSizes &a) {
                                         : (double)a.rows / tile + a.experts / 2.0;
     return ceil(m * n / at_once);
   };
+  if (a.size == 4 && a.kind == DWEIGHTS && a.part < a.rows) return TILES_128;
   if (a.size == 4) return 7.3 * turns(256, 256) <= 1.95 * turns(128, 256) ? TILES_256 : TILES_128;
   return 1.7 * turns(256, 256) <= 1.3 * turns(128, 512) ? TILES_256 : TILES_128;
 }

@@ -74,3 +74,10 @@ def test_one_matrix_is_not_copied_for_its_distance():
     two = torch.zeros(2 * 200 * 128 + 1, dtype=torch.bfloat16).as_strided((2, 200, 128), (200 * 128 + 1, 128, 1))
     assert experts._at_words(one) and not experts._at_words(two)
     assert experts._at_words(torch.zeros(2, 3, 5)) and not experts._at_words(torch.zeros(2, 3, 5, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("rows,experts,out,cols", [(16384, 8, 1025, 1023), (16384, 8, 512, 2048), (8192, 16, 1024, 1024),
+                                                   (65536, 64, 1024, 1024), (20000, 4, 640, 640)])
+def test_parts_of_float32_are_taken_in_small_tiles(rules, rows, experts, out, cols):
+    assert rules.part("float32", rows, experts, out, cols) < rows
+    assert rules.way("dweights", "float32", rows, experts, out, cols) == "128"
