@@ -74,7 +74,16 @@ __device__ __forceinline__ const char *same_in_all(const char *p) {
 }
 // 16 bytes at each lane's own offset behind a buffer's start to 64 consecutive places from `lds` on (the same in every
 // lane); nothing is read behind the buffer's size. Written out, because the compiler would wait for all of these before
-// a read of LDS that it cannot tell from where they write; who reads there waits for vmcnt by hand.
+// a read of LDS that it cannot tell from where they write; who reads there waits for vmcnt by hand. That is also why no
+// memory is named as changed: stages and scales are read behind meet(), which is a barrier to the compiler too, and which
+// every load has behind it before its stage is read; before the first stages it is s_waitcnt and __syncthreads(). (Row
+// numbers are ordinary stores.) The compiler does not look in here either for the five states that a memory instruction has
+// to stay behind a vector instruction, as readfirstlane is, that wrote one of its scalar registers: settled() is called
+// where a buffer's start or size may come from such, once for a tile. (Waiting here, for every load, cost 800 x 2048 x 8192
+// in 4 bits 57 -> 60 us.) m0 is named, so that no value of the compiler's own is kept there; it warns of every such name,
+// since it gives m0 to no variable.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ u32x4 buffer_of(const char *start, unsigned size) {
   return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(size_t)start),
                (unsigned)__builtin_amdgcn_readfirstlane((unsigned)((size_t)start >> 32) & 0xffffu),
@@ -84,7 +93,20 @@ __device__ __forceinline__ void to_lds_16(u32x4 buffer, unsigned offset, unsigne
 #if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
-               : "s"(lds), "v"(offset), "s"(buffer));
+               : "s"(lds), "v"(offset), "s"(buffer)
+               : "m0");
+#endif
+}
+#pragma clang diagnostic pop
+// A memory instruction may read these scalar registers, whatever wrote them.
+__device__ __forceinline__ void settled(const char *&a, const char *&b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 4" : "+s"(a), "+s"(b));
+#endif
+}
+__device__ __forceinline__ void settled(const char *&start, unsigned &size) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 4" : "+s"(start), "+s"(size));
 #endif
 }
 
@@ -407,6 +429,7 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       in_w += (size_t)r.expert * a.w_expert + (WC ? (size_t)r.n0 * SIZE : (size_t)r.n0 * a.w_stride);
     }
     in_x = same_in_all(in_x), in_w = same_in_all(in_w);
+    settled(in_x, in_w);
     in_left = r.k_end, in_stages = r.m_here ? stages_of(r.k_end) : 0x7fffffff, in_stage = 0;
     if (r.m_here == 0) in_left = 0;
     rows_in ^= BM;
@@ -415,7 +438,8 @@ __global__ __launch_bounds__(WM *WN * 64) void pipe_kernel(PipeArgs a) {
       const size_t row = of_x ? (GATHER ? 0 : (size_t)r.first) : (size_t)r.expert * a.n + r.n0;
       const unsigned rows = of_x ? (GATHER ? (unsigned)(a.x_bytes / a.x_stride) : (unsigned)r.m_here) : (unsigned)r.n_here;
       in_s = same_in_all((const char *)(of_x ? a.x_scales : a.w_scales) + row * a.scales_stride);
-      in_s_size = (rows - 1) * (unsigned)a.scales_stride + 16;
+      in_s_size = __builtin_amdgcn_readfirstlane((rows - 1) * (unsigned)a.scales_stride + 16);
+      settled(in_s, in_s_size);
     }
   };
   unsigned x_size = 0, w_size = 0;
