@@ -118,7 +118,8 @@ class Microscale4:
 
 
 def quantize(values):
-    """Microscale4 of `values`, (rows, cols) or (experts, rows, cols), float32, bfloat16 or float16.
+    """Microscale4 of `values`, (rows, cols) with contiguous rows or (experts, rows, cols) of any strides (which are
+    copied if need be), float32, bfloat16 or float16.
 
     The power of two of 32 columns is that of their largest magnitude over 4, at least 2^-127; elements
     are rounded to the nearest number, a tie to the one of even code, and what is then beyond 6 is 6
@@ -135,7 +136,7 @@ def quantize(values):
     out._allocate(values, shape[:-1], shape[-1], values.dtype)
     if len(shape) == 3:
         values = values.reshape(-1, shape[-1])
-        if values.shape[0] > 1 and not (values.stride(1) == 1 and values.stride(0) >= shape[-1]):
+        if not (values.stride(1) == 1 and (values.shape[0] < 2 or values.stride(0) >= shape[-1])):
             values = values.contiguous()
     ptr, stride = _rows("values", values)
     _call(out.device.index, "h2o4gpu_microscale4_quantize", _TYPES[out.dtype], values.shape[0], out.cols, ptr, stride,

@@ -1,5 +1,5 @@
 """The cases of test_gpu_large_products.py: products that the rules send to pipe_kernel's tiles, and which of these each
-pass takes (forward, rows' gradient, matrices' gradient). Plain values, so that the collecting process needs no torch."""
+pass takes (forward, rows' gradient, matrices' gradient); and numbers into 4 bits. Plain values, so that the collecting process needs no torch."""
 
 HALVES = ("bfloat16", "float16")
 
@@ -50,6 +50,7 @@ def all_cases():
         for in_order in (False, True):
             cases.append(dict(op="large_fours", tokens=tokens, top_k=top_k, experts=experts, out=out, cols=cols, most=False,
                               dtype=(HALVES + ("float32",))[(i + in_order) % 3], in_order=in_order, ways=[way]))
+    cases.append(dict(op="rows_of_any_stride", ways=[]))
     for i, c in enumerate(cases):
         c["name"] = "%02d_%s" % (i, "_".join(str(v) for k, v in c.items() if k != "ways"))
     return cases

@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, os.path.dirname(HERE))
 sys.path.insert(0, HERE)
 from large_products_cases import DROPPED, all_cases  # noqa: E402
-from products_device_check import DT, LEVELS, ROUND, TINY, U32, roundings, stretches  # noqa: E402
+from products_device_check import DT, LEVELS, ROUND, TINY, U32, numbers, roundings, stretches  # noqa: E402
 from h2o4gpu_amd import experts, microscale4  # noqa: E402
 
 
@@ -131,6 +131,16 @@ def check_large_fours(c):
             found.add("y", y[lo:hi], a @ b.t(), (K / 8 + 16) * U32 * (a.abs() @ b.t().abs()))
     found.add("y behind", y[held:], torch.zeros_like(y[held:], dtype=torch.float64), 0.0 * y.new_zeros((), dtype=torch.float64))
     found.check()
+
+
+def check_rows_of_any_stride(_):
+    """A matrix per expert is copied where its rows are not contiguous, of one row as of several."""
+    for E, rows in ((1, 1), (2, 1), (1, 3), (3, 4)):
+        for v in (torch.randn(E, rows, 80, generator=drawn(5), device="cuda")[..., ::2],
+                  torch.randn(E, 40, rows, generator=drawn(6), device="cuda").transpose(1, 2),
+                  torch.randn(E, 1, 40, generator=drawn(7), device="cuda").expand(E, rows, 40)):
+            m, (code, scale, _) = microscale4.quantize(v), numbers(v.reshape(-1, 40).cpu())
+            assert m.codes().reshape(-1, 40).cpu().equal(code) and m.scales().reshape(-1, 2).cpu().equal(scale)
 
 
 def main():
