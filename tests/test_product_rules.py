@@ -26,7 +26,9 @@ def test_way(rules, kind, dtype, rows, experts, out, cols, way):
 
 
 @pytest.mark.parametrize("rows,out,cols,experts,gathered,way", [
-    (1, 4096, 4096, 0, 0, "few rows"), (33, 11003, 8190, 0, 0, "kept"), (64, 2048, 4096, 0, 0, "few rows"),
+    (1, 4096, 4096, 0, 0, "few rows"), (33, 11003, 8190, 0, 0, "kept"), (64, 2048, 4096, 0, 0, "kept"),
+    (17, 16, 512, 0, 0, "kept"), (16, 4096, 4096, 0, 0, "few rows"), (65, 2048, 4096, 0, 0, "few rows"),
+    (33, 4096, 8193, 0, 0, "few rows"), (33, 2048, 4096, 4, 33, "few rows"),
     (800, 2048, 8192, 0, 0, "128"), (8192, 8192, 8192, 0, 0, "256"), (256, 2048, 4096, 64, 64, "few rows"),
     (65536, 4096, 2048, 64, 16384, "256"), (1 << 23, 4096, 2048, 64, 1 << 23, "few rows"),
 ])
