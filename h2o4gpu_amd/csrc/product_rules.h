@@ -32,7 +32,11 @@ struct ProductSizes {
 // matrix are about as many as the CUs. Such tiles would be too few, and each has all of the columns: in one matrix of
 // 2048 x 8192, 200 rows take 45 us here and 77 there, float16; 400 (432 workgroups) 89 and 77. In 4 bits and in float32 a
 // tile's turn takes as long as three of these (4 bits, 400 rows 32 and 56 us, 800 60 and 55; float32 of 2048 x 4096, 400
-// rows 114 and 244, 800 219 and 245).
+// rows 114 and 244, 800 219 and 245). The average is what the host knows; the offsets lie on the GPU. Where one expert has
+// most rows, its matrix is read for every 16 of them: 1024 rows of 64 experts of 4096 x 4096, bfloat16, take 549 us evenly
+// shared (in tiles 372) and 473 all in one (52), in 4 bits 209 (138) and 182 (34). Matrices as large and as many as these, and
+// those of few columns, would be faster in tiles from fewer rows on (8 rows each of the former 423 and 366, of 64 experts of
+// 4096 x 1024 148 and 97), smaller and fewer ones not (of 8 experts of 2048 x 2048 20 and 26).
 inline bool few_rows(int size, int rows, int experts, int n) {
   const int matrices = experts ? experts : 1;
   return rows / matrices <= (size == 4 ? 48 : 16) ||
@@ -61,8 +65,10 @@ inline bool between_words(const ProductSizes &a) {
 // 1024 with 1024 take 37 us in parts of 1024 and 23 in none. Narrow matrices are product_kernel's, which does not:
 // four tiles for each CU, and no fewer than 512 rows (1000 experts of 77 x 101 float32, 300 rows on average and one with
 // 3794, take 130 us, in parts of 1024 156, of 2048 199; 16 experts' 64000 rows of 64 with 2048, in parts of 1024, 217, in
-// one part an expert 325). Where a matrix has 128 tiles there are enough whoever has the rows. All parts' sums are at most
-// 2 (1024 + 128) tiles of 64 KB.
+// one part an expert 325). A matrix of 128 tiles and more is in one part, which leaves CUs idle where few such have the rows:
+// one expert's 65536 rows of 1024 with 2048, bfloat16, take 890 us, of 1024 with 1920 in parts 407; 64 experts' 65536 of 2048
+// with 2048 530 us evenly shared, and 1930 where one expert has all of them. All parts' sums are at most 2 (1024 + 128) tiles of
+// 64 KB.
 inline int rows_of_part(int size, size_t rows, int experts, size_t out, size_t cols) {
   const size_t tiles = ((out + 127) / 128) * ((cols + 127) / 128);
   if (tiles >= 128) return INT_MAX;
@@ -110,7 +116,7 @@ inline Way way_of(const ProductSizes &a) {
   const int each = a.rows / a.experts;
   // few rows of an expert, see few_rows (the rows' gradient: 8 experts of 4096 x 4096, 24 rows each, bfloat16, 46 us there
   // and 54 in tiles, but 300 experts of 512 x 512, 20 rows each, 50 and 32; float32 of the first with 48 rows each 173 and
-  // 262, of 300 experts with 50 rows each 144 and 357); far: an offset of a tile's last row would not fit a buffer
+  // 262, of 300 experts with 50 rows each 173 and 176); far: an offset of a tile's last row would not fit a buffer
   const bool far = a.x_stride * a.size >= BUFFER_BYTES / 512 || a.w_stride * a.size >= BUFFER_BYTES / 512;
   const bool few = a.kind == FORWARD ? few_rows(a.size, a.rows, a.experts, a.n) : each <= (a.size == 4 ? 64 : 16);
   if (a.kind != DWEIGHTS && (far || few)) return FEW_ROWS;

@@ -473,9 +473,13 @@ def product(rows, weights, order):
     rows has a gradient of zeros.
 
     Sizes, types, strides and addresses choose between kernels that add up in another order: the same numbers laid out
-    otherwise may differ in the last bit. Fastest are rows that begin at multiples of 4 bytes (of 16-bit types, an even
-    number of columns); of others a long product makes copies that do. The gradient of matrices of less than 128
-    x 128 x 128 elements takes up to 151 MB for partial sums while it runs."""
+    otherwise may differ in the last bit. Fastest are rows that begin at multiples of 4 bytes (float32 always, of 16-bit
+    types an even number of columns). Of others a long product makes copies that do, anew in each forward and backward pass and
+    for its time: as much memory again as the rows, the incoming gradient and all experts' matrices take. The gradient of
+    matrices of less than 128 tiles of 128 x 128 takes up to 151 MB for partial sums while it runs.
+
+    Which kernel is fast for few rows is decided by the rows of an expert on average: a batch nearly all of whose rows have one
+    of many experts may take several times as long as an evenly shared one of as many."""
     if not (isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _TYPES):
         _tensor("rows", rows, 2)
         _type_of("rows", rows)
